@@ -116,6 +116,72 @@ int ti_amd_softmax_f32(const float* x, float* y, int rows, int cols, uintptr_t s
  * the memory traffic.  Validation as ti_amd_layernorm_f32; y must not overlap x. */
 int ti_amd_layernorm_softmax_f32(const float* x, const float* gamma, const float* beta, float* y,
                                  int rows, int cols, float eps, uintptr_t stream, int device);
+
+/* The int8 KV cache: no counterpart in the reference, whose caches are fp16.
+ * A row of head_dim fp16 values (one token, one key head) is held as head_dim
+ * bytes and one fp32 scale = fp32_rn(max|x| / 127) (1 for a row of zeros, NaN
+ * for a row with an infinity or NaN, which then reads as NaN); its value is
+ * c * scale with c the whole number nearest x / scale, ties to even.  The caller
+ * owns the buffers, all 16-byte aligned: k and v of slots * kv_heads * capacity *
+ * head_dim bytes, k_scales and v_scales of slots * kv_heads * capacity floats.
+ * Their inner order is the kernels' own (k's rows one after another, v in blocks
+ * of 64 tokens); rows never written are never read as part of a request.
+ * capacity is a multiple of 64, head_dim 64 or 128. */
+typedef struct ti_amd_kv_i8 {
+  uint8_t* k;
+  uint8_t* v;
+  float* k_scales;
+  float* v_scales;
+  int32_t slots, kv_heads, capacity, head_dim;
+} ti_amd_kv_i8;
+/* ti_amd_kv_append_i8: k, v fp16 [batch][kv_heads][rows][head_dim]; row i <
+ * lengths[b] (null: every row) becomes token positions[b] + i of slots[b].  The
+ * metadata is int32 [batch] on the device.  What lies outside the cache (a slot,
+ * a token) is not written; where two requests write the same token the later
+ * request's row stays. */
+int ti_amd_kv_append_i8(const ti_amd_kv_i8* cache, const uint16_t* k, const uint16_t* v, const int32_t* slots,
+                        const int32_t* positions, const int32_t* lengths, int batch, int rows, uintptr_t stream, int device);
+/* ti_amd_kv_read_i8: the same rows back, fp16_rn(fp32(c * scale)); zeros past
+ * lengths[b] and outside the cache. */
+int ti_amd_kv_read_i8(const ti_amd_kv_i8* cache, uint16_t* k, uint16_t* v, const int32_t* slots, const int32_t* positions,
+                      const int32_t* lengths, int batch, int rows, uintptr_t stream, int device);
+/* ti_amd_attention_i8kv: q, y fp16 [batch][heads][q_len][head_dim] over the
+ * cache; query head h reads key head h / (heads / kv_heads).  Request b's keys
+ * are tokens 0 .. kv_lengths[b] - 1 of slots[b] (clamped to the capacity; a slot
+ * outside the cache has none).  Query i < q_lengths[b] (null: q_len) sees them
+ * all, or with causal = 1 those up to offsets[b] + i; offsets null means
+ * kv_lengths[b] - q_lengths[b]: the queries are the request's last tokens.  Rows
+ * that see no key, and queries past q_lengths[b], are exactly 0.
+ * prefix_len > 0: in front of its own keys every query also sees tokens 0 ..
+ * prefix_len - 1 of prefix_slot, whose bytes are read once for the batch.
+ * Scores, softmax and sums are fp32; probabilities are rounded to fp16.
+ * max_kv (0: the capacity) is what kv_lengths are expected to stay within: it
+ * plans the launch and its workspace, and longer requests are answered too.
+ * workspace: ti_amd_attention_i8kv_workspace bytes (-1 for invalid arguments, 0
+ * if none is needed), used by this call alone until its work is done. */
+int64_t ti_amd_attention_i8kv_workspace(const ti_amd_kv_i8* cache, int batch, int heads, int q_len, int max_kv,
+                                        int prefix_len);
+int ti_amd_attention_i8kv(const ti_amd_kv_i8* cache, const uint16_t* q, uint16_t* y, const int32_t* slots,
+                          const int32_t* kv_lengths, const int32_t* q_lengths, const int32_t* offsets, void* workspace,
+                          int64_t workspace_bytes, int batch, int heads, int q_len, int max_kv, int causal,
+                          int prefix_slot, int prefix_len, uintptr_t stream, int device);
+
+/* ti_amd_sample: one token per row of logits [batch][vocab] (dtype 0 fp16, 1
+ * fp32; vocab at most 262144) from uniforms[batch] in [0, 1) (others are taken
+ * as the nearest of them, NaN as 0).  Tokens are ordered by logit, ties by
+ * index; kept are the first top_k (<= 0: all), of these the shortest run from
+ * the front with top_p of their probability (>= 1: all), of these those with at
+ * least min_p of the likeliest one's (<= 0: all), the likeliest always.  The
+ * token is the first whose cumulative probability among the kept ones exceeds
+ * uniforms[b], probs[b] its probability among them.  A temperature that is not
+ * above 0, or a logit of +inf, gives the likeliest token with probability 1; a
+ * row without a logit above -inf gives 2^31 - 1 with probability 0.  NaN logits
+ * are never chosen.  temperature, top_k, top_p and min_p are per row on the
+ * device, or null: then the *_all values hold for every row.  The answer depends
+ * on nothing but its row. */
+int ti_amd_sample(const void* logits, int dtype, const float* uniforms, const float* temperature, const int32_t* top_k,
+                  const float* top_p, const float* min_p, float temperature_all, int top_k_all, float top_p_all,
+                  float min_p_all, int32_t* tokens, float* probs, int batch, int vocab, uintptr_t stream, int device);
 #ifdef __cplusplus
 }
 #endif

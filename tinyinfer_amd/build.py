@@ -32,7 +32,8 @@ HIP_FLAGS = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-ffp-contr
 HOST_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-march=x86-64-v3", "-ffp-contract=fast",
               "-fno-math-errno", "-I", str(ROOT / "include")]
 
-BACKEND_HIP = ["gemm.hip", "attention.hip", "rowops.hip", "backend_v2.hip", "backend_legacy.hip"]
+BACKEND_HIP = ["gemm.hip", "attention.hip", "rowops.hip", "kv_cache.hip", "kv_attention.hip", "sample.hip",
+               "backend_v2.hip", "backend_legacy.hip"]
 LLM_HIP = ["llm_runtime.hip"]
 
 

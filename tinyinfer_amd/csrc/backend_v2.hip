@@ -96,6 +96,53 @@ int run_gemm(const uint16_t* a, const void* w, bool int8, const float* scales, c
   return hip_status(err);
 }
 
+
+// The int8 cache a caller hands over: every buffer and extent its kernels index.
+int check_cache(const ti_amd_kv_i8* c, tia::KvI8& out) {
+  if (!c || (c->head_dim != 64 && c->head_dim != 128) || c->slots <= 0 || c->kv_heads <= 0 || c->kv_heads > 65535 ||
+      c->capacity <= 0 || c->capacity % 64 != 0 || !shape_fits({c->slots, c->kv_heads, c->capacity, c->head_dim}, 1) ||
+      !aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scales, 16) || !aligned(c->v_scales, 16))
+    return fail(TI_V2_INVALID_ARGUMENT,
+                "int8 cache: 16-byte aligned buffers, head_dim 64 or 128, capacity a multiple of 64 and positive extents");
+  out.k = c->k;
+  out.v = c->v;
+  out.k_scales = c->k_scales;
+  out.v_scales = c->v_scales;
+  out.slots = c->slots;
+  out.kv_heads = c->kv_heads;
+  out.capacity = c->capacity;
+  out.head_dim = c->head_dim;
+  return TI_V2_OK;
+}
+bool optional_aligned(const void* p, size_t bytes) { return !p || aligned(p, bytes); }
+
+int check_kv_rows(const void* k, const void* v, const int32_t* slots, const int32_t* positions, const int32_t* lengths,
+                  int batch, int rows, const tia::KvI8& c) {
+  if (!aligned(k, 2) || !aligned(v, 2) || !aligned(slots, 4) || !aligned(positions, 4) || !optional_aligned(lengths, 4) ||
+      batch <= 0 || batch > 65535 || rows <= 0 || !shape_fits({batch, c.kv_heads, rows, c.head_dim}, 2))
+    return fail(TI_V2_INVALID_ARGUMENT, "invalid int8 cache rows: shape, pointers or alignment (batch at most 65535)");
+  return TI_V2_OK;
+}
+
+int check_kv_attention(const ti_amd_kv_i8* cache, int batch, int heads, int q_len, int max_kv, int prefix_slot,
+                       int prefix_len, tia::KvAttnArgs& a) {
+  const int status = check_cache(cache, a.cache);
+  if (status) return status;
+  const int64_t most = std::numeric_limits<int32_t>::max();
+  if (batch <= 0 || batch > 65535 || heads <= 0 || heads > 65535 || q_len <= 0 || heads % a.cache.kv_heads != 0 ||
+      int64_t(batch) * heads > most / q_len || max_kv < 0 || prefix_len < 0 || prefix_len > a.cache.capacity ||
+      (prefix_len > 0 && (prefix_slot < 0 || prefix_slot >= a.cache.slots)))
+    return fail(TI_V2_INVALID_ARGUMENT,
+                "invalid int8 cache attention: heads a multiple of kv_heads, at most 2^31 - 1 query rows, the prefix inside the cache");
+  a.batch = batch;
+  a.heads = heads;
+  a.q_len = q_len;
+  a.max_kv = max_kv == 0 || max_kv > a.cache.capacity ? a.cache.capacity : max_kv;
+  a.prefix_slot = prefix_slot;
+  a.prefix_len = prefix_len;
+  return TI_V2_OK;
+}
+
 }  // namespace
 
 extern "C" int ti_v2_abi_version(void) { return 2; }
@@ -429,4 +476,103 @@ extern "C" int ti_amd_softmax_f32(const float* x, float* y, int rows, int cols, 
   if (!shape_fits({rows, cols}, 4) || !aligned(x, 4) || !aligned(y, 4))
     return fail(TI_V2_INVALID_ARGUMENT, "invalid softmax arguments");
   return hip_status(tia::softmax_f32(x, y, rows, cols, reinterpret_cast<hipStream_t>(stream)));
+}
+
+extern "C" int ti_amd_kv_append_i8(const ti_amd_kv_i8* cache, const uint16_t* k, const uint16_t* v, const int32_t* slots,
+                                   const int32_t* positions, const int32_t* lengths, int batch, int rows,
+                                   uintptr_t stream, int device) {
+  int status = begin(device);
+  if (status) return status;
+  tia::KvAppendArgs a;
+  if ((status = check_cache(cache, a.cache))) return status;
+  if ((status = check_kv_rows(k, v, slots, positions, lengths, batch, rows, a.cache))) return status;
+  a.k = k;
+  a.v = v;
+  a.slots = slots;
+  a.positions = positions;
+  a.lengths = lengths;
+  a.batch = batch;
+  a.rows = rows;
+  return hip_status(tia::kv_append_i8(a, reinterpret_cast<hipStream_t>(stream)));
+}
+
+extern "C" int ti_amd_kv_read_i8(const ti_amd_kv_i8* cache, uint16_t* k, uint16_t* v, const int32_t* slots,
+                                 const int32_t* positions, const int32_t* lengths, int batch, int rows, uintptr_t stream,
+                                 int device) {
+  int status = begin(device);
+  if (status) return status;
+  tia::KvReadArgs a;
+  if ((status = check_cache(cache, a.cache))) return status;
+  if ((status = check_kv_rows(k, v, slots, positions, lengths, batch, rows, a.cache))) return status;
+  a.k = k;
+  a.v = v;
+  a.slots = slots;
+  a.positions = positions;
+  a.lengths = lengths;
+  a.batch = batch;
+  a.rows = rows;
+  return hip_status(tia::kv_read_i8(a, reinterpret_cast<hipStream_t>(stream)));
+}
+
+extern "C" int64_t ti_amd_attention_i8kv_workspace(const ti_amd_kv_i8* cache, int batch, int heads, int q_len, int max_kv,
+                                                   int prefix_len) {
+  tia::KvAttnArgs a;
+  error_text[0] = '\0';
+  if (check_kv_attention(cache, batch, heads, q_len, max_kv, 0, prefix_len, a)) return -1;
+  return tia::kv_attention_workspace(a);
+}
+
+extern "C" int ti_amd_attention_i8kv(const ti_amd_kv_i8* cache, const uint16_t* q, uint16_t* y, const int32_t* slots,
+                                     const int32_t* kv_lengths, const int32_t* q_lengths, const int32_t* offsets,
+                                     void* workspace, int64_t workspace_bytes, int batch, int heads, int q_len, int max_kv,
+                                     int causal, int prefix_slot, int prefix_len, uintptr_t stream, int device) {
+  int status = begin(device);
+  if (status) return status;
+  tia::KvAttnArgs a;
+  if ((status = check_kv_attention(cache, batch, heads, q_len, max_kv, prefix_slot, prefix_len, a))) return status;
+  if (!aligned(q, 2) || !aligned(y, 2) || !aligned(slots, 4) || !aligned(kv_lengths, 4) || !optional_aligned(q_lengths, 4) ||
+      !optional_aligned(offsets, 4) || (causal != 0 && causal != 1))
+    return fail(TI_V2_INVALID_ARGUMENT, "invalid int8 cache attention pointers, alignment or causal flag");
+  const int64_t needed = tia::kv_attention_workspace(a);
+  if (needed > 0 && (!aligned(workspace, 16) || workspace_bytes < needed))
+    return fail(TI_V2_INVALID_ARGUMENT, "the call needs a 16-byte aligned workspace of ti_amd_attention_i8kv_workspace bytes");
+  a.q = q;
+  a.out = y;
+  a.slots = slots;
+  a.kv_lengths = kv_lengths;
+  a.q_lengths = q_lengths;
+  a.offsets = offsets;
+  a.causal = causal != 0;
+  a.workspace = static_cast<float*>(workspace);
+  return hip_status(tia::kv_attention(a, reinterpret_cast<hipStream_t>(stream)));
+}
+
+extern "C" int ti_amd_sample(const void* logits, int dtype, const float* uniforms, const float* temperature,
+                             const int32_t* top_k, const float* top_p, const float* min_p, float temperature_all,
+                             int top_k_all, float top_p_all, float min_p_all, int32_t* tokens, float* probs, int batch,
+                             int vocab, uintptr_t stream, int device) {
+  int status = begin(device);
+  if (status) return status;
+  if ((dtype != TI_V2_FP16 && dtype != TI_V2_FP32) || !aligned(logits, dtype == TI_V2_FP16 ? 2 : 4) || !aligned(uniforms, 4) ||
+      !optional_aligned(temperature, 4) || !optional_aligned(top_k, 4) || !optional_aligned(top_p, 4) ||
+      !optional_aligned(min_p, 4) || !aligned(tokens, 4) || !aligned(probs, 4) || vocab > (1 << 18) ||
+      !shape_fits({batch, vocab}, 4))
+    return fail(TI_V2_INVALID_ARGUMENT, "invalid sampling arguments: fp16 or fp32 logits, at most 262144 of a row");
+  tia::SampleArgs a;
+  a.logits = logits;
+  a.f32 = dtype == TI_V2_FP32;
+  a.uniforms = uniforms;
+  a.temperature = temperature;
+  a.top_k = top_k;
+  a.top_p = top_p;
+  a.min_p = min_p;
+  a.temperature_all = temperature_all;
+  a.top_k_all = top_k_all;
+  a.top_p_all = top_p_all;
+  a.min_p_all = min_p_all;
+  a.tokens = tokens;
+  a.probs = probs;
+  a.batch = batch;
+  a.vocab = vocab;
+  return hip_status(tia::sample(a, reinterpret_cast<hipStream_t>(stream)));
 }

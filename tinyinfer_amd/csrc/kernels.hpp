@@ -223,4 +223,81 @@ hipError_t softmax_f32(const float* x, float* y, int rows, int cols, hipStream_t
 hipError_t layernorm_softmax_f32(const float* x, const float* g, const float* b, float* y, int rows,
                                 int cols, float eps, hipStream_t stream);
 
+// The int8 KV cache (layout in kv_cache.hip); capacity is a multiple of 64.
+struct KvI8 {
+  uint8_t* k = nullptr;
+  uint8_t* v = nullptr;
+  float* k_scales = nullptr;
+  float* v_scales = nullptr;
+  int slots = 0, kv_heads = 0, capacity = 0, head_dim = 64;
+};
+// k, v fp16 [batch][kv_heads][rows][D]: row i < lengths[b] (null: all) goes to
+// token positions[b] + i of slots[b].  What the kernels find outside the cache
+// (a slot, a token) is not written.
+struct KvAppendArgs {
+  KvI8 cache;
+  const uint16_t* k = nullptr;
+  const uint16_t* v = nullptr;
+  const int32_t* slots = nullptr;
+  const int32_t* positions = nullptr;
+  const int32_t* lengths = nullptr;
+  int batch = 0, rows = 0;
+};
+constexpr int kKvAppendRowsMax = 8;  // rows per request up to which rows are stored one by one
+hipError_t kv_append_i8(const KvAppendArgs& args, hipStream_t stream);
+// The way back: k, v fp16 [batch][kv_heads][rows][D], zeros past lengths[b] and
+// outside the cache.
+struct KvReadArgs {
+  KvI8 cache;
+  uint16_t* k = nullptr;
+  uint16_t* v = nullptr;
+  const int32_t* slots = nullptr;
+  const int32_t* positions = nullptr;
+  const int32_t* lengths = nullptr;
+  int batch = 0, rows = 0;
+};
+hipError_t kv_read_i8(const KvReadArgs& args, hipStream_t stream);
+
+// Attention over the int8 cache: q, out fp16 [batch][heads][q_len][D], query head
+// h reads key head h / (heads / kv_heads).  Request b's keys are tokens
+// [0, kv_lengths[b]) of slots[b]; query i < q_lengths[b] (null: q_len) sees those
+// up to offsets[b] + i where causal (offsets null: kv_lengths[b] - q_lengths[b],
+// the queries are the last tokens).  prefix_len > 0: every query sees tokens
+// [0, prefix_len) of prefix_slot in front of its own.  Rows without a key are 0.
+struct KvAttnArgs {
+  KvI8 cache;
+  const uint16_t* q = nullptr;
+  uint16_t* out = nullptr;
+  const int32_t* slots = nullptr;
+  const int32_t* kv_lengths = nullptr;
+  const int32_t* q_lengths = nullptr;
+  const int32_t* offsets = nullptr;
+  int batch = 0, heads = 0, q_len = 0, max_kv = 0;
+  int prefix_slot = 0, prefix_len = 0;
+  bool causal = true;
+  float* workspace = nullptr;  // kv_attention_workspace() bytes, 16-byte aligned
+};
+// The bytes of workspace a call needs (the shape and max_kv decide, 0 where no
+// keys are split); max_kv only plans: longer requests are answered all the same.
+int64_t kv_attention_workspace(const KvAttnArgs& args);
+hipError_t kv_attention(const KvAttnArgs& args, hipStream_t stream);
+
+// One token per row of logits [batch][vocab] (sample.hip has the definition).
+struct SampleArgs {
+  const void* logits = nullptr;
+  bool f32 = true;
+  const float* uniforms = nullptr;
+  // One per row, or null: the value for all.
+  const float* temperature = nullptr;
+  const int32_t* top_k = nullptr;
+  const float* top_p = nullptr;
+  const float* min_p = nullptr;
+  float temperature_all = 1.f, top_p_all = 1.f, min_p_all = 0.f;
+  int top_k_all = 0;
+  int32_t* tokens = nullptr;
+  float* probs = nullptr;
+  int batch = 0, vocab = 0;
+};
+hipError_t sample(const SampleArgs& args, hipStream_t stream);
+
 }  // namespace tia

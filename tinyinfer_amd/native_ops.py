@@ -55,6 +55,10 @@ _ABI = {
     "ti_v2_layernorm_f16": "ppppiif",
     "ti_v2_gelu_new_f16": "ppq",
     "ti_v2_softmax_f16": "ppii",
+    "ti_amd_kv_append_i8": "ppppppii",
+    "ti_amd_kv_read_i8": "ppppppii",
+    "ti_amd_attention_i8kv": "ppppppppqiiiiiii",
+    "ti_amd_sample": "pippppp" "fiff" "ppii",
 }
 _CTYPE = {"p": ctypes.c_void_p, "i": ctypes.c_int, "f": ctypes.c_float, "q": ctypes.c_int64}
 _TRAILER = [ctypes.c_size_t, ctypes.c_int]   # hipStream_t as uintptr_t, device ordinal
@@ -174,6 +178,34 @@ class _Call:
         at = held.data_ptr()
         self.args.extend(at + 4 * len(lists[0]) * i for i in range(len(lists)))
 
+    def cache(self, cache):
+        if type(cache) is not Int8KVCache:
+            raise TypeError("cache: an Int8KVCache (NativeOps.kv_cache_int8) is required")
+        self.device = cache.buffer.device
+        self.held.append(cache.buffer)
+        self.args.append(cache._at)
+
+    def per_request(self, batch, *items):
+        """One int per request, each item (value, upper, name): int32 [batch] tensors on
+        the call's device, whose values the kernels bound, or host ints or sequences
+        of them in [0, upper], checked here.  None stays null."""
+        torch, host, where = self.ops.torch, [], []
+        for value, upper, name in items:
+            if value is None:
+                self.args.append(None)
+            elif isinstance(value, self.ops.tensor_type):
+                self.operand(value, torch.int32, name, shape=(batch,))
+            else:
+                host.append(_per_request(value, batch, 0, upper, name))
+                where.append(len(self.args))
+                self.args.append(None)
+        if host:
+            at = len(self.args)
+            self.metadata(*host)
+            for i, pointer in zip(where, self.args[at:]):
+                self.args[i] = pointer
+            del self.args[at:]
+
     def scalars(self, *values):
         self.args.extend(values)
 
@@ -193,6 +225,39 @@ class _Call:
             raise RuntimeError(f"{self.symbol} failed ({status}): {detail}")
 
 
+class _KvI8(ctypes.Structure):
+    """ti_amd_kv_i8."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scales", ctypes.c_void_p),
+                ("v_scales", ctypes.c_void_p), ("slots", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("capacity", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+class Int8KVCache:
+    """An int8 KV cache of `slots` requests, made by ``NativeOps.kv_cache_int8``.
+
+    One zeroed buffer holds K's and V's bytes and their fp32 scales (one per
+    token and head), in the order include/tinyinfer_amd_ext.h describes; rows go in
+    through ``kv_append_int8`` and come back through ``kv_read_int8``.  `capacity`
+    is the requested one rounded up to a multiple of 64.  The cache keeps no
+    lengths: every call names the slots, positions and lengths it means."""
+
+    __slots__ = ("slots", "kv_heads", "capacity", "head_dim", "buffer", "_native", "_at")
+
+    def __init__(self, torch, slots, kv_heads, capacity, head_dim, device):
+        self.slots, self.kv_heads, self.head_dim = slots, kv_heads, head_dim
+        self.capacity = (capacity + 63) // 64 * 64
+        tokens = slots * kv_heads * self.capacity
+        self.buffer = torch.zeros(tokens * (2 * head_dim + 8), dtype=torch.uint8, device=device)
+        at = self.buffer.data_ptr()
+        self._native = _KvI8(at, at + tokens * head_dim, at + 2 * tokens * head_dim,
+                             at + 2 * tokens * head_dim + 4 * tokens, slots, kv_heads, self.capacity, head_dim)
+        self._at = ctypes.addressof(self._native)
+
+    @property
+    def device(self):
+        return self.buffer.device
+
+
 class NativeOps:
     """Inference-only device ops over the v2 ABI; operands are torch GPU tensors,
     work is queued on the current torch stream of their device."""
@@ -210,6 +275,7 @@ class NativeOps:
             self._declare(symbol, [_CTYPE[c] for c in codes] + _TRAILER, ctypes.c_int)
         if self.lib.ti_v2_abi_version() != 2:
             raise RuntimeError("native v2 ABI version mismatch: version 2 required")
+        self._declare("ti_amd_attention_i8kv_workspace", [ctypes.c_void_p] + [ctypes.c_int] * 5, ctypes.c_int64)
         self.catalog = json.loads(self.lib.ti_v2_gemm_catalog_json())
         listed = tuple({**entry, "tile": tuple(entry["tile"])} for entry in self.catalog["configs"])
         if listed != GEMM_CATALOG:
@@ -343,3 +409,177 @@ class NativeOps:
         call.scalars(batch, heads, nq, nk, dim, int(causal), config)
         call.run()
         return y
+
+    # -- int8 KV cache ---------------------------------------------------------
+    def kv_cache_int8(self, slots, kv_heads, capacity, head_dim, *, device=None):
+        """A zeroed cache for `slots` requests of up to `capacity` tokens (rounded up
+        to a multiple of 64), `kv_heads` key heads of 64 or 128 dims."""
+        torch = self.torch
+        _count(slots, "slots")
+        _count(kv_heads, "kv_heads", high=65535)
+        _count(capacity, "capacity", high=INT32_MAX - 63)
+        if type(head_dim) is not int or head_dim not in (64, 128):
+            raise ValueError("head_dim must be 64 or 128")
+        where = torch.device("cuda" if device is None else device)
+        if where.type != "cuda":
+            raise TypeError("device: a GPU (torch 'cuda' device) is required")
+        return Int8KVCache(torch, slots, kv_heads, capacity, head_dim, where)
+
+    def kv_append_int8(self, cache, k, v, slots, positions, *, lengths=None):
+        """Quantise k, v fp16 [B,G,Q,D] into the cache as they are: row i < lengths[b]
+        (None: Q) becomes token positions[b] + i of slots[b].
+
+        slots, positions and lengths are int32 [B] tensors, or host ints (one for
+        all, or B of them).  Host values must lie inside the cache; rows that device
+        values put outside it are not written.  Where two requests write the same
+        token, the later request's row stays."""
+        torch = self.torch
+        call = _Call(self, "ti_amd_kv_append_i8")
+        call.cache(cache)
+        call.operand(k, torch.float16, "k", rank=4)
+        batch, heads, rows, dim = k.shape
+        if heads != cache.kv_heads or dim != cache.head_dim:
+            raise ValueError(f"k must be [B, {cache.kv_heads}, Q, {cache.head_dim}], got {list(k.shape)}")
+        call.operand(v, torch.float16, "v", shape=k.shape)
+        self._batch_rows(batch, slots, positions, lengths, rows, cache)
+        call.per_request(batch, (slots, cache.slots - 1, "slots"), (positions, cache.capacity - 1, "positions"),
+                         (lengths, rows, "lengths"))
+        call.scalars(batch, rows)
+        call.run()
+
+    def kv_read_int8(self, cache, slots, positions, lengths, rows):
+        """fp16 k, v [B,G,rows,D]: row i < lengths[b] (None: rows) is token positions[b]
+        + i of slots[b]; zeros past the length and outside the cache.  slots, positions
+        and lengths as in ``kv_append_int8``."""
+        torch = self.torch
+        call = _Call(self, "ti_amd_kv_read_i8")
+        call.cache(cache)
+        batch = self._batch_of(slots, positions, lengths)
+        _count(rows, "rows")
+        self._batch_rows(batch, slots, positions, lengths, rows, cache)
+        shape = (batch, cache.kv_heads, rows, cache.head_dim)
+        k = call.output(shape, torch.float16)
+        v = call.output(shape, torch.float16)
+        call.per_request(batch, (slots, cache.slots - 1, "slots"), (positions, cache.capacity - 1, "positions"),
+                         (lengths, rows, "lengths"))
+        call.scalars(batch, rows)
+        call.run()
+        return k, v
+
+    def _batch_of(self, *values):
+        for value in values:
+            if value is not None and type(value) is not int:
+                return len(value)
+        return 1
+
+    def _batch_rows(self, batch, slots, positions, lengths, rows, cache):
+        """Host positions and lengths must stay inside the cache."""
+        if slots is None or positions is None:
+            raise ValueError("slots and positions are required")
+        if batch > 65535:
+            raise ValueError("batch must be at most 65535")
+        tensor = self.tensor_type
+        if isinstance(positions, tensor) or isinstance(lengths, tensor):
+            return
+        first = _per_request(positions, batch, 0, cache.capacity - 1, "positions")
+        count = _per_request(lengths, batch, rows, rows, "lengths")
+        if max(map(int.__add__, first, count)) > cache.capacity:
+            raise ValueError(f"positions + lengths pass the cache's capacity of {cache.capacity}")
+
+    def attention_int8kv(self, q, cache, slots, kv_lengths, *, q_lengths=None, query_offsets=None, causal=True,
+                         max_kv_length=None):
+        """q [B,H,Q,D] fp16 over the int8 cache, H a multiple of its key heads (query
+        head h reads key head h // (H // G)): request b's keys are tokens 0 ..
+        kv_lengths[b] - 1 of slots[b].
+
+        Causal: query i sees keys up to query_offsets[b] + i; None means
+        kv_lengths[b] - q_lengths[b], the queries being the request's last tokens
+        (append first, then attend).  Rows that see no key and queries past
+        q_lengths[b] are 0.  slots, kv_lengths, q_lengths and query_offsets are int32
+        [B] tensors or host ints; tensors make a call that a graph can capture.
+        max_kv_length: what kv_lengths stay within where the capacity is much larger
+        (it plans the launch only)."""
+        return self._attend_int8(q, cache, 0, 0, slots, kv_lengths, q_lengths, query_offsets, causal, max_kv_length)
+
+    def attention_shared_prefix(self, q, cache, prefix_slot, prefix_length, slots, kv_lengths, *, q_lengths=None,
+                                query_offsets=None, causal=True, max_kv_length=None):
+        """``attention_int8kv`` for a batch whose requests share a prefix: in front of its
+        own keys every query sees tokens 0 .. prefix_length - 1 (host ints) of
+        prefix_slot, which are read once for the whole batch.  kv_lengths and
+        query_offsets count the request's own tokens."""
+        if type(cache) is not Int8KVCache:
+            raise TypeError("cache: an Int8KVCache (NativeOps.kv_cache_int8) is required")
+        _count(prefix_slot, "prefix_slot", 0, cache.slots - 1)
+        _count(prefix_length, "prefix_length", 0, cache.capacity)
+        return self._attend_int8(q, cache, prefix_slot, prefix_length, slots, kv_lengths, q_lengths, query_offsets,
+                                 causal, max_kv_length)
+
+    def _attend_int8(self, q, cache, prefix_slot, prefix_length, slots, kv_lengths, q_lengths, query_offsets, causal,
+                     max_kv_length):
+        torch = self.torch
+        call = _Call(self, "ti_amd_attention_i8kv")
+        call.cache(cache)
+        call.operand(q, torch.float16, "q", rank=4)
+        batch, heads, nq, dim = q.shape
+        if dim != cache.head_dim or heads % cache.kv_heads:
+            raise ValueError(f"q must be [B, H, Q, {cache.head_dim}] with H a multiple of {cache.kv_heads}, got {list(q.shape)}")
+        if batch > 65535 or heads > 65535:
+            raise ValueError("batch and heads must each be at most 65535")
+        if type(causal) is not bool:
+            raise ValueError("causal must be a bool")
+        if slots is None or kv_lengths is None:
+            raise ValueError("slots and kv_lengths are required")
+        bound = 0 if max_kv_length is None else _count(max_kv_length, "max_kv_length", 0)
+        y = call.output(q.shape, torch.float16)
+        call.per_request(batch, (slots, cache.slots - 1, "slots"), (kv_lengths, cache.capacity, "kv_lengths"),
+                         (q_lengths, nq, "q_lengths"), (query_offsets, INT32_MAX - nq, "query_offsets"))
+        needed = self.lib.ti_amd_attention_i8kv_workspace(cache._at, batch, heads, nq, bound, prefix_length)
+        if needed > 0:
+            call.output((needed,), torch.uint8)
+        else:
+            call.args.append(None)
+        call.scalars(max(needed, 0), batch, heads, nq, bound, int(causal), prefix_slot, prefix_length)
+        call.run()
+        return y
+
+    # -- sampling ----------------------------------------------------------------
+    def sample(self, logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """One token per row of logits [B,V] (fp16 or fp32) from uniforms fp32 [B] in
+        [0, 1): (tokens int32 [B], probs fp32 [B], the tokens' probabilities among the
+        kept ones).
+
+        Tokens are ordered by logit, ties by index.  Kept are the first top_k (0: all),
+        of these the shortest run from the front with top_p of their probability, of
+        these those with at least min_p of the likeliest one's; the token is the first
+        whose cumulative probability among them exceeds the row's uniform.  Each of
+        temperature, top_p, min_p (fp32) and top_k (int32) is a number for all rows or
+        a [B] tensor.  Temperature 0 takes the likeliest token."""
+        torch = self.torch
+        call = _Call(self, "ti_amd_sample")
+        wide = isinstance(logits, self.tensor_type) and logits.dtype == torch.float32
+        call.operand(logits, torch.float32 if wide else torch.float16, "logits", rank=2)
+        batch, vocab = logits.shape
+        if vocab > 1 << 18:
+            raise ValueError("logits: at most 262144 columns")
+        call.scalars(int(wide))
+        call.operand(uniforms, torch.float32, "uniforms", shape=(batch,))
+        values = []
+        for x, dtype, name, high in ((temperature, torch.float32, "temperature", math.inf),
+                                     (top_k, torch.int32, "top_k", INT32_MAX), (top_p, torch.float32, "top_p", 1.0),
+                                     (min_p, torch.float32, "min_p", 1.0)):
+            if isinstance(x, self.tensor_type):
+                call.operand(x, dtype, name, shape=(batch,))
+                values.append(0)
+                continue
+            if dtype == torch.int32:
+                _count(x, name, 0)
+            elif type(x) not in (int, float) or not 0 <= x <= high or x == math.inf:
+                raise ValueError(f"{name} must be a number in [0, {'inf)' if high == math.inf else '1]'}")
+            call.scalars(None)
+            values.append(x)
+        call.scalars(*values)
+        tokens = call.output((batch,), torch.int32)
+        probs = call.output((batch,), torch.float32)
+        call.scalars(batch, vocab)
+        call.run()
+        return tokens, probs
