@@ -68,6 +68,22 @@ __device__ __forceinline__ half8_t widen8(uint32_t w0, uint32_t w1) {
   return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// x times the value that lane N of this lane's row of 16 holds (the broadcast is an
+// operand modifier of the multiplication).
+template <int N>
+__device__ __forceinline__ float mul_row_lane(float x, float of) {
+  const float y = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, of), 0x150 + N, 0xF, 0xF, true));
+  return x * y;
+}
+// x[kb][v] times lane 4 kb + v's value.
+__device__ __forceinline__ void mul_row(float4_t (&x)[4], float of) {
+#define TIA_MUL(kb, v) x[kb][v] = mul_row_lane<4 * kb + v>(x[kb][v], of);
+#define TIA_MUL4(kb) TIA_MUL(kb, 0) TIA_MUL(kb, 1) TIA_MUL(kb, 2) TIA_MUL(kb, 3)
+  TIA_MUL4(0) TIA_MUL4(1) TIA_MUL4(2) TIA_MUL4(3)
+#undef TIA_MUL4
+#undef TIA_MUL
+}
+
 template <int D, int QB>
 struct Merge {
   float4_t acc[kWaves][QB * D / 16][64];
@@ -130,25 +146,26 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
   const int64_t base = (int64_t(slot) * a.cache.kv_heads + head) * a.cache.capacity;
   const uint8_t* kp = a.cache.k + base * D + j * D + 16 * g;
   const uint8_t* vp = a.cache.v + base * D + lane * 16;
-  const float* ksp = a.cache.k_scales + base + 4 * g;
-  const float* vsp = a.cache.v_scales + base + 4 * g;
+  // Lane (j, g) holds the scales of the tile's key 16 (j / 4) + 4 g + j % 4: of row g's
+  // 16 scores of a tile, number 4 kb + v in order, lane 4 kb + v has the scale.
+  const int my_key = 16 * (j >> 2) + 4 * g + (j & 3);
+  const float* ksp = a.cache.k_scales + base + my_key;
+  const float* vsp = a.cache.v_scales + base + my_key;
   u32x4_t kr[4][D / 64], vr[D / 16];
-  float4_t ksr[4], vsr[4];
+  float ksr = 0.f, vsr = 0.f;
   auto load_k = [&](int tt) {
     const uint8_t* at = kp + int64_t(tt) * (kTile * D);
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) kr[kb][c] = *reinterpret_cast<const u32x4_t*>(at + 16 * kb * D + 64 * c);
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb) ksr[kb] = *reinterpret_cast<const float4_t*>(ksp + int64_t(tt) * kTile + 16 * kb);
+    ksr = ksp[int64_t(tt) * kTile];
   };
   auto load_v = [&](int tt) {
     const uint8_t* at = vp + int64_t(tt) * (kTile * D);
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) vr[d] = *reinterpret_cast<const u32x4_t*>(at + 1024 * d);
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb) vsr[kb] = *reinterpret_cast<const float4_t*>(vsp + int64_t(tt) * kTile + 16 * kb);
+    vsr = vsp[int64_t(tt) * kTile];
   };
   if (t < t_end) {
     load_k(t);
@@ -183,9 +200,10 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
   // the weight p * vs / unit that is rounded to fp16 is then at most p.
   float unit = 0.f, inv_unit = 1.f;
 
-  auto step = [&](auto full_c, int tt, int next) {
-    constexpr bool FULL = decltype(full_c)::value;
-    const int key0 = tt * kTile + 4 * g;
+  // One tile; MORE: this wave has a next one, whose loads are issued as the registers fall free.
+  auto step = [&](auto more_c, int tt) {
+    constexpr bool MORE = decltype(more_c)::value;
+    const bool full = (tt + 1) * kTile <= first;
     float4_t sc[QB][4];
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
@@ -200,22 +218,14 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
           for (int u = 0; u < QB; ++u)
             sc[u][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[u][2 * c + s], sc[u][kb], 0, 0, 0);
         }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    float4_t ck[4], wv[4];
-    float top = 0.f;
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        ck[kb][v] = ksr[kb][v] * p.scale;
-        // (Past the last key any row sees, scales may be anything.)
-        wv[kb][v] = FULL || key0 + 16 * kb + v < last ? vsr[kb][v] : 0.f;
-        top = fmaxf(top, wv[kb][v]);
-      }
-    if (next < t_end) load_k(next);
-    if (__ballot(top > unit)) {
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float ck = ksr * p.scale;
+    // (Past the last key any row sees, scales may be anything.)
+    const float vs = tt * kTile + my_key < last ? vsr : 0.f;
+    if constexpr (MORE) load_k(tt + kWaves);
+    if (__ballot(vs > unit)) {
+      const float top = wave_max(vs);
       const float raised = __builtin_amdgcn_ldexpf(1.f, __builtin_amdgcn_frexp_expf(top));  // > top
       const float f = unit / raised;
       unit = raised;
@@ -225,20 +235,24 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) acc[u][d] *= f;
     }
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb) wv[kb] *= inv_unit;
+    const float wv = vs * inv_unit;
     half8_t pp[QB][2];
 #pragma unroll
     for (int u = 0; u < QB; ++u) {
+      mul_row(sc[u], ck);
+      const int lim = end[u] - tt * kTile - 4 * g;  // key 16 kb + v of this lane is visible iff < lim
+      const auto mask = [&](float with) {
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) sc[u][kb][v] = 16 * kb + v < lim ? sc[u][kb][v] : with;
+      };
+      if (!full) mask(kNegInf);
       float high = kNegInf;
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const float x = sc[u][kb][v] * ck[kb][v];
-          sc[u][kb][v] = FULL || key0 + 16 * kb + v < end[u] ? x : kNegInf;
-          high = fmaxf(high, sc[u][kb][v]);
-        }
+        for (int v = 0; v < 4; ++v) high = fmaxf(high, sc[u][kb][v]);
       if (__ballot(high > m[u] + kRaise)) {
         high = fmaxf(high, __shfl_xor(high, 16, 64));
         high = fmaxf(high, __shfl_xor(high, 32, 64));
@@ -254,26 +268,31 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
       for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const float pr = __builtin_amdgcn_exp2f(sc[u][kb][v] - ref);
-          l[u] += pr;
-          const float w = pr * wv[kb][v];
-          pp[u][kb >> 1][4 * (kb & 1) + v] = f16(FULL || key0 + 16 * kb + v < end[u] ? w : 0.f);
+          sc[u][kb][v] = __builtin_amdgcn_exp2f(sc[u][kb][v] - ref);
+          l[u] += sc[u][kb][v];
         }
+      mul_row(sc[u], wv);
+      if (!full) mask(0.f);  // (0 times a scale that is not finite)
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          pp[u][kb >> 1][4 * (kb & 1) + v] = f16(sc[u][kb][v]);
     }
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d)
+    for (int d = 0; d < D / 16; ++d) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const half8_t vf = widen8(vr[d][2 * c], vr[d][2 * c + 1]);
 #pragma unroll
         for (int u = 0; u < QB; ++u) acc[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pp[u][c], acc[u][d], 0, 0, 0);
       }
-    if (next < t_end) load_v(next);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (MORE) load_v(tt + kWaves);
   };
-  for (; t < t_end; t += kWaves) {
-    if ((t + 1) * kTile <= first) step(std::true_type{}, t, t + kWaves);
-    else step(std::false_type{}, t, t + kWaves);
-  }
+  for (; t + kWaves < t_end; t += kWaves) step(std::true_type{}, t);
+  if (t < t_end) step(std::false_type{}, t);
 
   // The waves' states meet in LDS; wave w joins every fourth (block, 16 dims).
   auto& mg = *reinterpret_cast<Merge<D, QB>*>(lds);
@@ -332,8 +351,11 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
   }
 }
 
+// Waves per SIMD that the registers are budgeted for.
+constexpr int waves_for(int dim, int qb) { return dim == 64 ? (qb == 1 ? 4 : qb == 2 ? 3 : 2) : (qb == 1 ? 3 : 2); }
+
 template <int D, int QB, int PB>
-__global__ __launch_bounds__(64 * kWaves) void kv_attention_kernel(AttnPlan p) {
+__global__ __launch_bounds__(64 * kWaves, waves_for(D, QB > PB ? QB : PB)) void kv_attention_kernel(AttnPlan p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   int64_t id = blockIdx.x;
   const int heads = p.a.cache.kv_heads;
