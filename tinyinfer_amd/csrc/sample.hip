@@ -8,42 +8,53 @@
 // exceeds u times the mass of the kept ones.
 //
 // All three filters keep a run from the front, so nothing is sorted: a histogram
-// of (count, mass) over the distance from the maximum finds the bin in which a
-// count or a mass is reached, and only that bin's tokens are ordered.  Masses are
-// whole numbers of 2^-44 of the heaviest token's, computed from 64-bit
-// exponentials: their sums are the same in any order, so an answer depends on
-// its row alone, and cumulative masses are right to about 1e-12, so a token is
-// the one that 64-bit arithmetic gives.  A token lighter than 2^-45 counts as 0.
+// over the distance from the maximum, 256 bins to a unit of (max - logit) / T,
+// finds the bin in which a count or a mass is reached, and only the tokens of the
+// few bins in question are gathered and ordered.  A token of bin b at distance
+// (b + f) / 256 weighs e^(-b/256) (1 - q), q = 1 - e^(-f/256) < 2^-8: bins hold
+// their count and the sum of q in units of 2^-35, one 64-bit LDS addition per token,
+// and masses are whole numbers of 2^-44: sums are the same in any order, and an
+// answer depends on its row alone.  A token's mass is right to about 2^-31 of itself, so
+// the token is the one that 64-bit arithmetic gives but for a random number within
+// about 1e-10 of a border.  Tokens 32 units from the maximum (e^-32) weigh nothing.
 //
-// One workgroup per row: its passes after the first read the row from cache.
+// One workgroup per row reads it three times, the second and third time from cache.
+// (Keeping it in registers needs every pass unrolled over them: 50 KB of code that runs
+// once per wave, fetched from memory, took 20 us a pass; a pass over 201 KB in L2 reads
+// in 1.6 us.)
 #include "common.hpp"
 #include "kernels.hpp"
+#include "lds_limit.hpp"
 
 namespace tia {
 namespace {
 
-constexpr int kThreads = 1024, kBins = 2048, kList = 512;
-constexpr double kUnit = 17592186044416.0;  // 2^44
-constexpr double kPerNat = 64.0;            // bins per unit of (max - logit) / T
-constexpr float kNegInf = -__builtin_huge_valf();
-constexpr int kNoToken = 0x7fffffff;
-
 typedef unsigned long long u64;
 
-struct Bins {
-  u64 mass[kBins];      // then: mass in front of the bin
-  unsigned count[kBins];  // then: tokens in front of the bin
-};
+constexpr int kThreads = 1024, kPerThread = 8, kBins = kThreads * kPerThread, kList = 512, kRuns = 2048;
+constexpr unsigned kShort = 256;
+constexpr double kPerUnit = 256.0;  // bins per unit of (max - logit) / T
+constexpr int kCountShift = 45;     // a bin: count << 45 | sum of q
+constexpr u64 kOne = u64(1) << 35;  // weight of a token at its bin's near edge
+constexpr double kMass = 512.0;     // a mass: weight * e^(-b/256) * 2^9
+constexpr int kNoToken = 0x7fffffff;
+constexpr float kNegInf = -__builtin_huge_valf();
 struct SampleLds {
-  Bins all, sub;
-  u64 key[kList], w[kList];
+  union {
+    u64 bin[kBins];   // while the row is counted
+    u64 mass[kBins];  // then: the mass in front of each bin
+  };
+  unsigned count[kBins];  // tokens in front of each bin
+  u64 runs[kRuns];
+  u64 key[kList];         // the gathered tokens,
+  unsigned at[kList], q[kList];  // their bins and losses
+  unsigned wanted[kBins / 32 + 1];  // a bit per bin whose tokens are gathered (and a word of none)
   u64 wave_mass[kThreads / 64];
   unsigned wave_count[kThreads / 64];
   float wave_max[kThreads / 64];
   int wave_at[kThreads / 64];
-  u64 total_mass, low, high, answer_key, answer_mass;
-  unsigned total_count, list_count;
-  int bin;
+  u64 low, high, answer_key, answer_mass;
+  unsigned answer_count, list_count;
 };
 
 // 64-bit key whose ascending order is the row's: value descending, then index.
@@ -53,46 +64,147 @@ __device__ __forceinline__ u64 order_key(float x, int i) {
   return u64(~up) << 32 | unsigned(i);
 }
 
+__device__ __forceinline__ float value_of(u64 key) {
+  const unsigned up = ~unsigned(key >> 32);
+  return __builtin_bit_cast(float, up & 0x80000000u ? up & 0x7fffffffu : ~up);
+}
+
+// A row.  f(value, index) is called for every token (and, value NaN, for places outside
+// the row).  Vectors lie on 16-byte boundaries of memory, so the first and the last may
+// hold places outside the row, which are not read.
 template <typename T>
 struct Row {
+  static constexpr int W = 16 / int(sizeof(T)), kAhead = 16 / W;
+  typedef T vec __attribute__((ext_vector_type(W)));
   const T* p;
-  int n;
-  // f(value, index) for every token of the row.
+  int n, shift;  // places of the first vector in front of the row
+
+  __device__ __forceinline__ Row(const T* row, int length)
+      : p(row), n(length), shift(int(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T))) {}
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    constexpr int W = 16 / sizeof(T);
-    for (int i = int(threadIdx.x) * W; i < n; i += kThreads * W) {
-      if (i + W <= n) {
-        T x[W];
-        __builtin_memcpy(x, p + i, 16);
+    constexpr int kStep = kThreads * W;
+    int i = int(threadIdx.x) * W - shift;
+    // Whole vectors, kAhead loads in flight.
+    for (; i >= 0 && i + (kAhead - 1) * kStep + W <= n; i += kAhead * kStep) {
+      vec x[kAhead];
 #pragma unroll
-        for (int e = 0; e < W; ++e) f(float(x[e]), i + e);
-      } else {
-        for (int e = i; e < n; ++e) f(float(p[e]), e);
+      for (int c = 0; c < kAhead; ++c) x[c] = *reinterpret_cast<const vec*>(p + i + c * kStep);
+#pragma unroll
+      for (int c = 0; c < kAhead; ++c)
+#pragma unroll
+        for (int e = 0; e < W; ++e) f(float(x[c][e]), i + c * kStep + e);
+    }
+    for (; i < n; i += kStep) {
+      const vec x = load(i);
+#pragma unroll
+      for (int e = 0; e < W; ++e) f(float(x[e]), i + e);
+    }
+  }
+  // f(value, index) for the few tokens that `rare` holds for (which may hold for no NaN).
+  template <typename P, typename F>
+  __device__ __forceinline__ void pick(P rare, F f) const {
+    constexpr int kStep = kThreads * W;
+    for (int i = int(threadIdx.x) * W - shift; i < n; i += kAhead * kStep) {
+      vec x[kAhead];
+#pragma unroll
+      for (int c = 0; c < kAhead; ++c) x[c] = load(i + c * kStep);
+      unsigned hits = 0;
+#pragma unroll
+      for (int c = 0; c < kAhead; ++c)
+#pragma unroll
+        for (int e = 0; e < W; ++e) hits |= unsigned(rare(float(x[c][e]))) << (c * W + e);
+      while (hits) {
+        const int k = __builtin_ctz(hits), at = i + k / W * kStep + k % W;
+        hits &= hits - 1;
+        f(float(p[at]), at);
       }
     }
   }
+  // f(value) for one vector per thread, spread evenly over a row of more.
+  template <typename F>
+  __device__ __forceinline__ void sample(F f) const {
+    const int vectors = (n + shift + W - 1) / W;
+    const int at = vectors <= kThreads ? int(threadIdx.x) : int(unsigned(vectors) * u64(threadIdx.x) / kThreads);
+    if (at * W - shift >= n) return;
+    const vec x = load(at * W - shift);
+#pragma unroll
+    for (int e = 0; e < W; ++e) f(float(x[e]));
+  }
+  __device__ __forceinline__ vec load(int i) const {
+    if (i >= 0 && i + W <= n) return *reinterpret_cast<const vec*>(p + i);
+    vec x;
+#pragma unroll
+    for (int e = 0; e < W; ++e) x[e] = i + e >= 0 && i + e < n ? p[i + e] : T(__builtin_nanf(""));
+    return x;
+  }
 };
 
+// Distances from the maximum in bins, in fp32 with what its roundings leave out: D =
+// max - logit is a sum of two fp32 numbers exactly, 256 / T of two to 2^-48.  The
+// rounded distance, monotone in the logit, gives the bin (of tokens in order the bins
+// are in order); its fraction, taken with the rest, is right to about 2^-23 of a bin.
 struct Scale {
-  double top, per;  // max, 1 / T
-  __device__ __forceinline__ double distance(float x) const { return (top - double(x)) * per; }
+  float top, per, per_rest;  // max; 256 / T
+  double temp;
+  __device__ __forceinline__ Scale(float max, float t) : top(max), temp(t) {
+    const double p = kPerUnit / temp;
+    per = float(fmin(p, 3e38));  // (T below 1e-36: every smaller logit is past the last bin)
+    per_rest = float(p - double(per));
+    if (!(fabsf(per_rest) < 1e30f)) per_rest = 0.f;
+  }
+  // Not below kBins for -inf, neither below nor above for NaN.
+  __device__ __forceinline__ float distance(float x) const { return (top - x) * per; }
+  // The part of the distance behind its bin's near edge: in [-2^-10, 1 + 2^-10].
+  __device__ __forceinline__ float fraction(float x) const {
+    const float d = top - x, back = d - top, rest = (top - (d - back)) - (x + back);
+    return fmaf(d, per, -floorf(d * per)) + fmaf(d, per_rest, rest * per);
+  }
+  __device__ __noinline__ double weight_of(float x) const { return exp((double(x) - double(top)) / temp); }
 };
-// Bin of a distance; kBins where its token weighs nothing.
-__device__ __forceinline__ int bin_of(double d) {
-  const double at = d * kPerNat;
-  return at < double(kBins) ? int(at) : kBins;  // (NaN: kBins)
+// (1 - e^(-f/256)) 2^35 of a fraction f, made positive by f + kSlack, to its terms of
+// third order (the fourth is below 2^-36); a bin's near edge is kSlack in front of it.
+constexpr float kSlack = 1.f / 64;
+__device__ __forceinline__ unsigned loss(float fraction) {
+  constexpr double h = 1.0 / kPerUnit, one = double(kOne);
+  const float f = fraction + kSlack;
+  return unsigned(f * fmaf(f, fmaf(f, float(one * h * h * h / 6), float(-one * h * h / 2)), float(one * h)));
 }
-__device__ __forceinline__ u64 mass_of(double e) { return u64(e * kUnit + 0.5); }
+__device__ __forceinline__ u64 packed(float fraction) { return (u64(1) << kCountShift) + loss(fraction); }
+__device__ __forceinline__ unsigned count_of(u64 packed) { return unsigned(packed >> kCountShift); }
+__device__ __forceinline__ u64 weight_of(u64 packed) {
+  return count_of(packed) * kOne - (packed & ((u64(1) << kCountShift) - 1));
+}
+// e^(-i/256)
+__device__ __forceinline__ double step(int i) {
+  constexpr double k[kPerThread] = {1.0, 0.9961013694701175, 0.9922179382602435, 0.9883496471138451,
+                                    0.9844964370054085, 0.9806582491395386, 0.976835024950062, 0.9730267060991332};
+  double x = k[0];
+#pragma unroll
+  for (int e = 1; e < kPerThread; ++e) x = i == e ? k[e] : x;
+  return x;
+}
+__device__ __noinline__ double run_edge(unsigned run) { return exp((double(run) * -kPerThread + double(kSlack)) / kPerUnit); }
+// Mass of a weight in a bin whose edge is e = run_edge * step.
+__device__ __forceinline__ u64 mass_of(u64 weight, double e) { return u64(fma(double(weight), e * kMass, 0.5)); }
 
-// Exclusive sums over the bins, totals in total_mass and total_count.
-__device__ void scan(SampleLds& s, Bins& b) {
+// Turns the counted bins into what stands in front of each; all threads return the totals.
+__device__ void scan(SampleLds& s, u64& mass_all, unsigned& count_all) {
   const int t = int(threadIdx.x), lane = t & 63, wave = t >> 6;
   __syncthreads();
-  u64 m = b.mass[2 * t] + b.mass[2 * t + 1];
-  unsigned c = b.count[2 * t] + b.count[2 * t + 1];
-  u64 mi = m;
-  unsigned ci = c;
+  const double edge = run_edge(unsigned(t));
+  u64 m[kPerThread], mi = 0;
+  unsigned c[kPerThread], ci = 0;
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) {
+    const u64 b = s.bin[kPerThread * t + i];
+    m[i] = mi;
+    c[i] = ci;
+    mi += mass_of(weight_of(b), edge * step(i));
+    ci += count_of(b);
+  }
+  const u64 mine = mi;
+  const unsigned many = ci;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const u64 mu = __shfl_up(mi, o, 64);
@@ -107,21 +219,21 @@ __device__ void scan(SampleLds& s, Bins& b) {
     s.wave_count[wave] = ci;
   }
   __syncthreads();
-  u64 mb = 0;
-  unsigned cb = 0;
-  for (int w = 0; w < wave; ++w) {
-    mb += s.wave_mass[w];
-    cb += s.wave_count[w];
+  u64 front = mi - mine;
+  unsigned before = ci - many;
+  mass_all = 0;
+  count_all = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) {
+    front += w < wave ? s.wave_mass[w] : 0;
+    before += w < wave ? s.wave_count[w] : 0;
+    mass_all += s.wave_mass[w];
+    count_all += s.wave_count[w];
   }
-  const u64 m0 = b.mass[2 * t];
-  const unsigned c0 = b.count[2 * t];
-  b.mass[2 * t] = mb + mi - m;
-  b.mass[2 * t + 1] = mb + mi - m + m0;
-  b.count[2 * t] = cb + ci - c;
-  b.count[2 * t + 1] = cb + ci - c + c0;
-  if (t == kThreads - 1) {
-    s.total_mass = mb + mi;
-    s.total_count = cb + ci;
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) {
+    s.mass[kPerThread * t + i] = front + m[i];
+    s.count[kPerThread * t + i] = before + c[i];
   }
   __syncthreads();
 }
@@ -138,38 +250,97 @@ struct Place {
   u64 key;
 };
 
-__device__ __forceinline__ void clear(Bins& b) {
-  for (int i = int(threadIdx.x); i < kBins; i += kThreads) {
-    b.mass[i] = 0;
-    b.count[i] = 0;
+// floor(f m) for 0 <= f < 1 exactly (bits of f below 2^-64 count as 0); whole: f m is a whole number.
+__device__ __forceinline__ u64 part_of(float f, u64 m, bool& whole) {
+  const u64 fx = f > 0.f ? u64(ldexp(double(f), 64)) : 0;
+  whole = fx * m == 0;
+  return __umul64hi(fx, m);
+}
+// Goal of the first token with cumulative mass >= top_p m, and of the first above u m.
+__device__ __forceinline__ Goal goal_p(float top_p, u64 m) {
+  bool whole;
+  const u64 g = part_of(top_p, m, whole), up = whole ? g : g + 1;
+  return Goal{false, up > 0 ? up : 1};
+}
+__device__ __forceinline__ Goal goal_u(float u, u64 m) {
+  bool whole;
+  return Goal{false, part_of(u, m, whole) + 1};
+}
+
+// The bin in which the goal is reached: the last one that begins in front of it.  Every
+// wave searches for itself: its lanes look at 64 bins in even steps, then at the 128 of
+// one step.
+__device__ __forceinline__ unsigned find_bin(const SampleLds& s, const Goal& g) {
+  const unsigned lane = threadIdx.x & 63;
+  const auto in_front = [&](unsigned bin) { return __ballot((g.by_count ? u64(s.count[bin]) : s.mass[bin]) < g.goal); };
+  static_assert(kBins == 64 * 128, "two steps of the search");
+  const unsigned run = 128 * (__popcll(in_front(128 * lane)) - 1);  // (bin 0 always is)
+  return run + __popcll(in_front(run + lane)) + __popcll(in_front(run + 64 + lane)) - 1;
+}
+
+__device__ __forceinline__ bool is_wanted(const SampleLds& s, unsigned bin) { return s.wanted[bin >> 5] >> (bin & 31) & 1; }
+__device__ __forceinline__ void take(SampleLds& s, u64 key, unsigned bin, float fraction) {
+  const unsigned i = atomicAdd(&s.list_count, 1u);
+  if (i < kList) {
+    s.key[i] = key;
+    s.at[i] = bin;
+    s.q[i] = loss(fraction);
   }
 }
 
-// The last bin in front of which the goal is not yet reached, in s.bin.
-__device__ void find_bin(SampleLds& s, const Bins& b, const Goal& g, u64 mass0, unsigned count0, u64 mass_all,
-                         unsigned count_all) {
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int i = 2 * int(threadIdx.x) + e;
-    const u64 before = g.by_count ? count0 + u64(b.count[i]) : mass0 + b.mass[i];
-    const u64 after = i + 1 < kBins ? (g.by_count ? count0 + u64(b.count[i + 1]) : mass0 + b.mass[i + 1])
-                                    : (g.by_count ? count0 + u64(count_all) : mass0 + mass_all);
-    if (before < g.goal && g.goal <= after) s.bin = i;
+// A gathered token's place in the row's order, one per thread.
+struct Gathered {
+  u64 key = 0, before = 0, after = 0;  // mass in front of the token, and with it
+  unsigned rank = 0, bin = ~0u;
+  // weight0, count0: what stands in front of the list within its (single) bin.
+  __device__ __forceinline__ void order(const SampleLds& s, u64 weight0, unsigned count0) {
+    const unsigned n = min(s.list_count, unsigned(kList));
+    bin = ~0u;
+    if (threadIdx.x >= n) return;
+    key = s.key[threadIdx.x];
+    bin = s.at[threadIdx.x];
+    u64 front = weight0;
+    rank = s.count[bin] + count0;
+#pragma unroll 8
+    for (unsigned o = 0; o < n; ++o) {
+      const u64 k = s.key[o];
+      const unsigned q = s.q[o], at = s.at[o];
+      const bool ahead = (at == bin) & (k < key);
+      front += ahead ? kOne - q : 0;
+      rank += ahead;
+    }
+    const double e = run_edge(bin / kPerThread) * step(int(bin % kPerThread));
+    before = s.mass[bin] + mass_of(front, e);
+    after = s.mass[bin] + mass_of(front + kOne - s.q[threadIdx.x], e);
   }
-  __syncthreads();
-}
+  __device__ __forceinline__ Place resolve(SampleLds& s, unsigned of, const Goal& g) const {
+    if (bin == of && (g.by_count ? rank : before) < g.goal && g.goal <= (g.by_count ? rank + 1 : after)) {
+      s.answer_key = key;
+      s.answer_mass = after;
+      s.answer_count = rank + 1;
+    }
+    __syncthreads();
+    const Place got{s.answer_mass, s.answer_count, s.answer_key};
+    __syncthreads();
+    return got;
+  }
+};
 
+// Gathers the tokens of `bin`, or where they are too many those of a run of it in which
+// the goal is reached.
 template <typename T>
-__device__ Place locate(SampleLds& s, const Row<T>& row, const Scale& sc, const Goal& g, u64 mass_all, unsigned count_all) {
-  find_bin(s, s.all, g, 0, 0, mass_all, count_all);
-  const int bin = s.bin;
-  u64 mass0 = s.all.mass[bin];
-  unsigned count0 = s.all.count[bin];
-  unsigned n = (bin + 1 < kBins ? s.all.count[bin + 1] : count_all) - count0;
-  u64 low = 0, high = ~u64(0);
+__device__ __noinline__ Gathered gather(SampleLds& s, const Row<T>& row, const Scale& sc, const Goal& g, unsigned bin,
+                                        unsigned count_all) {
+  u64 low = 0, high = ~u64(0), weight0 = 0;
+  unsigned count0 = 0, n = (bin + 1 < kBins ? s.count[bin + 1] : count_all) - s.count[bin];
+  const auto in_bin = [&](float x) {
+    const float d = sc.distance(x);
+    return d >= float(bin) && d < float(bin + 1);
+  };
+  __syncthreads();
   if (n > kList) {
-    // A crowded bin: its keys' range, cut into kBins runs of equal width until
-    // one run's tokens fit the list.  (Keys are distinct, so this ends.)
+    // A crowded bin: its keys' range, cut into runs of equal width until one run's
+    // tokens fit the list.  (Keys are distinct, so this ends.)
     if (threadIdx.x == 0) {
       s.low = ~u64(0);
       s.high = 0;
@@ -177,7 +348,7 @@ __device__ Place locate(SampleLds& s, const Row<T>& row, const Scale& sc, const 
     __syncthreads();
     u64 lo = ~u64(0), hi = 0;
     row.each([&](float x, int i) {
-      if (bin_of(sc.distance(x)) != bin) return;
+      if (!in_bin(x)) return;
       const u64 k = order_key(x, i);
       lo = min(lo, k);
       hi = max(hi, k);
@@ -187,181 +358,361 @@ __device__ Place locate(SampleLds& s, const Row<T>& row, const Scale& sc, const 
     __syncthreads();
     low = s.low;
     high = s.high;
+    const double e = run_edge(bin / kPerThread) * step(int(bin % kPerThread));
     while (n > kList) {
       int shift = 0;
-      while (((high - low) >> shift) >= kBins) ++shift;
+      while (((high - low) >> shift) >= kRuns) ++shift;
       __syncthreads();
-      clear(s.sub);
+      for (int i = int(threadIdx.x); i < kRuns; i += kThreads) s.runs[i] = 0;
       __syncthreads();
       row.each([&](float x, int i) {
-        const double d = sc.distance(x);
-        if (bin_of(d) != bin) return;
+        if (!in_bin(x)) return;
         const u64 k = order_key(x, i);
-        if (k < low || k > high) return;
-        const int at = int((k - low) >> shift);
-        atomicAdd(&s.sub.mass[at], mass_of(exp(-d)));
-        atomicAdd(&s.sub.count[at], 1u);
+        if (k >= low && k <= high) atomicAdd(&s.runs[(k - low) >> shift], packed(sc.fraction(x)));
       });
-      scan(s, s.sub);
-      const u64 m_all = s.total_mass;
-      const unsigned c_all = s.total_count;
-      find_bin(s, s.sub, g, mass0, count0, m_all, c_all);
-      const int at = s.bin;
-      n = (at + 1 < kBins ? s.sub.count[at + 1] : c_all) - s.sub.count[at];
-      mass0 += s.sub.mass[at];
-      count0 += s.sub.count[at];
+      __syncthreads();
+      // (Rare enough that every thread walks the runs by itself.)
+      int at = 0;
+      for (; at < kRuns - 1; ++at) {
+        const u64 b = s.runs[at], w = weight0 + weight_of(b);
+        const unsigned c = count0 + count_of(b);
+        if (g.goal <= (g.by_count ? u64(s.count[bin] + c) : s.mass[bin] + mass_of(w, e))) break;
+        weight0 = w;
+        count0 = c;
+      }
+      n = count_of(s.runs[at]);
       low += u64(at) << shift;
       high = min(high, low + ((u64(1) << shift) - 1));
-      __syncthreads();
     }
   }
-  // The list: every token of the run, each ranked by all the others.
+  __syncthreads();
+  if (threadIdx.x < kBins / 32) s.wanted[threadIdx.x] = 0;
   if (threadIdx.x == 0) s.list_count = 0;
   __syncthreads();
-  row.each([&](float x, int i) {
-    const double d = sc.distance(x);
-    if (bin_of(d) != bin) return;
+  // The whole bin is at hand for the next goal, a run of it is not.
+  if (threadIdx.x == 0 && weight0 == 0 && high == ~u64(0)) s.wanted[bin >> 5] = 1u << (bin & 31);
+  row.pick(in_bin, [&](float x, int i) {
     const u64 k = order_key(x, i);
-    if (k < low || k > high) return;
-    const unsigned at = atomicAdd(&s.list_count, 1u);
-    if (at < kList) {
-      s.key[at] = k;
-      s.w[at] = mass_of(exp(-d));
-    }
+    if (k >= low && k <= high) take(s, k, bin, sc.fraction(x));
   });
   __syncthreads();
-  const unsigned t = threadIdx.x;
-  if (t < min(n, unsigned(kList))) {
-    const u64 k = s.key[t], w = s.w[t];
-    u64 before = mass0;
-    unsigned rank = count0;
-    for (unsigned o = 0; o < n; ++o)
-      if (s.key[o] < k) {
-        before += s.w[o];
-        ++rank;
-      }
-    const u64 b = g.by_count ? rank : before, a = g.by_count ? rank + 1 : before + w;
-    if (b < g.goal && g.goal <= a) {
-      s.answer_key = k;
-      s.answer_mass = before + w;
-      s.total_count = rank + 1;
-    }
-  }
-  __syncthreads();
-  const Place got{s.answer_mass, s.total_count, s.answer_key};
-  __syncthreads();
-  return got;
+  Gathered mine;
+  mine.order(s, weight0, count0);
+  return mine;
 }
 
-// floor(f * m) for 0 <= f < 1, exact: f is a 24-bit number times a power of two.
-__device__ __forceinline__ u64 part_of(float f, u64 m, bool& whole) {
-  // f * 2^64 as a whole number (what lies below 2^-64 counts as 0).
-  const u64 fx = f > 0.f ? u64(ldexp(double(f), 64)) : 0;
-  whole = fx * m == 0;
-  return __umul64hi(fx, m);
+template <typename T>
+__device__ __forceinline__ Place locate(SampleLds& s, const Row<T>& row, const Scale& sc, Gathered& mine, const Goal& g,
+                                        unsigned count_all) {
+  const unsigned bin = find_bin(s, g);
+  if (!is_wanted(s, bin)) mine = gather(s, row, sc, g, bin, count_all);
+  return mine.resolve(s, bin, g);
+}
+
+
+// The bin of the token with `goal` - 1 others in front of it, from the counts per bin;
+// before: the tokens in front of the bin.  kBins if there are fewer.  Every wave sums
+// 1024 bins at a time, 16 to a lane, then those of one lane.
+__device__ __forceinline__ unsigned bin_of_rank(const SampleLds& s, unsigned goal, unsigned& before) {
+  const unsigned lane = threadIdx.x & 63;
+  before = 0;
+  for (unsigned run = 0; run < kBins; run += 1024) {
+    unsigned sum = 0;
+#pragma unroll
+    for (unsigned i = 0; i < 16; ++i) sum += s.count[run + 16 * lane + ((i + lane) & 15)];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const unsigned up = __shfl_up(sum, o, 64);
+      sum += lane >= unsigned(o) ? up : 0;
+    }
+    const int over = __popcll(__ballot(before + sum < goal));
+    if (over < 64) {
+      if (over > 0) before += __shfl(sum, over - 1, 64);
+      unsigned bin = run + 16 * over;
+      while (before + s.count[bin] < goal) before += s.count[bin++];
+      return bin;
+    }
+    before += __shfl(sum, 63, 64);
+  }
+  return kBins;
+}
+
+__device__ __forceinline__ float block_top(SampleLds& s, float top) {
+  top = wave_max(top);
+  if ((threadIdx.x & 63) == 0) s.wave_max[threadIdx.x >> 6] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) top = fmaxf(top, s.wave_max[w]);
+  return top;
+}
+
+// At most kShort tokens kept, by top_k or because the row has no more, in one pass over
+// the row: a sample of it says which logits are likely to be among four times as many as
+// may be kept, the tokens with those are gathered, and everything else is read off the
+// list: the maximum, the bin of the last token that may be kept, the order up to that bin
+// and the cumulative masses.  False, nothing written: too few tokens were found, or more
+// than the lists hold.
+template <typename T>
+__device__ __forceinline__ bool sample_short(SampleLds& s, const Row<T>& row, float temp, unsigned most, float top_p,
+                                             float min_p, float u, int32_t* token, float* prob) {
+  const unsigned t = threadIdx.x, lane = t & 63;
+  const auto clear = [&] {
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) s.count[i * kThreads + t] = 0;
+    if (t == 0) s.list_count = 0;
+  };
+  clear();
+  float top = kNegInf;
+  row.sample([&](float x) { top = fmaxf(top, x); });
+  top = block_top(s, top);
+  if (top == kNegInf || top == -kNegInf) return false;
+  const Scale about(top, temp);
+  row.sample([&](float x) {
+    const float d = about.distance(x);
+    if (d < float(kBins)) atomicAdd(&s.count[unsigned(d)], 1u);
+  });
+  __syncthreads();
+  unsigned before;
+  const unsigned sampled = Row<T>::W * kThreads;
+  const unsigned enough = unsigned(row.n) <= sampled ? most : 4 * most * sampled / unsigned(row.n) + 8;
+  const float least = top - float(min(bin_of_rank(s, enough, before) + 1, unsigned(kBins))) / about.per;
+  __syncthreads();
+  clear();
+  __syncthreads();
+  row.pick([&](float x) { return x >= least; },
+           [&](float x, int i) {
+             const unsigned at = atomicAdd(&s.list_count, 1u);
+             if (at < kBins) s.bin[at] = order_key(x, i);
+           });
+  __syncthreads();
+  const unsigned found = s.list_count;
+  if (found < most || found > kBins) return false;
+  for (unsigned i = t; i < found; i += kThreads) top = fmaxf(top, value_of(s.bin[i]));
+  top = block_top(s, top);
+  if (top == -kNegInf) return false;
+  const Scale sc(top, temp);
+  unsigned counted = 0;
+  for (unsigned i = t; i < found; i += kThreads) {
+    const float d = sc.distance(value_of(s.bin[i]));
+    if (d < float(kBins)) {
+      atomicAdd(&s.count[unsigned(d)], 1u);
+      ++counted;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) counted += __shfl_xor(counted, o, 64);
+  if (lane == 0) s.wave_count[t >> 6] = counted;
+  __syncthreads();
+  counted = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) counted += s.wave_count[w];
+  most = min(most, counted);
+  const unsigned last = bin_of_rank(s, most, before);
+  const unsigned n = before + s.count[last];
+  if (n > kList) return false;
+  __syncthreads();
+  if (t == 0) s.list_count = 0;
+  __syncthreads();
+  for (unsigned i = t; i < found; i += kThreads) {
+    const u64 key = s.bin[i];
+    if (sc.distance(value_of(key)) < float(last + 1)) s.key[atomicAdd(&s.list_count, 1u)] = key;
+  }
+  __syncthreads();
+  // Masses in the row's order, in units of 2^-44 of the heaviest token's, and their sums.
+  constexpr double unit = 17592186044416.0;
+  u64 key = 0;
+  double weight = 0;
+  unsigned rank = ~0u;
+  if (t < n) {
+    key = s.key[t];
+    rank = 0;
+#pragma unroll 8
+    for (unsigned o = 0; o < n; ++o) rank += s.key[o] < key;
+    weight = sc.weight_of(value_of(key));
+    s.runs[rank] = u64(fma(weight, unit, 0.5));
+  }
+  __syncthreads();
+  u64 sum = t < n ? s.runs[t] : 0;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const u64 up = __shfl_up(sum, o, 64);
+    sum += lane >= unsigned(o) ? up : 0;
+  }
+  if (lane == 63) s.wave_mass[t >> 6] = sum;
+  __syncthreads();
+  for (unsigned w = 0; w < t >> 6; ++w) sum += s.wave_mass[w];
+  if (t < n) s.runs[t] = sum;
+  unsigned kept = most;
+  if (min_p > 0.f) {
+    const unsigned heavy = __syncthreads_count(t < n && weight >= double(min_p));
+    kept = min(kept, max(heavy, 1u));
+  } else {
+    __syncthreads();
+  }
+  if (top_p < 1.f) {
+    const u64 goal = goal_p(top_p, s.runs[most - 1]).goal;
+    kept = min(kept, 1u + unsigned(__syncthreads_count(t < n && s.runs[t] < goal)));
+  }
+  const u64 mass = s.runs[kept - 1], goal = goal_u(u, mass).goal;
+  if (rank < n && s.runs[rank] >= goal && (rank == 0 || s.runs[rank - 1] < goal)) {
+    *token = int(key & 0xffffffffu);
+    *prob = float(weight * unit / double(mass));
+  }
+  return true;
 }
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
-  __shared__ SampleLds s;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  SampleLds& s = *reinterpret_cast<SampleLds*>(lds);
   const int b = int(blockIdx.x), t = int(threadIdx.x);
-  const Row<T> row{static_cast<const T*>(a.logits) + int64_t(b) * a.vocab, a.vocab};
+  Row<T> row(static_cast<const T*>(a.logits) + int64_t(b) * a.vocab, a.vocab);
   const float temp = a.temperature ? a.temperature[b] : a.temperature_all;
   const int top_k = a.top_k ? a.top_k[b] : a.top_k_all;
   const float top_p = a.top_p ? a.top_p[b] : a.top_p_all, min_p = a.min_p ? a.min_p[b] : a.min_p_all;
   float u = a.uniforms[b];
   u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
 
-  clear(s.all);
-  float bv = kNegInf;
-  int bi = kNoToken;
-  row.each([&](float x, int i) {
-    if (x > bv) {
-      bv = x;
-      bi = i;
-    }
-  });
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float ov = __shfl_xor(bv, o, 64);
-    const int oi = __shfl_xor(bi, o, 64);
-    amax_merge(bv, bi, ov, oi);
-  }
-  if ((t & 63) == 0) {
-    s.wave_max[t >> 6] = bv;
-    s.wave_at[t >> 6] = bi;
-  }
+  const unsigned most = top_k > 0 && top_k < a.vocab ? unsigned(top_k) : unsigned(a.vocab);
+  if (most <= kShort && temp > 0.f && sample_short(s, row, temp, most, top_p, min_p, u, a.tokens + b, a.probs + b)) return;
+
+  float top = kNegInf;
+  row.each([&](float x, int) { top = fmaxf(top, x); });
   __syncthreads();
-  for (int w = 0; w < kThreads / 64; ++w) amax_merge(bv, bi, s.wave_max[w], s.wave_at[w]);
-  if (bi == kNoToken || !(temp > 0.f) || bv == -kNegInf) {
-    // No token above -inf, or the greedy one.
+  top = block_top(s, top);
+  if (top == kNegInf || !(temp > 0.f) || top == -kNegInf) {
+    // No token above -inf, or the likeliest one.
+    int at = kNoToken;
+    if (top != kNegInf) row.each([&](float x, int i) { at = x == top ? min(at, i) : at; });
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
+    if ((t & 63) == 0) s.wave_at[t >> 6] = at;
+    __syncthreads();
     if (t == 0) {
-      a.tokens[b] = bi;
-      a.probs[b] = bi == kNoToken ? 0.f : 1.f;
+      for (int w = 1; w < kThreads / 64; ++w) at = min(at, s.wave_at[w]);
+      a.tokens[b] = at;
+      a.probs[b] = at == kNoToken ? 0.f : 1.f;
     }
     return;
   }
-  const Scale sc{double(bv), 1.0 / double(temp)};
-  u64 min_mass = 0;
-  unsigned min_count = 0;
-  const bool use_min = min_p > 0.f;
+  const Scale sc(top, temp);
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) s.bin[i * kThreads + t] = 0;
+  if (t <= kBins / 32) s.wanted[t] = 0;
+  if (t == 0) s.list_count = 0;
+  __syncthreads();
   row.each([&](float x, int) {
-    const double d = sc.distance(x);
-    const int at = bin_of(d);
-    if (at >= kBins) return;
-    const double e = exp(-d);
-    const u64 w = mass_of(e);
-    atomicAdd(&s.all.mass[at], w);
-    atomicAdd(&s.all.count[at], 1u);
-    if (use_min && e >= double(min_p)) {
-      min_mass += w;
-      ++min_count;
-    }
+    const float d = sc.distance(x);
+    if (d < float(kBins)) atomicAdd(&s.bin[unsigned(d)], packed(sc.fraction(x)));
   });
-  scan(s, s.all);
-  const u64 mass_all = s.total_mass;
-  const unsigned count_all = s.total_count;
+  u64 mass_all;
+  unsigned count_all;
+  scan(s, mass_all, count_all);
+
+  const bool use_k = top_k > 0 && unsigned(top_k) < count_all, use_p = top_p < 1.f, use_m = min_p > 0.f;
+  // The bin of the logit whose weight is min_p: all tokens in front of it are heavier.
+  unsigned far = 0;
+  if (use_m) {
+    const float d = sc.distance(float(double(top) + sc.temp * log(fmin(double(min_p), 1.0))));
+    far = unsigned(fminf(fmaxf(d, 0.f), float(kBins - 1)));
+  }
+
+  // The bins in question, from masses known to a bin: their tokens are gathered in one pass.
+  {
+    const auto behind = [&](unsigned bin) { return bin + 1 < kBins ? s.mass[bin + 1] : mass_all; };
+    constexpr int kRanges = 4;
+    unsigned from[kRanges] = {1, 1, 1, 1}, to[kRanges] = {0, 0, 0, 0};
+    u64 low = mass_all, high = mass_all;  // the kept mass lies between
+    if (use_k) {
+      from[0] = to[0] = find_bin(s, Goal{true, u64(top_k)});
+      low = s.mass[to[0]];
+      high = behind(to[0]);
+    }
+    if (use_p) {
+      from[1] = find_bin(s, goal_p(top_p, max(low, u64(1))));
+      to[1] = find_bin(s, goal_p(top_p, high));
+      low = s.mass[from[1]];
+      high = behind(to[1]);
+    }
+    if (use_m) {
+      from[2] = to[2] = far;
+      low = min(low, s.mass[far]);
+      high = min(high, behind(far));
+    }
+    from[3] = find_bin(s, goal_u(u, max(low, u64(1))));
+    to[3] = find_bin(s, goal_u(u, max(high, u64(1))));
+    unsigned last = 0, tokens = 0;
+#pragma unroll
+    for (int r = 0; r < kRanges; ++r) {
+      if (from[r] > to[r]) continue;
+      last = max(last, to[r]);
+      tokens += (to[r] + 1 < kBins ? s.count[to[r] + 1] : count_all) - s.count[from[r]];
+    }
+    if (tokens <= kList) {  // (bins in two ranges count twice)
+      if (t < kBins / 32) {
+        unsigned bits = 0;
+#pragma unroll
+        for (int r = 0; r < kRanges; ++r) {
+          const int first = int(from[r]) - 32 * t, end = int(to[r]) - 32 * t;  // bits first .. end of this word
+          if (from[r] <= to[r] && first < 32 && end >= 0)
+            bits |= (~0u << max(first, 0)) & (~0u >> (31 - min(end, 31)));
+        }
+        s.wanted[t] = bits;
+      }
+      __syncthreads();
+      const float end = float(last + 1);
+      row.pick(
+          [&](float x) {
+            const float d = sc.distance(x);
+            return is_wanted(s, d < end ? unsigned(d) : unsigned(kBins));
+          },
+          [&](float x, int i) { take(s, order_key(x, i), unsigned(sc.distance(x)), sc.fraction(x)); });
+      __syncthreads();
+    }
+  }
+  Gathered mine;
+  mine.order(s, 0, 0);
 
   // The kept run: its length and mass.
-  u64 kept = mass_all, k_mass = mass_all;
+  u64 kept = mass_all;
   unsigned length = count_all;
-  if (top_k > 0 && unsigned(top_k) < count_all) {
-    const Place p = locate(s, row, sc, Goal{true, u64(top_k)}, mass_all, count_all);
-    kept = k_mass = p.mass;
-    length = p.count;
-  }
-  if (top_p < 1.f) {
-    // The last token kept is the first with cumulative mass >= top_p * k_mass.
-    bool whole;
-    u64 goal = part_of(top_p, k_mass, whole);
-    goal = max(whole ? goal : goal + 1, u64(1));
-    const Place p = locate(s, row, sc, Goal{false, goal}, mass_all, count_all);
+  if (use_k) {
+    const Place p = locate(s, row, sc, mine, Goal{true, u64(top_k)}, count_all);
     kept = p.mass;
     length = p.count;
   }
-  if (use_min) {
-    __syncthreads();
-    if (t == 0) {
-      s.total_mass = 0;
-      s.total_count = 0;
-    }
-    __syncthreads();
-    atomicAdd(&s.total_mass, min_mass);
-    atomicAdd(&s.total_count, min_count);
-    __syncthreads();
-    const unsigned n = s.total_count;
-    const u64 m = s.total_mass;
-    __syncthreads();
-    if (n < length) {
-      kept = n == 0 ? mass_of(1.0) : m;  // min_p above 1: the first token
-    }
+  if (use_p) {
+    const Place p = locate(s, row, sc, mine, goal_p(top_p, kept), count_all);
+    kept = p.mass;
+    length = p.count;
   }
-  bool whole;
-  const Place p = locate(s, row, sc, Goal{false, part_of(u, kept, whole) + 1}, mass_all, count_all);
+  if (use_m) {
+    // The tokens of bin `far` with w >= min_p stand in front of its others.
+    __syncthreads();
+    if (t == 0) s.low = 0;
+    __syncthreads();
+    u64 heavy = 0;
+    if (is_wanted(s, far)) {
+      const float x = value_of(mine.key);
+      if (mine.bin == far && sc.weight_of(x) >= double(min_p)) heavy = packed(sc.fraction(x));
+    } else {
+      row.each([&](float x, int) {
+        const float d = sc.distance(x);
+        if (d >= float(far) && d < float(far + 1) && sc.weight_of(x) >= double(min_p)) heavy += packed(sc.fraction(x));
+      });
+    }
+    if (heavy) atomicAdd(&s.low, heavy);
+    __syncthreads();
+    const unsigned n = s.count[far] + count_of(s.low);
+    const u64 m = s.mass[far] + mass_of(weight_of(s.low), run_edge(far / kPerThread) * step(int(far % kPerThread)));
+    __syncthreads();
+    if (n < length) kept = n == 0 ? mass_of(kOne - loss(0.f), run_edge(0)) : m;  // (n = 0: min_p above 1)
+  }
+  const Place p = locate(s, row, sc, mine, goal_u(u, kept), count_all);
   if (t == 0) {
     const int token = int(p.key & 0xffffffffu);
     a.tokens[b] = token;
-    a.probs[b] = float(exp(-sc.distance(float(row.p[token]))) * kUnit / double(kept));
+    a.probs[b] = float(sc.weight_of(float(row.p[token])) * (double(kOne) * kMass) / double(kept));
   }
 }
 
@@ -369,8 +720,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
 
 hipError_t sample(const SampleArgs& a, hipStream_t stream) {
   const dim3 grid(unsigned(a.batch)), block(kThreads);
-  if (a.f32) hipLaunchKernelGGL((sample_kernel<float>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((sample_kernel<f16>), grid, block, 0, stream, a);
+  static LdsLimit limits[2];
+  const void* kernel = a.f32 ? reinterpret_cast<const void*>(&sample_kernel<float>) : reinterpret_cast<const void*>(&sample_kernel<f16>);
+  const hipError_t e = limits[a.f32].raise(kernel, int(sizeof(SampleLds)));
+  if (e != hipSuccess) return e;
+  if (a.f32) hipLaunchKernelGGL((sample_kernel<float>), grid, block, sizeof(SampleLds), stream, a);
+  else hipLaunchKernelGGL((sample_kernel<f16>), grid, block, sizeof(SampleLds), stream, a);
   return hipGetLastError();
 }
 
