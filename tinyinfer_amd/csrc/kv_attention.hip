@@ -36,7 +36,6 @@ namespace tia {
 namespace {
 
 constexpr int kTile = 64;   // keys per wave and step
-constexpr int kWaves = 4;
 constexpr float kNegInf = -__builtin_huge_valf();
 // The reference of a row's exponents: 6 below its largest score when set, raised
 // when a score is 14 above it.  Probabilities then lie around 2^6 and below 2^14:
@@ -44,12 +43,27 @@ constexpr float kNegInf = -__builtin_huge_valf();
 // heavy as the heaviest still keeps 11 bits.
 constexpr float kBelow = 6.f, kRaise = 14.f;
 
+// n / d for 0 <= n < 2^31 by a multiplication: with 2^(shift-1) < d <= 2^shift and mul =
+// floor(2^32 (2^shift - d) / d) + 1, n / d = (hi32(n mul) + n) >> shift.
+struct Divisor {
+  uint32_t d, mul, shift;
+};
+Divisor divisor(uint32_t d) {
+  uint32_t shift = 0;
+  while ((uint64_t(1) << shift) < d) ++shift;
+  return {d, uint32_t(((uint64_t(1) << 32) * ((uint64_t(1) << shift) - d)) / d + 1), shift};
+}
+__device__ __forceinline__ int div_by(int n, Divisor v) {
+  return int((uint64_t(__umulhi(uint32_t(n), v.mul)) + uint32_t(n)) >> v.shift);
+}
+
 struct AttnPlan {
   KvAttnArgs a;
   float scale;                   // D^-1/2 log2 e
-  int group, rows;               // query heads per key head; rows of one request and key head
-  int row_blocks, splits;        // of the requests' own keys
-  int prefix_blocks, prefix_splits;
+  Divisor group, rows;           // query heads per key head; rows of one request and key head
+  Divisor heads, pairs;          // key heads; (request, key head) pairs
+  Divisor row_block_div, prefix_block_div;  // row blocks of a pair, and of the prefix
+  int splits, prefix_splits;     // of the requests' own keys, and of the prefix's
   int64_t own_wgs, prefix_wgs;
   int64_t all_rows;              // batch * heads * q_len
   bool parts;                    // states to the workspace, joined by the second kernel
@@ -84,22 +98,27 @@ __device__ __forceinline__ void mul_row(float4_t (&x)[4], float of) {
 #undef TIA_MUL
 }
 
-template <int D, int QB>
+template <bool NT>
+__device__ __forceinline__ u32x4_t load16(const uint8_t* p) {
+  if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
+  return *reinterpret_cast<const u32x4_t*>(p);
+}
+
+template <int D, int QB, int KW>
 struct Merge {
-  float4_t acc[kWaves][QB * D / 16][64];
-  float m[kWaves][QB][16], l[kWaves][QB][16];
+  float4_t acc[KW][QB * D / 16][64];
+  float m[KW][QB][16], l[KW][QB][16];
 };
 
 // Row block `rb` of one set of keys.  PREFIX: rows run over the batch, key head
 // `head`, the keys are the prefix's; else over request b's.
-template <int D, int QB, bool PREFIX>
+template <int D, int QB, int KW, bool PREFIX>
 __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb, int split, int splits, int state) {
   const KvAttnArgs& a = p.a;
   const int lane = int(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
   const int j = lane & 15, g = lane >> 4;
   constexpr int ROWS = 16 * QB;
-  const int64_t r0 = int64_t(rb) * ROWS;
-  const int64_t row_count = PREFIX ? int64_t(a.batch) * p.rows : p.rows;
+  const int r0 = rb * ROWS, row_count = PREFIX ? a.batch * int(p.rows.d) : int(p.rows.d);
 
   int slot, kv;
   if constexpr (PREFIX) {
@@ -112,15 +131,14 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
   }
 
   // This lane's rows: block u, column j.
-  int64_t row_id[QB];  // in q's order, -1 past the last row
-  int end[QB];         // keys [0, end) are visible
+  int row_id[QB];  // in q's order, -1 past the last row
+  int end[QB];     // keys [0, end) are visible
 #pragma unroll
   for (int u = 0; u < QB; ++u) {
-    const int64_t r = r0 + 16 * u + j;
-    const int b = PREFIX ? int(min(r, row_count - 1) / p.rows) : b0;
-    const int rr = int(min(r, row_count - 1) - (PREFIX ? int64_t(b) * p.rows : 0));
-    const int qi = rr / p.group, hg = rr - qi * p.group;
-    row_id[u] = r < row_count ? (int64_t(b) * a.heads + int64_t(head) * p.group + hg) * a.q_len + qi : -1;
+    const int r = r0 + 16 * u + j, rc = min(r, row_count - 1);
+    const int b = PREFIX ? div_by(rc, p.rows) : b0, rr = PREFIX ? rc - b * int(p.rows.d) : rc;
+    const int qi = div_by(rr, p.group), hg = rr - qi * int(p.group.d);
+    row_id[u] = r < row_count ? (b * a.heads + head * int(p.group.d) + hg) * a.q_len + qi : -1;
     const int ql = a.q_lengths ? min(max(a.q_lengths[b], 0), a.q_len) : a.q_len;
     int64_t e = kv;
     if (!PREFIX && a.causal) e = min(e, (a.offsets ? int64_t(a.offsets[b]) : int64_t(kv) - ql) + qi + 1);
@@ -133,7 +151,7 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
     last = first = kv;
   } else {
     const int ql = a.q_lengths ? min(max(a.q_lengths[b0], 0), a.q_len) : a.q_len;
-    const int q_first = int(r0 / p.group), q_last = min(int((min(r0 + ROWS, row_count) - 1) / p.group), ql - 1);
+    const int q_first = div_by(r0, p.group), q_last = min(div_by(min(r0 + ROWS, row_count) - 1, p.group), ql - 1);
     const int64_t off = a.offsets ? int64_t(a.offsets[b0]) : int64_t(kv) - ql;
     const auto seen = [&](int qi) { return int(max(a.causal ? min(int64_t(kv), off + qi + 1) : int64_t(kv), int64_t(0))); };
     last = q_last < q_first ? 0 : seen(q_last);
@@ -144,13 +162,14 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
   int t = split * per + wave;
 
   const int64_t base = (int64_t(slot) * a.cache.kv_heads + head) * a.cache.capacity;
-  const uint8_t* kp = a.cache.k + base * D + j * D + 16 * g;
+  const uint8_t* kp = a.cache.k + base * D + j * 64 + 16 * g;
   const uint8_t* vp = a.cache.v + base * D + lane * 16;
   // Lane (j, g) holds the scales of the tile's key 16 (j / 4) + 4 g + j % 4: of row g's
   // 16 scores of a tile, number 4 kb + v in order, lane 4 kb + v has the scale.
   const int my_key = 16 * (j >> 2) + 4 * g + (j & 3);
   const float* ksp = a.cache.k_scales + base + my_key;
   const float* vsp = a.cache.v_scales + base + my_key;
+  constexpr bool NT = !PREFIX && QB == 1;
   u32x4_t kr[4][D / 64], vr[D / 16];
   float ksr = 0.f, vsr = 0.f;
   auto load_k = [&](int tt) {
@@ -158,25 +177,21 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) kr[kb][c] = *reinterpret_cast<const u32x4_t*>(at + 16 * kb * D + 64 * c);
+      for (int c = 0; c < D / 64; ++c) kr[kb][c] = load16<NT>(at + 16 * kb * D + 1024 * c);
     ksr = ksp[int64_t(tt) * kTile];
   };
   auto load_v = [&](int tt) {
     const uint8_t* at = vp + int64_t(tt) * (kTile * D);
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) vr[d] = *reinterpret_cast<const u32x4_t*>(at + 1024 * d);
+    for (int d = 0; d < D / 16; ++d) vr[d] = load16<NT>(at + 1024 * d);
     vsr = vsp[int64_t(tt) * kTile];
   };
-  if (t < t_end) {
-    load_k(t);
-    load_v(t);
-  }
 
   // Step (c, s) of a dot product takes dims 64 c + 16 g + 8 s .. + 7 from lane (., g).
   half8_t qf[QB][D / 32];
 #pragma unroll
   for (int u = 0; u < QB; ++u) {
-    const uint16_t* qp = a.q + max(row_id[u], int64_t(0)) * D + 16 * g;
+    const uint16_t* qp = a.q + int64_t(max(row_id[u], 0)) * D + 16 * g;
 #pragma unroll
     for (int c = 0; c < D / 64; ++c)
 #pragma unroll
@@ -200,10 +215,10 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
   // the weight p * vs / unit that is rounded to fp16 is then at most p.
   float unit = 0.f, inv_unit = 1.f;
 
-  // One tile; MORE: this wave has a next one, whose loads are issued as the registers fall free.
-  auto step = [&](auto more_c, int tt) {
-    constexpr bool MORE = decltype(more_c)::value;
-    const bool full = (tt + 1) * kTile <= first;
+  for (; t < t_end; t += KW) {
+    load_k(t);
+    load_v(t);
+    const bool full = (t + 1) * kTile <= first;
     float4_t sc[QB][4];
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
@@ -222,8 +237,7 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
     }
     const float ck = ksr * p.scale;
     // (Past the last key any row sees, scales may be anything.)
-    const float vs = tt * kTile + my_key < last ? vsr : 0.f;
-    if constexpr (MORE) load_k(tt + kWaves);
+    const float vs = t * kTile + my_key < last ? vsr : 0.f;
     if (__ballot(vs > unit)) {
       const float top = wave_max(vs);
       const float raised = __builtin_amdgcn_ldexpf(1.f, __builtin_amdgcn_frexp_expf(top));  // > top
@@ -240,7 +254,7 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
 #pragma unroll
     for (int u = 0; u < QB; ++u) {
       mul_row(sc[u], ck);
-      const int lim = end[u] - tt * kTile - 4 * g;  // key 16 kb + v of this lane is visible iff < lim
+      const int lim = end[u] - t * kTile - 4 * g;  // key 16 kb + v of this lane is visible iff < lim
       const auto mask = [&](float with) {
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb)
@@ -289,91 +303,109 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (MORE) load_v(tt + kWaves);
-  };
-  for (; t + kWaves < t_end; t += kWaves) step(std::true_type{}, t);
-  if (t < t_end) step(std::false_type{}, t);
+  }
 
-  // The waves' states meet in LDS; wave w joins every fourth (block, 16 dims).
-  auto& mg = *reinterpret_cast<Merge<D, QB>*>(lds);
 #pragma unroll
   for (int u = 0; u < QB; ++u) {
     l[u] += __shfl_xor(l[u], 16, 64);
     l[u] += __shfl_xor(l[u], 32, 64);
     if (end[u] == 0) l[u] = 0.f;
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) mg.acc[wave][u * (D / 16) + d][lane] = acc[u][d] * unit;
-    if (g == 0) {
-      mg.m[wave][u][j] = m[u];
-      mg.l[wave][u][j] = l[u];
-    }
+    for (int d = 0; d < D / 16; ++d) acc[u][d] *= unit;
   }
-  __syncthreads();
-#pragma unroll
-  for (int u = 0; u < QB; ++u) {
-    float top = kNegInf, total = 0.f, f[kWaves];
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = mg.l[w][u][j] == 0.f ? top : fmaxf(top, mg.m[w][u][j]);
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float lw = mg.l[w][u][j];
-      f[w] = lw == 0.f ? 0.f : __builtin_amdgcn_exp2f(mg.m[w][u][j] - top);
-      total += lw * f[w];
+  // Dims 16 d + 4 g .. + 3 of row (u, j), of `total` weight at exponent reference `top`.
+  const auto put = [&](int u, int d, float4_t o, float total) {
+    if (row_id[u] < 0) return;
+    if (p.parts) {
+      const int64_t at = int64_t(state) * p.all_rows + row_id[u];
+      if (total != 0.f) *reinterpret_cast<float4_t*>(a.workspace + at * D + 16 * d + 4 * g) = o;
+      return;
     }
-    if (row_id[u] < 0) continue;
     const float inv = total == 0.f ? 0.f : 1.f / total;
+    half4_t y;
 #pragma unroll
-    for (int d0 = 0; d0 < D / 16; d0 += kWaves) {
-      const int d = d0 + wave;
-      float4_t o = {0.f, 0.f, 0.f, 0.f};
+    for (int e = 0; e < 4; ++e) y[e] = f16r(total == 0.f ? 0.f : o[e] * inv);
+    __builtin_memcpy(a.out + int64_t(row_id[u]) * D + 16 * d + 4 * g, &y, 8);
+  };
+  const auto put_weight = [&](int u, float top, float total) {
+    if (!p.parts || g != 0 || row_id[u] < 0) return;
+    const int64_t states = int64_t(p.splits + p.prefix_splits) * p.all_rows;
+    float* ml = a.workspace + states * D + 2 * (int64_t(state) * p.all_rows + row_id[u]);
+    ml[0] = top;
+    ml[1] = total;
+  };
+  if constexpr (KW == 1) {
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float4_t x = mg.acc[w][u * (D / 16) + d][lane];
+    for (int u = 0; u < QB; ++u) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = f[w] == 0.f ? o[e] : fmaf(x[e], f[w], o[e]);
-      }
-      if (p.parts) {
-        const int64_t at = int64_t(state) * p.all_rows + row_id[u];
-        if (total != 0.f) *reinterpret_cast<float4_t*>(a.workspace + at * D + 16 * d + 4 * g) = o;
-      } else {
-        half4_t y;
+      for (int d = 0; d < D / 16; ++d) put(u, d, acc[u][d], l[u]);
+      put_weight(u, m[u], l[u]);
+    }
+  } else {
+    // The waves' states meet in LDS; wave w joins every KW-th piece of 16 dims.
+    auto& mg = *reinterpret_cast<Merge<D, QB, KW>*>(lds);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = f16r(total == 0.f ? 0.f : o[e] * inv);
-        __builtin_memcpy(a.out + row_id[u] * D + 16 * d + 4 * g, &y, 8);
+    for (int u = 0; u < QB; ++u) {
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) mg.acc[wave][u * (D / 16) + d][lane] = acc[u][d];
+      if (g == 0) {
+        mg.m[wave][u][j] = m[u];
+        mg.l[wave][u][j] = l[u];
       }
     }
-    if (p.parts && wave == 0 && g == 0) {
-      const int64_t states = int64_t(p.splits + p.prefix_splits) * p.all_rows;
-      float* ml = a.workspace + states * D + 2 * (int64_t(state) * p.all_rows + row_id[u]);
-      ml[0] = top;
-      ml[1] = total;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < QB; ++u) {
+      float top = kNegInf, total = 0.f, f[KW];
+#pragma unroll
+      for (int w = 0; w < KW; ++w) top = mg.l[w][u][j] == 0.f ? top : fmaxf(top, mg.m[w][u][j]);
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        const float lw = mg.l[w][u][j];
+        f[w] = lw == 0.f ? 0.f : __builtin_amdgcn_exp2f(mg.m[w][u][j] - top);
+        total += lw * f[w];
+      }
+#pragma unroll
+      for (int d0 = 0; d0 < D / 16; d0 += KW) {
+        const int d = d0 + wave;
+        float4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+          const float4_t x = mg.acc[w][u * (D / 16) + d][lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = f[w] == 0.f ? o[e] : fmaf(x[e], f[w], o[e]);
+        }
+        put(u, d, o, total);
+      }
+      if (wave == 0) put_weight(u, top, total);
     }
   }
 }
 
 // Waves per SIMD that the registers are budgeted for.
-constexpr int waves_for(int dim, int qb) { return dim == 64 ? (qb == 1 ? 4 : qb == 2 ? 3 : 2) : (qb == 1 ? 3 : 2); }
+constexpr int waves_for(int dim, int qb) { return dim == 64 ? (qb == 1 ? 4 : 3) : (qb == 1 ? 3 : 2); }
 
-template <int D, int QB, int PB>
-__global__ __launch_bounds__(64 * kWaves, waves_for(D, QB > PB ? QB : PB)) void kv_attention_kernel(AttnPlan p) {
+// QB, PB: row blocks of 16 per wave over the requests' own keys and the prefix's (0:
+// no prefix); KW: waves that share a row block's keys.
+template <int D, int QB, int PB, int KW>
+__global__ __launch_bounds__(64 * KW, waves_for(D, QB > PB ? QB : PB)) void kv_attention_kernel(AttnPlan p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  int64_t id = blockIdx.x;
+  int id = int(blockIdx.x);
   const int heads = p.a.cache.kv_heads;
   if constexpr (PB > 0) {
     if (id < p.prefix_wgs) {
-      const int head = int(id % heads);
-      id /= heads;
-      attend<D, PB, true>(p, lds, 0, head, int(id % p.prefix_blocks), int(id / p.prefix_blocks), p.prefix_splits,
-                          p.splits + int(id / p.prefix_blocks));
+      const int blocks = div_by(id, p.heads), split = div_by(blocks, p.prefix_block_div);
+      attend<D, PB, KW, true>(p, lds, 0, id - blocks * heads, blocks - split * int(p.prefix_block_div.d), split, p.prefix_splits,
+                              p.splits + split);
       return;
     }
-    id -= p.prefix_wgs;
+    id -= int(p.prefix_wgs);
   }
-  const int64_t bh = int64_t(p.a.batch) * heads;
-  const int at = int(id % bh);
-  const int rest = int(id / bh);
-  attend<D, QB, false>(p, lds, at / heads, at % heads, p.row_blocks - 1 - rest % p.row_blocks, rest / p.row_blocks,
-                       p.splits, rest / p.row_blocks);
+  // The last row blocks of all (request, key head) pairs first: under the causal mask
+  // they are the longest.
+  const int block = div_by(id, p.pairs), at = id - block * int(p.pairs.d), b = div_by(at, p.heads);
+  const int split = div_by(block, p.row_block_div), blocks = int(p.row_block_div.d);
+  attend<D, QB, KW, false>(p, lds, b, at - b * heads, blocks - 1 - (block - split * blocks), split, p.splits, split);
 }
 
 // One wave per row joins its splits' states.
@@ -420,50 +452,89 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(AttnPlan p) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// 16-row blocks per wave: as many as the rows fill, up to what the registers hold.
-int blocks_for(int64_t rows, int dim) { return rows <= 16 ? 1 : rows <= 32 || dim == 128 ? 2 : 4; }
+// How a set of keys is walked: `blocks` row blocks of 16 per wave, `waves` waves to a
+// row block, `splits` workgroups to its keys.
+struct Walk {
+  int blocks, waves, splits;
+};
 
-constexpr int64_t kWantedWgs = 1024;
-
-int splits_for(int64_t wgs, int keys) {
+// From the number of (request, key head) pairs, the rows of one and the tiles of 64 keys
+// of the longest.  Two blocks of 16 rows use every converted key and value twice; they
+// pay where there are plenty of row blocks (GPT-2 XL prefill, 100 pairs of 1024 rows:
+// 38.4 against 44.7 us; 12 pairs: 12.2 against 11.1) or many keys to a row block (64
+// queries over 16000 keys, D 128: 40 against 50 us).
+// Waves: with enough row blocks to fill every SIMD three times a wave takes a whole one
+// and nothing is merged (100 pairs of 1024 rows: 38.4 us, 46.6 with four waves); below
+// that two waves, or four where keys are many (12 pairs of 4096 rows: 56 us, 66 with
+// two, 100 with one).
+// Splits: a second launch and the states' traffic cost 2 us and more, so short caches
+// are not split (96 pairs, 1024 keys: 8.8 us, 9.4 in four), longer ones into about
+// 384 or, from 4096 keys on, 512 workgroups (8 pairs of 4096 keys, D 128: 31 us whole,
+// 10.6 in 16; 128 pairs of 32768: 253 us whole, 136 in 4).
+Walk walk_for(int64_t pairs, int rows, int keys) {
+  const int64_t tiles = ceil_div(keys, kTile), twos = pairs * ceil_div(rows, 32);
+  Walk w{1, 4, 1};
+  if (rows > 16 && (twos >= 1024 || tiles >= 128)) w.blocks = 2;
+  if (w.blocks == 2 && twos >= 1024) {
+    w.waves = twos >= 3072 ? 1 : tiles < 32 ? 2 : 4;
+    return w;
+  }
+  const int64_t wgs = pairs * ceil_div(rows, 16 * w.blocks);
+  if (tiles > 16 && (tiles >= 64 || wgs < 256))
+    w.splits = int(std::min(ceil_div(tiles >= 64 ? 512 : 384, wgs), tiles / 4));
+  return w;
+}
+// A prefix's states are joined with the requests' own in any case, so splitting it costs
+// less: into about 192 workgroups, 256 from 8192 keys on (64 requests of 4 rows, 8 heads,
+// 16001 keys: 97 us in 128 workgroups, 44 in 256).
+Walk prefix_walk_for(int heads, int64_t rows, int keys) {
   const int64_t tiles = ceil_div(keys, kTile);
-  return int(std::max<int64_t>(1, std::min(ceil_div(kWantedWgs, wgs), tiles / kWaves)));
+  Walk w{rows > 16 && (heads * ceil_div(rows, 32) >= 1024 || tiles >= 128) ? 2 : 1, 4, 1};
+  const int64_t wgs = heads * ceil_div(rows, 16 * w.blocks);
+  w.splits = int(std::max<int64_t>(1, std::min(ceil_div(tiles >= 128 ? 256 : 192, wgs), tiles / 4)));
+  return w;
 }
 
-AttnPlan plan_of(const KvAttnArgs& a, int& qb, int& pb) {
+AttnPlan plan_of(const KvAttnArgs& a, Walk& own, Walk& prefix) {
   AttnPlan p{};
   p.a = a;
-  const int dim = a.cache.head_dim;
-  p.scale = float(1.4426950408889634 / __builtin_sqrt(double(dim)));
-  p.group = a.heads / a.cache.kv_heads;
-  p.rows = p.group * a.q_len;
-  p.all_rows = int64_t(a.batch) * a.heads * a.q_len;
-  qb = blocks_for(p.rows, dim);
-  p.row_blocks = int(ceil_div(p.rows, 16 * qb));
-  p.own_wgs = int64_t(a.batch) * a.cache.kv_heads * p.row_blocks;
-  p.splits = splits_for(p.own_wgs, a.max_kv);
-  p.own_wgs *= p.splits;
-  pb = 0;
+  p.scale = float(1.4426950408889634 / __builtin_sqrt(double(a.cache.head_dim)));
+  const int group = a.heads / a.cache.kv_heads, rows = group * a.q_len;
+  const int64_t pairs = int64_t(a.batch) * a.cache.kv_heads;
+  p.group = divisor(group);
+  p.rows = divisor(rows);
+  p.heads = divisor(a.cache.kv_heads);
+  p.pairs = divisor(uint32_t(pairs));
+  p.all_rows = pairs * rows;
+  own = walk_for(pairs, rows, a.max_kv);
+  prefix = Walk{0, 4, 0};
   if (a.prefix_len > 0) {
-    pb = blocks_for(int64_t(a.batch) * p.rows, dim);
-    p.prefix_blocks = int(ceil_div(int64_t(a.batch) * p.rows, 16 * pb));
-    p.prefix_wgs = int64_t(a.cache.kv_heads) * p.prefix_blocks;
-    p.prefix_splits = splits_for(p.prefix_wgs, a.prefix_len);
-    p.prefix_wgs *= p.prefix_splits;
+    const int64_t all = int64_t(a.batch) * rows;
+    prefix = prefix_walk_for(a.cache.kv_heads, all, a.prefix_len);
+    own.waves = 4;
+    const int64_t blocks = ceil_div(all, 16 * prefix.blocks);
+    p.prefix_block_div = divisor(uint32_t(blocks));
+    p.prefix_wgs = a.cache.kv_heads * blocks * prefix.splits;
   }
+  const int64_t blocks = ceil_div(rows, 16 * own.blocks);
+  p.row_block_div = divisor(uint32_t(blocks));
+  p.own_wgs = pairs * blocks * own.splits;
+  p.splits = own.splits;
+  p.prefix_splits = prefix.splits;
   p.parts = p.splits + p.prefix_splits > 1;
   return p;
 }
 
-template <int D, int QB, int PB>
+template <int D, int QB, int PB, int KW>
 hipError_t launch(const AttnPlan& p, hipStream_t stream) {
-  constexpr int bytes = int(std::max(sizeof(Merge<D, QB>), PB > 0 ? sizeof(Merge<D, (PB > 0 ? PB : 1)>) : size_t(0)));
-  static LdsLimit limit;
-  if (bytes > 64 * 1024) {
-    const hipError_t e = limit.raise(reinterpret_cast<const void*>(&kv_attention_kernel<D, QB, PB>), bytes);
+  constexpr int bytes =
+      KW == 1 ? 0 : int(std::max(sizeof(Merge<D, QB, KW>), PB > 0 ? sizeof(Merge<D, (PB > 0 ? PB : 1), KW>) : size_t(0)));
+  if constexpr (bytes > 64 * 1024) {  // (two blocks of 128-dim rows)
+    static LdsLimit limit;
+    const hipError_t e = limit.raise(reinterpret_cast<const void*>(&kv_attention_kernel<D, QB, PB, KW>), bytes);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((kv_attention_kernel<D, QB, PB>), dim3(unsigned(p.prefix_wgs + p.own_wgs)), dim3(64 * kWaves), bytes,
+  hipLaunchKernelGGL((kv_attention_kernel<D, QB, PB, KW>), dim3(unsigned(p.prefix_wgs + p.own_wgs)), dim3(64 * KW), bytes,
                      stream, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !p.parts) return e;
@@ -471,35 +542,30 @@ hipError_t launch(const AttnPlan& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <int D, int QB>
-hipError_t launch_prefix(const AttnPlan& p, int pb, hipStream_t stream) {
-  if (pb == 0) return launch<D, QB, 0>(p, stream);
-  if (pb == 1) return launch<D, QB, 1>(p, stream);
-  if constexpr (D == 64)
-    if (pb == 4) return launch<D, QB, 4>(p, stream);
-  return launch<D, QB, 2>(p, stream);
-}
-
 template <int D>
-hipError_t launch_blocks(const AttnPlan& p, int qb, int pb, hipStream_t stream) {
-  if (qb == 1) return launch_prefix<D, 1>(p, pb, stream);
-  if constexpr (D == 64)
-    if (qb == 4) return launch_prefix<D, 4>(p, pb, stream);
-  return launch_prefix<D, 2>(p, pb, stream);
+hipError_t launch_walk(const AttnPlan& p, const Walk& own, const Walk& prefix, hipStream_t stream) {
+  if (own.waves == 1) return launch<D, 2, 0, 1>(p, stream);
+  if (own.waves == 2) return launch<D, 2, 0, 2>(p, stream);
+  if (own.blocks == 1) {
+    if (prefix.blocks == 0) return launch<D, 1, 0, 4>(p, stream);
+    return prefix.blocks == 1 ? launch<D, 1, 1, 4>(p, stream) : launch<D, 1, 2, 4>(p, stream);
+  }
+  if (prefix.blocks == 0) return launch<D, 2, 0, 4>(p, stream);
+  return prefix.blocks == 1 ? launch<D, 2, 1, 4>(p, stream) : launch<D, 2, 2, 4>(p, stream);
 }
 
 }  // namespace
 
 int64_t kv_attention_workspace(const KvAttnArgs& a) {
-  int qb, pb;
-  const AttnPlan p = plan_of(a, qb, pb);
+  Walk own, prefix;
+  const AttnPlan p = plan_of(a, own, prefix);
   return p.parts ? int64_t(p.splits + p.prefix_splits) * p.all_rows * (a.cache.head_dim + 2) * 4 : 0;
 }
 
 hipError_t kv_attention(const KvAttnArgs& a, hipStream_t stream) {
-  int qb, pb;
-  const AttnPlan p = plan_of(a, qb, pb);
-  return a.cache.head_dim == 64 ? launch_blocks<64>(p, qb, pb, stream) : launch_blocks<128>(p, qb, pb, stream);
+  Walk own, prefix;
+  const AttnPlan p = plan_of(a, own, prefix);
+  return a.cache.head_dim == 64 ? launch_walk<64>(p, own, prefix, stream) : launch_walk<128>(p, own, prefix, stream);
 }
 
 }  // namespace tia

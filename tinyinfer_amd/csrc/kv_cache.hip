@@ -13,7 +13,7 @@
 // Layout (T = capacity, a multiple of 64), made for the attention kernel's
 // matrix operands so that it loads 16 bytes per lane and moves nothing between
 // lanes:
-//   K  [slot][head][T][D]
+//   K  [slot][head][T / 16][D / 64][16 tokens][64 dims]
 //   V  [slot][head][T / 64][D / 16][64 lanes][16 bytes]: byte i of lane l of
 //      record d of a block of 64 tokens is token 16 (i / 4) + 4 (l / 16) + i % 4,
 //      dim 16 d + l % 16
@@ -66,6 +66,10 @@ __device__ __forceinline__ unsigned quantise(uint16_t bits, RowScale r) {
   return unsigned(int(q) + 128);
 }
 
+// Offsets of (token, dim) from the start of a slot's head.
+__device__ __forceinline__ int64_t k_byte(int64_t t, int dim, int D) {
+  return (t >> 4) * 16 * D + (dim >> 6) * 1024 + (t & 15) * 64 + (dim & 63);
+}
 __device__ __forceinline__ int64_t v_byte(int64_t t, int dim, int D) {
   const int r = int(t & 63);
   return (t >> 6) * 64 * D + (dim >> 4) * 1024 + ((dim & 15) + 16 * ((r >> 2) & 3)) * 16 + 4 * (r >> 4) + (r & 3);
@@ -118,7 +122,7 @@ __global__ __launch_bounds__(64) void append_rows_kernel(KvAppendArgs a) {
     kq |= uint64_t(quantise(k[e], kr)) << (8 * e);
     vd[v_byte(t, 8 * seg + e, D)] = uint8_t(quantise(v[e], vr));
   }
-  *reinterpret_cast<uint64_t*>(a.cache.k + (at + t) * D + 8 * seg) = kq;
+  *reinterpret_cast<uint64_t*>(a.cache.k + at * D + k_byte(t, 8 * seg, D)) = kq;
   if (seg == 0) {
     a.cache.k_scales[at + t] = kr.s;
     a.cache.v_scales[at + t] = vr.s;
@@ -161,7 +165,7 @@ __global__ __launch_bounds__(256) void append_block_kernel(KvAppendArgs a) {
     *reinterpret_cast<uint32_t*>(&vt[r][8 * seg + 4]) = vq[1];
     if (seg == 0) lives[r] = live;
     if (live) {
-      *reinterpret_cast<uint64_t*>(a.cache.k + (at + t) * D + 8 * seg) = uint64_t(kq[1]) << 32 | kq[0];
+      *reinterpret_cast<uint64_t*>(a.cache.k + at * D + k_byte(t, 8 * seg, D)) = uint64_t(kq[1]) << 32 | kq[0];
       if (seg == 0) {
         a.cache.k_scales[at + t] = kr.s;
         a.cache.v_scales[at + t] = vr.s;
@@ -233,7 +237,7 @@ __global__ __launch_bounds__(256) void read_kernel(KvReadArgs a) {
     if (i < 0 || i >= a.rows) continue;
     u16x8_t k = {}, v = {};
     if (i < n) {
-      const uint64_t kq = *reinterpret_cast<const uint64_t*>(a.cache.k + (at + t) * D + 8 * seg);
+      const uint64_t kq = *reinterpret_cast<const uint64_t*>(a.cache.k + at * D + k_byte(t, 8 * seg, D));
       const float ks = a.cache.k_scales[at + t], vs = a.cache.v_scales[at + t];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
