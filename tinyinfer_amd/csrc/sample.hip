@@ -39,16 +39,20 @@ constexpr u64 kOne = u64(1) << 35;  // weight of a token at its bin's near edge
 constexpr double kMass = 512.0;     // a mass: weight * e^(-b/256) * 2^9
 constexpr int kNoToken = 0x7fffffff;
 constexpr float kNegInf = -__builtin_huge_valf();
+// Place of a bin in LDS: a thread's kPerThread bins are followed by a gap, so that the
+// threads of a wave, each at its own run, meet in no bank.
+__device__ __forceinline__ constexpr unsigned slot(unsigned bin) { return bin + (bin >> 3); }
+
 struct SampleLds {
   union {
-    u64 bin[kBins];   // while the row is counted
-    u64 mass[kBins];  // then: the mass in front of each bin
+    u64 bin[slot(kBins)];   // while the row is counted
+    u64 mass[slot(kBins)];  // then: the mass in front of each bin
   };
-  unsigned count[kBins];  // tokens in front of each bin
+  unsigned count[slot(kBins)];  // tokens in front of each bin
   u64 runs[kRuns];
   u64 key[kList];         // the gathered tokens,
   unsigned at[kList], q[kList];  // their bins and losses
-  unsigned wanted[kBins / 32 + 1];  // a bit per bin whose tokens are gathered (and a word of none)
+  unsigned wanted[kBins / 32];   // a bit per bin whose tokens are gathered
   u64 wave_mass[kThreads / 64];
   unsigned wave_count[kThreads / 64];
   float wave_max[kThreads / 64];
@@ -69,74 +73,86 @@ __device__ __forceinline__ float value_of(u64 key) {
   return __builtin_bit_cast(float, up & 0x80000000u ? up & 0x7fffffffu : ~up);
 }
 
-// A row.  f(value, index) is called for every token (and, value NaN, for places outside
-// the row).  Vectors lie on 16-byte boundaries of memory, so the first and the last may
-// hold places outside the row, which are not read.
+// A row: its 16-byte vectors on 16-byte boundaries of memory, and the few tokens in
+// front of the first and behind the last of them.
 template <typename T>
 struct Row {
-  static constexpr int W = 16 / int(sizeof(T)), kAhead = 16 / W;
+  static constexpr int W = 16 / int(sizeof(T));
   typedef T vec __attribute__((ext_vector_type(W)));
   const T* p;
-  int n, shift;  // places of the first vector in front of the row
+  int n, head, vectors;  // tokens; those in front of the first vector
 
-  __device__ __forceinline__ Row(const T* row, int length)
-      : p(row), n(length), shift(int(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T))) {}
+  __device__ __forceinline__ Row(const T* row, int length) : p(row), n(length) {
+    head = min(n, int(-(reinterpret_cast<uintptr_t>(row) / sizeof(T))) & (W - 1));
+    vectors = (n - head) / W;
+  }
+  // The vectors at, at + kThreads, ... (the last one's values past it).
+  template <int A>
+  __device__ __forceinline__ void load(vec (&x)[A], int at) const {
+#pragma unroll
+    for (int c = 0; c < A; ++c) x[c] = *reinterpret_cast<const vec*>(p + head + min(at + c * kThreads, vectors - 1) * W);
+  }
   template <typename F>
+  __device__ __forceinline__ void edges(F f) const {
+    const int t = int(threadIdx.x), at = t < head ? t : t + vectors * W;
+    if (at < n && (t < head || t < n - vectors * W)) f(float(p[at]), at);
+  }
+  // f(value, index) for every token, the next vectors on their way while A are worked on.
+  template <int A, typename F>
   __device__ __forceinline__ void each(F f) const {
-    constexpr int kStep = kThreads * W;
-    int i = int(threadIdx.x) * W - shift;
-    // Whole vectors, kAhead loads in flight.
-    for (; i >= 0 && i + (kAhead - 1) * kStep + W <= n; i += kAhead * kStep) {
-      vec x[kAhead];
+    edges(f);
+    int at = int(threadIdx.x);
+    if (at >= vectors) return;
+    vec x[A];
+    load(x, at);
+    while (at < vectors) {
+      vec next[A];
+      load(next, at + A * kThreads);
 #pragma unroll
-      for (int c = 0; c < kAhead; ++c) x[c] = *reinterpret_cast<const vec*>(p + i + c * kStep);
+      for (int c = 0; c < A; ++c) {
+        if (at + c * kThreads >= vectors) break;
 #pragma unroll
-      for (int c = 0; c < kAhead; ++c)
+        for (int e = 0; e < W; ++e) f(float(x[c][e]), head + (at + c * kThreads) * W + e);
+      }
 #pragma unroll
-        for (int e = 0; e < W; ++e) f(float(x[c][e]), i + c * kStep + e);
-    }
-    for (; i < n; i += kStep) {
-      const vec x = load(i);
-#pragma unroll
-      for (int e = 0; e < W; ++e) f(float(x[e]), i + e);
+      for (int c = 0; c < A; ++c) x[c] = next[c];
+      at += A * kThreads;
     }
   }
-  // f(value, index) for the few tokens that `rare` holds for (which may hold for no NaN).
+  // f(value, index) for the few tokens that `rare` holds for.
   template <typename P, typename F>
   __device__ __forceinline__ void pick(P rare, F f) const {
-    constexpr int kStep = kThreads * W;
-    for (int i = int(threadIdx.x) * W - shift; i < n; i += kAhead * kStep) {
-      vec x[kAhead];
-#pragma unroll
-      for (int c = 0; c < kAhead; ++c) x[c] = load(i + c * kStep);
+    constexpr int A = 32 / W;
+    edges([&](float x, int i) {
+      if (rare(x)) f(x, i);
+    });
+    for (int at = int(threadIdx.x); at < vectors; at += A * kThreads) {
+      vec x[A];
+      load(x, at);
       unsigned hits = 0;
 #pragma unroll
-      for (int c = 0; c < kAhead; ++c)
+      for (int c = 0; c < A; ++c)
 #pragma unroll
         for (int e = 0; e < W; ++e) hits |= unsigned(rare(float(x[c][e]))) << (c * W + e);
+#pragma unroll
+      for (int c = 1; c < A; ++c)
+        if (at + c * kThreads >= vectors) hits &= (1u << (c * W)) - 1;
       while (hits) {
-        const int k = __builtin_ctz(hits), at = i + k / W * kStep + k % W;
+        const int k = __builtin_ctz(hits), i = head + (at + k / W * kThreads) * W + k % W;
         hits &= hits - 1;
-        f(float(p[at]), at);
+        f(float(p[i]), i);
       }
     }
   }
-  // f(value) for one vector per thread, spread evenly over a row of more.
+  // f(value) for one vector per thread, spread evenly over a row of more (and the edges).
   template <typename F>
   __device__ __forceinline__ void sample(F f) const {
-    const int vectors = (n + shift + W - 1) / W;
+    edges([&](float x, int) { f(x); });
     const int at = vectors <= kThreads ? int(threadIdx.x) : int(unsigned(vectors) * u64(threadIdx.x) / kThreads);
-    if (at * W - shift >= n) return;
-    const vec x = load(at * W - shift);
+    if (at >= vectors) return;
+    const vec x = *reinterpret_cast<const vec*>(p + head + at * W);
 #pragma unroll
     for (int e = 0; e < W; ++e) f(float(x[e]));
-  }
-  __device__ __forceinline__ vec load(int i) const {
-    if (i >= 0 && i + W <= n) return *reinterpret_cast<const vec*>(p + i);
-    vec x;
-#pragma unroll
-    for (int e = 0; e < W; ++e) x[e] = i + e >= 0 && i + e < n ? p[i + e] : T(__builtin_nanf(""));
-    return x;
   }
 };
 
@@ -197,7 +213,7 @@ __device__ void scan(SampleLds& s, u64& mass_all, unsigned& count_all) {
   unsigned c[kPerThread], ci = 0;
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
-    const u64 b = s.bin[kPerThread * t + i];
+    const u64 b = s.bin[slot(kPerThread * t + i)];
     m[i] = mi;
     c[i] = ci;
     mi += mass_of(weight_of(b), edge * step(i));
@@ -232,8 +248,8 @@ __device__ void scan(SampleLds& s, u64& mass_all, unsigned& count_all) {
   }
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
-    s.mass[kPerThread * t + i] = front + m[i];
-    s.count[kPerThread * t + i] = before + c[i];
+    s.mass[slot(kPerThread * t + i)] = front + m[i];
+    s.count[slot(kPerThread * t + i)] = before + c[i];
   }
   __syncthreads();
 }
@@ -272,7 +288,7 @@ __device__ __forceinline__ Goal goal_u(float u, u64 m) {
 // one step.
 __device__ __forceinline__ unsigned find_bin(const SampleLds& s, const Goal& g) {
   const unsigned lane = threadIdx.x & 63;
-  const auto in_front = [&](unsigned bin) { return __ballot((g.by_count ? u64(s.count[bin]) : s.mass[bin]) < g.goal); };
+  const auto in_front = [&](unsigned bin) { return __ballot((g.by_count ? u64(s.count[slot(bin)]) : s.mass[slot(bin)]) < g.goal); };
   static_assert(kBins == 64 * 128, "two steps of the search");
   const unsigned run = 128 * (__popcll(in_front(128 * lane)) - 1);  // (bin 0 always is)
   return run + __popcll(in_front(run + lane)) + __popcll(in_front(run + 64 + lane)) - 1;
@@ -300,7 +316,7 @@ struct Gathered {
     key = s.key[threadIdx.x];
     bin = s.at[threadIdx.x];
     u64 front = weight0;
-    rank = s.count[bin] + count0;
+    rank = s.count[slot(bin)] + count0;
 #pragma unroll 8
     for (unsigned o = 0; o < n; ++o) {
       const u64 k = s.key[o];
@@ -310,8 +326,8 @@ struct Gathered {
       rank += ahead;
     }
     const double e = run_edge(bin / kPerThread) * step(int(bin % kPerThread));
-    before = s.mass[bin] + mass_of(front, e);
-    after = s.mass[bin] + mass_of(front + kOne - s.q[threadIdx.x], e);
+    before = s.mass[slot(bin)] + mass_of(front, e);
+    after = s.mass[slot(bin)] + mass_of(front + kOne - s.q[threadIdx.x], e);
   }
   __device__ __forceinline__ Place resolve(SampleLds& s, unsigned of, const Goal& g) const {
     if (bin == of && (g.by_count ? rank : before) < g.goal && g.goal <= (g.by_count ? rank + 1 : after)) {
@@ -332,7 +348,7 @@ template <typename T>
 __device__ __noinline__ Gathered gather(SampleLds& s, const Row<T>& row, const Scale& sc, const Goal& g, unsigned bin,
                                         unsigned count_all) {
   u64 low = 0, high = ~u64(0), weight0 = 0;
-  unsigned count0 = 0, n = (bin + 1 < kBins ? s.count[bin + 1] : count_all) - s.count[bin];
+  unsigned count0 = 0, n = (bin + 1 < kBins ? s.count[slot(bin + 1)] : count_all) - s.count[slot(bin)];
   const auto in_bin = [&](float x) {
     const float d = sc.distance(x);
     return d >= float(bin) && d < float(bin + 1);
@@ -347,7 +363,7 @@ __device__ __noinline__ Gathered gather(SampleLds& s, const Row<T>& row, const S
     }
     __syncthreads();
     u64 lo = ~u64(0), hi = 0;
-    row.each([&](float x, int i) {
+    row.template each<2>([&](float x, int i) {
       if (!in_bin(x)) return;
       const u64 k = order_key(x, i);
       lo = min(lo, k);
@@ -365,7 +381,7 @@ __device__ __noinline__ Gathered gather(SampleLds& s, const Row<T>& row, const S
       __syncthreads();
       for (int i = int(threadIdx.x); i < kRuns; i += kThreads) s.runs[i] = 0;
       __syncthreads();
-      row.each([&](float x, int i) {
+      row.template each<2>([&](float x, int i) {
         if (!in_bin(x)) return;
         const u64 k = order_key(x, i);
         if (k >= low && k <= high) atomicAdd(&s.runs[(k - low) >> shift], packed(sc.fraction(x)));
@@ -376,7 +392,7 @@ __device__ __noinline__ Gathered gather(SampleLds& s, const Row<T>& row, const S
       for (; at < kRuns - 1; ++at) {
         const u64 b = s.runs[at], w = weight0 + weight_of(b);
         const unsigned c = count0 + count_of(b);
-        if (g.goal <= (g.by_count ? u64(s.count[bin] + c) : s.mass[bin] + mass_of(w, e))) break;
+        if (g.goal <= (g.by_count ? u64(s.count[slot(bin)] + c) : s.mass[slot(bin)] + mass_of(w, e))) break;
         weight0 = w;
         count0 = c;
       }
@@ -419,7 +435,7 @@ __device__ __forceinline__ unsigned bin_of_rank(const SampleLds& s, unsigned goa
   for (unsigned run = 0; run < kBins; run += 1024) {
     unsigned sum = 0;
 #pragma unroll
-    for (unsigned i = 0; i < 16; ++i) sum += s.count[run + 16 * lane + ((i + lane) & 15)];
+    for (unsigned i = 0; i < 16; ++i) sum += s.count[slot(run + 16 * lane + i)];
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const unsigned up = __shfl_up(sum, o, 64);
@@ -428,9 +444,15 @@ __device__ __forceinline__ unsigned bin_of_rank(const SampleLds& s, unsigned goa
     const int over = __popcll(__ballot(before + sum < goal));
     if (over < 64) {
       if (over > 0) before += __shfl(sum, over - 1, 64);
-      unsigned bin = run + 16 * over;
-      while (before + s.count[bin] < goal) before += s.count[bin++];
-      return bin;
+      unsigned upto = s.count[slot(run + 16 * over + (lane & 15))];
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) {
+        const unsigned up = __shfl_up(upto, o, 16);
+        upto += (lane & 15) >= unsigned(o) ? up : 0;
+      }
+      const int bin = __popcll(__ballot(lane < 16 && before + upto < goal));
+      if (bin > 0) before += __shfl(upto, bin - 1, 64);
+      return run + 16 * over + bin;
     }
     before += __shfl(sum, 63, 64);
   }
@@ -457,8 +479,7 @@ __device__ __forceinline__ bool sample_short(SampleLds& s, const Row<T>& row, fl
                                              float min_p, float u, int32_t* token, float* prob) {
   const unsigned t = threadIdx.x, lane = t & 63;
   const auto clear = [&] {
-#pragma unroll
-    for (int i = 0; i < kPerThread; ++i) s.count[i * kThreads + t] = 0;
+    for (unsigned i = t; i < slot(kBins); i += kThreads) s.count[i] = 0;
     if (t == 0) s.list_count = 0;
   };
   clear();
@@ -469,12 +490,12 @@ __device__ __forceinline__ bool sample_short(SampleLds& s, const Row<T>& row, fl
   const Scale about(top, temp);
   row.sample([&](float x) {
     const float d = about.distance(x);
-    if (d < float(kBins)) atomicAdd(&s.count[unsigned(d)], 1u);
+    if (d < float(kBins)) atomicAdd(&s.count[slot(unsigned(d))], 1u);
   });
   __syncthreads();
   unsigned before;
   const unsigned sampled = Row<T>::W * kThreads;
-  const unsigned enough = unsigned(row.n) <= sampled ? most : 4 * most * sampled / unsigned(row.n) + 8;
+  const unsigned enough = row.vectors <= kThreads ? most : 4 * most * sampled / unsigned(row.n) + 8;
   const float least = top - float(min(bin_of_rank(s, enough, before) + 1, unsigned(kBins))) / about.per;
   __syncthreads();
   clear();
@@ -495,7 +516,7 @@ __device__ __forceinline__ bool sample_short(SampleLds& s, const Row<T>& row, fl
   for (unsigned i = t; i < found; i += kThreads) {
     const float d = sc.distance(value_of(s.bin[i]));
     if (d < float(kBins)) {
-      atomicAdd(&s.count[unsigned(d)], 1u);
+      atomicAdd(&s.count[slot(unsigned(d))], 1u);
       ++counted;
     }
   }
@@ -508,7 +529,7 @@ __device__ __forceinline__ bool sample_short(SampleLds& s, const Row<T>& row, fl
   for (int w = 0; w < kThreads / 64; ++w) counted += s.wave_count[w];
   most = min(most, counted);
   const unsigned last = bin_of_rank(s, most, before);
-  const unsigned n = before + s.count[last];
+  const unsigned n = before + s.count[slot(last)];
   if (n > kList) return false;
   __syncthreads();
   if (t == 0) s.list_count = 0;
@@ -518,16 +539,27 @@ __device__ __forceinline__ bool sample_short(SampleLds& s, const Row<T>& row, fl
     if (sc.distance(value_of(key)) < float(last + 1)) s.key[atomicAdd(&s.list_count, 1u)] = key;
   }
   __syncthreads();
+  // Ranks: `parts` threads to a token, each comparing it with a part of the others.
+  unsigned wide = 64;
+  while (wide < n) wide *= 2;
+  const unsigned mine = t & (wide - 1), part = t / wide, parts = kThreads / wide, chunk = (n + parts - 1) / parts;
+  if (t < n) s.q[t] = 0;
+  __syncthreads();
+  const u64 key = s.key[min(mine, n - 1)];
+  {
+    unsigned ahead = 0;
+    const unsigned end = min(n, (part + 1) * chunk);
+#pragma unroll 4
+    for (unsigned o = part * chunk; o < end; ++o) ahead += s.key[o] < key;
+    if (mine < n) atomicAdd(&s.q[mine], ahead);
+  }
+  __syncthreads();
   // Masses in the row's order, in units of 2^-44 of the heaviest token's, and their sums.
   constexpr double unit = 17592186044416.0;
-  u64 key = 0;
   double weight = 0;
   unsigned rank = ~0u;
-  if (t < n) {
-    key = s.key[t];
-    rank = 0;
-#pragma unroll 8
-    for (unsigned o = 0; o < n; ++o) rank += s.key[o] < key;
+  if (t < n) {  // (mine = t)
+    rank = s.q[t];
     weight = sc.weight_of(value_of(key));
     s.runs[rank] = u64(fma(weight, unit, 0.5));
   }
@@ -540,7 +572,8 @@ __device__ __forceinline__ bool sample_short(SampleLds& s, const Row<T>& row, fl
   }
   if (lane == 63) s.wave_mass[t >> 6] = sum;
   __syncthreads();
-  for (unsigned w = 0; w < t >> 6; ++w) sum += s.wave_mass[w];
+#pragma unroll
+  for (unsigned w = 0; w < kList / 64; ++w) sum += w < t >> 6 ? s.wave_mass[w] : 0;
   if (t < n) s.runs[t] = sum;
   unsigned kept = most;
   if (min_p > 0.f) {
@@ -577,13 +610,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   if (most <= kShort && temp > 0.f && sample_short(s, row, temp, most, top_p, min_p, u, a.tokens + b, a.probs + b)) return;
 
   float top = kNegInf;
-  row.each([&](float x, int) { top = fmaxf(top, x); });
+  row.template each<4>([&](float x, int) { top = fmaxf(top, x); });
   __syncthreads();
   top = block_top(s, top);
   if (top == kNegInf || !(temp > 0.f) || top == -kNegInf) {
     // No token above -inf, or the likeliest one.
     int at = kNoToken;
-    if (top != kNegInf) row.each([&](float x, int i) { at = x == top ? min(at, i) : at; });
+    if (top != kNegInf) row.template each<2>([&](float x, int i) { at = x == top ? min(at, i) : at; });
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
     if ((t & 63) == 0) s.wave_at[t >> 6] = at;
@@ -596,14 +629,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     return;
   }
   const Scale sc(top, temp);
-#pragma unroll
-  for (int i = 0; i < kPerThread; ++i) s.bin[i * kThreads + t] = 0;
-  if (t <= kBins / 32) s.wanted[t] = 0;
+  for (unsigned i = unsigned(t); i < slot(kBins); i += kThreads) s.bin[i] = 0;
+  if (t < kBins / 32) s.wanted[t] = 0;
   if (t == 0) s.list_count = 0;
   __syncthreads();
-  row.each([&](float x, int) {
+  row.template each<4>([&](float x, int) {
     const float d = sc.distance(x);
-    if (d < float(kBins)) atomicAdd(&s.bin[unsigned(d)], packed(sc.fraction(x)));
+    if (d < float(kBins)) atomicAdd(&s.bin[slot(unsigned(d))], packed(sc.fraction(x)));
   });
   u64 mass_all;
   unsigned count_all;
@@ -619,34 +651,33 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
 
   // The bins in question, from masses known to a bin: their tokens are gathered in one pass.
   {
-    const auto behind = [&](unsigned bin) { return bin + 1 < kBins ? s.mass[bin + 1] : mass_all; };
+    const auto behind = [&](unsigned bin) { return bin + 1 < kBins ? s.mass[slot(bin + 1)] : mass_all; };
     constexpr int kRanges = 4;
     unsigned from[kRanges] = {1, 1, 1, 1}, to[kRanges] = {0, 0, 0, 0};
     u64 low = mass_all, high = mass_all;  // the kept mass lies between
     if (use_k) {
       from[0] = to[0] = find_bin(s, Goal{true, u64(top_k)});
-      low = s.mass[to[0]];
+      low = s.mass[slot(to[0])];
       high = behind(to[0]);
     }
     if (use_p) {
       from[1] = find_bin(s, goal_p(top_p, max(low, u64(1))));
       to[1] = find_bin(s, goal_p(top_p, high));
-      low = s.mass[from[1]];
+      low = s.mass[slot(from[1])];
       high = behind(to[1]);
     }
     if (use_m) {
       from[2] = to[2] = far;
-      low = min(low, s.mass[far]);
+      low = min(low, s.mass[slot(far)]);
       high = min(high, behind(far));
     }
     from[3] = find_bin(s, goal_u(u, max(low, u64(1))));
     to[3] = find_bin(s, goal_u(u, max(high, u64(1))));
-    unsigned last = 0, tokens = 0;
+    unsigned tokens = 0;
 #pragma unroll
     for (int r = 0; r < kRanges; ++r) {
       if (from[r] > to[r]) continue;
-      last = max(last, to[r]);
-      tokens += (to[r] + 1 < kBins ? s.count[to[r] + 1] : count_all) - s.count[from[r]];
+      tokens += (to[r] + 1 < kBins ? s.count[slot(to[r] + 1)] : count_all) - s.count[slot(from[r])];
     }
     if (tokens <= kList) {  // (bins in two ranges count twice)
       if (t < kBins / 32) {
@@ -660,13 +691,38 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
         s.wanted[t] = bits;
       }
       __syncthreads();
-      const float end = float(last + 1);
-      row.pick(
-          [&](float x) {
-            const float d = sc.distance(x);
-            return is_wanted(s, d < end ? unsigned(d) : unsigned(kBins));
-          },
-          [&](float x, int i) { take(s, order_key(x, i), unsigned(sc.distance(x)), sc.fraction(x)); });
+      int ranges = 0;  // those that are, in front
+#pragma unroll
+      for (int r = 0; r < kRanges; ++r) {
+        if (from[r] > to[r]) continue;
+#pragma unroll
+        for (int o = 0; o <= r; ++o)
+          if (o == ranges) {
+            const unsigned f = from[r], e = to[r];
+            from[o] = f;
+            to[o] = e;
+          }
+        ++ranges;
+      }
+      const auto act = [&](float x, int i) { take(s, order_key(x, i), unsigned(sc.distance(x)), sc.fraction(x)); };
+      const auto within = [&](float d, int r) { return d >= float(from[r]) && d < float(to[r] + 1); };
+      if (ranges <= 2) {
+        if (ranges == 1) from[1] = 1, to[1] = 0;
+        row.pick(
+            [&](float x) {
+              const float d = sc.distance(x);
+              return within(d, 0) || within(d, 1);
+            },
+            act);
+      } else {
+        if (ranges == 3) from[3] = 1, to[3] = 0;
+        row.pick(
+            [&](float x) {
+              const float d = sc.distance(x);
+              return within(d, 0) || within(d, 1) || within(d, 2) || within(d, 3);
+            },
+            act);
+      }
       __syncthreads();
     }
   }
@@ -696,15 +752,15 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
       const float x = value_of(mine.key);
       if (mine.bin == far && sc.weight_of(x) >= double(min_p)) heavy = packed(sc.fraction(x));
     } else {
-      row.each([&](float x, int) {
+      row.template each<2>([&](float x, int) {
         const float d = sc.distance(x);
         if (d >= float(far) && d < float(far + 1) && sc.weight_of(x) >= double(min_p)) heavy += packed(sc.fraction(x));
       });
     }
     if (heavy) atomicAdd(&s.low, heavy);
     __syncthreads();
-    const unsigned n = s.count[far] + count_of(s.low);
-    const u64 m = s.mass[far] + mass_of(weight_of(s.low), run_edge(far / kPerThread) * step(int(far % kPerThread)));
+    const unsigned n = s.count[slot(far)] + count_of(s.low);
+    const u64 m = s.mass[slot(far)] + mass_of(weight_of(s.low), run_edge(far / kPerThread) * step(int(far % kPerThread)));
     __syncthreads();
     if (n < length) kept = n == 0 ? mass_of(kOne - loss(0.f), run_edge(0)) : m;  // (n = 0: min_p above 1)
   }

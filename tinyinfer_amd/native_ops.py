@@ -154,6 +154,12 @@ class _Call:
         self.args.append(y.data_ptr())
         return y
 
+    def output_like(self, x):
+        y = self.ops.torch.empty_like(x)
+        self.made.append(y)
+        self.args.append(y.data_ptr())
+        return y
+
     def workspace(self, shape, needed):
         if not needed:
             self.args.append(None)
@@ -210,18 +216,23 @@ class _Call:
         self.args.extend(values)
 
     def run(self):
-        cuda = self.ops.torch.cuda
-        index = self.device.index
-        stream = cuda.current_stream(index)
+        ops, index = self.ops, self.device.index
+        cuda = ops.torch.cuda
+        # (The current stream's handle costs a tenth of making its Stream object, which
+        # record_stream wants and which stays the same for a handle.)
+        handle = ops.stream_handle(index)
+        stream = ops.streams.get((index, handle))
+        if stream is None:
+            stream = ops.streams[index, handle] = cuda.current_stream(index)
         for x in self.held:
             x.record_stream(stream)
         if cuda.current_device() == index:
-            status = getattr(self.ops.lib, self.symbol)(*self.args, stream.cuda_stream, index)
+            status = getattr(ops.lib, self.symbol)(*self.args, handle, index)
         else:
             with cuda.device(self.device):
-                status = getattr(self.ops.lib, self.symbol)(*self.args, stream.cuda_stream, index)
+                status = getattr(ops.lib, self.symbol)(*self.args, handle, index)
         if status != 0:
-            detail = self.ops.lib.ti_v2_last_error().decode("utf-8", errors="replace")
+            detail = ops.lib.ti_v2_last_error().decode("utf-8", errors="replace")
             raise RuntimeError(f"{self.symbol} failed ({status}): {detail}")
 
 
@@ -265,6 +276,7 @@ class NativeOps:
     def __init__(self, library_path=None):
         import torch
         self.torch, self.tensor_type = torch, torch.Tensor
+        self.stream_handle, self.streams = torch._C._cuda_getCurrentRawStream, {}
         where = require(BACKEND_LIB) if library_path is None else library_path
         self.library_path = str(Path(where).expanduser().resolve(strict=True))
         self.lib = ctypes.CDLL(self.library_path)
@@ -530,7 +542,7 @@ class NativeOps:
         if slots is None or kv_lengths is None:
             raise ValueError("slots and kv_lengths are required")
         bound = 0 if max_kv_length is None else _count(max_kv_length, "max_kv_length", 0)
-        y = call.output(q.shape, torch.float16)
+        y = call.output_like(q)
         call.per_request(batch, (slots, cache.slots - 1, "slots"), (kv_lengths, cache.capacity, "kv_lengths"),
                          (q_lengths, nq, "q_lengths"), (query_offsets, INT32_MAX - nq, "query_offsets"))
         needed = self.lib.ti_amd_attention_i8kv_workspace(cache._at, batch, heads, nq, bound, prefix_length)
