@@ -138,7 +138,7 @@ typedef struct ti_amd_kv_i8 {
  * lengths[b] (null: every row) becomes token positions[b] + i of slots[b].  The
  * metadata is int32 [batch] on the device.  What lies outside the cache (a slot,
  * a token) is not written; where two requests write the same token the later
- * request's row stays. */
+ * request's row stays.  batch is at most 65535, rows at most 2^28. */
 int ti_amd_kv_append_i8(const ti_amd_kv_i8* cache, const uint16_t* k, const uint16_t* v, const int32_t* slots,
                         const int32_t* positions, const int32_t* lengths, int batch, int rows, uintptr_t stream, int device);
 /* ti_amd_kv_read_i8: the same rows back, fp16_rn(fp32(c * scale)); zeros past
@@ -151,7 +151,8 @@ int ti_amd_kv_read_i8(const ti_amd_kv_i8* cache, uint16_t* k, uint16_t* v, const
  * outside the cache has none).  Query i < q_lengths[b] (null: q_len) sees them
  * all, or with causal = 1 those up to offsets[b] + i; offsets null means
  * kv_lengths[b] - q_lengths[b]: the queries are the request's last tokens.  Rows
- * that see no key, and queries past q_lengths[b], are exactly 0.
+ * that see no key, and queries past q_lengths[b], are exactly 0.  batch and heads
+ * are at most 65535, batch * heads * q_len at most 2^23.
  * prefix_len > 0: in front of its own keys every query also sees tokens 0 ..
  * prefix_len - 1 of prefix_slot, whose bytes are read once for the batch.
  * Scores, softmax and sums are fp32; probabilities are rounded to fp16.
@@ -167,7 +168,7 @@ int ti_amd_attention_i8kv(const ti_amd_kv_i8* cache, const uint16_t* q, uint16_t
                           int prefix_slot, int prefix_len, uintptr_t stream, int device);
 
 /* ti_amd_sample: one token per row of logits [batch][vocab] (dtype 0 fp16, 1
- * fp32; vocab at most 262144) from uniforms[batch] in [0, 1) (others are taken
+ * fp32; batch at most 2^20, vocab 2^18) from uniforms[batch] in [0, 1) (others are taken
  * as the nearest of them, NaN as 0).  Tokens are ordered by logit, ties by
  * index; kept are the first top_k (<= 0: all), of these the shortest run from
  * the front with top_p of their probability (>= 1: all), of these those with at

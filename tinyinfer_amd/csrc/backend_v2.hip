@@ -119,8 +119,9 @@ bool optional_aligned(const void* p, size_t bytes) { return !p || aligned(p, byt
 int check_kv_rows(const void* k, const void* v, const int32_t* slots, const int32_t* positions, const int32_t* lengths,
                   int batch, int rows, const tia::KvI8& c) {
   if (!aligned(k, 2) || !aligned(v, 2) || !aligned(slots, 4) || !aligned(positions, 4) || !optional_aligned(lengths, 4) ||
-      batch <= 0 || batch > 65535 || rows <= 0 || !shape_fits({batch, c.kv_heads, rows, c.head_dim}, 2))
-    return fail(TI_V2_INVALID_ARGUMENT, "invalid int8 cache rows: shape, pointers or alignment (batch at most 65535)");
+      batch <= 0 || batch > 65535 || rows <= 0 || rows > (1 << 28) || !shape_fits({batch, c.kv_heads, rows, c.head_dim}, 2))
+    return fail(TI_V2_INVALID_ARGUMENT,
+                "invalid int8 cache rows: shape, pointers or alignment (batch at most 65535, rows 2^28)");
   return TI_V2_OK;
 }
 
@@ -128,12 +129,13 @@ int check_kv_attention(const ti_amd_kv_i8* cache, int batch, int heads, int q_le
                        int prefix_len, tia::KvAttnArgs& a) {
   const int status = check_cache(cache, a.cache);
   if (status) return status;
-  const int64_t most = std::numeric_limits<int32_t>::max();
+  // (Row numbers and one-dimensional grids of 256 threads per 1 row and more stay below 2^32.)
+  const int most = 1 << 23;
   if (batch <= 0 || batch > 65535 || heads <= 0 || heads > 65535 || q_len <= 0 || heads % a.cache.kv_heads != 0 ||
       int64_t(batch) * heads > most / q_len || max_kv < 0 || prefix_len < 0 || prefix_len > a.cache.capacity ||
       (prefix_len > 0 && (prefix_slot < 0 || prefix_slot >= a.cache.slots)))
     return fail(TI_V2_INVALID_ARGUMENT,
-                "invalid int8 cache attention: heads a multiple of kv_heads, at most 2^31 - 1 query rows, the prefix inside the cache");
+                "invalid int8 cache attention: heads a multiple of kv_heads, at most 2^23 query rows, the prefix inside the cache");
   a.batch = batch;
   a.heads = heads;
   a.q_len = q_len;
@@ -555,9 +557,9 @@ extern "C" int ti_amd_sample(const void* logits, int dtype, const float* uniform
   if (status) return status;
   if ((dtype != TI_V2_FP16 && dtype != TI_V2_FP32) || !aligned(logits, dtype == TI_V2_FP16 ? 2 : 4) || !aligned(uniforms, 4) ||
       !optional_aligned(temperature, 4) || !optional_aligned(top_k, 4) || !optional_aligned(top_p, 4) ||
-      !optional_aligned(min_p, 4) || !aligned(tokens, 4) || !aligned(probs, 4) || vocab > (1 << 18) ||
+      !optional_aligned(min_p, 4) || !aligned(tokens, 4) || !aligned(probs, 4) || vocab > (1 << 18) || batch > (1 << 20) ||
       !shape_fits({batch, vocab}, 4))
-    return fail(TI_V2_INVALID_ARGUMENT, "invalid sampling arguments: fp16 or fp32 logits, at most 262144 of a row");
+    return fail(TI_V2_INVALID_ARGUMENT, "invalid sampling arguments: fp16 or fp32 logits, at most 2^20 rows of 2^18");
   tia::SampleArgs a;
   a.logits = logits;
   a.f32 = dtype == TI_V2_FP32;

@@ -110,15 +110,26 @@ struct Merge {
   float m[KW][QB][16], l[KW][QB][16];
 };
 
+// A tile's operands as the waves of a workgroup share them, in the order in which a
+// lane reads them: 16 bytes per lane, one conflict-free kilobyte per operand.
+template <int D>
+struct Tiles {
+  half8_t k[2][4][D / 32][64], v[2][D / 16][2][64];
+};
+
 // Row block `rb` of one set of keys.  PREFIX: rows run over the batch, key head
 // `head`, the keys are the prefix's; else over request b's.
+// KW waves share the row block, each with its own tiles; kShared: 4 waves have a row
+// block each (`rb` counts those groups) and share every tile, each widening a quarter of
+// it into LDS while the tile before is worked on.
+constexpr int kShared = 0;
 template <int D, int QB, int KW, bool PREFIX>
 __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb, int split, int splits, int state) {
   const KvAttnArgs& a = p.a;
   const int lane = int(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
   const int j = lane & 15, g = lane >> 4;
-  constexpr int ROWS = 16 * QB;
-  const int r0 = rb * ROWS, row_count = PREFIX ? a.batch * int(p.rows.d) : int(p.rows.d);
+  constexpr int ROWS = 16 * QB, GROUP = KW == kShared ? 4 * ROWS : ROWS;
+  const int group0 = rb * GROUP, r0 = KW == kShared ? group0 + wave * ROWS : group0, row_count = PREFIX ? a.batch * int(p.rows.d) : int(p.rows.d);
 
   int slot, kv;
   if constexpr (PREFIX) {
@@ -144,22 +155,28 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
     if (!PREFIX && a.causal) e = min(e, (a.offsets ? int64_t(a.offsets[b]) : int64_t(kv) - ql) + qi + 1);
     end[u] = r < row_count && qi < ql ? int(max(e, int64_t(0))) : 0;
   }
-  // Keys that some row of the block sees, and keys that every row with a query
-  // sees (a row without one may compute anything: it is cleared at the end).
-  int last, first;
+  // Keys that some row of the wave sees, and keys that every row of it with a query sees
+  // (a row without one may compute anything: it is cleared at the end); keys that some
+  // row of the workgroup sees.
+  int last, first, group_last;
   if constexpr (PREFIX) {
-    last = first = kv;
+    last = r0 < row_count ? kv : 0;
+    first = group_last = kv;
   } else {
     const int ql = a.q_lengths ? min(max(a.q_lengths[b0], 0), a.q_len) : a.q_len;
-    const int q_first = div_by(r0, p.group), q_last = min(div_by(min(r0 + ROWS, row_count) - 1, p.group), ql - 1);
     const int64_t off = a.offsets ? int64_t(a.offsets[b0]) : int64_t(kv) - ql;
     const auto seen = [&](int qi) { return int(max(a.causal ? min(int64_t(kv), off + qi + 1) : int64_t(kv), int64_t(0))); };
-    last = q_last < q_first ? 0 : seen(q_last);
-    first = q_last < q_first ? 0 : seen(q_first);
+    const auto last_of = [&](int from, int rows) {
+      const int q_last = min(div_by(min(from + rows, row_count) - 1, p.group), ql - 1);
+      return from >= row_count || q_last < div_by(from, p.group) ? 0 : seen(q_last);
+    };
+    last = last_of(r0, ROWS);
+    first = last == 0 ? 0 : seen(div_by(r0, p.group));
+    group_last = KW == kShared ? last_of(group0, GROUP) : last;
   }
-  const int tiles = (last + kTile - 1) / kTile, per = (tiles + splits - 1) / splits;
+  const int tiles = (group_last + kTile - 1) / kTile, per = (tiles + splits - 1) / splits;
   const int t_end = min(tiles, (split + 1) * per);
-  int t = split * per + wave;
+  int t = split * per + (KW == kShared ? 0 : wave);
 
   const int64_t base = (int64_t(slot) * a.cache.kv_heads + head) * a.cache.capacity;
   const uint8_t* kp = a.cache.k + base * D + j * 64 + 16 * g;
@@ -170,22 +187,40 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
   const float* ksp = a.cache.k_scales + base + my_key;
   const float* vsp = a.cache.v_scales + base + my_key;
   constexpr bool NT = !PREFIX && QB == 1;
-  u32x4_t kr[4][D / 64], vr[D / 16];
+  u32x4_t kr[KW == kShared ? 1 : 4][D / 64], vr[KW == kShared ? D / 64 : D / 16];
   float ksr = 0.f, vsr = 0.f;
+  auto& shared = *reinterpret_cast<Tiles<D>*>(lds);
+  // A tile's bytes, or this wave's quarter of them: 16 keys, and a quarter of the dims of
+  // all values.
   auto load_k = [&](int tt) {
-    const uint8_t* at = kp + int64_t(tt) * (kTile * D);
+    const uint8_t* at = kp + int64_t(tt) * (kTile * D) + (KW == kShared ? 16 * wave * D : 0);
 #pragma unroll
-    for (int kb = 0; kb < 4; ++kb)
+    for (int kb = 0; kb < (KW == kShared ? 1 : 4); ++kb)
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) kr[kb][c] = load16<NT>(at + 16 * kb * D + 1024 * c);
-    ksr = ksp[int64_t(tt) * kTile];
   };
   auto load_v = [&](int tt) {
-    const uint8_t* at = vp + int64_t(tt) * (kTile * D);
+    const uint8_t* at = vp + int64_t(tt) * (kTile * D) + (KW == kShared ? 1024 * wave * (D / 64) : 0);
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) vr[d] = load16<NT>(at + 1024 * d);
+    for (int d = 0; d < (KW == kShared ? D / 64 : D / 16); ++d) vr[d] = load16<NT>(at + 1024 * d);
+  };
+  auto load_scales = [&](int tt) {
+    ksr = ksp[int64_t(tt) * kTile];
     vsr = vsp[int64_t(tt) * kTile];
   };
+  auto share = [&](int buf) {
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        shared.k[buf][wave][2 * c + s][lane] = widen8(kr[0][c][2 * s], kr[0][c][2 * s + 1]);
+        shared.v[buf][wave * (D / 64) + c][s][lane] = widen8(vr[c][2 * s], vr[c][2 * s + 1]);
+      }
+  };
+  if (KW == kShared && t < t_end) {
+    load_k(t);
+    load_v(t);
+  }
 
   // Step (c, s) of a dot product takes dims 64 c + 16 g + 8 s .. + 7 from lane (., g).
   half8_t qf[QB][D / 32];
@@ -215,9 +250,7 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
   // the weight p * vs / unit that is rounded to fp16 is then at most p.
   float unit = 0.f, inv_unit = 1.f;
 
-  for (; t < t_end; t += KW) {
-    load_k(t);
-    load_v(t);
+  const auto tile = [&](int t, int buf, float ks, float vs_) {
     const bool full = (t + 1) * kTile <= first;
     float4_t sc[QB][4];
 #pragma unroll
@@ -228,16 +261,16 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
       for (int c = 0; c < D / 64; ++c)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const half8_t kf = widen8(kr[kb][c][2 * s], kr[kb][c][2 * s + 1]);
+          const half8_t kf = KW == kShared ? shared.k[buf][kb][2 * c + s][lane] : widen8(kr[KW == kShared ? 0 : kb][c][2 * s], kr[KW == kShared ? 0 : kb][c][2 * s + 1]);
 #pragma unroll
           for (int u = 0; u < QB; ++u)
             sc[u][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[u][2 * c + s], sc[u][kb], 0, 0, 0);
         }
-      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (KW != kShared) __builtin_amdgcn_sched_barrier(0);  // (widen one block of 16 keys at a time)
     }
-    const float ck = ksr * p.scale;
+    const float ck = ks * p.scale;
     // (Past the last key any row sees, scales may be anything.)
-    const float vs = t * kTile + my_key < last ? vsr : 0.f;
+    const float vs = t * kTile + my_key < last ? vs_ : 0.f;
     if (__ballot(vs > unit)) {
       const float top = wave_max(vs);
       const float raised = __builtin_amdgcn_ldexpf(1.f, __builtin_amdgcn_frexp_expf(top));  // > top
@@ -297,11 +330,41 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
     for (int d = 0; d < D / 16; ++d) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const half8_t vf = widen8(vr[d][2 * c], vr[d][2 * c + 1]);
+        const half8_t vf = KW == kShared ? shared.v[buf][d][c][lane] : widen8(vr[KW == kShared ? 0 : d][2 * c], vr[KW == kShared ? 0 : d][2 * c + 1]);
 #pragma unroll
         for (int u = 0; u < QB; ++u) acc[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pp[u][c], acc[u][d], 0, 0, 0);
       }
-      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (KW != kShared) __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  if constexpr (KW == kShared) {
+    if (t < t_end) {
+      share(0);
+      load_scales(t);
+      if (t + 1 < t_end) {
+        load_k(t + 1);
+        load_v(t + 1);
+      }
+    }
+    for (int buf = 0; t < t_end; ++t, buf ^= 1) {
+      lds_barrier();  // (the next tile's loads stay in flight)
+      const float ks = ksr, vs = vsr;
+      if (t + 1 < t_end) {
+        share(buf ^ 1);
+        load_scales(t + 1);
+        if (t + 2 < t_end) {
+          load_k(t + 2);
+          load_v(t + 2);
+        }
+      }
+      if (t * kTile < last) tile(t, buf, ks, vs);
+    }
+  } else {
+    for (; t < t_end; t += KW) {
+      load_k(t);
+      load_scales(t);
+      load_v(t);
+      tile(t, 0, ksr, vsr);
     }
   }
 
@@ -334,7 +397,7 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
     ml[0] = top;
     ml[1] = total;
   };
-  if constexpr (KW == 1) {
+  if constexpr (KW == kShared) {
 #pragma unroll
     for (int u = 0; u < QB; ++u) {
 #pragma unroll
@@ -388,7 +451,7 @@ constexpr int waves_for(int dim, int qb) { return dim == 64 ? (qb == 1 ? 4 : 3) 
 // QB, PB: row blocks of 16 per wave over the requests' own keys and the prefix's (0:
 // no prefix); KW: waves that share a row block's keys.
 template <int D, int QB, int PB, int KW>
-__global__ __launch_bounds__(64 * KW, waves_for(D, QB > PB ? QB : PB)) void kv_attention_kernel(AttnPlan p) {
+__global__ __launch_bounds__(KW == kShared ? 256 : 64 * KW, waves_for(D, QB > PB ? QB : PB)) void kv_attention_kernel(AttnPlan p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   int id = int(blockIdx.x);
   const int heads = p.a.cache.kv_heads;
@@ -453,30 +516,33 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(AttnPlan p) {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // How a set of keys is walked: `blocks` row blocks of 16 per wave, `waves` waves to a
-// row block, `splits` workgroups to its keys.
+// row block or kShared, `splits` workgroups to its keys.
 struct Walk {
   int blocks, waves, splits;
 };
 
 // From the number of (request, key head) pairs, the rows of one and the tiles of 64 keys
-// of the longest.  Two blocks of 16 rows use every converted key and value twice; they
+// of the longest.  Two blocks of 16 rows use every widened key and value twice; they
 // pay where there are plenty of row blocks (GPT-2 XL prefill, 100 pairs of 1024 rows:
-// 38.4 against 44.7 us; 12 pairs: 12.2 against 11.1) or many keys to a row block (64
-// queries over 16000 keys, D 128: 40 against 50 us).
-// Waves: with enough row blocks to fill every SIMD three times a wave takes a whole one
-// and nothing is merged (100 pairs of 1024 rows: 38.4 us, 46.6 with four waves); below
-// that two waves, or four where keys are many (12 pairs of 4096 rows: 56 us, 66 with
-// two, 100 with one).
+// 38.4 us against 44.7; 64 pairs of 333 rows, D 128: 37 against 53; 12 pairs of 1024:
+// 12.2 against 11.1) or many keys to a row block (64 queries of 4 heads over 16000 keys,
+// D 128: 40 against 50 us).
+// Waves: with row blocks to fill every SIMD three times a workgroup takes four of them
+// and its waves share the tiles, each widened once instead of four times and nothing
+// merged (100 pairs of 1024 rows: 34.5 us, 39 with a wave to a row block of its own, 47
+// with four waves to one; 32 pairs of 4096 rows, D 128: 176, 191 and 213 us); below that
+// two waves share a row block, or four where keys are many (12 pairs of 4096 rows: 56 us,
+// 66 with two, 87 with shared tiles).
 // Splits: a second launch and the states' traffic cost 2 us and more, so short caches
 // are not split (96 pairs, 1024 keys: 8.8 us, 9.4 in four), longer ones into about
 // 384 or, from 4096 keys on, 512 workgroups (8 pairs of 4096 keys, D 128: 31 us whole,
 // 10.6 in 16; 128 pairs of 32768: 253 us whole, 136 in 4).
-Walk walk_for(int64_t pairs, int rows, int keys) {
-  const int64_t tiles = ceil_div(keys, kTile), twos = pairs * ceil_div(rows, 32);
+Walk walk_for(int64_t pairs, int rows, int keys, int dim) {
+  const int64_t tiles = ceil_div(keys, kTile), twos = pairs * ceil_div(rows, 32), plenty = dim == 64 ? 1024 : 512;
   Walk w{1, 4, 1};
-  if (rows > 16 && (twos >= 1024 || tiles >= 128)) w.blocks = 2;
-  if (w.blocks == 2 && twos >= 1024) {
-    w.waves = twos >= 3072 ? 1 : tiles < 32 ? 2 : 4;
+  if (rows > 16 && (twos >= plenty || tiles >= 128)) w.blocks = 2;
+  if (w.blocks == 2 && twos >= plenty) {
+    w.waves = twos >= 3072 ? kShared : twos >= 1024 && tiles < 32 ? 2 : 4;
     return w;
   }
   const int64_t wgs = pairs * ceil_div(rows, 16 * w.blocks);
@@ -506,7 +572,7 @@ AttnPlan plan_of(const KvAttnArgs& a, Walk& own, Walk& prefix) {
   p.heads = divisor(a.cache.kv_heads);
   p.pairs = divisor(uint32_t(pairs));
   p.all_rows = pairs * rows;
-  own = walk_for(pairs, rows, a.max_kv);
+  own = walk_for(pairs, rows, a.max_kv, a.cache.head_dim);
   prefix = Walk{0, 4, 0};
   if (a.prefix_len > 0) {
     const int64_t all = int64_t(a.batch) * rows;
@@ -516,7 +582,7 @@ AttnPlan plan_of(const KvAttnArgs& a, Walk& own, Walk& prefix) {
     p.prefix_block_div = divisor(uint32_t(blocks));
     p.prefix_wgs = a.cache.kv_heads * blocks * prefix.splits;
   }
-  const int64_t blocks = ceil_div(rows, 16 * own.blocks);
+  const int64_t blocks = ceil_div(rows, 16 * own.blocks * (own.waves == kShared ? 4 : 1));
   p.row_block_div = divisor(uint32_t(blocks));
   p.own_wgs = pairs * blocks * own.splits;
   p.splits = own.splits;
@@ -528,13 +594,13 @@ AttnPlan plan_of(const KvAttnArgs& a, Walk& own, Walk& prefix) {
 template <int D, int QB, int PB, int KW>
 hipError_t launch(const AttnPlan& p, hipStream_t stream) {
   constexpr int bytes =
-      KW == 1 ? 0 : int(std::max(sizeof(Merge<D, QB, KW>), PB > 0 ? sizeof(Merge<D, (PB > 0 ? PB : 1), KW>) : size_t(0)));
+      KW == kShared ? int(sizeof(Tiles<D>)) : int(std::max(sizeof(Merge<D, QB, (KW > 0 ? KW : 1)>), PB > 0 ? sizeof(Merge<D, (PB > 0 ? PB : 1), (KW > 0 ? KW : 1)>) : size_t(0)));
   if constexpr (bytes > 64 * 1024) {  // (two blocks of 128-dim rows)
     static LdsLimit limit;
     const hipError_t e = limit.raise(reinterpret_cast<const void*>(&kv_attention_kernel<D, QB, PB, KW>), bytes);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((kv_attention_kernel<D, QB, PB, KW>), dim3(unsigned(p.prefix_wgs + p.own_wgs)), dim3(64 * KW), bytes,
+  hipLaunchKernelGGL((kv_attention_kernel<D, QB, PB, KW>), dim3(unsigned(p.prefix_wgs + p.own_wgs)), dim3(KW == kShared ? 256 : 64 * KW), bytes,
                      stream, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !p.parts) return e;
@@ -544,7 +610,7 @@ hipError_t launch(const AttnPlan& p, hipStream_t stream) {
 
 template <int D>
 hipError_t launch_walk(const AttnPlan& p, const Walk& own, const Walk& prefix, hipStream_t stream) {
-  if (own.waves == 1) return launch<D, 2, 0, 1>(p, stream);
+  if (own.waves == kShared) return launch<D, 2, 0, kShared>(p, stream);
   if (own.waves == 2) return launch<D, 2, 0, 2>(p, stream);
   if (own.blocks == 1) {
     if (prefix.blocks == 0) return launch<D, 1, 0, 4>(p, stream);

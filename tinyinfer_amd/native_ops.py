@@ -488,8 +488,8 @@ class NativeOps:
         """Host positions and lengths must stay inside the cache."""
         if slots is None or positions is None:
             raise ValueError("slots and positions are required")
-        if batch > 65535:
-            raise ValueError("batch must be at most 65535")
+        if batch > 65535 or rows > 1 << 28:
+            raise ValueError("batch must be at most 65535, rows at most 2^28")
         tensor = self.tensor_type
         if isinstance(positions, tensor) or isinstance(lengths, tensor):
             return
@@ -537,6 +537,8 @@ class NativeOps:
             raise ValueError(f"q must be [B, H, Q, {cache.head_dim}] with H a multiple of {cache.kv_heads}, got {list(q.shape)}")
         if batch > 65535 or heads > 65535:
             raise ValueError("batch and heads must each be at most 65535")
+        if batch * heads * nq > 1 << 23:
+            raise ValueError("at most 2^23 query rows (batch * heads * queries)")
         if type(causal) is not bool:
             raise ValueError("causal must be a bool")
         if slots is None or kv_lengths is None:
@@ -571,8 +573,8 @@ class NativeOps:
         wide = isinstance(logits, self.tensor_type) and logits.dtype == torch.float32
         call.operand(logits, torch.float32 if wide else torch.float16, "logits", rank=2)
         batch, vocab = logits.shape
-        if vocab > 1 << 18:
-            raise ValueError("logits: at most 262144 columns")
+        if vocab > 1 << 18 or batch > 1 << 20:
+            raise ValueError("logits: at most 2^20 rows of 2^18")
         call.scalars(int(wide))
         call.operand(uniforms, torch.float32, "uniforms", shape=(batch,))
         values = []
