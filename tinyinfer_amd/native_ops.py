@@ -252,7 +252,7 @@ class Int8KVCache:
     is the requested one rounded up to a multiple of 64.  The cache keeps no
     lengths: every call names the slots, positions and lengths it means."""
 
-    __slots__ = ("slots", "kv_heads", "capacity", "head_dim", "buffer", "_native", "_at")
+    __slots__ = ("slots", "kv_heads", "capacity", "head_dim", "buffer", "_native", "_at", "_workspace")
 
     def __init__(self, torch, slots, kv_heads, capacity, head_dim, device):
         self.slots, self.kv_heads, self.head_dim = slots, kv_heads, head_dim
@@ -263,6 +263,7 @@ class Int8KVCache:
         self._native = _KvI8(at, at + tokens * head_dim, at + 2 * tokens * head_dim,
                              at + 2 * tokens * head_dim + 4 * tokens, slots, kv_heads, self.capacity, head_dim)
         self._at = ctypes.addressof(self._native)
+        self._workspace = {}  # bytes an attention call needs, by its shape
 
     @property
     def device(self):
@@ -547,12 +548,15 @@ class NativeOps:
         y = call.output_like(q)
         call.per_request(batch, (slots, cache.slots - 1, "slots"), (kv_lengths, cache.capacity, "kv_lengths"),
                          (q_lengths, nq, "q_lengths"), (query_offsets, INT32_MAX - nq, "query_offsets"))
-        needed = self.lib.ti_amd_attention_i8kv_workspace(cache._at, batch, heads, nq, bound, prefix_length)
-        if needed > 0:
+        shape = (batch, heads, nq, bound, prefix_length)
+        needed = cache._workspace.get(shape)
+        if needed is None:
+            needed = cache._workspace[shape] = max(0, self.lib.ti_amd_attention_i8kv_workspace(cache._at, *shape))
+        if needed:
             call.output((needed,), torch.uint8)
         else:
             call.args.append(None)
-        call.scalars(max(needed, 0), batch, heads, nq, bound, int(causal), prefix_slot, prefix_length)
+        call.scalars(needed, batch, heads, nq, bound, int(causal), prefix_slot, prefix_length)
         call.run()
         return y
 
