@@ -6,9 +6,11 @@
 //       infinity or NaN (whose bytes are those of c = 0), so that what reads it
 //       answers NaN instead of a number the row does not stand for;
 //   c = the whole number nearest x / s, ties to even, |c| <= 127.
-// x / s is decided exactly: q = rint(x * rcp(s)) is at most one off, and x - q s
-// is an fp32 number (a multiple of s's last place, at most about s), so one fma
-// gives it without rounding and comparing it with s / 2 settles the last step.
+// The quotient is decided exactly: t = x * rcp(s) is off by less than 2^-15, so
+// rint(t) is right unless t lies that near half way between whole numbers; then q =
+// rint(t) is at most one off, and x - q s is an fp32 number (a multiple of s's last
+// place, at most about s), so one fma gives it without rounding and comparing it with
+// s / 2 settles the last step.
 //
 // Layout (T = capacity, a multiple of 64), made for the attention kernel's
 // matrix operands so that it loads 16 bytes per lane and moves nothing between
@@ -56,14 +58,34 @@ __device__ __forceinline__ RowScale row_scale(unsigned top) {
   return {s, __builtin_amdgcn_rcpf(s)};
 }
 
-__device__ __forceinline__ unsigned quantise(uint16_t bits, RowScale r) {
-  const float x = r.inv == 0.f ? 0.f : h2f(bits);
+__device__ __forceinline__ float nearest(float x, RowScale r) {
   float q = rintf(x * r.inv);
   const float rest = 2.f * fmaf(-q, r.s, x);
   const bool odd = int(q) & 1;
   if (rest > r.s || (rest == r.s && odd)) q += 1.f;
   else if (rest < -r.s || (rest == -r.s && odd)) q -= 1.f;
-  return unsigned(int(q) + 128);
+  return q;
+}
+// The bytes of 8 values.
+__device__ __forceinline__ uint64_t quantise(u16x8_t bits, RowScale r) {
+  float q[8], close = 1.f;  // close: the least distance from half way
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float t = h2f(bits[e]) * r.inv;
+    q[e] = rintf(t);
+    close = fminf(close, fabsf(fabsf(t - q[e]) - 0.5f));
+  }
+  if (r.inv == 0.f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = 0.f;
+  } else if (close < 0x1p-14f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = nearest(h2f(bits[e]), r);
+  }
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e >> 2] = __builtin_amdgcn_cvt_pk_u8_f32(q[e] + 128.f, e & 3, w[e >> 2]);
+  return uint64_t(w[1]) << 32 | w[0];
 }
 
 // Offsets of (token, dim) from the start of a slot's head.
@@ -115,13 +137,10 @@ __global__ __launch_bounds__(64) void append_rows_kernel(KvAppendArgs a) {
   if (!live) return;
   const RowScale kr = row_scale(ktop), vr = row_scale(vtop);
   const int64_t at = (int64_t(slot) * a.cache.kv_heads + head) * a.cache.capacity;
-  uint64_t kq = 0;
+  const uint64_t kq = quantise(k, kr), vq = quantise(v, vr);
   uint8_t* vd = a.cache.v + at * D;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    kq |= uint64_t(quantise(k[e], kr)) << (8 * e);
-    vd[v_byte(t, 8 * seg + e, D)] = uint8_t(quantise(v[e], vr));
-  }
+  for (int e = 0; e < 8; ++e) vd[v_byte(t, 8 * seg + e, D)] = uint8_t(vq >> (8 * e));
   *reinterpret_cast<uint64_t*>(a.cache.k + at * D + k_byte(t, 8 * seg, D)) = kq;
   if (seg == 0) {
     a.cache.k_scales[at + t] = kr.s;
@@ -155,17 +174,12 @@ __global__ __launch_bounds__(256) void append_block_kernel(KvAppendArgs a) {
     const int64_t src = ((int64_t(b) * a.cache.kv_heads + head) * a.rows + min(max(i, int64_t(0)), int64_t(n - 1))) * D + 8 * seg;
     const u16x8_t k = load_row8(a.k + src), v = load_row8(a.v + src);
     const RowScale kr = row_scale(row_top<LPR>(k)), vr = row_scale(row_top<LPR>(v));
-    uint32_t kq[2] = {0, 0}, vq[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      kq[e >> 2] |= quantise(k[e], kr) << (8 * (e & 3));
-      vq[e >> 2] |= quantise(v[e], vr) << (8 * (e & 3));
-    }
-    *reinterpret_cast<uint32_t*>(&vt[r][8 * seg]) = vq[0];
-    *reinterpret_cast<uint32_t*>(&vt[r][8 * seg + 4]) = vq[1];
+    const uint64_t kq = quantise(k, kr), vq = quantise(v, vr);
+    *reinterpret_cast<uint32_t*>(&vt[r][8 * seg]) = uint32_t(vq);
+    *reinterpret_cast<uint32_t*>(&vt[r][8 * seg + 4]) = uint32_t(vq >> 32);
     if (seg == 0) lives[r] = live;
     if (live) {
-      *reinterpret_cast<uint64_t*>(a.cache.k + at * D + k_byte(t, 8 * seg, D)) = uint64_t(kq[1]) << 32 | kq[0];
+      *reinterpret_cast<uint64_t*>(a.cache.k + at * D + k_byte(t, 8 * seg, D)) = kq;
       if (seg == 0) {
         a.cache.k_scales[at + t] = kr.s;
         a.cache.v_scales[at + t] = vr.s;
