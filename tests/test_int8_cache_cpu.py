@@ -42,6 +42,16 @@ def test_cache_layout(cache):
     assert all(x % 16 == 0 for x in (n.k, n.v, n.k_scales, n.v_scales))
 
 
+def test_cache_cannot_be_changed_or_copied(cache):
+    """Its native descriptor holds the buffer's address."""
+    import copy
+    for name in ("buffer", "capacity", "slots", "other"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, 1)
+    with pytest.raises((TypeError, ValueError, AttributeError)):
+        copy.deepcopy(cache)
+
+
 @pytest.mark.parametrize("args", [
     ([0, 3], 0, 4, 4), ([0, -1], 0, 4, 4), (0, 126, 4, 4), ([0, 1], [0, 1, 2], 4, 4), (0, 0, 5, 4), (0, 0, -1, 4), (0, 0, 4, 0),
     (0, 0, 4, 4.0), (None, 0, 4, 4), (0, None, 4, 4), ([0, 1], [0], 4, 4), (0, 128, 0, 4), (0.5, 0, 4, 4)])

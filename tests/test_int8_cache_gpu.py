@@ -324,6 +324,126 @@ def test_attention_masks_that_leave_rows_empty(ops, heads, kv_heads, dim, nq):
     check(got, q, case, range(6), ends_of([2] * 6, nq))
 
 
+def some_of(got, q, case, slots, ends, rng, count, prefix=None):
+    """check() for `count` of the (request, head) pairs; all are finite."""
+    batch, heads = q.shape[:2]
+    assert np.isfinite(host(got)).all()
+    group = heads // case.kv_heads
+    for _ in range(count):
+        b, h = int(rng.integers(batch)), int(rng.integers(heads))
+        one = Case.__new__(Case)
+        one.kv_heads, one.dim, g = 1, case.dim, h // group
+        one.hk, one.hv = case.hk[:, g:g + 1], case.hv[:, g:g + 1]
+        check(got[b:b + 1, h:h + 1], q[b:b + 1, h:h + 1], one, [slots[b]], [ends[b]], prefix)
+
+
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,nq,kv", [
+    (48, 16, 16, 64, 128, 140),     # shared tiles
+    (40, 32, 8, 128, 81, 200),      # shared tiles, groups of rows that end inside one, 128 dims
+    (3, 25, 25, 64, 450, 450),      # two waves to a block of 32 rows
+    (6, 8, 8, 64, 700, 2100),       # four waves, long
+    (4, 16, 16, 128, 300, 310),     # four waves, 128 dims
+    (1, 8, 2, 64, 16, 8300),        # few rows, many keys: two blocks, split
+])
+def test_attention_plans(ops, batch, heads, kv_heads, dim, nq, kv):
+    """Shapes of every way the rows are walked, with ragged lengths, queries and offsets."""
+    say("plan", batch, heads, kv_heads, dim, nq, kv)
+    rng = np.random.default_rng(batch + nq)
+    lengths = [int(x) for x in rng.integers(0, kv + 1, batch)]
+    lengths[0], lengths[-1] = kv, kv - 1
+    case = Case(ops, rng, batch, kv_heads, dim, [kv])
+    q = (rng.standard_normal((batch, heads, nq, dim)) * 2).astype(np.float16)
+    slots = rng.permutation(batch)
+    got = ops.attention_int8kv(dev(q), case.cache, i32(slots), i32(lengths))
+    some_of(got, q, case, slots, ends_of(lengths, nq), rng, 12)
+    q_lengths = [int(x) for x in rng.integers(0, nq + 1, batch)]
+    offsets = [int(x) for x in rng.integers(-nq // 2, kv, batch)]
+    for causal in (True, False):
+        got = ops.attention_int8kv(dev(q), case.cache, i32(slots), i32(lengths), q_lengths=i32(q_lengths),
+                                   query_offsets=i32(offsets), causal=causal)
+        some_of(got, q, case, slots, ends_of(lengths, nq, q_lengths, offsets, causal), rng, 8)
+    # A row whose token is not finite reaches only those who see it.
+    bad = np.full((1, kv_heads, 1, dim), np.nan, np.float16)
+    ops.kv_append_int8(case.cache, dev(bad), dev(bad), int(slots[0]), kv - 2)
+    got = host(ops.attention_int8kv(dev(q), case.cache, i32(slots), i32(lengths)))
+    sees = np.asarray(ends_of(lengths, nq)[0]) > kv - 2
+    assert sees.any() and np.isnan(got[0, :, sees]).all() and np.isfinite(got[0, :, ~sees]).all() and np.isfinite(got[1:]).all()
+
+
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,nq,prefix,kv", [
+    (64, 16, 2, 64, 1, 8200, 40), (30, 24, 8, 128, 1, 700, 100), (2, 8, 8, 64, 40, 300, 8300), (3, 40, 40, 64, 300, 8200, 310)])
+def test_shared_prefix_plans(ops, batch, heads, kv_heads, dim, nq, prefix, kv):
+    say("prefix plan", batch, heads, kv_heads, dim, nq, prefix, kv)
+    rng = np.random.default_rng(batch + prefix)
+    lengths = [int(x) for x in rng.integers(0, kv + 1, batch)]
+    case = Case(ops, rng, batch + 1, kv_heads, dim, [kv], capacity=max(prefix, kv))
+    q = (rng.standard_normal((batch, heads, nq, dim)) * 2).astype(np.float16)
+    order = rng.permutation(batch + 1)
+    got = ops.attention_shared_prefix(dev(q), case.cache, int(order[-1]), prefix, i32(order[:-1]), i32(lengths),
+                                      max_kv_length=kv)
+    some_of(got, q, case, order[:-1], ends_of(lengths, nq), rng, 10, prefix=(int(order[-1]), prefix))
+
+
+def test_split_calls_on_two_streams_at_once(ops):
+    """Each call has its own workspace."""
+    say("two streams")
+    t = torch()
+    rng = np.random.default_rng(21)
+    case = Case(ops, rng, 2, 2, 128, [6000])
+    qs = [dev(rng.standard_normal((2, 8, 1, 128)).astype(np.float16)) for _ in range(2)]
+    lens, slots = i32([6000, 4321]), i32([0, 1])
+    want = [host(ops.attention_int8kv(q, case.cache, slots, lens)) for q in qs]
+    t.cuda.synchronize()
+    streams = [t.cuda.Stream(), t.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for i in (0, 1):
+            with t.cuda.stream(streams[i]):
+                got[i].append(ops.attention_int8kv(qs[i], case.cache, slots, lens))
+    t.cuda.synchronize()
+    for i in (0, 1):
+        for y in got[i]:
+            assert np.array_equal(bits(host(y)), bits(want[i]))
+
+
+def test_first_calls_of_a_process_can_be_captured():
+    """In a fresh process: the first calls ever, among them kernels with more than 64 KiB of
+    LDS, inside a capture."""
+    import subprocess
+    import sys
+    say("first calls captured")
+    script = """
+import torch
+from tinyinfer_amd.native_ops import NativeOps
+ops = NativeOps()
+cache = ops.kv_cache_int8(2, 2, 256, 128)
+i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+torch.manual_seed(0)
+k, v = torch.randn(2, 2, 200, 128, device="cuda").half(), torch.randn(2, 2, 200, 128, device="cuda").half()
+q, x = torch.randn(2, 4, 200, 128, device="cuda").half(), torch.randn(2, 5000, device="cuda")
+u, slots, zero, n = torch.rand(2, device="cuda"), i(0, 1), i(0, 0), i(200, 150)
+def step():
+    ops.kv_append_int8(cache, k, v, slots, zero, lengths=n)
+    return (ops.attention_int8kv(q, cache, slots, n), ops.attention_shared_prefix(q, cache, 0, 180, slots, n),
+            *ops.kv_read_int8(cache, slots, zero, n, 200), *ops.sample(x, u, top_p=0.9), *ops.sample(x, u, top_k=50))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = step()
+for turn in range(3):
+    k.normal_(); q.normal_(); u.uniform_()
+    graph.replay()
+    torch.cuda.synchronize()
+    got = [y.clone() for y in out]
+    for a, b in zip(got, step()):
+        assert torch.equal(a, b)
+print("captured")
+"""
+    from tests.conftest import ROOT
+    done = subprocess.run([sys.executable, "-c", script], cwd=ROOT, capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
 def test_attention_metadata_outside_the_cache(ops):
     """A slot outside the cache has no keys, lengths are clamped to the capacity and to zero."""
     say("metadata outside")

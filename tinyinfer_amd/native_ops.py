@@ -255,15 +255,20 @@ class Int8KVCache:
     __slots__ = ("slots", "kv_heads", "capacity", "head_dim", "buffer", "_native", "_at", "_workspace")
 
     def __init__(self, torch, slots, kv_heads, capacity, head_dim, device):
-        self.slots, self.kv_heads, self.head_dim = slots, kv_heads, head_dim
-        self.capacity = (capacity + 63) // 64 * 64
-        tokens = slots * kv_heads * self.capacity
-        self.buffer = torch.zeros(tokens * (2 * head_dim + 8), dtype=torch.uint8, device=device)
-        at = self.buffer.data_ptr()
-        self._native = _KvI8(at, at + tokens * head_dim, at + 2 * tokens * head_dim,
-                             at + 2 * tokens * head_dim + 4 * tokens, slots, kv_heads, self.capacity, head_dim)
-        self._at = ctypes.addressof(self._native)
-        self._workspace = {}  # bytes an attention call needs, by its shape
+        capacity = (capacity + 63) // 64 * 64
+        tokens = slots * kv_heads * capacity
+        buffer = torch.zeros(tokens * (2 * head_dim + 8), dtype=torch.uint8, device=device)
+        at = buffer.data_ptr()
+        native = _KvI8(at, at + tokens * head_dim, at + 2 * tokens * head_dim, at + 2 * tokens * head_dim + 4 * tokens,
+                       slots, kv_heads, capacity, head_dim)
+        # _workspace: bytes an attention call needs, by its shape.
+        for name, value in (("slots", slots), ("kv_heads", kv_heads), ("capacity", capacity), ("head_dim", head_dim),
+                            ("buffer", buffer), ("_native", native), ("_at", ctypes.addressof(native)),
+                            ("_workspace", {})):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"{name}: a cache's buffer and extents stay as they were made")
 
     @property
     def device(self):
