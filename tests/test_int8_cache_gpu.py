@@ -205,6 +205,31 @@ def test_the_later_of_two_requests_stays(ops, rows):
     same(host(gv), want)
 
 
+@pytest.mark.parametrize("dim,heads", [(64, 3), (128, 2)])
+@pytest.mark.parametrize("rows", [9, 31, 32, 33, 65, 128])
+def test_rows_on_both_sides_of_the_append_rule(ops, dim, heads, rows):
+    """Ragged requests that share slots and cross blocks of 64 tokens, in an order that says
+    which row stays; what no request writes stays as it was."""
+    say("append rule", dim, heads, rows)
+    rng = np.random.default_rng(dim + rows)
+    cache = ops.kv_cache_int8(4, heads, 192, dim)
+    base = random_rows(rng, 4, heads, 192, dim)
+    ops.kv_append_int8(cache, dev(base), dev(base[..., ::-1]), [0, 1, 2, 3], 0)
+    want_k, want_v = held(base)[1], held(base[..., ::-1])[1]
+    slots = np.array([0, 1, 1, 3, 1, 0], np.int32)
+    pos = np.array([0, 5, 33, 192 - rows, 63, 64], np.int32)
+    lens = np.array([rows, rows, max(rows - 7, 1), rows, 1, 0], np.int32)
+    k, v = random_rows(rng, 6, heads, rows, dim), random_rows(rng, 6, heads, rows, dim)
+    ops.kv_append_int8(cache, dev(k), dev(v), dev(slots), dev(pos), lengths=dev(lens))
+    for b in range(6):
+        n = min(lens[b], 192 - pos[b])
+        want_k[slots[b], :, pos[b]:pos[b] + n] = held(k)[1][b, :, :n]
+        want_v[slots[b], :, pos[b]:pos[b] + n] = held(v)[1][b, :, :n]
+    gk, gv = ops.kv_read_int8(cache, [0, 1, 2, 3], 0, 192, 192)
+    same(host(gk), want_k)
+    same(host(gv), want_v)
+
+
 # ---------------------------------------------------------------- attention
 def reference(q, keys, values, ends):
     """float64 outputs and their tolerance: rows q [R, D] over keys, values [N, D]
