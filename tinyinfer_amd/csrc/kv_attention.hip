@@ -20,13 +20,25 @@
 // straight from memory into registers, 16 bytes per lane, and nothing moves
 // between lanes or through LDS but the running maximum, when it rises.
 //
-// A workgroup's 4 waves take every fourth tile of 64 keys of one row block and
-// merge their states (m, l, O) through LDS.  With few row blocks the keys are cut
-// into splits as well, each split's state goes to the caller's workspace and a
-// second kernel joins them.  A prefix is one such set of splits, its row blocks
-// running over the whole batch: its keys are read once for all requests.
+// Waves (walk_for has the rules and both sides' times).  Two or four waves share a row
+// block: each takes every second or fourth tile of 64 keys, and their states (m, l, O)
+// merge through LDS.  Where row blocks are plenty four waves have one each and share the
+// tiles instead: each widens a quarter of the next one into LDS (operand by operand, a
+// conflict-free kilobyte) while all work on this one, two buffers and one barrier a tile.
+// With few row blocks the keys are cut into splits as well, each split's state goes to the
+// caller's workspace and a second kernel joins them.  A prefix is one such set of splits,
+// its row blocks running over the whole batch: its keys are read once for all requests.
+//
+// What bounds it.  Single tokens: memory where caches are long (16 requests of 8 x 128,
+// 12000 to 32768 keys: 138 us, 5.8 TB/s; the loads are the plain ones of a stream,
+// past the caches), launch and one tile's chain of latencies where they are short (one
+// request of 12 heads, 300 keys: 5.7 us).  Prompts: vector instructions beside the matrix
+// products.  Of a tile of 64 keys x 32 rows at D 128 the 64 matrix instructions are 1024
+// cycles of a SIMD; widening K and V is 192 vector instructions and a score takes 6 and an
+// exponential, 1900 cycles together.  2 requests of 777 queries, 32 heads over 8 of 128,
+// 4500 to 6001 keys: 200 us, 670 TFLOP/s; 4 prompts of 1024, 25 heads of 64: 30 us, 445
+// TFLOP/s, its scores' exponentials and scales more than the products.
 #include <algorithm>
-#include <type_traits>
 
 #include "common.hpp"
 #include "kernels.hpp"
@@ -80,6 +92,13 @@ __device__ __forceinline__ half8_t widen8(uint32_t w0, uint32_t w1) {
   widen4(w0, a, b);
   widen4(w1, c, d);
   return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// The same bytes as the whole numbers c + 1152: half the work.
+__device__ __forceinline__ half8_t raise8(uint32_t w0, uint32_t w1) {
+  const u32x4_t r = {__builtin_amdgcn_perm(0x64646464u, w0, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, w0, 0x04030402u),
+                     __builtin_amdgcn_perm(0x64646464u, w1, 0x04010400u), __builtin_amdgcn_perm(0x64646464u, w1, 0x04030402u)};
+  return __builtin_bit_cast(half8_t, r);
 }
 
 // x times the value that lane N of this lane's row of 16 holds (the broadcast is an
@@ -191,6 +210,10 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
   // so the result is as near as fp32 weights would bring it.  Two blocks (prompts) take
   // the rounded weights alone: a third less matrix work, 1.3 times the error.
   constexpr bool NT = !PREFIX && QB == 1, FINE = QB == 1;
+  // Two blocks whose waves widen every tile themselves are bound by that, so K stays at
+  // c + 1152 and q . c is summed from -1152 sum_d q_d on: sums of up to 1152 / 127 times the
+  // terms of q . c, which are fp32 sums still (their last place 2^-20 of q . c's terms).
+  constexpr bool RAISED = QB == 2 && KW != kShared;
   u32x4_t kr[KW == kShared ? 1 : 4][D / 64], vr[KW == kShared ? D / 64 : D / 16];
   float ksr = 0.f, vsr = 0.f;
   auto& shared = *reinterpret_cast<Tiles<D>*>(lds);
@@ -241,6 +264,18 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
       }
   }
 
+  float4_t from[QB];  // where the sums of S start
+#pragma unroll
+  for (int u = 0; u < QB; ++u) {
+    from[u] = float4_t{0.f, 0.f, 0.f, 0.f};
+    if constexpr (RAISED) {
+      const f16 o = f16(-1152.f);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+        from[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(half8_t{o, o, o, o, o, o, o, o}, qf[u][i], from[u], 0, 0, 0);
+    }
+  }
+
   float m[QB], l[QB];
   float4_t acc[QB][D / 16];
 #pragma unroll
@@ -260,12 +295,15 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
 #pragma unroll
-      for (int u = 0; u < QB; ++u) sc[u][kb] = float4_t{0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < QB; ++u) sc[u][kb] = from[u];
 #pragma unroll
       for (int c = 0; c < D / 64; ++c)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const half8_t kf = KW == kShared ? shared.k[buf][kb][2 * c + s][lane] : widen8(kr[KW == kShared ? 0 : kb][c][2 * s], kr[KW == kShared ? 0 : kb][c][2 * s + 1]);
+          const u32x4_t w = kr[KW == kShared ? 0 : kb][c];
+          const half8_t kf = KW == kShared ? shared.k[buf][kb][2 * c + s][lane]
+                             : RAISED      ? raise8(w[2 * s], w[2 * s + 1])
+                                           : widen8(w[2 * s], w[2 * s + 1]);
 #pragma unroll
           for (int u = 0; u < QB; ++u)
             sc[u][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[u][2 * c + s], sc[u][kb], 0, 0, 0);
@@ -457,7 +495,8 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
   }
 }
 
-// Waves per SIMD that the registers are budgeted for.
+// Waves per SIMD that the registers are budgeted for: the most that spills nothing (103,
+// 164, 153 and 228 registers are used of 128, 168, 168 and 256).
 constexpr int waves_for(int dim, int qb) { return dim == 64 ? (qb == 1 ? 4 : 3) : (qb == 1 ? 3 : 2); }
 
 // QB, PB: row blocks of 16 per wave over the requests' own keys and the prefix's (0:
@@ -483,7 +522,9 @@ __global__ __launch_bounds__(KW == kShared ? 256 : 64 * KW, waves_for(D, QB > PB
   attend<D, QB, KW, false>(p, lds, b, at - b * heads, blocks - 1 - (block - split * blocks), split, p.splits, split);
 }
 
-// One wave per row joins its splits' states.
+// One wave per row joins its splits' states: D / 4 lanes a state, 2 or 4 states at a time.
+// 3.2 us for 384 rows of 3 states of 64, 4.2 for 512 rows of 4 and 4.3 for 2048 rows of 5
+// of 128: a launch and its dependent loads.
 template <int D>
 __global__ __launch_bounds__(256) void kv_attention_join_kernel(AttnPlan p) {
   constexpr int LPR = D / 4, PARTS = 64 / LPR;
@@ -539,12 +580,13 @@ struct Walk {
 // 38.4 us against 44.7; 64 pairs of 333 rows, D 128: 37 against 53; 12 pairs of 1024:
 // 12.2 against 11.1) or many keys to a row block (64 queries of 4 heads over 16000 keys,
 // D 128: 40 against 50 us).
-// Waves: with row blocks to fill every SIMD three times a workgroup takes four of them
-// and its waves share the tiles, each widened once instead of four times and nothing
-// merged (100 pairs of 1024 rows: 34.5 us, 39 with a wave to a row block of its own, 47
-// with four waves to one; 32 pairs of 4096 rows, D 128: 176, 191 and 213 us); below that
+// Waves: with row blocks to fill every SIMD twice a workgroup takes four of them and its
+// waves share the tiles, each widened once instead of four times and nothing merged (100
+// pairs of 1024 rows: 31.3 us, 35.7 with two waves to a row block, 44 with four; 75 pairs:
+// 29.8, 32.6, 39.8; 8 pairs of 8192 rows over 8000 keys, D 128: 278, 301, 298); below that
 // two waves share a row block, or four where keys are many (12 pairs of 4096 rows: 56 us,
-// 66 with two, 87 with shared tiles).
+// 66 with two, 87 with shared tiles; 24 pairs of 2048 rows without a mask: 52, 50, 61; 16
+// pairs of 3108 rows over 6001 keys, D 128: 205, 224, 212).
 // Splits: a second launch and the states' traffic cost 2 us and more, so short caches
 // are not split (96 pairs, 1024 keys: 8.8 us, 9.4 in four), longer ones into about
 // 384 or, from 4096 keys on, 512 workgroups (8 pairs of 4096 keys, D 128: 31 us whole,
@@ -554,7 +596,7 @@ Walk walk_for(int64_t pairs, int rows, int keys, int dim) {
   Walk w{1, 4, 1};
   if (rows > 16 && (twos >= plenty || tiles >= 128)) w.blocks = 2;
   if (w.blocks == 2 && twos >= plenty) {
-    w.waves = twos >= 3072 ? kShared : twos >= 1024 && tiles < 32 ? 2 : 4;
+    w.waves = twos >= 2048 ? kShared : twos >= 1024 && tiles < 32 ? 2 : 4;
     return w;
   }
   const int64_t wgs = pairs * ceil_div(rows, 16 * w.blocks);
