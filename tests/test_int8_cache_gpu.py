@@ -409,6 +409,38 @@ def test_shared_prefix_plans(ops, batch, heads, kv_heads, dim, nq, prefix, kv):
     some_of(got, q, case, order[:-1], ends_of(lengths, nq), rng, 10, prefix=(int(order[-1]), prefix))
 
 
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,nq,kv,mean", [
+    (3, 25, 25, 64, 440, 440, 30.0),    # two waves to a block of 32 rows
+    (4, 16, 16, 128, 520, 530, 30.0),   # the same, 128 dims
+    (1, 4, 2, 128, 9, 8300, 30.0),      # four waves, split
+    (40, 16, 16, 64, 120, 130, 30.0),   # shared tiles
+    (2, 3, 3, 128, 1, 200, 30.0),       # single tokens
+])
+def test_attention_queries_of_one_sign(ops, batch, heads, kv_heads, dim, nq, kv, mean):
+    """Queries whose dims share a sign, where sums that start at -1152 sum q run furthest from
+    q . c: one rounding per 8 dims of terms up to 1280 sum |q| adds to d of the tolerance
+      2 (D / 8) 2^-24 1280 / 127 max|K| sum |q| / sqrt(D)."""
+    say("one sign", batch, heads, kv_heads, dim, nq, kv)
+    rng = np.random.default_rng(batch + kv)
+    case = Case(ops, rng, batch, kv_heads, dim, [kv])
+    q = ((rng.standard_normal((batch, heads, nq, dim)) + mean) / (8 * mean)).astype(np.float16)
+    got = host(ops.attention_int8kv(dev(q), case.cache, list(range(batch)), [kv] * batch)).astype(np.float64)
+    ends = np.asarray(ends_of([kv], nq)[0])
+    for _ in range(10):
+        b, h = int(rng.integers(batch)), int(rng.integers(heads))
+        rows = rng.choice(nq, min(nq, 20), replace=False)
+        keys, values = case.hk[b, h * kv_heads // heads], case.hv[b, h * kv_heads // heads]
+        x = q[b, h, rows].astype(np.float64)
+        want, tol = reference(x, keys, values, ends[rows])
+        more = 2 * dim / 8 * 2.0 ** -24 * 1280 / 127 * np.abs(keys).max() * np.abs(x).sum(-1, keepdims=True) / math.sqrt(dim)
+        for i, end in enumerate(ends[rows]):
+            s = keys[:end] @ x[i] / math.sqrt(dim)
+            p = np.exp(s - s.max())
+            tol[i] += 1.02 * more[i] * (p @ np.abs(values[:end]) / p.sum())
+        err = np.abs(got[b, h, rows] - want)
+        assert (err <= tol).all(), f"b {b} h {h}: {(err / tol).max():.3g} of the tolerance"
+
+
 def test_split_calls_on_two_streams_at_once(ops):
     """Each call has its own workspace."""
     say("two streams")
