@@ -198,18 +198,24 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
   int t = split * per + (KW == kShared ? 0 : wave);
 
   const int64_t base = (int64_t(slot) * a.cache.kv_heads + head) * a.cache.capacity;
-  const uint8_t* kp = a.cache.k + base * D + j * 64 + 16 * g;
-  const uint8_t* vp = a.cache.v + base * D + lane * 16;
+  const uint8_t* kp = a.cache.k + base * D;
+  const uint8_t* vp = a.cache.v + base * D;
+  const uint32_t k_lane = j * 64 + 16 * g, v_lane = lane * 16;
   // Lane (j, g) holds the scales of the tile's key 16 (j / 4) + 4 g + j % 4: of row g's
   // 16 scores of a tile, number 4 kb + v in order, lane 4 kb + v has the scale.
   const int my_key = 16 * (j >> 2) + 4 * g + (j & 3);
-  const float* ksp = a.cache.k_scales + base + my_key;
-  const float* vsp = a.cache.v_scales + base + my_key;
+  const float* ksp = a.cache.k_scales + base;
+  const float* vsp = a.cache.v_scales + base;
   // One block of rows (single tokens): memory has no use for the keys again, and a second
   // product with what the weights' rounding to fp16 leaves out costs nothing that shows,
   // so the result is as near as fp32 weights would bring it.  Two blocks (prompts) take
   // the rounded weights alone: a third less matrix work, 1.3 times the error.
   constexpr bool NT = !PREFIX && QB == 1, FINE = QB == 1;
+  // The next tile's K and scales are loaded once the scores have used this one's (one token
+  // of 12 heads, 1000 keys: 8.0 us, 9.3 without; 32 of them 11.2 and 12.7), but for two
+  // blocks of 64 dims, whose third wave per SIMD that would cost (12 pairs of 4096 rows:
+  // 62 us, 57 without).
+  constexpr bool AHEAD = QB == 1 || D == 128;
   // Two blocks whose waves widen every tile themselves are bound by that, so K stays at
   // c + 1152 and q . c is summed from -1152 sum_d q_d on: sums of up to 1152 / 127 times the
   // terms of q . c, which are fp32 sums still (their last place 2^-20 of q . c's terms).
@@ -224,16 +230,16 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
 #pragma unroll
     for (int kb = 0; kb < (KW == kShared ? 1 : 4); ++kb)
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) kr[kb][c] = load16<NT>(at + 16 * kb * D + 1024 * c);
+      for (int c = 0; c < D / 64; ++c) kr[kb][c] = load16<NT>(at + 16 * kb * D + 1024 * c + k_lane);
   };
   auto load_v = [&](int tt) {
     const uint8_t* at = vp + int64_t(tt) * (kTile * D) + (KW == kShared ? 1024 * wave * (D / 64) : 0);
 #pragma unroll
-    for (int d = 0; d < (KW == kShared ? D / 64 : D / 16); ++d) vr[d] = load16<NT>(at + 1024 * d);
+    for (int d = 0; d < (KW == kShared ? D / 64 : D / 16); ++d) vr[d] = load16<NT>(at + 1024 * d + v_lane);
   };
   auto load_scales = [&](int tt) {
-    ksr = ksp[int64_t(tt) * kTile];
-    vsr = vsp[int64_t(tt) * kTile];
+    ksr = (ksp + int64_t(tt) * kTile)[uint32_t(my_key)];
+    vsr = (vsp + int64_t(tt) * kTile)[uint32_t(my_key)];
   };
   auto share = [&](int buf) {
 #pragma unroll
@@ -289,7 +295,7 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
   // the weight p * vs / unit that is rounded to fp16 is then at most p.
   float unit = 0.f, inv_unit = 1.f;
 
-  const auto tile = [&](int t, int buf, float ks, float vs_) {
+  const auto tile = [&](int t, int buf, float ks, float vs_, auto after_scores) {
     const bool full = (t + 1) * kTile <= first;
     float4_t sc[QB][4];
 #pragma unroll
@@ -310,6 +316,7 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
         }
       if constexpr (KW != kShared) __builtin_amdgcn_sched_barrier(0);  // (widen one block of 16 keys at a time)
     }
+    after_scores();
     const float ck = ks * p.scale;
     // (Past the last key any row sees, scales may be anything.)
     const float vs = t * kTile + my_key < last ? vs_ : 0.f;
@@ -407,14 +414,30 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
           load_v(t + 2);
         }
       }
-      if (t * kTile < last) tile(t, buf, ks, vs);
+      if (t * kTile < last) tile(t, buf, ks, vs, [] {});
     }
   } else {
-    for (; t < t_end; t += KW) {
+    if (AHEAD && t < t_end) {
       load_k(t);
       load_scales(t);
+    }
+    for (; t < t_end; t += KW) {
+      if (!AHEAD) {
+        load_k(t);
+        load_scales(t);
+      }
+      const float ks = ksr, vs = vsr;
       load_v(t);
-      tile(t, 0, ksr, vsr);
+      __builtin_amdgcn_sched_barrier(0);
+      tile(t, 0, ks, vs, [&] {
+        if constexpr (AHEAD) {
+          if (t + KW < t_end) {
+            load_k(t + KW);
+            load_scales(t + KW);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      });
     }
   }
 
@@ -497,7 +520,7 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
 
 // Waves per SIMD that the registers are budgeted for: the most that spills nothing (103,
 // 164, 153 and 228 registers are used of 128, 168, 168 and 256).
-constexpr int waves_for(int dim, int qb) { return dim == 64 ? (qb == 1 ? 4 : 3) : (qb == 1 ? 3 : 2); }
+constexpr int waves_for(int dim, int qb) { return dim == 64 ? (qb == 1 ? 4 : 2) : (qb == 1 ? 2 : 2); }
 
 // QB, PB: row blocks of 16 per wave over the requests' own keys and the prefix's (0:
 // no prefix); KW: waves that share a row block's keys.
@@ -522,15 +545,18 @@ __global__ __launch_bounds__(KW == kShared ? 256 : 64 * KW, waves_for(D, QB > PB
   attend<D, QB, KW, false>(p, lds, b, at - b * heads, blocks - 1 - (block - split * blocks), split, p.splits, split);
 }
 
-// One wave per row joins its splits' states: D / 4 lanes a state, 2 or 4 states at a time.
-// 3.2 us for 384 rows of 3 states of 64, 4.2 for 512 rows of 4 and 4.3 for 2048 rows of 5
-// of 128: a launch and its dependent loads.
-template <int D>
+// W waves of a workgroup of 4 join a row's states: D / 4 lanes a state, 2 or 4 states at a
+// time and wave.  A launch and its dependent loads: 3.2 us for 384 rows of 3 states of 64,
+// 4.2 for 512 rows of 4 and 4.3 for 2048 rows of 5 of 128.  Four waves from 17 states on:
+// one token of 12 heads over 9000 keys in 36 splits takes 11.2 us, 13.3 with one wave.
+template <int D, int W>
 __global__ __launch_bounds__(256) void kv_attention_join_kernel(AttnPlan p) {
   constexpr int LPR = D / 4, PARTS = 64 / LPR;
-  const int lane = int(threadIdx.x & 63), part = lane / LPR, at = 4 * (lane % LPR);
-  const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (row >= p.all_rows) return;
+  __shared__ float4_t sums[W][LPR];
+  __shared__ float weights[W];
+  const int lane = int(threadIdx.x & 63), wave = int(threadIdx.x >> 6) % W, part = lane / LPR, at = 4 * (lane % LPR);
+  const int64_t row = int64_t(blockIdx.x) * (4 / W) + int(threadIdx.x >> 6) / W;
+  if (row >= p.all_rows) return;  // (a workgroup of one row has it)
   const int states = p.splits + p.prefix_splits;
   const float* ml = p.a.workspace + int64_t(states) * p.all_rows * D;
   float top = kNegInf;
@@ -542,21 +568,31 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(AttnPlan p) {
   float total = 0.f;
   float4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = part; s < states; s += PARTS) {
+  for (int s = wave * PARTS + part; s < states; s += W * PARTS) {
     const float* x = ml + 2 * (s * p.all_rows + row);
-    const float lw = x[1];
-    if (lw == 0.f) continue;
-    const float f = __builtin_amdgcn_exp2f(x[0] - top);
+    const float lw = x[1], f = lw == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[0] - top);
+    // (A state without weight was not written.)
     const float4_t y = *reinterpret_cast<const float4_t*>(p.a.workspace + (s * p.all_rows + row) * D + at);
     total = fmaf(lw, f, total);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = fmaf(y[e], f, o[e]);
+    for (int e = 0; e < 4; ++e) o[e] = lw == 0.f ? o[e] : fmaf(y[e], f, o[e]);
   }
 #pragma unroll
   for (int x = LPR; x < 64; x <<= 1) {
     total += __shfl_xor(total, x, 64);
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], x, 64);
+  }
+  if constexpr (W > 1) {
+    if (part == 0) sums[wave][lane % LPR] = o;
+    if (lane == 0) weights[wave] = total;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      total += weights[w];
+      o += sums[w][lane % LPR];
+    }
   }
   if (part != 0) return;
   const float inv = total == 0.f ? 0.f : 1.f / total;
@@ -588,9 +624,11 @@ struct Walk {
 // 66 with two, 87 with shared tiles; 24 pairs of 2048 rows without a mask: 52, 50, 61; 16
 // pairs of 3108 rows over 6001 keys, D 128: 205, 224, 212).
 // Splits: a second launch and the states' traffic cost 2 us and more, so short caches
-// are not split (96 pairs, 1024 keys: 8.8 us, 9.4 in four), longer ones into about
-// 384 or, from 4096 keys on, 512 workgroups (8 pairs of 4096 keys, D 128: 31 us whole,
-// 10.6 in 16; 128 pairs of 32768: 253 us whole, 136 in 4).
+// are not split (96 pairs, 1024 keys: 8.8 us, 9.4 in four).  Longer ones are, into at most
+// one workgroup a CU (8 pairs of 16000 keys, D 128: 13.3 us in 256 workgroups, 17 in 320 or
+// 512; 24 of 60000: 65 in 192, 87 in 264) and 64 splits (one pair of 100000 keys: 21 us, 25
+// in 256), but where the pairs alone take more than half of the CUs into about 512 (160
+// pairs of 10000 to 20000 keys: 114 us, 130 whole; 272 of 4000 to 12000: 108, 117).
 Walk walk_for(int64_t pairs, int rows, int keys, int dim) {
   const int64_t tiles = ceil_div(keys, kTile), twos = pairs * ceil_div(rows, 32), plenty = dim == 64 ? 1024 : 512;
   Walk w{1, 4, 1};
@@ -600,8 +638,8 @@ Walk walk_for(int64_t pairs, int rows, int keys, int dim) {
     return w;
   }
   const int64_t wgs = pairs * ceil_div(rows, 16 * w.blocks);
-  if (tiles > 16 && (tiles >= 64 || wgs < 256))
-    w.splits = int(std::min(ceil_div(tiles >= 64 ? 512 : 384, wgs), tiles / 4));
+  if (tiles > 16)
+    w.splits = int(wgs > 128 && tiles >= 64 ? ceil_div(512, wgs) : std::max<int64_t>(1, std::min<int64_t>({256 / wgs, tiles / 4, 64})));
   return w;
 }
 // A prefix's states are joined with the requests' own in any case, so splitting it costs
@@ -658,7 +696,10 @@ hipError_t launch(const AttnPlan& p, hipStream_t stream) {
                      stream, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !p.parts) return e;
-  hipLaunchKernelGGL((kv_attention_join_kernel<D>), dim3(unsigned(ceil_div(p.all_rows, 4))), dim3(256), 0, stream, p);
+  if (p.splits + p.prefix_splits > 16)
+    hipLaunchKernelGGL((kv_attention_join_kernel<D, 4>), dim3(unsigned(p.all_rows)), dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL((kv_attention_join_kernel<D, 1>), dim3(unsigned(ceil_div(p.all_rows, 4))), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
