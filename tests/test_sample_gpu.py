@@ -265,3 +265,16 @@ def test_refusals(ops):
         with pytest.raises(error):
             call()
             pytest.fail(f"call {i} was accepted")
+
+
+@pytest.mark.parametrize("vocab,top_k", [(399, 40), (400, 40), (401, 41), (16383, 256), (16384, 256), (16384, 257),
+                                         (256, 256), (300, 256), (5, 3), (5, 4), (4, 4)])
+def test_both_sides_of_the_one_pass_rule(ops, vocab, top_k):
+    say("one pass rule", vocab, top_k)
+    rng = np.random.default_rng(vocab + top_k)
+    rows = rows_of(rng, 6, vocab)
+    rows[4] = np.float32(0.25)                      # equal logits
+    rows[5, ::2] = -np.inf                          # fewer tokens than a large top-k
+    uniforms = (rng.random(6) * 0.999 + 0.0005).astype(np.float32)
+    check(ops, rows, uniforms, 0.8, top_k)
+    check(ops, rows, uniforms, 1.2, top_k, top_p=0.8, min_p=0.01)

@@ -18,10 +18,18 @@
 // the token is the one that 64-bit arithmetic gives but for a random number within
 // about 1e-10 of a border.  Tokens 32 units from the maximum (e^-32) weigh nothing.
 //
-// One workgroup per row reads it three times, the second and third time from cache.
-// (Keeping it in registers needs every pass unrolled over them: 50 KB of code that runs
-// once per wave, fetched from memory, took 20 us a pass; a pass over 201 KB in L2 reads
-// in 1.6 us.)
+// One workgroup per row reads it three times (maximum, bins, gathering), the second and
+// third time from cache.  (Keeping it in registers needs every pass unrolled over them: 50
+// KB of code that runs once per wave, fetched from memory, took 20 us a pass; a pass over
+// 201 KB in L2 reads in 1.6 us.)  Rows with a small top-k take a shorter way that
+// reads them once.
+//
+// What bounds it.  32 rows of 50257 with top-p take 27 us: 3.5 for the maximum (one CU's
+// loads), 6.5 for the bins and 6.3 for the gathering (20 and 9 vector instructions a token),
+// 4 for the sums over the bins, 2.3 for the searches, 4 for ordering and answers; without
+// data (a few tokens) 13 are left.  32 CUs are busy.  Several workgroups to a row would
+// have to bring their bins together, 64 KB each, which costs what they save.  256 rows of
+// 128257 with every filter take 39 us at 3.4 TB/s, 76 by top-p alone.
 #include "common.hpp"
 #include "kernels.hpp"
 #include "lds_limit.hpp"
@@ -32,7 +40,14 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int kThreads = 1024, kPerThread = 8, kBins = kThreads * kPerThread, kList = 512, kRuns = 2048;
+// A top-k up to which a row may be sampled in one pass: half of what the list holds, so
+// that a bin which ends past the k-th token still fits.
 constexpr unsigned kShort = 256;
+// Whether it is: ordering the k costs k^2, the longer way the row twice more.  In one pass
+// against the longer way, us: 64 rows of 1000 tokens, k = 40 12.6 and 14.1, k = 256 17.1 and
+// 14.2; of 10000, 13.2 and 17.2, 18.2 and 17.3; of 20000, 13.3 and 18.9, 18.2 and 19.1; 32
+// rows of 50257, 14.9 and 30.8, 19.7 and 30.6.
+__device__ __forceinline__ bool is_short(unsigned k, unsigned vocab) { return k <= kShort && k < vocab && k * k / 4 <= vocab; }
 constexpr double kPerUnit = 256.0;  // bins per unit of (max - logit) / T
 constexpr int kCountShift = 45;     // a bin: count << 45 | sum of q
 constexpr u64 kOne = u64(1) << 35;  // weight of a token at its bin's near edge
@@ -468,12 +483,11 @@ __device__ __forceinline__ float block_top(SampleLds& s, float top) {
   return top;
 }
 
-// At most kShort tokens kept, by top_k or because the row has no more, in one pass over
-// the row: a sample of it says which logits are likely to be among four times as many as
-// may be kept, the tokens with those are gathered, and everything else is read off the
-// list: the maximum, the bin of the last token that may be kept, the order up to that bin
-// and the cumulative masses.  False, nothing written: too few tokens were found, or more
-// than the lists hold.
+// A top-k that is_short, in one pass over the row: a sample of it says which logits are
+// likely to be among four times as many as may be kept, the tokens with those are gathered,
+// and everything else is read off the list: the maximum, the bin of the last token that may
+// be kept, the order up to that bin and the cumulative masses.  False, nothing written: too
+// few tokens were found, or more than the lists hold.
 template <typename T>
 __device__ __forceinline__ bool sample_short(SampleLds& s, const Row<T>& row, float temp, unsigned most, float top_p,
                                              float min_p, float u, int32_t* token, float* prob) {
@@ -607,7 +621,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   u = u > 0.f ? fminf(u, 0.99999994f) : 0.f;
 
   const unsigned most = top_k > 0 && top_k < a.vocab ? unsigned(top_k) : unsigned(a.vocab);
-  if (most <= kShort && temp > 0.f && sample_short(s, row, temp, most, top_p, min_p, u, a.tokens + b, a.probs + b)) return;
+  if (is_short(most, unsigned(a.vocab)) && temp > 0.f && sample_short(s, row, temp, most, top_p, min_p, u, a.tokens + b, a.probs + b)) return;
 
   float top = kNegInf;
   row.template each<4>([&](float x, int) { top = fmaxf(top, x); });

@@ -8,6 +8,10 @@ and the exception contract -- ``TypeError`` for an operand that is not a
 contiguous device tensor of the right dtype, ``ValueError`` for a bad rank,
 extent, device, integer argument or a tensor that requires grad,
 ``RuntimeError`` carrying ``ti_v2_last_error()`` for a nonzero native status.
+Beyond it: an int8 KV cache (``kv_cache_int8``, ``kv_append_int8``,
+``kv_read_int8``), attention over it for single tokens and prompts
+(``attention_int8kv``, ``attention_shared_prefix``) and ``sample``, one token per
+row of logits.
 
 How it is built here: every native symbol is described by a string of
 parameter codes (``_ABI``); each call goes through a ``_Call`` that validates
@@ -556,6 +560,8 @@ class NativeOps:
         shape = (batch, heads, nq, bound, prefix_length)
         needed = cache._workspace.get(shape)
         if needed is None:
+            if len(cache._workspace) >= 1024:  # (a caller whose lengths are all different)
+                cache._workspace.clear()
             needed = cache._workspace[shape] = max(0, self.lib.ti_amd_attention_i8kv_workspace(cache._at, *shape))
         if needed:
             call.output((needed,), torch.uint8)
