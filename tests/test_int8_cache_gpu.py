@@ -409,6 +409,33 @@ def test_shared_prefix_plans(ops, batch, heads, kv_heads, dim, nq, prefix, kv):
     some_of(got, q, case, order[:-1], ends_of(lengths, nq), rng, 10, prefix=(int(order[-1]), prefix))
 
 
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,nq,prefix,kv", [
+    (64, 32, 8, 128, 1, 4000, 40),      # single tokens, two blocks of rows over the prefix
+    (2, 8, 8, 128, 40, 300, 8300),      # two blocks over the own keys alone
+    (3, 24, 24, 128, 300, 2000, 310),   # over both
+    (5, 6, 2, 64, 33, 2000, 70),
+])
+def test_shared_prefix_plans_of_more_shapes(ops, batch, heads, kv_heads, dim, nq, prefix, kv):
+    test_shared_prefix_plans(ops, batch, heads, kv_heads, dim, nq, prefix, kv)
+
+
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,nq,kv", [
+    (8, 16, 16, 128, 64, 2000),         # rows for two blocks by their keys
+    (2, 25, 25, 64, 90, 3000),
+    (1, 8, 1, 128, 1, 40000),           # one pair, as many splits as there may be
+    (160, 2, 1, 64, 1, 5000),           # pairs on more than half of the units
+])
+def test_attention_plans_of_more_shapes(ops, batch, heads, kv_heads, dim, nq, kv):
+    say("more plans", batch, heads, kv_heads, dim, nq, kv)
+    rng = np.random.default_rng(batch + kv)
+    lengths = [int(x) for x in rng.integers(0, kv + 1, batch)]
+    lengths[0] = kv
+    case = Case(ops, rng, batch, kv_heads, dim, [kv])
+    q = (rng.standard_normal((batch, heads, nq, dim)) * 2).astype(np.float16)
+    got = ops.attention_int8kv(dev(q), case.cache, list(range(batch)), i32(lengths))
+    some_of(got, q, case, range(batch), ends_of(lengths, nq), rng, 10)
+
+
 @pytest.mark.parametrize("batch,heads,kv_heads,dim,nq,kv,mean", [
     (3, 25, 25, 64, 440, 440, 30.0),    # two waves to a block of 32 rows
     (4, 16, 16, 128, 520, 530, 30.0),   # the same, 128 dims

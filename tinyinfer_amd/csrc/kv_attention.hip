@@ -30,13 +30,13 @@
 // its row blocks running over the whole batch: its keys are read once for all requests.
 //
 // What bounds it.  Single tokens: memory where caches are long (16 requests of 8 x 128,
-// 12000 to 32768 keys: 138 us, 5.8 TB/s; the loads are the plain ones of a stream,
+// 12000 to 32768 keys: 135 us, 5.9 TB/s; the loads are the plain ones of a stream,
 // past the caches), launch and one tile's chain of latencies where they are short (one
-// request of 12 heads, 300 keys: 5.7 us).  Prompts: vector instructions beside the matrix
+// request of 12 heads, 300 keys: 6 us).  Prompts: vector instructions beside the matrix
 // products.  Of a tile of 64 keys x 32 rows at D 128 the 64 matrix instructions are 1024
 // cycles of a SIMD; widening K and V is 192 vector instructions and a score takes 6 and an
 // exponential, 1900 cycles together.  2 requests of 777 queries, 32 heads over 8 of 128,
-// 4500 to 6001 keys: 200 us, 670 TFLOP/s; 4 prompts of 1024, 25 heads of 64: 30 us, 445
+// 4500 to 6001 keys: 198 us, 680 TFLOP/s; 4 prompts of 1024, 25 heads of 64: 30 us, 440
 // TFLOP/s, its scores' exponentials and scales more than the products.
 #include <algorithm>
 
@@ -612,27 +612,29 @@ struct Walk {
 
 // From the number of (request, key head) pairs, the rows of one and the tiles of 64 keys
 // of the longest.  Two blocks of 16 rows use every widened key and value twice; they
-// pay where there are plenty of row blocks (GPT-2 XL prefill, 100 pairs of 1024 rows:
-// 38.4 us against 44.7; 64 pairs of 333 rows, D 128: 37 against 53; 12 pairs of 1024:
-// 12.2 against 11.1) or many keys to a row block (64 queries of 4 heads over 16000 keys,
-// D 128: 40 against 50 us).
+// pay where there are plenty of row blocks (100 pairs of 1024 rows: 31 us against 60; 288
+// pairs of 100 rows: 8.9 against 10.7), or many keys to them (128 pairs of 64 rows over 2000
+// keys, D 128: 22 against 30; 8 pairs of 256 rows over 16000: 37 against 52), not where
+// both are few (12 pairs of 512 rows: 8.2 against 6.9; 128 pairs of 20 rows over 2000 keys,
+// D 128: 20 against 19).
 // Waves: with row blocks to fill every SIMD twice a workgroup takes four of them and its
 // waves share the tiles, each widened once instead of four times and nothing merged (100
 // pairs of 1024 rows: 31.3 us, 35.7 with two waves to a row block, 44 with four; 75 pairs:
 // 29.8, 32.6, 39.8; 8 pairs of 8192 rows over 8000 keys, D 128: 278, 301, 298); below that
-// two waves share a row block, or four where keys are many (12 pairs of 4096 rows: 56 us,
-// 66 with two, 87 with shared tiles; 24 pairs of 2048 rows without a mask: 52, 50, 61; 16
+// two waves share a row block, or four where keys are many (12 pairs of 4096 rows: 51 us,
+// 60 with two, 81 with shared tiles; 24 pairs of 2048 rows without a mask: 52, 50, 61; 16
 // pairs of 3108 rows over 6001 keys, D 128: 205, 224, 212).
 // Splits: a second launch and the states' traffic cost 2 us and more, so short caches
-// are not split (96 pairs, 1024 keys: 8.8 us, 9.4 in four).  Longer ones are, into at most
-// one workgroup a CU (8 pairs of 16000 keys, D 128: 13.3 us in 256 workgroups, 17 in 320 or
-// 512; 24 of 60000: 65 in 192, 87 in 264) and 64 splits (one pair of 100000 keys: 21 us, 25
-// in 256), but where the pairs alone take more than half of the CUs into about 512 (160
-// pairs of 10000 to 20000 keys: 114 us, 130 whole; 272 of 4000 to 12000: 108, 117).
+// are not split (96 pairs, 1024 keys: 8.4 us, 9.4 in four; 12 pairs, 7.6 and 7.8).  Longer
+// ones are, into at most one workgroup a CU (8 pairs of 16000 keys, D 128: 13.3 us in 256
+// workgroups, 17 in 320 or 512; 24 of 60000: 65 in 192, 87 in 264) and 64 splits (one pair
+// of 100000 keys: 21 us, 25 in 256), but where the pairs alone take more than half of the
+// CUs into about 512 (160 pairs of 10000 to 20000 keys: 114 us, 130 whole; 272 of 4000 to
+// 12000: 108, 117).
 Walk walk_for(int64_t pairs, int rows, int keys, int dim) {
   const int64_t tiles = ceil_div(keys, kTile), twos = pairs * ceil_div(rows, 32), plenty = dim == 64 ? 1024 : 512;
   Walk w{1, 4, 1};
-  if (rows > 16 && (twos >= plenty || tiles >= 128)) w.blocks = 2;
+  if (rows > 16 && (twos >= plenty || tiles >= 128 || (twos >= 128 && twos * tiles > 4096))) w.blocks = 2;
   if (w.blocks == 2 && twos >= plenty) {
     w.waves = twos >= 2048 ? kShared : twos >= 1024 && tiles < 32 ? 2 : 4;
     return w;
@@ -642,12 +644,15 @@ Walk walk_for(int64_t pairs, int rows, int keys, int dim) {
     w.splits = int(wgs > 128 && tiles >= 64 ? ceil_div(512, wgs) : std::max<int64_t>(1, std::min<int64_t>({256 / wgs, tiles / 4, 64})));
   return w;
 }
-// A prefix's states are joined with the requests' own in any case, so splitting it costs
-// less: into about 192 workgroups, 256 from 8192 keys on (64 requests of 4 rows, 8 heads,
-// 16001 keys: 97 us in 128 workgroups, 44 in 256).
+// A prefix: two blocks by the work alone (its keys are re-read from the L2 by all its row
+// blocks: 64 requests of 4 rows, 8 heads of 128, 4000 keys 23.5 us against 24.7, 256
+// requests over 2000 42 against 52; 8 requests over 9000 18.1 against 15.7, 400 requests of
+// 12 heads of 64 over 1000 39 against 34).  Its states are joined with the requests' own in
+// any case, so splitting it costs less: into about 192 workgroups, 256 from 8192 keys on (64
+// requests of 4 rows, 8 heads, 16001 keys: 63 us in 128 workgroups, 42 in 256, 44 in 512).
 Walk prefix_walk_for(int heads, int64_t rows, int keys) {
   const int64_t tiles = ceil_div(keys, kTile);
-  Walk w{rows > 16 && (heads * ceil_div(rows, 32) >= 1024 || tiles >= 128) ? 2 : 1, 4, 1};
+  Walk w{rows > 16 && heads * ceil_div(rows, 32) * tiles >= 3000 ? 2 : 1, 4, 1};
   const int64_t wgs = heads * ceil_div(rows, 16 * w.blocks);
   w.splits = int(std::max<int64_t>(1, std::min(ceil_div(tiles >= 128 ? 256 : 192, wgs), tiles / 4)));
   return w;
