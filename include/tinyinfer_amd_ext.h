@@ -125,7 +125,8 @@ int ti_amd_layernorm_softmax_f32(const float* x, const float* gamma, const float
  * owns the buffers, all 16-byte aligned: k and v of slots * kv_heads * capacity *
  * head_dim bytes, k_scales and v_scales of slots * kv_heads * capacity floats.
  * Their inner order is the kernels' own (k's rows one after another, v in blocks
- * of 64 tokens); rows never written are never read as part of a request.
+ * of 64 tokens).  A call reads the rows that its lengths name: those that were
+ * never written count as what the buffers hold (zeros in zeroed ones).
  * capacity is a multiple of 64, head_dim 64 or 128. */
 typedef struct ti_amd_kv_i8 {
   uint8_t* k;
@@ -155,7 +156,8 @@ int ti_amd_kv_read_i8(const ti_amd_kv_i8* cache, uint16_t* k, uint16_t* v, const
  * are at most 65535, batch * heads * q_len at most 2^23.
  * prefix_len > 0: in front of its own keys every query also sees tokens 0 ..
  * prefix_len - 1 of prefix_slot, whose bytes are read once for the batch.
- * Scores, softmax and sums are fp32; probabilities are rounded to fp16.
+ * Scores, softmax and sums are fp32; probabilities are rounded to fp16 (up to 16
+ * query rows per key head and request twice: what the first leaves out is added).
  * max_kv (0: the capacity) is what kv_lengths are expected to stay within: it
  * plans the launch and its workspace, and longer requests are answered too.
  * workspace: ti_amd_attention_i8kv_workspace bytes (-1 for invalid arguments, 0
