@@ -156,8 +156,10 @@ int ti_amd_kv_read_i8(const ti_amd_kv_i8* cache, uint16_t* k, uint16_t* v, const
  * are at most 65535, batch * heads * q_len at most 2^23.
  * prefix_len > 0: in front of its own keys every query also sees tokens 0 ..
  * prefix_len - 1 of prefix_slot, whose bytes are read once for the batch.
- * Scores, softmax and sums are fp32; probabilities are rounded to fp16 (up to 16
- * query rows per key head and request twice: what the first leaves out is added).
+ * Scores, softmax and sums are fp32; probabilities are rounded to fp16 (where few
+ * rows share the keys twice: what the first rounding leaves out is added).  How rows
+ * and keys are divided follows from the shape arguments, so a request's last bits
+ * may differ between batches of other sizes; equal calls give equal bits.
  * max_kv (0: the capacity) is what kv_lengths are expected to stay within: it
  * plans the launch and its workspace, and longer requests are answered too.
  * workspace: ti_amd_attention_i8kv_workspace bytes (-1 for invalid arguments, 0
