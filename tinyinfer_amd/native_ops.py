@@ -112,9 +112,9 @@ class _Call:
         tensor = self.ops.tensor_type
         # (At most INT32_MAX elements: then every extent and the byte count fit.)
         if not ((type(x) is tensor or isinstance(x, tensor)) and x.is_cuda and x.dtype == dtype
-                and x.is_contiguous() and not x.requires_grad and 0 < x.numel() <= INT32_MAX and x.dim()
-                and (rank is None or x.dim() == rank) and (self.device is None or x.device == self.device)
-                and (shape is None or x.shape == shape)):
+                and x.is_contiguous() and not x.requires_grad and 0 < x.numel() <= INT32_MAX
+                and (x.shape == shape if shape is not None else x.dim() == rank if rank is not None else x.dim())
+                and (self.device is None or x.device == self.device)):
             self._checked(x, dtype, name, rank, shape)
         if self.device is None:
             self.device = x.device
@@ -230,7 +230,7 @@ class _Call:
             stream = ops.streams[index, handle] = cuda.current_stream(index)
         for x in self.held:
             x.record_stream(stream)
-        if cuda.current_device() == index:
+        if ops.current_device() == index:
             status = getattr(ops.lib, self.symbol)(*self.args, handle, index)
         else:
             with cuda.device(self.device):
@@ -287,6 +287,7 @@ class NativeOps:
         import torch
         self.torch, self.tensor_type = torch, torch.Tensor
         self.stream_handle, self.streams = torch._C._cuda_getCurrentRawStream, {}
+        self.current_device = torch._C._cuda_getDevice   # (operands are on a GPU: it is initialised)
         where = require(BACKEND_LIB) if library_path is None else library_path
         self.library_path = str(Path(where).expanduser().resolve(strict=True))
         self.lib = ctypes.CDLL(self.library_path)
