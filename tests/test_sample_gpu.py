@@ -278,3 +278,16 @@ def test_both_sides_of_the_one_pass_rule(ops, vocab, top_k):
     uniforms = (rng.random(6) * 0.999 + 0.0005).astype(np.float32)
     check(ops, rows, uniforms, 0.8, top_k)
     check(ops, rows, uniforms, 1.2, top_k, top_p=0.8, min_p=0.01)
+
+
+@pytest.mark.parametrize("temperature", [1e-30, 1e-3, 0.7, 300.0, 1e30, float("inf")])
+@pytest.mark.parametrize("shift,spread", [(0.0, 3.0), (1e5, 2.0), (-1e5, 2.0), (1e30, 1e28), (0.0, 1e-6), (-3.0, 1e-30)])
+def test_scales_and_shifts(ops, temperature, shift, spread):
+    """Where rounding moves logits and bins furthest against each other."""
+    say("scales", temperature, shift, spread)
+    rng = np.random.default_rng(int(abs(shift) % 97) + 7)
+    rows = (rng.standard_normal((4, 9001)) * spread + shift).astype(np.float32)
+    uniforms = (rng.random(4) * 0.999 + 0.0005).astype(np.float32)
+    t = np.full(4, temperature, np.float32)
+    check(ops, rows, uniforms, t, top_p=0.9, borders=False)
+    check(ops, rows, uniforms, t, 2000, top_p=0.95, min_p=0.001, borders=False)

@@ -23,8 +23,9 @@
 // The stored byte is c + 128: 0x6400 | byte is then the fp16 number 1152 + c.
 //
 // Both directions are bound by memory where there is much of it: 8 prompts of up to 1000
-// rows, 25 heads of 64, are quantised in 17 us (up to 51 MB in, 27 out), 65536 rows of 8 heads of 128 read back in 74 us (403 MB, 5.4
-// TB/s); single tokens by the launch (32 requests of 12 heads: 4.3 us, 4.2 back).
+// rows, 25 heads of 64, are quantised in 17 us (up to 51 MB in, 27 out), 65536 rows of 8
+// heads of 128 read back in 74 us (403 MB, 5.4 TB/s); single tokens by the launch (32
+// requests of 12 heads: 4.3 us, 4.2 back).
 #include "common.hpp"
 #include "kernels.hpp"
 
