@@ -69,7 +69,7 @@ struct SampleLds {
   unsigned at[kList], q[kList];  // their bins and losses
   unsigned wanted[kBins / 32];   // a bit per bin whose tokens are gathered
   u64 wave_mass[kThreads / 64];
-  unsigned wave_count[kThreads / 64];
+  unsigned wave_count[kThreads / 64], run_count[kBins / 1024];
   float wave_max[kThreads / 64];
   int wave_at[kThreads / 64];
   u64 low, high, answer_key, answer_mass;
@@ -187,15 +187,14 @@ struct Row {
       }
     }
   }
-  // f(value) for one vector per thread, spread evenly over a row of more (and the edges).
-  template <typename F>
-  __device__ __forceinline__ void sample(F f) const {
-    edges([&](float x, int) { f(x); });
-    const int at = vectors <= kThreads ? int(threadIdx.x) : int(unsigned(vectors) * u64(threadIdx.x) / kThreads);
-    if (at >= vectors) return;
-    const vec x = *reinterpret_cast<const vec*>(p + head + at * W);
-#pragma unroll
-    for (int e = 0; e < W; ++e) f(float(x[e]));
+  // A vector per thread, spread evenly over a row of more, and of the edges a token; -inf
+  // where there is none.
+  __device__ __forceinline__ vec sample(T& edge) const {
+    const int t = int(threadIdx.x), i = t < head ? t : t + vectors * W;
+    edge = t < head || t < n - vectors * W ? p[i] : T(kNegInf);
+    const int at = vectors <= kThreads ? t : int(unsigned(vectors) * u64(t) / kThreads);
+    if (at < vectors) return *reinterpret_cast<const vec*>(p + head + at * W);
+    return vec(T(kNegInf));
   }
 };
 
@@ -478,12 +477,11 @@ __device__ __forceinline__ Place locate(SampleLds& s, const Row<T>& row, const S
 
 
 // The bin of the token with `goal` - 1 others in front of it, from the counts per bin;
-// before: the tokens in front of the bin.  kBins if there are fewer.  Every wave sums
-// 1024 bins at a time, 16 to a lane, then those of one lane.
-__device__ __forceinline__ unsigned bin_of_rank(const SampleLds& s, unsigned goal, unsigned& before) {
-  const unsigned lane = threadIdx.x & 63;
-  before = 0;
-  for (unsigned run = 0; run < kBins; run += 1024) {
+// before: the tokens in front of the bin.  kBins if there are fewer.  A wave sums 1024 bins,
+// 16 to a lane; every wave then looks into the thousand in question and into one lane's.
+__device__ __forceinline__ unsigned bin_of_rank(SampleLds& s, unsigned goal, unsigned& before) {
+  const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const auto sum_of = [&](unsigned run) {
     unsigned sum = 0;
 #pragma unroll
     for (unsigned i = 0; i < 16; ++i) sum += s.count[slot(run + 16 * lane + i)];
@@ -492,22 +490,30 @@ __device__ __forceinline__ unsigned bin_of_rank(const SampleLds& s, unsigned goa
       const unsigned up = __shfl_up(sum, o, 64);
       sum += lane >= unsigned(o) ? up : 0;
     }
-    const int over = __popcll(__ballot(before + sum < goal));
-    if (over < 64) {
-      if (over > 0) before += __shfl(sum, over - 1, 64);
-      unsigned upto = s.count[slot(run + 16 * over + (lane & 15))];
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) {
-        const unsigned up = __shfl_up(upto, o, 16);
-        upto += (lane & 15) >= unsigned(o) ? up : 0;
-      }
-      const int bin = __popcll(__ballot(lane < 16 && before + upto < goal));
-      if (bin > 0) before += __shfl(upto, bin - 1, 64);
-      return run + 16 * over + bin;
-    }
-    before += __shfl(sum, 63, 64);
+    return sum;
+  };
+  if (wave < kBins / 1024) {
+    const unsigned sum = sum_of(1024 * wave);
+    if (lane == 63) s.run_count[wave] = sum;
   }
-  return kBins;
+  __syncthreads();
+  before = 0;
+  unsigned run = 0;
+  while (run < kBins / 1024 && before + s.run_count[run] < goal) before += s.run_count[run++];
+  if (run == kBins / 1024) return kBins;
+  run *= 1024;
+  const unsigned sum = sum_of(run);
+  const int over = __popcll(__ballot(before + sum < goal));
+  if (over > 0) before += __shfl(sum, over - 1, 64);
+  unsigned upto = s.count[slot(run + 16 * over + (lane & 15))];
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    const unsigned up = __shfl_up(upto, o, 16);
+    upto += (lane & 15) >= unsigned(o) ? up : 0;
+  }
+  const int bin = __popcll(__ballot(lane < 16 && before + upto < goal));
+  if (bin > 0) before += __shfl(upto, bin - 1, 64);
+  return run + 16 * over + bin;
 }
 
 __device__ __forceinline__ float block_top(SampleLds& s, float top) {
@@ -534,18 +540,24 @@ __device__ __forceinline__ bool sample_short(SampleLds& s, const Row<T>& row, fl
   };
   clear();
   float top = kNegInf;
-  row.sample([&](float x) { top = fmaxf(top, x); });
+  T edge;
+  const auto sampled = row.sample(edge);
+  top = fmaxf(top, float(edge));
+#pragma unroll
+  for (int e = 0; e < Row<T>::W; ++e) top = fmaxf(top, float(sampled[e]));
   top = block_top(s, top);
   if (top == kNegInf || top == -kNegInf) return false;
   const Scale about(top, temp);
-  row.sample([&](float x) {
+  const auto counts = [&](float x) {
     const float d = about.distance(x);
     if (d < float(kBins)) atomicAdd(&s.count[slot(unsigned(d))], 1u);
-  });
+  };
+  counts(float(edge));
+#pragma unroll
+  for (int e = 0; e < Row<T>::W; ++e) counts(float(sampled[e]));
   __syncthreads();
   unsigned before;
-  const unsigned sampled = Row<T>::W * kThreads;
-  const unsigned enough = row.vectors <= kThreads ? most : 4 * most * sampled / unsigned(row.n) + 8;
+  const unsigned enough = row.vectors <= kThreads ? most : 4 * most * Row<T>::W * kThreads / unsigned(row.n) + 8;
   const float least = top - float(min(bin_of_rank(s, enough, before) + 1, unsigned(kBins))) / about.per;
   __syncthreads();
   clear();
