@@ -30,13 +30,13 @@
 // its row blocks running over the whole batch: its keys are read once for all requests.
 //
 // What bounds it.  Single tokens: memory where caches are long (16 requests of 8 x 128,
-// 12000 to 32768 keys: 135 us, 5.9 TB/s; the loads are the plain ones of a stream,
+// 12000 to 32768 keys: 134 us, 6.0 TB/s; the loads are the plain ones of a stream,
 // past the caches), launch and one tile's chain of latencies where they are short (one
 // request of 12 heads, 300 keys: 6 us).  Prompts: vector instructions beside the matrix
 // products.  Of a tile of 64 keys x 32 rows at D 128 the 64 matrix instructions are 1024
 // cycles of a SIMD; widening K and V is 192 vector instructions and a score takes 6 and an
 // exponential, 1900 cycles together.  2 requests of 777 queries, 32 heads over 8 of 128,
-// 4500 to 6001 keys: 198 us, 680 TFLOP/s; 4 prompts of 1024, 25 heads of 64: 30 us, 440
+// 4500 to 6001 keys: 197 us, 686 TFLOP/s; 4 prompts of 1024, 25 heads of 64: 30 us, 445
 // TFLOP/s, its scores' exponentials and scales more than the products.
 #include <algorithm>
 
