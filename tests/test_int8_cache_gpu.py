@@ -849,3 +849,37 @@ def test_c_entry_refuses_a_missing_or_small_workspace(ops):
     assert call(ws.data_ptr(), needed) == 0
     t.cuda.synchronize()
     assert not y.any()
+
+
+def test_a_cache_dropped_while_another_stream_still_reads_it(ops):
+    """The allocator waits for every stream that a call used the cache on."""
+    say("dropped cache")
+    t = torch()
+    rng = np.random.default_rng(15)
+    n = 4096
+    k, v = random_rows(rng, 4, 8, n, 128), random_rows(rng, 4, 8, n, 128)
+    q = dev(rng.standard_normal((4, 8, 1, 128)).astype(np.float16))
+    slots, lengths = i32([0, 1, 2, 3]), i32([n] * 4)
+    dk, dv = dev(k), dev(v)
+
+    def filled():
+        cache = ops.kv_cache_int8(4, 8, n, 128)
+        ops.kv_append_int8(cache, dk, dv, slots, 0)
+        return cache
+
+    cache = filled()
+    want = host(ops.attention_int8kv(q, cache, slots, lengths))
+    size = cache.buffer.numel()
+    del cache
+    side = t.cuda.Stream()
+    for _ in range(4):
+        cache = filled()
+        side.wait_stream(t.cuda.current_stream())
+        with t.cuda.stream(side):
+            for _ in range(20):                # (work in front of the call that counts)
+                ops.attention_int8kv(q, cache, slots, lengths)
+            got = ops.attention_int8kv(q, cache, slots, lengths)
+        del cache
+        t.zeros(size, dtype=t.uint8, device="cuda").fill_(255)   # takes the freed block, if it was
+        side.synchronize()
+        assert np.array_equal(got.cpu().numpy(), want)

@@ -100,24 +100,26 @@ class _Call:
     device is switched only when it is not current.  ``gemm_int8`` at M = 1,
     768 -> 2304, call after call: 15.6 -> 11.7 us."""
 
-    __slots__ = ("ops", "symbol", "args", "held", "made", "device")
+    __slots__ = ("ops", "symbol", "args", "held", "made", "device", "index", "over")
 
     def __init__(self, ops, symbol):
         self.ops, self.symbol = ops, symbol
         self.args = []
         self.held, self.made = [], []   # the caller's tensors, and this call's own
-        self.device = None
+        self.device = self.index = None
+        self.over = None                # the int8 cache it works on
 
     def operand(self, x, dtype, name, rank=None, shape=None):
         tensor = self.ops.tensor_type
         # (At most INT32_MAX elements: then every extent and the byte count fit.)
-        if not ((type(x) is tensor or isinstance(x, tensor)) and x.is_cuda and x.dtype == dtype
+        if not ((type(x) is tensor or isinstance(x, tensor)) and x.dtype == dtype
                 and x.is_contiguous() and not x.requires_grad and 0 < x.numel() <= INT32_MAX
                 and (x.shape == shape if shape is not None else x.dim() == rank if rank is not None else x.dim())
-                and (self.device is None or x.device == self.device)):
+                and x.is_cuda and (self.index is None or x.get_device() == self.index)):
             self._checked(x, dtype, name, rank, shape)
-        if self.device is None:
+        if self.index is None:
             self.device = x.device
+            self.index = x.get_device()
         self.held.append(x)
         self.args.append(x.data_ptr())
         return x
@@ -192,7 +194,8 @@ class _Call:
         if type(cache) is not Int8KVCache:
             raise TypeError("cache: an Int8KVCache (NativeOps.kv_cache_int8) is required")
         self.device = cache.buffer.device
-        self.held.append(cache.buffer)
+        self.index = cache.buffer.get_device()
+        self.over = cache
         self.args.append(cache._at)
 
     def per_request(self, batch, *items):
@@ -220,7 +223,7 @@ class _Call:
         self.args.extend(values)
 
     def run(self):
-        ops, index = self.ops, self.device.index
+        ops, index = self.ops, self.index
         cuda = ops.torch.cuda
         # (The current stream's handle costs a tenth of making its Stream object, which
         # record_stream wants and which stays the same for a handle.)
@@ -230,6 +233,10 @@ class _Call:
             stream = ops.streams[index, handle] = cuda.current_stream(index)
         for x in self.held:
             x.record_stream(stream)
+        # (The allocator keeps a stream with a block until the block is freed: once does.)
+        if self.over is not None and handle not in self.over._streams:
+            self.over.buffer.record_stream(stream)
+            self.over._streams.add(handle)
         if ops.current_device() == index:
             status = getattr(ops.lib, self.symbol)(*self.args, handle, index)
         else:
@@ -256,7 +263,7 @@ class Int8KVCache:
     is the requested one rounded up to a multiple of 64.  The cache keeps no
     lengths: every call names the slots, positions and lengths it means."""
 
-    __slots__ = ("slots", "kv_heads", "capacity", "head_dim", "buffer", "_native", "_at", "_workspace")
+    __slots__ = ("slots", "kv_heads", "capacity", "head_dim", "buffer", "_native", "_at", "_workspace", "_streams")
 
     def __init__(self, torch, slots, kv_heads, capacity, head_dim, device):
         capacity = (capacity + 63) // 64 * 64
@@ -265,10 +272,11 @@ class Int8KVCache:
         at = buffer.data_ptr()
         native = _KvI8(at, at + tokens * head_dim, at + 2 * tokens * head_dim, at + 2 * tokens * head_dim + 4 * tokens,
                        slots, kv_heads, capacity, head_dim)
-        # _workspace: bytes an attention call needs, by its shape.
+        # _workspace: bytes an attention call needs, by its shape; _streams: those that
+        # the allocator has been told of.
         for name, value in (("slots", slots), ("kv_heads", kv_heads), ("capacity", capacity), ("head_dim", head_dim),
                             ("buffer", buffer), ("_native", native), ("_at", ctypes.addressof(native)),
-                            ("_workspace", {})):
+                            ("_workspace", {}), ("_streams", set())):
             object.__setattr__(self, name, value)
 
     def __setattr__(self, name, value):
