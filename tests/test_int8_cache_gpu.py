@@ -419,6 +419,45 @@ def test_shared_prefix_plans_of_more_shapes(ops, batch, heads, kv_heads, dim, nq
     test_shared_prefix_plans(ops, batch, heads, kv_heads, dim, nq, prefix, kv)
 
 
+@pytest.mark.parametrize("prefix", [1, 63, 64, 65, 500])
+@pytest.mark.parametrize("heads,kv_heads,dim,nq", [(4, 4, 64, 1), (8, 2, 128, 1), (3, 3, 64, 5), (6, 2, 128, 5), (4, 4, 64, 17)])
+def test_short_prefixes(ops, heads, kv_heads, dim, nq, prefix):
+    """A prefix that ends inside a tile, own keys from none on, queries that see none of their
+    own, requests of slots outside the cache, and a row that is not finite in each."""
+    say("short prefix", heads, kv_heads, dim, nq, prefix)
+    rng = np.random.default_rng(heads + nq + prefix)
+    lengths, kv = [0, 1, 64, 70, 129, 3], 130
+    batch = len(lengths)
+    case = Case(ops, rng, batch + 1, kv_heads, dim, [kv], capacity=640)
+    order = [4, 0, 6, 2, 1, 5]
+    q = (rng.standard_normal((batch, heads, nq, dim)) * 2).astype(np.float16)
+
+    def run(**more):
+        return ops.attention_shared_prefix(dev(q), case.cache, 3, prefix, i32(order), i32(lengths), max_kv_length=kv, **more)
+
+    check(run(), q, case, order, ends_of(lengths, nq), prefix=(3, prefix))
+    q_lengths = [nq, nq - 1, 0, nq, 1, nq]
+    offsets = [0, -nq, 5, 200, 60, -1]
+    for causal in (True, False):
+        got = run(q_lengths=i32(q_lengths), query_offsets=i32(offsets), causal=causal)
+        check(got, q, case, order, ends_of(lengths, nq, q_lengths, offsets, causal), prefix=(3, prefix))
+    got = host(ops.attention_shared_prefix(dev(q), case.cache, 3, prefix, i32([-1, 7, 99, 2, 2, 2]), i32(lengths), max_kv_length=kv))
+    none = host(ops.attention_shared_prefix(dev(q), case.cache, 3, prefix, i32([2] * 6), i32([0, 0, 0] + lengths[3:]), max_kv_length=kv,
+                                            causal=False))
+    if nq == 1:
+        assert np.array_equal(got[:3], none[:3]) and got[:3].any()
+    bad = np.full((1, kv_heads, 1, dim), np.nan, np.float16)
+    ops.kv_append_int8(case.cache, dev(bad), dev(bad), 2, 69)         # request 3's last key
+    got = host(run())
+    assert np.isnan(got[3, :, -1]).all() and np.isfinite(np.delete(got, 3, 0)).all() and np.isfinite(got[3, :, :-1]).all()
+    ops.kv_append_int8(case.cache, dev(bad), dev(bad), 3, prefix - 1)  # every row's
+    assert np.isnan(host(run())).all()
+    if prefix < 500:
+        ops.kv_append_int8(case.cache, dev(case.k[3:4, :, prefix - 1:prefix]), dev(case.v[3:4, :, prefix - 1:prefix]), 3, prefix - 1)
+        ops.kv_append_int8(case.cache, dev(bad), dev(bad), 3, prefix)  # nobody's
+        assert np.isfinite(np.delete(host(run()), 3, 0)).all()
+
+
 @pytest.mark.parametrize("batch,heads,kv_heads,dim,nq,kv", [
     (8, 16, 16, 128, 64, 2000),         # rows for two blocks by their keys
     (2, 25, 25, 64, 90, 3000),

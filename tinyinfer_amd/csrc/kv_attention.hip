@@ -27,7 +27,8 @@
 // conflict-free kilobyte) while all work on this one, two buffers and one barrier a tile.
 // With few row blocks the keys are cut into splits as well, each split's state goes to the
 // caller's workspace and a second kernel joins them.  A prefix is one such set of splits,
-// its row blocks running over the whole batch: its keys are read once for all requests.
+// its row blocks running over the whole batch: its keys are read once for all requests (but
+// for a few short ones, whose rows walk it in front of their own keys: prefix_inline).
 //
 // What bounds it.  Single tokens: memory where caches are long (16 requests of 8 x 128,
 // 12000 to 32768 keys: 134 us, 6.0 TB/s; the loads are the plain ones of a stream,
@@ -136,14 +137,17 @@ struct Tiles {
   half8_t k[2][4][D / 32][64], v[2][D / 16][2][64];
 };
 
-// Row block `rb` of one set of keys.  PREFIX: rows run over the batch, key head
-// `head`, the keys are the prefix's; else over request b's.
+// Row block `rb` of one set of keys.  kPrefix: rows run over the batch, key head
+// `head`, the keys are the prefix's; else over request b's, the keys its own, behind the
+// prefix's for kBoth.
 // KW waves share the row block, each with its own tiles; kShared: 4 waves have a row
 // block each (`rb` counts those groups) and share every tile, each widening a quarter of
 // it into LDS while the tile before is worked on.
 constexpr int kShared = 0;
-template <int D, int QB, int KW, bool PREFIX>
+enum Keys { kOwn, kPrefix, kBoth };
+template <int D, int QB, int KW, Keys KEYS>
 __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb, int split, int splits, int state) {
+  constexpr bool PREFIX = KEYS == kPrefix, BOTH = KEYS == kBoth;
   const KvAttnArgs& a = p.a;
   const int lane = int(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
   const int j = lane & 15, g = lane >> 4;
@@ -163,6 +167,7 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
   // This lane's rows: block u, column j.
   int row_id[QB];  // in q's order, -1 past the last row
   int end[QB];     // keys [0, end) are visible
+  bool asks[QB];   // it has a query
 #pragma unroll
   for (int u = 0; u < QB; ++u) {
     const int r = r0 + 16 * u + j, rc = min(r, row_count - 1);
@@ -172,7 +177,8 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
     const int ql = a.q_lengths ? min(max(a.q_lengths[b], 0), a.q_len) : a.q_len;
     int64_t e = kv;
     if (!PREFIX && a.causal) e = min(e, (a.offsets ? int64_t(a.offsets[b]) : int64_t(kv) - ql) + qi + 1);
-    end[u] = r < row_count && qi < ql ? int(max(e, int64_t(0))) : 0;
+    asks[u] = r < row_count && qi < ql;
+    end[u] = asks[u] ? int(max(e, int64_t(0))) : 0;
   }
   // Keys that some row of the wave sees, and keys that every row of it with a query sees
   // (a row without one may compute anything: it is cleared at the end); keys that some
@@ -193,24 +199,25 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
     first = last == 0 ? 0 : seen(div_by(r0, p.group));
     group_last = KW == kShared ? last_of(group0, GROUP) : last;
   }
-  const int tiles = (group_last + kTile - 1) / kTile, per = (tiles + splits - 1) / splits;
+  // (kBoth: tiles [0, shift) are the prefix's.)
+  const int shift = BOTH ? (a.prefix_len + kTile - 1) / kTile : 0;
+  const int tiles = shift + (group_last + kTile - 1) / kTile, per = (tiles + splits - 1) / splits;
   const int t_end = min(tiles, (split + 1) * per);
   int t = split * per + (KW == kShared ? 0 : wave);
 
-  const int64_t base = (int64_t(slot) * a.cache.kv_heads + head) * a.cache.capacity;
-  const uint8_t* kp = a.cache.k + base * D;
-  const uint8_t* vp = a.cache.v + base * D;
+  // The first tile of the slot's head; kBoth: in front of it by `shift`, and the prefix's.
+  const int64_t base = (int64_t(slot) * a.cache.kv_heads + head) * (a.cache.capacity / kTile) - shift;
+  const int64_t prefix_base = (int64_t(a.prefix_slot) * a.cache.kv_heads + head) * (a.cache.capacity / kTile);
+  const auto tile_of = [&](int tt) { return (BOTH && tt < shift ? prefix_base : base) + tt; };
   const uint32_t k_lane = j * 64 + 16 * g, v_lane = lane * 16;
   // Lane (j, g) holds the scales of the tile's key 16 (j / 4) + 4 g + j % 4: of row g's
   // 16 scores of a tile, number 4 kb + v in order, lane 4 kb + v has the scale.
   const int my_key = 16 * (j >> 2) + 4 * g + (j & 3);
-  const float* ksp = a.cache.k_scales + base;
-  const float* vsp = a.cache.v_scales + base;
   // One block of rows (single tokens): memory has no use for the keys again, and a second
   // product with what the weights' rounding to fp16 leaves out costs nothing that shows,
   // so the result is as near as fp32 weights would bring it.  Two blocks (prompts) take
   // the rounded weights alone: a third less matrix work, 1.3 times the error.
-  constexpr bool NT = !PREFIX && QB == 1, FINE = QB == 1;
+  constexpr bool NT = KEYS == kOwn && QB == 1, FINE = QB == 1;
   // The next tile's K and scales are loaded once the scores have used this one's (one token
   // of 12 heads, 1000 keys: 8.0 us, 9.3 without; 32 of them 11.2 and 12.7), but for two
   // blocks of 64 dims, whose third wave per SIMD that would cost (12 pairs of 4096 rows:
@@ -226,20 +233,20 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
   // A tile's bytes, or this wave's quarter of them: 16 keys, and a quarter of the dims of
   // all values.
   auto load_k = [&](int tt) {
-    const uint8_t* at = kp + int64_t(tt) * (kTile * D) + (KW == kShared ? 16 * wave * D : 0);
+    const uint8_t* at = a.cache.k + tile_of(tt) * (kTile * D) + (KW == kShared ? 16 * wave * D : 0);
 #pragma unroll
     for (int kb = 0; kb < (KW == kShared ? 1 : 4); ++kb)
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) kr[kb][c] = load16<NT>(at + 16 * kb * D + 1024 * c + k_lane);
   };
   auto load_v = [&](int tt) {
-    const uint8_t* at = vp + int64_t(tt) * (kTile * D) + (KW == kShared ? 1024 * wave * (D / 64) : 0);
+    const uint8_t* at = a.cache.v + tile_of(tt) * (kTile * D) + (KW == kShared ? 1024 * wave * (D / 64) : 0);
 #pragma unroll
     for (int d = 0; d < (KW == kShared ? D / 64 : D / 16); ++d) vr[d] = load16<NT>(at + 1024 * d + v_lane);
   };
   auto load_scales = [&](int tt) {
-    ksr = (ksp + int64_t(tt) * kTile)[uint32_t(my_key)];
-    vsr = (vsp + int64_t(tt) * kTile)[uint32_t(my_key)];
+    ksr = (a.cache.k_scales + tile_of(tt) * kTile)[uint32_t(my_key)];
+    vsr = (a.cache.v_scales + tile_of(tt) * kTile)[uint32_t(my_key)];
   };
   auto share = [&](int buf) {
 #pragma unroll
@@ -266,7 +273,7 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
       for (int s = 0; s < 2; ++s) {
         half8_t x;
         __builtin_memcpy(&x, qp + 64 * c + 8 * s, 16);
-        qf[u][2 * c + s] = end[u] > 0 ? x : half8_t{};
+        qf[u][2 * c + s] = (BOTH ? asks[u] : end[u] > 0) ? x : half8_t{};
       }
   }
 
@@ -296,7 +303,9 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
   float unit = 0.f, inv_unit = 1.f;
 
   const auto tile = [&](int t, int buf, float ks, float vs_, auto after_scores) {
-    const bool full = (t + 1) * kTile <= first;
+    const bool of_prefix = BOTH && t < shift;
+    const int key0 = (t - (of_prefix ? 0 : shift)) * kTile;  // the tile's first key
+    const bool full = key0 + kTile <= (of_prefix ? a.prefix_len : first);
     float4_t sc[QB][4];
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
@@ -319,7 +328,7 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
     after_scores();
     const float ck = ks * p.scale;
     // (Past the last key any row sees, scales may be anything.)
-    const float vs = t * kTile + my_key < last ? vs_ : 0.f;
+    const float vs = key0 + my_key < (of_prefix ? a.prefix_len : last) ? vs_ : 0.f;
     if (__ballot(vs > unit)) {
       const float top = wave_max(vs);
       const float raised = __builtin_amdgcn_ldexpf(1.f, __builtin_amdgcn_frexp_expf(top));  // > top
@@ -336,7 +345,7 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
 #pragma unroll
     for (int u = 0; u < QB; ++u) {
       mul_row(sc[u], ck);
-      const int lim = end[u] - t * kTile - 4 * g;  // key 16 kb + v of this lane is visible iff < lim
+      const int lim = (of_prefix ? a.prefix_len : end[u]) - key0 - 4 * g;  // key 16 kb + v of this lane is visible iff < lim
       const auto mask = [&](float with) {
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb)
@@ -445,7 +454,7 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
   for (int u = 0; u < QB; ++u) {
     l[u] += __shfl_xor(l[u], 16, 64);
     l[u] += __shfl_xor(l[u], 32, 64);
-    if (end[u] == 0) l[u] = 0.f;
+    if (BOTH ? !asks[u] : end[u] == 0) l[u] = 0.f;
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) acc[u][d] *= unit;
   }
@@ -523,7 +532,9 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
 constexpr int waves_for(int dim, int qb) { return dim == 64 ? (qb == 1 ? 4 : 2) : (qb == 1 ? 2 : 2); }
 
 // QB, PB: row blocks of 16 per wave over the requests' own keys and the prefix's (0:
-// no prefix); KW: waves that share a row block's keys.
+// no prefix, kInline: walked in front of the own keys); KW: waves that share a row block's
+// keys.
+constexpr int kInline = -1;
 template <int D, int QB, int PB, int KW>
 __global__ __launch_bounds__(KW == kShared ? 256 : 64 * KW, waves_for(D, QB > PB ? QB : PB)) void kv_attention_kernel(AttnPlan p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -532,7 +543,7 @@ __global__ __launch_bounds__(KW == kShared ? 256 : 64 * KW, waves_for(D, QB > PB
   if constexpr (PB > 0) {
     if (id < p.prefix_wgs) {
       const int blocks = div_by(id, p.heads), split = div_by(blocks, p.prefix_block_div);
-      attend<D, PB, KW, true>(p, lds, 0, id - blocks * heads, blocks - split * int(p.prefix_block_div.d), split, p.prefix_splits,
+      attend<D, PB, KW, kPrefix>(p, lds, 0, id - blocks * heads, blocks - split * int(p.prefix_block_div.d), split, p.prefix_splits,
                               p.splits + split);
       return;
     }
@@ -542,7 +553,7 @@ __global__ __launch_bounds__(KW == kShared ? 256 : 64 * KW, waves_for(D, QB > PB
   // they are the longest.
   const int block = div_by(id, p.pairs), at = id - block * int(p.pairs.d), b = div_by(at, p.heads);
   const int split = div_by(block, p.row_block_div), blocks = int(p.row_block_div.d);
-  attend<D, QB, KW, false>(p, lds, b, at - b * heads, blocks - 1 - (block - split * blocks), split, p.splits, split);
+  attend<D, QB, KW, PB == kInline ? kBoth : kOwn>(p, lds, b, at - b * heads, blocks - 1 - (block - split * blocks), split, p.splits, split);
 }
 
 // W waves of a workgroup of 4 join a row's states: D / 4 lanes a state, 2 or 4 states at a
@@ -658,6 +669,17 @@ Walk prefix_walk_for(int heads, int64_t rows, int keys) {
   return w;
 }
 
+// Whether every request walks the prefix in front of its own keys by itself: one launch in
+// place of two, no workspace and no states, where that is little work.  By itself against
+// shared, us: 12 heads of 64, prefix 700, 1 / 8 / 32 / 64 requests 7.1 / 7.3 / 10.0 / 13.1 and
+// 8.5 / 8.7 / 9.5 / 9.8 (but for 32 the second launch's 4 us of the caller's time are saved);
+// prefix 960, 32 requests 11.6 and 9.1; 1500, 4 requests 10.8 and 8.4; 8 heads of 128, 700,
+// 64 requests 14.4 and 16.2, 200, 10.1 and 13.5.
+bool prefix_inline(int64_t pairs, int rows, int keys, int prefix, int dim) {
+  const int64_t tiles = ceil_div(keys, kTile) + ceil_div(prefix, kTile);
+  return rows <= 16 && tiles <= 16 && pairs * tiles <= (dim == 64 ? 5000 : 6500);
+}
+
 AttnPlan plan_of(const KvAttnArgs& a, Walk& own, Walk& prefix) {
   AttnPlan p{};
   p.a = a;
@@ -671,7 +693,10 @@ AttnPlan plan_of(const KvAttnArgs& a, Walk& own, Walk& prefix) {
   p.all_rows = pairs * rows;
   own = walk_for(pairs, rows, a.max_kv, a.cache.head_dim);
   prefix = Walk{0, 4, 0};
-  if (a.prefix_len > 0) {
+  if (a.prefix_len > 0 && prefix_inline(pairs, rows, a.max_kv, a.prefix_len, a.cache.head_dim)) {
+    own = Walk{1, 4, 1};
+    prefix.blocks = kInline;
+  } else if (a.prefix_len > 0) {
     const int64_t all = int64_t(a.batch) * rows;
     prefix = prefix_walk_for(a.cache.kv_heads, all, a.prefix_len);
     own.waves = 4;
@@ -713,6 +738,7 @@ hipError_t launch_walk(const AttnPlan& p, const Walk& own, const Walk& prefix, h
   if (own.waves == kShared) return launch<D, 2, 0, kShared>(p, stream);
   if (own.waves == 2) return launch<D, 2, 0, 2>(p, stream);
   if (own.blocks == 1) {
+    if (prefix.blocks == kInline) return launch<D, 1, kInline, 4>(p, stream);
     if (prefix.blocks == 0) return launch<D, 1, 0, 4>(p, stream);
     return prefix.blocks == 1 ? launch<D, 1, 1, 4>(p, stream) : launch<D, 1, 2, 4>(p, stream);
   }
