@@ -155,7 +155,8 @@ int ti_amd_kv_read_i8(const ti_amd_kv_i8* cache, uint16_t* k, uint16_t* v, const
  * that see no key, and queries past q_lengths[b], are exactly 0.  batch and heads
  * are at most 65535, batch * heads * q_len at most 2^23.
  * prefix_len > 0: in front of its own keys every query also sees tokens 0 ..
- * prefix_len - 1 of prefix_slot, whose bytes are read once for the batch.
+ * prefix_len - 1 of prefix_slot, whose bytes are read once for the batch (a short
+ * prefix of a few requests by each of them).
  * Scores, softmax and sums are fp32; probabilities are rounded to fp16 (where few
  * rows share the keys twice: what the first rounding leaves out is added).  How rows
  * and keys are divided follows from the shape arguments, so a request's last bits

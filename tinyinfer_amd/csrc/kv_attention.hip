@@ -635,9 +635,10 @@ struct Walk {
 // two waves share a row block, or four where keys are many (12 pairs of 4096 rows: 51 us,
 // 60 with two, 81 with shared tiles; 24 pairs of 2048 rows without a mask: 52, 50, 61; 16
 // pairs of 3108 rows over 6001 keys, D 128: 205, 224, 212).
-// Splits: a second launch and the states' traffic cost 2 us and more, so short caches
-// are not split (96 pairs, 1024 keys: 8.4 us, 9.4 in four; 12 pairs, 7.6 and 7.8).  Longer
-// ones are, into at most one workgroup a CU (8 pairs of 16000 keys, D 128: 13.3 us in 256
+// Splits: a second launch and the states' traffic cost 2 us and more, and 4 us of the
+// caller's time, so short caches are not split (96 pairs, 1024 keys: 8.4 us, 9.4 in four; 12
+// pairs, 7.6 and 7.8, of 1500 keys 9.5 and 8.3; 8 of 1024, D 128, 9.7 and 8.7).  Longer ones
+// are, into at most one workgroup a CU (8 pairs of 16000 keys, D 128: 13.3 us in 256
 // workgroups, 17 in 320 or 512; 24 of 60000: 65 in 192, 87 in 264) and 64 splits (one pair
 // of 100000 keys: 21 us, 25 in 256), but where the pairs alone take more than half of the
 // CUs into about 512 (160 pairs of 10000 to 20000 keys: 114 us, 130 whole; 272 of 4000 to
@@ -651,7 +652,7 @@ Walk walk_for(int64_t pairs, int rows, int keys, int dim) {
     return w;
   }
   const int64_t wgs = pairs * ceil_div(rows, 16 * w.blocks);
-  if (tiles > 16)
+  if (tiles > (dim == 64 ? 24 : 16))
     w.splits = int(wgs > 128 && tiles >= 64 ? ceil_div(512, wgs) : std::max<int64_t>(1, std::min<int64_t>({256 / wgs, tiles / 4, 64})));
   return w;
 }

@@ -536,7 +536,7 @@ class NativeOps:
                                 query_offsets=None, causal=True, max_kv_length=None):
         """``attention_int8kv`` for a batch whose requests share a prefix: in front of its
         own keys every query sees tokens 0 .. prefix_length - 1 (host ints) of
-        prefix_slot, which are read once for the whole batch.  kv_lengths and
+        prefix_slot, which are read once for the whole batch where that is the faster way.  kv_lengths and
         query_offsets count the request's own tokens."""
         if type(cache) is not Int8KVCache:
             raise TypeError("cache: an Int8KVCache (NativeOps.kv_cache_int8) is required")
