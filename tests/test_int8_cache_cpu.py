@@ -85,7 +85,8 @@ def test_workspace_query(cpu_ops, cache):
     assert whole > 0 and whole % (2 * (64 + 2) * 4) == 0
     assert ask(at, 1, 2, 1, 1 << 20, 0) == whole                   # a bound past the capacity is the capacity
     assert 0 <= ask(at, 1, 2, 1, 64, 0) < whole
-    assert ask(at, 4, 2, 1, 64, 0) == 0 < ask(at, 4, 2, 1, 64, 64)  # a prefix's states always join others
+    assert ask(at, 4, 2, 1, 64, 0) == 0 == ask(at, 4, 2, 1, 64, 64)  # a short prefix is walked with the own keys,
+    assert ask(at, 4, 2, 1, 64, 4096) > 0                           # a long one's states join theirs
     for args in ((0, 2, 1, 0, 0), (1, 3, 1, 0, 0), (1, 0, 1, 0, 0), (1, 2, 0, 0, 0), (65536, 2, 1, 0, 0),
                  (1, 2, 1, -1, 0), (1, 2, 1, 0, -1), (1, 2, 1, 0, (1 << 16) + 1), (65535, 65534, 2, 0, 0)):
         assert ask(at, *args) == -1, args
