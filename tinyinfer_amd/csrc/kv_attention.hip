@@ -37,7 +37,7 @@
 // products.  Of a tile of 64 keys x 32 rows at D 128 the 64 matrix instructions are 1024
 // cycles of a SIMD; widening K and V is 192 vector instructions and a score takes 6 and an
 // exponential, 1900 cycles together.  2 requests of 777 queries, 32 heads over 8 of 128,
-// 4500 to 6001 keys: 197 us, 686 TFLOP/s; 4 prompts of 1024, 25 heads of 64: 30 us, 445
+// 4500 to 6001 keys: 195 us, 690 TFLOP/s; 4 prompts of 1024, 25 heads of 64: 30 us, 445
 // TFLOP/s, its scores' exponentials and scales more than the products.
 #include <algorithm>
 

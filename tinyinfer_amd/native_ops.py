@@ -490,7 +490,7 @@ class NativeOps:
         self._batch_rows(batch, slots, positions, lengths, rows, cache)
         shape = (batch, cache.kv_heads, rows, cache.head_dim)
         k = call.output(shape, torch.float16)
-        v = call.output(shape, torch.float16)
+        v = call.output_like(k)
         call.per_request(batch, (slots, cache.slots - 1, "slots"), (positions, cache.capacity - 1, "positions"),
                          (lengths, rows, "lengths"))
         call.scalars(batch, rows)
