@@ -12,6 +12,7 @@
 #include "../../include/tinyinfer_amd_ext.h"
 #include "../../include/tinyinfer_backend_v2.h"
 #include "kernels.hpp"
+#include "sample_bins.hpp"
 
 namespace {
 
@@ -557,7 +558,7 @@ extern "C" int ti_amd_sample(const void* logits, int dtype, const float* uniform
   if (status) return status;
   if ((dtype != TI_V2_FP16 && dtype != TI_V2_FP32) || !aligned(logits, dtype == TI_V2_FP16 ? 2 : 4) || !aligned(uniforms, 4) ||
       !optional_aligned(temperature, 4) || !optional_aligned(top_k, 4) || !optional_aligned(top_p, 4) ||
-      !optional_aligned(min_p, 4) || !aligned(tokens, 4) || !aligned(probs, 4) || vocab > (1 << 18) || batch > (1 << 20) ||
+      !optional_aligned(min_p, 4) || !aligned(tokens, 4) || !aligned(probs, 4) || vocab > tia::sample_bins::kVocabMax || batch > (1 << 20) ||
       !shape_fits({batch, vocab}, 4))
     return fail(TI_V2_INVALID_ARGUMENT, "invalid sampling arguments: fp16 or fp32 logits, at most 2^20 rows of 2^18");
   tia::SampleArgs a;

@@ -11,9 +11,9 @@
 // over the distance from the maximum, 256 bins to a unit of (max - logit) / T,
 // finds the bin in which a count or a mass is reached, and only the tokens of the
 // few bins in question are gathered and ordered.  A token of bin b at distance
-// (b + f) / 256 weighs e^(-b/256) (1 - q), q = 1 - e^(-f/256) < 2^-8: bins hold
-// their count and the sum of q in units of 2^-35, one 64-bit LDS addition per token,
-// and masses are whole numbers of 2^-44: sums are the same in any order, and an
+// (b + f) / 256 weighs e^(-b/256) (1 - q), q = 1 - e^(-f/256) < 1.02 * 2^-8: bins hold
+// their count and the sum of q in units of 2^-34, one 64-bit LDS addition per token (a bin
+// that holds the whole vocabulary fits: sample_bins.hpp), and masses are whole numbers of 2^-44: sums are the same in any order, and an
 // answer depends on its row alone.  A token's mass is right to about 2^-31 of itself, so
 // the token is the one that 64-bit arithmetic gives but for a random number within
 // about 1e-10 of a border.  Tokens 32 units from the maximum (e^-32) weigh nothing.
@@ -34,11 +34,12 @@
 #include "common.hpp"
 #include "kernels.hpp"
 #include "lds_limit.hpp"
+#include "sample_bins.hpp"
 
 namespace tia {
 namespace {
 
-typedef unsigned long long u64;
+using namespace sample_bins;
 
 constexpr int kThreads = 1024, kPerThread = 8, kBins = kThreads * kPerThread, kList = 512, kRuns = 2048;
 // A top-k up to which a row may be sampled in one pass: half of what the list holds, so
@@ -49,10 +50,6 @@ constexpr unsigned kShort = 256;
 // 14.2; of 10000, 13.2 and 17.2, 18.2 and 17.3; of 20000, 13.3 and 18.9, 18.2 and 19.1; 32
 // rows of 50257, 14.9 and 30.8, 19.7 and 30.6.
 __device__ __forceinline__ bool is_short(unsigned k, unsigned vocab) { return k <= kShort && k < vocab && k * k / 4 <= vocab; }
-constexpr double kPerUnit = 256.0;  // bins per unit of (max - logit) / T
-constexpr int kCountShift = 45;     // a bin: count << 45 | sum of q
-constexpr u64 kOne = u64(1) << 35;  // weight of a token at its bin's near edge
-constexpr double kMass = 512.0;     // a mass: weight * e^(-b/256) * 2^9
 constexpr int kNoToken = 0x7fffffff;
 constexpr float kNegInf = -__builtin_huge_valf();
 // Place of a bin in LDS: a thread's kPerThread bins are followed by a gap, so that the
@@ -214,26 +211,13 @@ struct Scale {
   }
   // Not below kBins for -inf, neither below nor above for NaN.
   __device__ __forceinline__ float distance(float x) const { return (top - x) * per; }
-  // The part of the distance behind its bin's near edge: in [-2^-10, 1 + 2^-10].
+  // The part of the distance behind its bin's near edge: in [-kFraction, 1 + kFraction].
   __device__ __forceinline__ float fraction(float x) const {
     const float d = top - x, back = d - top, rest = (top - (d - back)) - (x + back);
     return fmaf(d, per, -floorf(d * per)) + fmaf(d, per_rest, rest * per);
   }
   __device__ __noinline__ double weight_of(float x) const { return exp((double(x) - double(top)) / temp); }
 };
-// (1 - e^(-f/256)) 2^35 of a fraction f, made positive by f + kSlack, to its terms of
-// third order (the fourth is below 2^-36); a bin's near edge is kSlack in front of it.
-constexpr float kSlack = 1.f / 64;
-__device__ __forceinline__ unsigned loss(float fraction) {
-  constexpr double h = 1.0 / kPerUnit, one = double(kOne);
-  const float f = fraction + kSlack;
-  return unsigned(f * fmaf(f, fmaf(f, float(one * h * h * h / 6), float(-one * h * h / 2)), float(one * h)));
-}
-__device__ __forceinline__ u64 packed(float fraction) { return (u64(1) << kCountShift) + loss(fraction); }
-__device__ __forceinline__ unsigned count_of(u64 packed) { return unsigned(packed >> kCountShift); }
-__device__ __forceinline__ u64 weight_of(u64 packed) {
-  return count_of(packed) * kOne - (packed & ((u64(1) << kCountShift) - 1));
-}
 // e^(-i/256)
 __device__ __forceinline__ double step(int i) {
   constexpr double k[kPerThread] = {1.0, 0.9961013694701175, 0.9922179382602435, 0.9883496471138451,
