@@ -71,7 +71,7 @@ struct SampleLds {
   float wave_max[kThreads / 64];
   int wave_at[kThreads / 64];
   u64 low, high, answer_key, answer_mass;
-  unsigned answer_count, list_count;
+  unsigned answer_count, list_count, claims[3];  // (a claim per goal of a row: top-k, top-p, the random number)
 };
 
 // 64-bit key whose ascending order is the row's: value descending, then index.
@@ -282,7 +282,8 @@ __device__ void scan(SampleLds& s, u64& mass_all, unsigned& count_all) {
 }
 
 // What a position is asked by: the first token whose count or mass, with all in
-// front of it, reaches `goal` (goal >= 1, and at most the total).
+// front of it, reaches `goal` (goal >= 1, and at most the total), which is the last one
+// that begins in front of it.
 struct Goal {
   bool by_count;
   u64 goal;
@@ -364,16 +365,20 @@ struct Gathered {
     before = s.mass[slot(bin)] + mass_of(front, e);
     after = s.mass[slot(bin)] + mass_of(front + kOne - s.q[t], e);
   }
-  __device__ __forceinline__ Place resolve(SampleLds& s, unsigned of, const Goal& g) const {
-    if (bin == of && (g.by_count ? rank : before) < g.goal && g.goal <= (g.by_count ? rank + 1 : after)) {
-      s.answer_key = key;
-      s.answer_mass = after;
-      s.answer_count = rank + 1;
+  // Goal number `which` of the row (its claim is still 0).  Without any token gathered from
+  // the bin the row's first one stands for all.
+  __device__ __forceinline__ Place resolve(SampleLds& s, unsigned of, const Goal& g, int which) const {
+    const unsigned claim = bin == of ? claim_of(g.by_count ? rank : before, g.goal, rank, threadIdx.x) : 0;
+    if (claim) atomicMax(&s.claims[which], claim);
+    __syncthreads();  // (the answer in front of this one has been read)
+    const unsigned best = s.claims[which];
+    if (threadIdx.x == claimant(best)) {
+      s.answer_key = best ? key : 0;
+      s.answer_mass = best ? after : s.mass[slot(of)] + 1;
+      s.answer_count = best ? rank + 1 : s.count[slot(of)] + 1;
     }
     __syncthreads();
-    const Place got{s.answer_mass, s.answer_count, s.answer_key};
-    __syncthreads();
-    return got;
+    return Place{s.answer_mass, s.answer_count, s.answer_key};
   }
 };
 
@@ -454,10 +459,10 @@ __device__ __noinline__ Gathered gather(SampleLds& s, const Row<T>& row, const S
 
 template <typename T>
 __device__ __forceinline__ Place locate(SampleLds& s, const Row<T>& row, const Scale& sc, Gathered& mine, const Goal& g,
-                                        unsigned count_all) {
+                                        unsigned count_all, int which) {
   const unsigned bin = find_bin(s, g);
   if (!is_wanted(s, bin)) mine = gather(s, row, sc, g, bin, count_all);
-  return mine.resolve(s, bin, g);
+  return mine.resolve(s, bin, g, which);
 }
 
 
@@ -678,6 +683,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   const Scale sc(top, temp);
   for (unsigned i = unsigned(t); i < slot(kBins); i += kThreads) s.bin[i] = 0;
   if (t < kBins / 32) s.wanted[t] = 0;
+  if (t < 3) s.claims[t] = 0;
   if (t == 0) s.list_count = 0;
   __syncthreads();
   row.template each<4>([&](float x, int) {
@@ -771,12 +777,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   u64 kept = mass_all;
   unsigned length = count_all;
   if (use_k) {
-    const Place p = locate(s, row, sc, mine, Goal{true, u64(top_k)}, count_all);
+    const Place p = locate(s, row, sc, mine, Goal{true, u64(top_k)}, count_all, 0);
     kept = p.mass;
     length = p.count;
   }
   if (use_p) {
-    const Place p = locate(s, row, sc, mine, goal_p(top_p, kept), count_all);
+    const Place p = locate(s, row, sc, mine, goal_p(top_p, kept), count_all, 1);
     kept = p.mass;
     length = p.count;
   }
@@ -802,7 +808,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     __syncthreads();
     if (n < length) kept = n == 0 ? mass_of(kOne - loss(0.f), run_edge(0)) : m;  // (n = 0: min_p above 1)
   }
-  const Place p = locate(s, row, sc, mine, goal_u(u, kept), count_all);
+  const Place p = locate(s, row, sc, mine, goal_u(u, kept), count_all, 2);
   if (t == 0) {
     const int token = int(p.key & 0xffffffffu);
     a.tokens[b] = token;

@@ -37,5 +37,16 @@ static_assert(u64(kVocabMax) * loss(1.f + kFraction) < u64(1) << kCountShift, "t
 static_assert(u64(kVocabMax) <= ~u64(0) >> kCountShift, "the count of a bin");
 static_assert(double(kVocabMax) * double(kOne) * kMass < 9.2e18, "the mass of a row");
 
+// The place a goal asks for is the last token that begins in front of it.  What a gathered
+// token, number `thread` of at most 1024, of `rank` in its row's order, claims: 0 if it
+// begins at the goal or behind, else the more the later it stands.  The largest claim wins,
+// so there is a place wherever masses that disagree would end (a token in front of the goal
+// is enough), and it is a gathered token.
+constexpr unsigned claim_of(u64 begin, u64 goal, unsigned rank, unsigned thread) {
+  return begin < goal ? (rank + 1) << 10 | thread : 0;
+}
+constexpr unsigned claimant(unsigned claim) { return claim & 1023; }
+static_assert(unsigned(kVocabMax) <= ~0u >> 10, "a rank in a claim");
+
 }  // namespace sample_bins
 }  // namespace tia
