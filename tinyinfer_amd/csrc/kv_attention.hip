@@ -1,11 +1,13 @@
 // Attention over the int8 KV cache for gfx950: single tokens, prompts, and a
 // prefix that a batch shares, by one kernel.
 //
-//   o[r] = sum_j p_rj V_j / sum_j p_rj,  p_rj = 2^(x_rj - m_r),
+//   o[r] = sum_j w_rj d_j / sum_j p_rj,  p_rj = 2^(x_rj - m_r),  w_rj = p_rj vs_j,
 //   x_rj = (q_r . c_j) * ks_j * D^-1/2 * log2 e,  V_j = vs_j * d_j
 // with c, d the whole numbers that the cache holds (exact in fp16) and ks, vs the
 // fp32 scales of token j: a key's scale is applied to its score, a value's to its
-// probability, so neither c nor d is rounded.
+// probability, so neither c nor d is rounded.  The weights w are, to fp16: the reference m_r
+// follows the largest x + log2 vs of the keys that row r sees, not the largest x, so the
+// rounding is relative to what the row weighs, whatever values others see.
 //
 // A query row is (request, query, query head of the key head's group): the rows
 // of a group share their keys, so they fill the 16 columns of a matrix operand.
@@ -50,11 +52,12 @@ namespace {
 
 constexpr int kTile = 64;   // keys per wave and step
 constexpr float kNegInf = -__builtin_huge_valf();
-// The reference of a row's exponents: 6 below its largest score when set, raised
-// when a score is 14 above it.  Probabilities then lie around 2^6 and below 2^14:
-// rounded to fp16, whose smallest normal number is 2^-14, a key 2^-20 times as
-// heavy as the heaviest still keeps 11 bits.
-constexpr float kBelow = 6.f, kRaise = 14.f;
+// The reference of a row's exponents: 6 below its largest x + log2 vs when set, raised
+// when one is 14 above it.  Weights then lie around 2^6 and below 2^14: rounded to
+// fp16, whose smallest normal number is 2^-14, a weight 2^-20 times the heaviest
+// still keeps 11 bits.  The scale of a row of zeros counts as 2^kLeast, below every
+// other (2^-24 / 127 at least): probabilities are fp32 and stay below 2^(14 - kLeast).
+constexpr float kBelow = 6.f, kRaise = 14.f, kLeast = -40.f;
 
 // n / d for 0 <= n < 2^31 by a multiplication: with 2^(shift-1) < d <= 2^shift and mul =
 // floor(2^32 (2^shift - d) / d) + 1, n / d = (hi32(n mul) + n) >> shift.
@@ -109,6 +112,10 @@ __device__ __forceinline__ float mul_row_lane(float x, float of) {
   const float y = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, of), 0x150 + N, 0xF, 0xF, true));
   return x * y;
 }
+template <int N>
+__device__ __forceinline__ float add_row_lane(float x, float of) {
+  return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, of), 0x150 + N, 0xF, 0xF, true));
+}
 // x[kb][v] times lane 4 kb + v's value.
 __device__ __forceinline__ void mul_row(float4_t (&x)[4], float of) {
 #define TIA_MUL(kb, v) x[kb][v] = mul_row_lane<4 * kb + v>(x[kb][v], of);
@@ -116,6 +123,17 @@ __device__ __forceinline__ void mul_row(float4_t (&x)[4], float of) {
   TIA_MUL4(0) TIA_MUL4(1) TIA_MUL4(2) TIA_MUL4(3)
 #undef TIA_MUL4
 #undef TIA_MUL
+}
+
+// The largest x[kb][v] + lane 4 kb + v's value.
+__device__ __forceinline__ float max_row_sum(const float4_t (&x)[4], float of) {
+  float high = kNegInf;
+#define TIA_MAX(kb, v) high = fmaxf(high, add_row_lane<4 * kb + v>(x[kb][v], of));
+#define TIA_MAX4(kb) TIA_MAX(kb, 0) TIA_MAX(kb, 1) TIA_MAX(kb, 2) TIA_MAX(kb, 3)
+  TIA_MAX4(0) TIA_MAX4(1) TIA_MAX4(2) TIA_MAX4(3)
+#undef TIA_MAX4
+#undef TIA_MAX
+  return high;
 }
 
 template <bool NT>
@@ -298,9 +316,10 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) acc[u][d] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
-  // O is kept in units of `unit`, a power of two not below any value scale seen:
-  // the weight p * vs / unit that is rounded to fp16 is then at most p.
-  float unit = 0.f, inv_unit = 1.f;
+  // A bound on the value scales so far, those of keys that only some rows see among them: a
+  // row's largest score is `room` above its reference, or more, before x + log2 vs can be
+  // kRaise above it.  It only spares the exact sums.
+  float bound = 0.f, room = kRaise - kLeast;
 
   const auto tile = [&](int t, int buf, float ks, float vs_, auto after_scores) {
     const bool of_prefix = BOTH && t < shift;
@@ -329,18 +348,11 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
     const float ck = ks * p.scale;
     // (Past the last key any row sees, scales may be anything.)
     const float vs = key0 + my_key < (of_prefix ? a.prefix_len : last) ? vs_ : 0.f;
-    if (__ballot(vs > unit)) {
-      const float top = wave_max(vs);
-      const float raised = __builtin_amdgcn_ldexpf(1.f, __builtin_amdgcn_frexp_expf(top));  // > top
-      const float f = unit / raised;
-      unit = raised;
-      inv_unit = 1.f / raised;
-#pragma unroll
-      for (int u = 0; u < QB; ++u)
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d) acc[u][d] *= f;
+    if (__ballot(vs > bound)) {
+      const int e = __builtin_amdgcn_frexp_expf(wave_max(vs));
+      bound = __builtin_amdgcn_ldexpf(1.f, e);  // > every scale
+      room = kRaise - fmaxf(float(e), kLeast);
     }
-    const float wv = vs * inv_unit;
     half8_t pp[QB][2], rest[2];
 #pragma unroll
     for (int u = 0; u < QB; ++u) {
@@ -358,7 +370,8 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
       for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
         for (int v = 0; v < 4; ++v) high = fmaxf(high, sc[u][kb][v]);
-      if (__ballot(high > m[u] + kRaise)) {
+      if (__ballot(high > m[u] + room)) {
+        high = max_row_sum(sc[u], fmaxf(__builtin_amdgcn_logf(vs), kLeast));
         high = fmaxf(high, __shfl_xor(high, 16, 64));
         high = fmaxf(high, __shfl_xor(high, 32, 64));
         const float nm = high > m[u] + kRaise ? high - kBelow : m[u];
@@ -376,7 +389,7 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
           sc[u][kb][v] = __builtin_amdgcn_exp2f(sc[u][kb][v] - ref);
           l[u] += sc[u][kb][v];
         }
-      mul_row(sc[u], wv);
+      mul_row(sc[u], vs);
       if (!full) mask(0.f);  // (0 times a scale that is not finite)
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb)
@@ -455,8 +468,6 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
     l[u] += __shfl_xor(l[u], 16, 64);
     l[u] += __shfl_xor(l[u], 32, 64);
     if (BOTH ? !asks[u] : end[u] == 0) l[u] = 0.f;
-#pragma unroll
-    for (int d = 0; d < D / 16; ++d) acc[u][d] *= unit;
   }
   // Dims 16 d + 4 g .. + 3 of row (u, j), of `total` weight at exponent reference `top`.
   const auto put = [&](int u, int d, float4_t o, float total) {
