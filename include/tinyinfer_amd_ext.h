@@ -119,9 +119,9 @@ int ti_amd_layernorm_softmax_f32(const float* x, const float* gamma, const float
 
 /* The int8 KV cache: no counterpart in the reference, whose caches are fp16.
  * A row of head_dim fp16 values (one token, one key head) is held as head_dim
- * bytes and one fp32 scale = fp32_rn(max|x| / 127) (1 for a row of zeros, NaN
+ * bytes and one fp32 scale = fp32_rn(max|x| / 127) (so 0 for a row of zeros; NaN
  * for a row with an infinity or NaN, which then reads as NaN); its value is
- * c * scale with c the whole number nearest x / scale, ties to even.  The caller
+ * c * scale with c the whole number nearest x / scale, ties to even (0 in a row of zeros).  The caller
  * owns the buffers, all 16-byte aligned: k and v of slots * kv_heads * capacity *
  * head_dim bytes, k_scales and v_scales of slots * kv_heads * capacity floats.
  * Their inner order is the kernels' own (k's rows one after another, v in blocks

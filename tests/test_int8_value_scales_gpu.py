@@ -135,3 +135,63 @@ def test_values_of_a_prefix_and_of_own_tokens(ops, batch, heads, kv_heads, dim, 
         lengths = [int(x) for x in rng.integers(0, kv, batch)]
         got = ops.attention_shared_prefix(dev(q), filled.cache, batch, prefix, list(range(batch)), i32(lengths), max_kv_length=kv)
         check(got, q, filled, range(batch), ends_of(lengths, nq), rng, 60, prefix=(batch, prefix))
+
+
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,nq,kv", PLANS)
+@pytest.mark.parametrize("score", [8, 60])
+def test_value_rows_of_zeros(ops, score, batch, heads, kv_heads, dim, nq, kv):
+    """Heavy tokens whose values are all 0 beside light ones of small values."""
+    say("zero values", score, batch, heads, kv_heads, dim, nq, kv)
+    rng = np.random.default_rng(batch + nq + dim + score)
+    way = rng.standard_normal(dim)
+    way *= math.sqrt(dim) / np.linalg.norm(way)
+    k = rng.standard_normal((batch, kv_heads, kv, dim)) * 0.3
+    v = rng.choice([-1, 1], (batch, kv_heads, kv, dim)) * 2.0 ** -10
+    zero = [3, kv // 2, kv - 2] if score == 8 else list(range(64, 128)) + [kv - 1]
+    k[:, :, zero] += score / math.sqrt(dim) * way
+    v[:, :, zero] = 0
+    filled = Filled(ops, k.astype(np.float16), v.astype(np.float16))
+    q = (way + 0.1 * rng.standard_normal((batch, heads, nq, dim))).astype(np.float16)
+    slots = rng.permutation(batch)
+    got = ops.attention_int8kv(dev(q), filled.cache, i32(slots), [kv] * batch, causal=nq > 1)
+    check(got, q, filled, slots, ends_of([kv] * batch, nq, causal=nq > 1), rng, 60)
+    k[...], v[...] = 1, 0                   # nothing but zeros
+    filled = Filled(ops, k.astype(np.float16), v.astype(np.float16))
+    assert not host(ops.attention_int8kv(dev(q), filled.cache, i32(slots), [kv] * batch)).any()
+
+
+@pytest.mark.parametrize("prefix,own", [(200, 50), (4000, 50)])
+def test_a_prefix_of_zeros(ops, prefix, own):
+    """Zero values, and rows never written, in front of own tokens of small values."""
+    say("zero prefix", prefix, own)
+    rng = np.random.default_rng(prefix)
+    batch, heads, dim = 4, 4, 64
+    k = rng.standard_normal((batch + 2, heads, prefix, dim)) * 0.3
+    v = rng.choice([-1, 1], (batch + 2, heads, prefix, dim)) * 2.0 ** -10
+    v[batch] = 0
+    k[batch + 1], v[batch + 1] = 0, 0       # what a slot that was never written stands for
+    k, v = k.astype(np.float16), v.astype(np.float16)
+    filled = Filled(ops, k, v)
+    filled.cache = ops.kv_cache_int8(batch + 2, heads, prefix, dim)
+    ops.kv_append_int8(filled.cache, dev(k[:-1]), dev(v[:-1]), list(range(batch + 1)), 0)
+    q = rng.standard_normal((batch, heads, 1, dim)).astype(np.float16)
+    for slot in (batch, batch + 1):
+        got = ops.attention_shared_prefix(dev(q), filled.cache, slot, prefix, [0, 1, 2, 3], own, max_kv_length=own)
+        check(got, q, filled, range(batch), ends_of([own] * batch, 1), rng, 16, prefix=(slot, prefix))
+        assert not host(ops.attention_shared_prefix(dev(q), filled.cache, slot, prefix, [batch] * 4, own)).any()
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+def test_a_row_of_zeros_has_the_scale_0(ops, rows):
+    """fp32_rn(max|x| / 127) as for every other row, negative zeros too; it reads as 0."""
+    say("zero scale", rows)
+    cache = ops.kv_cache_int8(1, 2, 64, 64)
+    x = np.ones((1, 2, rows, 64), np.float16)
+    x[0, 0, 1], x[0, 1, 2] = 0.0, -0.0
+    ops.kv_append_int8(cache, dev(x), dev(x), 0, 7)
+    size = 2 * 64 * 64
+    scales = host(cache.buffer)[2 * size:].view(np.float32).reshape(2, 2, 64)[:, :, 7:7 + rows]
+    want = np.where(x[0].any(-1), np.float32(1) / np.float32(127), np.float32(0))
+    assert np.array_equal(scales[0], want) and np.array_equal(scales[1], want)
+    for y in ops.kv_read_int8(cache, 0, 7, rows, rows):
+        assert np.array_equal(host(y), np.abs(x)) and not np.signbit(host(y)).any()

@@ -2,9 +2,10 @@
 //
 // A row x of D fp16 values (one token, one head) is held as D bytes c + 128 and
 // one fp32 scale s:
-//   s = fp32_rn(max|x| / 127), 1 for a row of zeros, NaN for a row with an
-//       infinity or NaN (whose bytes are those of c = 0), so that what reads it
-//       answers NaN instead of a number the row does not stand for;
+//   s = fp32_rn(max|x| / 127), so 0 for a row of zeros (a scale that no other row's
+//       weight is rounded against), NaN for a row with an infinity or NaN, so that what
+//       reads it answers NaN instead of a number the row does not stand for (the bytes
+//       of both are those of c = 0);
 //   c = the whole number nearest x / s, ties to even, |c| <= 127.
 // The quotient is decided exactly: t = x * rcp(s) is off by less than 2^-15, so
 // rint(t) is right unless t lies that near half way between whole numbers; then q =
@@ -54,11 +55,11 @@ __device__ __forceinline__ unsigned row_top(u16x8_t x) {
 }
 
 struct RowScale {
-  float s, inv;  // inv 0 for a row with a non-finite value: every byte 128
+  float s, inv;  // inv 0 for a row of zeros or with a non-finite value: every byte 128
 };
 __device__ __forceinline__ RowScale row_scale(unsigned top) {
   if (top >= 0x7c00u) return {__builtin_nanf(""), 0.f};
-  if (top == 0) return {1.f, 1.f};
+  if (top == 0) return {0.f, 0.f};
   const float s = h2f(uint16_t(top)) / 127.f;
   return {s, __builtin_amdgcn_rcpf(s)};
 }
