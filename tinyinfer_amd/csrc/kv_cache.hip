@@ -220,7 +220,8 @@ __global__ __launch_bounds__(256) void append_block_kernel(KvAppendArgs a) {
   }
 }
 
-__device__ __forceinline__ uint16_t value_of(unsigned byte, float s) { return f2h(float(int(byte) - 128) * s); }
+// (+ 0: a byte that was never written, -128, times its scale of 0 is -0.)
+__device__ __forceinline__ uint16_t value_of(unsigned byte, float s) { return f2h(float(int(byte) - 128) * s + 0.f); }
 
 // Rows [0, rows) of every request: token positions[b] + i, zeros where i is past
 // lengths[b] or the token is outside the cache.  A workgroup takes one request's,
