@@ -182,9 +182,11 @@ int ti_amd_attention_i8kv(const ti_amd_kv_i8* cache, const uint16_t* q, uint16_t
  * uniforms[b], probs[b] its probability among them.  A temperature that is not
  * above 0, or a logit of +inf, gives the likeliest token with probability 1; a
  * row without a logit above -inf gives 2^31 - 1 with probability 0.  NaN logits
- * are never chosen.  temperature, top_k, top_p and min_p are per row on the
- * device, or null: then the *_all values hold for every row.  The answer depends
- * on nothing but its row. */
+ * are never chosen.  Masses are right to 2^-29 of themselves, and tokens about 32
+ * temperatures below the likeliest one, whose weight is e^-32 of its, count as
+ * without any (3.4e-9 of it at most, all together).  temperature, top_k, top_p and
+ * min_p are per row on the device, or null: then the *_all values hold for every
+ * row.  The answer depends on nothing but its row. */
 int ti_amd_sample(const void* logits, int dtype, const float* uniforms, const float* temperature, const int32_t* top_k,
                   const float* top_p, const float* min_p, float temperature_all, int top_k_all, float top_p_all,
                   float min_p_all, int32_t* tokens, float* probs, int batch, int vocab, uintptr_t stream, int device);

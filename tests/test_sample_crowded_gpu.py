@@ -66,3 +66,26 @@ def test_the_largest_vocabulary_of_few_distinct_logits(ops, temperature):
     check(ops, x, uniforms, temperature, top_k=200003)
     check(ops, x, uniforms, temperature, top_p=0.9137)
     check(ops, x, uniforms, temperature, top_k=250001, top_p=0.31, min_p=0.9)
+
+
+@pytest.mark.parametrize("distance", [31.9, 32.5, 33.0])
+def test_a_vocabulary_far_behind_the_likeliest(ops, distance):
+    """Nearly all of the largest vocabulary about 32 temperatures behind the likeliest token:
+    from 32 on they count as without weight, at most V e^-32 of the likeliest one's, which
+    moves a border and a probability by as much (again for each goal)."""
+    say("far behind", distance)
+    rng = np.random.default_rng(int(10 * distance))
+    x = (-distance - rng.random((4, VOCAB)) * 0.05).astype(np.float32)
+    for row in x:
+        row[rng.permutation(VOCAB)[:5]] = [0, -1.5, -4, -9, -11.5]
+    uniforms = np.array([0.11, 0.79, 0.999, 1 - 2.0 ** -24], np.float32)
+    off = OFF + 1.001 * VOCAB * np.exp(-32.0)
+    for more in ({}, {"top_k": VOCAB - 100}, {"top_k": 3000}, {"min_p": 1e-14}, {"top_p": 0.9999}, {"top_k": 70000, "top_p": 0.87}):
+        tokens, probs = ops.sample(dev(x), dev(uniforms), **more)
+        torch().cuda.synchronize()
+        for b in range(4):
+            want, p, far = one(x[b], uniforms[b], np.float32(1), more.get("top_k", 0), np.float32(more.get("top_p", 1)),
+                               np.float32(more.get("min_p", 0)))
+            assert far > 4 * off, "the input is too near a border"
+            assert int(tokens[b]) == want, (more, b)
+            assert abs(float(probs[b]) - p) <= (2.0 ** -24 + 2 * off) * p, (more, b, float(probs[b]), p)

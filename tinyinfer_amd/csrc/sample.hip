@@ -14,9 +14,12 @@
 // (b + f) / 256 weighs e^(-b/256) (1 - q), q = 1 - e^(-f/256) < 1.02 * 2^-8: bins hold
 // their count and the sum of q in units of 2^-34, one 64-bit LDS addition per token (a bin
 // that holds the whole vocabulary fits: sample_bins.hpp), and masses are whole numbers of 2^-44: sums are the same in any order, and an
-// answer depends on its row alone.  A token's mass is right to about 2^-31 of itself, so
-// the token is the one that 64-bit arithmetic gives but for a random number within
-// about 1e-10 of a border.  Tokens 32 units from the maximum (e^-32) weigh nothing.
+// answer depends on its row alone.  A token's mass is right to 1.4 * 2^-30 of itself (the
+// fraction's 2^-23 of a bin, and fp32 roundings of q), a bin's rounded to 2^-45, and tokens
+// 32 units from the maximum weigh nothing: at most V e^-32 of the likeliest one's mass is left
+// out, 3.4e-9 at 2^18 tokens.  So the token is the one that 64-bit arithmetic gives but for a
+// random number (or a top-p) within twice 2^-29 + V e^-32 of a border, 1.1e-8 at most; fp32
+// numbers next to 1 are 6e-8 apart.
 //
 // One workgroup per row reads it three times (maximum, bins, gathering), the second and
 // third time from cache.  (Keeping it in registers needs every pass unrolled over them: 50
