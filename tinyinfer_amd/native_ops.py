@@ -294,8 +294,12 @@ class NativeOps:
     def __init__(self, library_path=None):
         import torch
         self.torch, self.tensor_type = torch, torch.Tensor
-        self.stream_handle, self.streams = torch._C._cuda_getCurrentRawStream, {}
-        self.current_device = torch._C._cuda_getDevice   # (operands are on a GPU: it is initialised)
+        # torch's own short ways to both (operands are on a GPU: it is initialised), which
+        # are not part of its interface and missing in a torch without GPU support.
+        self.stream_handle = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
+        self.current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+        self.streams = {}
         where = require(BACKEND_LIB) if library_path is None else library_path
         self.library_path = str(Path(where).expanduser().resolve(strict=True))
         self.lib = ctypes.CDLL(self.library_path)
