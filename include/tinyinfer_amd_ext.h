@@ -152,8 +152,9 @@ int ti_amd_kv_read_i8(const ti_amd_kv_i8* cache, uint16_t* k, uint16_t* v, const
  * outside the cache has none).  Query i < q_lengths[b] (null: q_len) sees them
  * all, or with causal = 1 those up to offsets[b] + i; offsets null means
  * kv_lengths[b] - q_lengths[b]: the queries are the request's last tokens.  Rows
- * that see no key, and queries past q_lengths[b], are exactly 0.  batch and heads
- * are at most 65535, batch * heads * q_len at most 2^23.
+ * that see no key, and queries past q_lengths[b], are exactly 0; a row that sees a
+ * key or value with an infinity or NaN, or has one in its query, is NaN.  batch and
+ * heads are at most 65535, batch * heads * q_len at most 2^23.
  * prefix_len > 0: in front of its own keys every query also sees tokens 0 ..
  * prefix_len - 1 of prefix_slot, whose bytes are read once for the batch (a short
  * prefix of a few requests by each of them).

@@ -85,6 +85,8 @@ struct AttnPlan {
   bool parts;                    // states to the workspace, joined by the second kernel
 };
 
+typedef unsigned short u16x8_t __attribute__((ext_vector_type(8)));
+
 // Whole numbers c of 4 stored bytes c + 128, as fp16.
 __device__ __forceinline__ void widen4(uint32_t w, half2_t& lo, half2_t& hi) {
   const half2_t bias = {f16(-1152.f), f16(-1152.f)};
@@ -282,8 +284,12 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
 
   // Step (c, s) of a dot product takes dims 64 c + 16 g + 8 s .. + 7 from lane (., g).
   half8_t qf[QB][D / 32];
+  // A row's sum starts at NaN if its query has an infinity or NaN: its scores are infinite, of
+  // either sign, or NaN (and all of -inf would pass for a row without a key).
+  float l[QB];
 #pragma unroll
   for (int u = 0; u < QB; ++u) {
+    u16x8_t top = {};
     const uint16_t* qp = a.q + int64_t(max(row_id[u], 0)) * D + 16 * g;
 #pragma unroll
     for (int c = 0; c < D / 64; ++c)
@@ -291,8 +297,13 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
       for (int s = 0; s < 2; ++s) {
         half8_t x;
         __builtin_memcpy(&x, qp + 64 * c + 8 * s, 16);
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x8_t, x) & uint16_t(0x7fff));
         qf[u][2 * c + s] = (BOTH ? asks[u] : end[u] > 0) ? x : half8_t{};
       }
+    bool inside = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) inside = inside && top[e] < 0x7c00;
+    l[u] = __ballot(!inside) >> j & 0x0001000100010001u ? __builtin_nanf("") : 0.f;
   }
 
   float4_t from[QB];  // where the sums of S start
@@ -307,12 +318,11 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
     }
   }
 
-  float m[QB], l[QB];
+  float m[QB];
   float4_t acc[QB][D / 16];
 #pragma unroll
   for (int u = 0; u < QB; ++u) {
     m[u] = kNegInf;
-    l[u] = 0.f;
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) acc[u][d] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
