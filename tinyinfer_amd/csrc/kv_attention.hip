@@ -523,12 +523,14 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
 #pragma unroll
     for (int u = 0; u < QB; ++u) {
       float top = kNegInf, total = 0.f, f[KW];
+      bool empty[KW];  // (what it holds is no row's; a state with keys counts however little it weighs: 0 times NaN is NaN)
 #pragma unroll
       for (int w = 0; w < KW; ++w) top = mg.l[w][u][j] == 0.f ? top : fmaxf(top, mg.m[w][u][j]);
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
         const float lw = mg.l[w][u][j];
-        f[w] = lw == 0.f ? 0.f : __builtin_amdgcn_exp2f(mg.m[w][u][j] - top);
+        empty[w] = lw == 0.f;
+        f[w] = empty[w] ? 0.f : __builtin_amdgcn_exp2f(mg.m[w][u][j] - top);
         total += lw * f[w];
       }
 #pragma unroll
@@ -539,7 +541,7 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
         for (int w = 0; w < KW; ++w) {
           const float4_t x = mg.acc[w][u * (D / 16) + d][lane];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = f[w] == 0.f ? o[e] : fmaf(x[e], f[w], o[e]);
+          for (int e = 0; e < 4; ++e) o[e] = empty[w] ? o[e] : fmaf(x[e], f[w], o[e]);
         }
         put(u, d, o, total);
       }
