@@ -4,7 +4,7 @@ import math
 import numpy as np
 import pytest
 
-from test_int8_cache_gpu import dev, host, say
+from test_int8_cache_gpu import dev, host, i32, say
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +33,23 @@ def test_a_value_of_nan_that_weighs_nothing(ops, dim, nq, kv, token, prefix):
     else:
         got = host(ops.attention_int8kv(dev(q), cache, 0, kv))
     assert bool(np.isnan(got).all())
+
+
+@pytest.mark.parametrize("batch,heads,dim,nq,kv", [
+    (48, 16, 64, 128, 140), (40, 16, 128, 81, 200), (3, 25, 64, 450, 450), (4, 16, 128, 300, 310), (6, 8, 64, 700, 2100),
+    (2, 4, 64, 1, 300), (1, 8, 64, 40, 8300)])
+def test_values_at_the_largest_number(ops, batch, heads, dim, nq, kv):
+    """Every value is fp16's largest number or its negative: so is every result, to 2^-11, and
+    none is infinite though the weights' roundings may sum up to more than theirs."""
+    say("largest values", batch, heads, dim, nq, kv)
+    rng = np.random.default_rng(batch + nq)
+    k = (rng.standard_normal((batch, heads, kv, dim)) * 2).astype(np.float16)
+    v = np.empty((batch, heads, kv, dim), np.float16)
+    v[...] = np.where(np.arange(dim) % 2, 65504, -65504)
+    cache = ops.kv_cache_int8(batch, heads, kv, dim)
+    ops.kv_append_int8(cache, dev(k), dev(v), list(range(batch)), 0)
+    q = (rng.standard_normal((batch, heads, nq, dim)) * 2).astype(np.float16)
+    got = host(ops.attention_int8kv(dev(q), cache, list(range(batch)), i32([kv] * batch))).astype(np.float64)
+    want = v[0, 0, 0].astype(np.float64)
+    assert bool(np.isfinite(got).all())
+    assert bool((np.abs(got - want) <= 1.02 * 2.0 ** -10 * 65504).all())

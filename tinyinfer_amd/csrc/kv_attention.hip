@@ -144,6 +144,20 @@ __device__ __forceinline__ u32x4_t load16(const uint8_t* p) {
   return *reinterpret_cast<const u32x4_t*>(p);
 }
 
+// The output of weighted values o of `total` probability (inv: its reciprocal).  It lies
+// between values, of at most 65504: what the rounded weights sum up to beyond is cut off.
+__device__ __forceinline__ half4_t output_of(float4_t o, float total, float inv) {
+  constexpr float most = 65504.f;
+  float x[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = total == 0.f ? 0.f : o[e] * inv;
+  if (__ballot(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))) > most)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = x[e] > most ? most : x[e] < -most ? -most : x[e];  // (NaN stays)
+  }
+  return half4_t{f16r(x[0]), f16r(x[1]), f16r(x[2]), f16r(x[3])};
+}
+
 template <int D, int QB, int KW>
 struct Merge {
   float4_t acc[KW][QB * D / 16][64];
@@ -488,9 +502,7 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
       return;
     }
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    half4_t y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = f16r(total == 0.f ? 0.f : o[e] * inv);
+    const half4_t y = output_of(o, total, inv);
     __builtin_memcpy(a.out + int64_t(row_id[u]) * D + 16 * d + 4 * g, &y, 8);
   };
   const auto put_weight = [&](int u, float top, float total) {
@@ -630,9 +642,7 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(AttnPlan p) {
   }
   if (part != 0) return;
   const float inv = total == 0.f ? 0.f : 1.f / total;
-  half4_t y;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = f16r(total == 0.f ? 0.f : o[e] * inv);
+  const half4_t y = output_of(o, total, inv);
   __builtin_memcpy(p.a.out + row * D + at, &y, 8);
 }
 
