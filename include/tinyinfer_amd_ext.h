@@ -139,7 +139,8 @@ typedef struct ti_amd_kv_i8 {
  * lengths[b] (null: every row) becomes token positions[b] + i of slots[b].  The
  * metadata is int32 [batch] on the device.  What lies outside the cache (a slot,
  * a token) is not written; where two requests write the same token the later
- * request's row stays.  batch is at most 65535, rows at most 2^28. */
+ * request's row stays (requests that share a slot look through the later ones, a
+ * time that grows with the batch).  batch is at most 65535, rows at most 2^28. */
 int ti_amd_kv_append_i8(const ti_amd_kv_i8* cache, const uint16_t* k, const uint16_t* v, const int32_t* slots,
                         const int32_t* positions, const int32_t* lengths, int batch, int rows, uintptr_t stream, int device);
 /* ti_amd_kv_read_i8: the same rows back, fp16_rn(fp32(c * scale)); zeros past
@@ -158,10 +159,11 @@ int ti_amd_kv_read_i8(const ti_amd_kv_i8* cache, uint16_t* k, uint16_t* v, const
  * prefix_len > 0: in front of its own keys every query also sees tokens 0 ..
  * prefix_len - 1 of prefix_slot, whose bytes are read once for the batch (a short
  * prefix of a few requests by each of them).
- * Scores, softmax and sums are fp32; probabilities are rounded to fp16 (where few
- * rows share the keys twice: what the first rounding leaves out is added).  How rows
- * and keys are divided follows from the shape arguments, so a request's last bits
- * may differ between batches of other sizes; equal calls give equal bits.
+ * Scores, softmax and sums are fp32; a key's probability times its value's scale is
+ * rounded to fp16, relative to what the row itself sees (where few rows share the keys
+ * twice: what the first rounding leaves out is added).  How rows and keys are
+ * divided follows from the shape arguments, so a request's last bits may differ
+ * between batches of other sizes; equal calls give equal bits.
  * max_kv (0: the capacity) is what kv_lengths are expected to stay within: it
  * plans the launch and its workspace, and longer requests are answered too.
  * workspace: ti_amd_attention_i8kv_workspace bytes (-1 for invalid arguments, 0

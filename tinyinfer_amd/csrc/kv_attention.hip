@@ -33,13 +33,13 @@
 // for a few short ones, whose rows walk it in front of their own keys: prefix_inline).
 //
 // What bounds it.  Single tokens: memory where caches are long (16 requests of 8 x 128,
-// 12000 to 32768 keys: 134 us, 6.0 TB/s; the loads are the plain ones of a stream,
+// 12000 to 32768 keys: 135 us, 6.0 TB/s; the loads are the plain ones of a stream,
 // past the caches), launch and one tile's chain of latencies where they are short (one
 // request of 12 heads, 300 keys: 6 us).  Prompts: vector instructions beside the matrix
 // products.  Of a tile of 64 keys x 32 rows at D 128 the 64 matrix instructions are 1024
 // cycles of a SIMD; widening K and V is 192 vector instructions and a score takes 6 and an
 // exponential, 1900 cycles together.  2 requests of 777 queries, 32 heads over 8 of 128,
-// 4500 to 6001 keys: 195 us, 690 TFLOP/s; 4 prompts of 1024, 25 heads of 64: 30 us, 445
+// 4500 to 6001 keys: 197 us, 685 TFLOP/s; 4 prompts of 1024, 25 heads of 64: 31 us, 430
 // TFLOP/s, its scores' exponentials and scales more than the products.
 #include <algorithm>
 
@@ -562,9 +562,11 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
   }
 }
 
-// Waves per SIMD that the registers are budgeted for: the most that spills nothing (103,
-// 164, 153 and 228 registers are used of 128, 168, 168 and 256).
-constexpr int waves_for(int dim, int qb) { return dim == 64 ? (qb == 1 ? 4 : 2) : (qb == 1 ? 2 : 2); }
+// Waves per SIMD that the registers are budgeted for.  What the compiler takes: 64 dims, one
+// block 121 registers of 128 (four waves), two 158 to 164 of 256 (three waves fit); 128 dims,
+// one block 177 of 256, two sharing tiles 218, two that widen for themselves all 256 and 1 to 5
+// more that are spilled (8 to 24 bytes a lane).
+constexpr int waves_for(int dim, int qb) { return dim == 64 && qb == 1 ? 4 : 2; }
 
 // QB, PB: row blocks of 16 per wave over the requests' own keys and the prefix's (0:
 // no prefix, kInline: walked in front of the own keys); KW: waves that share a row block's

@@ -27,11 +27,11 @@
 // 201 KB in L2 reads in 1.6 us.)  Rows with a small top-k take a shorter way that
 // reads them once.
 //
-// What bounds it.  32 rows of 50257 with top-p take 25 us: about 3 for the maximum (one CU's
+// What bounds it.  32 rows of 50257 with top-p take 26 us: about 3 for the maximum (one CU's
 // loads), 6.5 for the bins and 4 for the gathering (20 and 6 vector instructions a token), 3.5
 // for the sums over the bins, 2 for the searches, 3 for ordering and answers; without data (a
-// few tokens) 13 are left.  32 CUs are busy, their VALU 77 %.  Several workgroups to a row
-// would have to bring their bins together, 64 KB each, which costs what they save.  256 rows
+// few tokens) 13 are left.  32 CUs are busy, their VALU 76 %.  (Several workgroups to a row
+// would have to bring their bins together, 64 KB each; not tried.)  256 rows
 // of 128257 by a top-k up to 200, top-p and min-p take 39 us, 22 of them memory; by top-p
 // alone 75.
 #include "common.hpp"
