@@ -193,6 +193,77 @@ int ti_amd_attention_i8kv(const ti_amd_kv_i8* cache, const uint16_t* q, uint16_t
 int ti_amd_sample(const void* logits, int dtype, const float* uniforms, const float* temperature, const int32_t* top_k,
                   const float* top_p, const float* min_p, float temperature_all, int top_k_all, float top_p_all,
                   float min_p_all, int32_t* tokens, float* probs, int batch, int vocab, uintptr_t stream, int device);
+
+/* Rotary positions: no counterpart in the reference, whose positions are learned.  A
+ * row's first `rotated` dims (even) are turned in pairs, (2 i, 2 i + 1) if interleaved =
+ * 1, else (i, rotated / 2 + i): the pair (a, b) of position t becomes amplitude *
+ * (a cos w - b sin w, a sin w + b cos w), w = t f_i, in fp32, rounded to fp16 once; the
+ * dims behind pass unchanged.  turns holds the frequencies, uint64 [rotated / 2] on the
+ * device: turns[i] = 2^64 (f_i / 2 pi mod 1), so angles are exact to 2^-64 of a turn
+ * times the position at every int32 position, negative ones too.
+ * ti_amd_rotate: x fp16 [batch][heads][rows][dim] with strides in elements (dims
+ * contiguous), y contiguous and not overlapping x.  Row i of request b has position
+ * positions[b] + i, or positions[b * rows + i] with per_row = 1.  batch and heads are at
+ * most 65535, rows * dim at most 2^31. */
+int ti_amd_rotate(const uint16_t* x, int64_t x_batch, int64_t x_head, int64_t x_row, uint16_t* y, const int32_t* positions,
+                  int per_row, const uint64_t* turns, int rotated, int interleaved, float amplitude, int batch, int heads,
+                  int rows, int dim, uintptr_t stream, int device);
+
+/* The paged fp16 KV cache: no counterpart in the reference.  `pages` (16-byte aligned) is
+ * page_count pages of kv_heads * 2 * page_size * head_dim values in the kernels' own order; a
+ * page is contiguous and may be copied as a whole.  page_size is a power of two from 32 to
+ * 1024, head_dim 64 or 128.  Which pages hold a request's tokens is the caller's to say:
+ * token t of request b lies on page table[b * width + t / page_size] (int32 on the
+ * device).  What lies past the table, or on a page outside [0, page_count), does not exist:
+ * it is not written, reads as zeros and is not seen. */
+typedef struct ti_amd_kv_paged {
+  uint16_t* pages;
+  int32_t page_count, kv_heads, page_size, head_dim;
+} ti_amd_kv_paged;
+/* ti_amd_kv_append_paged: k, v fp16 [batch][kv_heads][rows][head_dim] with strides in
+ * elements; row i < lengths[b] (null: every row) becomes token positions[b] + i, its key
+ * turned by that position if turns is given (rotated a multiple of 16), its value as it
+ * is.  With q [batch][heads][rows][head_dim] its rows are turned alike into q_out
+ * (contiguous; zeros past lengths[b]; null q: none).  Rows of one call that name one
+ * place leave it with the values of either.  batch is at most 65535, rows at most 2^28. */
+int ti_amd_kv_append_paged(const ti_amd_kv_paged* cache, const uint16_t* k, int64_t k_batch, int64_t k_head, int64_t k_row,
+                           const uint16_t* v, int64_t v_batch, int64_t v_head, int64_t v_row, const uint16_t* q,
+                           int64_t q_batch, int64_t q_head, int64_t q_row, uint16_t* q_out, const int32_t* table, int width,
+                           const int32_t* positions, const int32_t* lengths, const uint64_t* turns, int rotated,
+                           int interleaved, float amplitude, int batch, int heads, int rows, uintptr_t stream, int device);
+/* ti_amd_kv_read_paged: the same rows back into contiguous k, v; zeros past lengths[b]. */
+int ti_amd_kv_read_paged(const ti_amd_kv_paged* cache, uint16_t* k, uint16_t* v, const int32_t* table, int width,
+                         const int32_t* positions, const int32_t* lengths, int batch, int rows, uintptr_t stream, int device);
+/* ti_amd_attention_paged: q, y fp16 [batch][heads][q_len][head_dim] over the paged cache;
+ * query head h reads key head h / (heads / kv_heads).  Request b's keys are tokens 0 ..
+ * kv_lengths[b] - 1 (as far as its table reaches).  Query i < q_lengths[b] (null: q_len) sees
+ * them all, or with causal = 1 those up to offsets[b] + i; offsets null means kv_lengths[b]
+ * - q_lengths[b].  Rows that see no key, and queries past q_lengths[b], are exactly 0.  A row
+ * that has an infinity or NaN in its query or sees a NaN in a key is NaN; one that sees an
+ * infinity or NaN in a value is not finite in that dim.  What a row does not see does not
+ * count, whatever memory holds there.  Scores, softmax and sums are fp32; a probability is
+ * rounded to fp16 for its product (for single tokens twice: what the first rounding leaves out
+ * is added).  batch and heads are at most 65535, batch * heads * q_len at most 2^23.
+ * max_kv (0: what the table holds) plans the launch and its workspace; longer requests are
+ * answered too.  workspace: ti_amd_attention_paged_workspace bytes (-1 for invalid arguments,
+ * 0 if none is needed), used by this call alone until its work is done. */
+int64_t ti_amd_attention_paged_workspace(const ti_amd_kv_paged* cache, int width, int batch, int heads, int q_len, int max_kv);
+int ti_amd_attention_paged(const ti_amd_kv_paged* cache, const uint16_t* q, uint16_t* y, const int32_t* table, int width,
+                           const int32_t* kv_lengths, const int32_t* q_lengths, const int32_t* offsets, void* workspace,
+                           int64_t workspace_bytes, int batch, int heads, int q_len, int max_kv, int causal, uintptr_t stream,
+                           int device);
+
+/* ti_amd_logprobs: of rows of logits [batch][vocab] (dtype 0 fp16, 1 fp32; batch at most
+ * 2^20, vocab 2^18) the natural log probabilities of tokens [batch][given] (1 <= given <= 2^16)
+ * under the row's softmax, its entropy in nats, and with 0 < top <= 64 its likeliest tokens
+ * [batch][top] and their log probabilities (top = 0: both null).  Tokens are ordered by logit,
+ * ties by index.  A token outside the vocabulary, or with a logit of -inf or NaN, has the log
+ * probability -inf and is no alternative: places left over hold 2^31 - 1 and -inf.  A
+ * logit of +inf has all the probability (the first such one).  A row without a logit above -inf
+ * has the entropy 0. */
+int ti_amd_logprobs(const void* logits, int dtype, const int32_t* tokens, float* logprobs, float* entropy,
+                    float* top_logprobs, int32_t* top_tokens, int batch, int vocab, int given, int top, uintptr_t stream,
+                    int device);
 #ifdef __cplusplus
 }
 #endif

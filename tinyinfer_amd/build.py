@@ -33,6 +33,7 @@ HOST_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-march=x86-64-v3", "-ffp-contract=f
               "-fno-math-errno", "-I", str(ROOT / "include")]
 
 BACKEND_HIP = ["gemm.hip", "attention.hip", "rowops.hip", "kv_cache.hip", "kv_attention.hip", "sample.hip",
+               "rotary.hip", "paged_cache.hip", "paged_attention.hip", "logprobs.hip",
                "backend_v2.hip", "backend_legacy.hip"]
 LLM_HIP = ["llm_runtime.hip"]
 

@@ -146,6 +146,62 @@ int check_kv_attention(const ti_amd_kv_i8* cache, int batch, int heads, int q_le
   return TI_V2_OK;
 }
 
+// Rotary arguments: `wide` for kernels that take the pairs 8 at a time.
+int check_rotary(const uint64_t* turns, int rotated, int interleaved, float amplitude, int dim, bool wide, tia::RotaryArgs& out) {
+  if (!aligned(turns, 8) || rotated <= 0 || rotated % 2 != 0 || rotated > dim || (wide && rotated % 16 != 0) ||
+      (interleaved != 0 && interleaved != 1) || !std::isfinite(amplitude))
+    return fail(TI_V2_INVALID_ARGUMENT, wide ? "rotary: 8-byte aligned turns, rotated a multiple of 16 within the head, a finite amplitude"
+                                             : "rotary: 8-byte aligned turns, rotated even and within the head, a finite amplitude");
+  out.turns = turns;
+  out.rotated = rotated;
+  out.interleaved = interleaved != 0;
+  out.amplitude = amplitude;
+  return TI_V2_OK;
+}
+bool strides_fit(int64_t batch, int64_t head, int64_t row) { return batch >= 0 && head >= 0 && row >= 0; }
+
+int check_paged(const ti_amd_kv_paged* c, const int32_t* table, int width, tia::KvPaged& out, tia::PageTable& pages) {
+  if (!c || (c->head_dim != 64 && c->head_dim != 128) || c->page_count <= 0 || c->kv_heads <= 0 || c->kv_heads > 65535 ||
+      c->page_size < 32 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)) != 0 ||
+      !shape_fits({c->page_count, c->kv_heads, c->page_size, c->head_dim}, 4) || !aligned(c->pages, 16))
+    return fail(TI_V2_INVALID_ARGUMENT,
+                "paged cache: 16-byte aligned pages, page_size a power of two from 32 to 1024, head_dim 64 or 128 and positive extents");
+  if (!aligned(table, 4) || width <= 0) return fail(TI_V2_INVALID_ARGUMENT, "page table: int32 [batch][width], width positive");
+  out.pages = c->pages;
+  out.page_count = c->page_count;
+  out.kv_heads = c->kv_heads;
+  out.page_size = c->page_size;
+  out.head_dim = c->head_dim;
+  pages.table = table;
+  pages.width = width;
+  return TI_V2_OK;
+}
+
+int check_paged_rows(const void* k, const void* v, const int32_t* positions, const int32_t* lengths, int batch, int rows,
+                     const tia::KvPaged& c) {
+  if (!aligned(k, 2) || !aligned(v, 2) || !aligned(positions, 4) || !optional_aligned(lengths, 4) || batch <= 0 || batch > 65535 ||
+      rows <= 0 || rows > (1 << 28) || !shape_fits({batch, c.kv_heads, rows, c.head_dim}, 2))
+    return fail(TI_V2_INVALID_ARGUMENT,
+                "invalid paged cache rows: shape, pointers or alignment (batch at most 65535, rows 2^28)");
+  return TI_V2_OK;
+}
+
+int check_paged_attention(const ti_amd_kv_paged* cache, const int32_t* table, int width, int batch, int heads, int q_len, int max_kv,
+                          tia::PagedAttnArgs& a) {
+  const int status = check_paged(cache, table, width, a.cache, a.pages);
+  if (status) return status;
+  const int most = 1 << 23;  // (row numbers and grids stay below 2^31)
+  if (batch <= 0 || batch > 65535 || heads <= 0 || heads > 65535 || q_len <= 0 || heads % a.cache.kv_heads != 0 ||
+      int64_t(batch) * heads > most / q_len || max_kv < 0)
+    return fail(TI_V2_INVALID_ARGUMENT, "invalid paged attention: heads a multiple of kv_heads, at most 2^23 query rows");
+  a.batch = batch;
+  a.heads = heads;
+  a.q_len = q_len;
+  const int64_t held = int64_t(width) * a.cache.page_size, all = held > INT32_MAX ? INT32_MAX : held;
+  a.max_kv = max_kv == 0 || max_kv > all ? int(all) : max_kv;
+  return TI_V2_OK;
+}
+
 }  // namespace
 
 extern "C" int ti_v2_abi_version(void) { return 2; }
@@ -578,4 +634,132 @@ extern "C" int ti_amd_sample(const void* logits, int dtype, const float* uniform
   a.batch = batch;
   a.vocab = vocab;
   return hip_status(tia::sample(a, reinterpret_cast<hipStream_t>(stream)));
+}
+
+extern "C" int ti_amd_rotate(const uint16_t* x, int64_t x_batch, int64_t x_head, int64_t x_row, uint16_t* y,
+                             const int32_t* positions, int per_row, const uint64_t* turns, int rotated, int interleaved,
+                             float amplitude, int batch, int heads, int rows, int dim, uintptr_t stream, int device) {
+  int status = begin(device);
+  if (status) return status;
+  tia::RotateArgs a;
+  if ((status = check_rotary(turns, rotated, interleaved, amplitude, dim, false, a.rotary))) return status;
+  if (!aligned(x, 2) || !aligned(y, 2) || !aligned(positions, 4) || (per_row != 0 && per_row != 1) || batch <= 0 || batch > 65535 ||
+      heads <= 0 || heads > 65535 || rows <= 0 || dim <= 0 || int64_t(rows) * dim > (int64_t(1) << 31) ||
+      !shape_fits({batch, heads, rows, dim}, 2) || !strides_fit(x_batch, x_head, x_row))
+    return fail(TI_V2_INVALID_ARGUMENT,
+                "invalid rows to rotate: shape, strides, pointers or alignment (batch and heads at most 65535, rows * dim 2^31)");
+  a.x = {x, x_batch, x_head, x_row};
+  a.y = y;
+  a.positions = positions;
+  a.per_row = per_row != 0;
+  a.batch = batch;
+  a.heads = heads;
+  a.rows = rows;
+  a.dim = dim;
+  return hip_status(tia::rotate(a, reinterpret_cast<hipStream_t>(stream)));
+}
+
+extern "C" int ti_amd_kv_append_paged(const ti_amd_kv_paged* cache, const uint16_t* k, int64_t k_batch, int64_t k_head,
+                                      int64_t k_row, const uint16_t* v, int64_t v_batch, int64_t v_head, int64_t v_row,
+                                      const uint16_t* q, int64_t q_batch, int64_t q_head, int64_t q_row, uint16_t* q_out,
+                                      const int32_t* table, int width, const int32_t* positions, const int32_t* lengths,
+                                      const uint64_t* turns, int rotated, int interleaved, float amplitude, int batch, int heads,
+                                      int rows, uintptr_t stream, int device) {
+  int status = begin(device);
+  if (status) return status;
+  tia::PagedAppendArgs a;
+  if ((status = check_paged(cache, table, width, a.cache, a.pages))) return status;
+  if ((status = check_paged_rows(k, v, positions, lengths, batch, rows, a.cache))) return status;
+  if (turns && (status = check_rotary(turns, rotated, interleaved, amplitude, a.cache.head_dim, true, a.rotary))) return status;
+  if (!strides_fit(k_batch, k_head, k_row) || !strides_fit(v_batch, v_head, v_row))
+    return fail(TI_V2_INVALID_ARGUMENT, "paged cache rows: strides must not be negative");
+  if (q && (!turns || !aligned(q, 2) || !aligned(q_out, 2) || heads <= 0 || heads > 65535 || !strides_fit(q_batch, q_head, q_row) ||
+            !shape_fits({batch, heads, rows, a.cache.head_dim}, 2)))
+    return fail(TI_V2_INVALID_ARGUMENT, "queries beside a paged append need turns, an output, at most 65535 heads and no negative strides");
+  a.k = {k, k_batch, k_head, k_row};
+  a.v = {v, v_batch, v_head, v_row};
+  a.q = {q, q_batch, q_head, q_row};
+  a.q_out = q_out;
+  a.positions = positions;
+  a.lengths = lengths;
+  a.batch = batch;
+  a.heads = q ? heads : 0;
+  a.rows = rows;
+  return hip_status(tia::paged_append(a, reinterpret_cast<hipStream_t>(stream)));
+}
+
+extern "C" int ti_amd_kv_read_paged(const ti_amd_kv_paged* cache, uint16_t* k, uint16_t* v, const int32_t* table, int width,
+                                    const int32_t* positions, const int32_t* lengths, int batch, int rows, uintptr_t stream,
+                                    int device) {
+  int status = begin(device);
+  if (status) return status;
+  tia::PagedReadArgs a;
+  if ((status = check_paged(cache, table, width, a.cache, a.pages))) return status;
+  if ((status = check_paged_rows(k, v, positions, lengths, batch, rows, a.cache))) return status;
+  a.k = k;
+  a.v = v;
+  a.positions = positions;
+  a.lengths = lengths;
+  a.batch = batch;
+  a.rows = rows;
+  return hip_status(tia::paged_read(a, reinterpret_cast<hipStream_t>(stream)));
+}
+
+extern "C" int64_t ti_amd_attention_paged_workspace(const ti_amd_kv_paged* cache, int width, int batch, int heads, int q_len,
+                                                    int max_kv) {
+  tia::PagedAttnArgs a;
+  error_text[0] = '\0';
+  static const int32_t none = 0;
+  if (check_paged_attention(cache, &none, width, batch, heads, q_len, max_kv, a)) return -1;
+  return tia::paged_attention_workspace(a);
+}
+
+extern "C" int ti_amd_attention_paged(const ti_amd_kv_paged* cache, const uint16_t* q, uint16_t* y, const int32_t* table,
+                                      int width, const int32_t* kv_lengths, const int32_t* q_lengths, const int32_t* offsets,
+                                      void* workspace, int64_t workspace_bytes, int batch, int heads, int q_len, int max_kv,
+                                      int causal, uintptr_t stream, int device) {
+  int status = begin(device);
+  if (status) return status;
+  tia::PagedAttnArgs a;
+  if ((status = check_paged_attention(cache, table, width, batch, heads, q_len, max_kv, a))) return status;
+  if (!aligned(q, 2) || !aligned(y, 2) || !aligned(kv_lengths, 4) || !optional_aligned(q_lengths, 4) ||
+      !optional_aligned(offsets, 4) || (causal != 0 && causal != 1))
+    return fail(TI_V2_INVALID_ARGUMENT, "invalid paged attention pointers, alignment or causal flag");
+  const int64_t needed = tia::paged_attention_workspace(a);
+  if (needed > 0 && (!aligned(workspace, 16) || workspace_bytes < needed))
+    return fail(TI_V2_INVALID_ARGUMENT, "the call needs a 16-byte aligned workspace of ti_amd_attention_paged_workspace bytes");
+  a.q = q;
+  a.out = y;
+  a.kv_lengths = kv_lengths;
+  a.q_lengths = q_lengths;
+  a.offsets = offsets;
+  a.causal = causal != 0;
+  a.workspace = static_cast<float*>(workspace);
+  return hip_status(tia::paged_attention(a, reinterpret_cast<hipStream_t>(stream)));
+}
+
+extern "C" int ti_amd_logprobs(const void* logits, int dtype, const int32_t* tokens, float* logprobs, float* entropy,
+                               float* top_logprobs, int32_t* top_tokens, int batch, int vocab, int given, int top,
+                               uintptr_t stream, int device) {
+  int status = begin(device);
+  if (status) return status;
+  if ((dtype != TI_V2_FP16 && dtype != TI_V2_FP32) || !aligned(logits, dtype == TI_V2_FP16 ? 2 : 4) || !aligned(tokens, 4) ||
+      !aligned(logprobs, 4) || !aligned(entropy, 4) || top < 0 || top > tia::kLogprobsTopMax ||
+      (top > 0 && (!aligned(top_logprobs, 4) || !aligned(top_tokens, 4))) || given <= 0 || given > tia::kLogprobsGivenMax ||
+      vocab > tia::sample_bins::kVocabMax || batch > (1 << 20) || !shape_fits({batch, vocab}, 4))
+    return fail(TI_V2_INVALID_ARGUMENT,
+                "invalid log probability arguments: fp16 or fp32 logits, at most 2^20 rows of 2^18, 64 alternatives and 2^16 given tokens");
+  tia::LogprobsArgs a;
+  a.logits = logits;
+  a.f32 = dtype == TI_V2_FP32;
+  a.tokens = tokens;
+  a.logprobs = logprobs;
+  a.entropy = entropy;
+  a.top_logprobs = top_logprobs;
+  a.top_tokens = top_tokens;
+  a.batch = batch;
+  a.vocab = vocab;
+  a.given = given;
+  a.top = top;
+  return hip_status(tia::logprobs(a, reinterpret_cast<hipStream_t>(stream)));
 }

@@ -304,4 +304,100 @@ struct SampleArgs {
 };
 hipError_t sample(const SampleArgs& args, hipStream_t stream);
 
+// Rotary positions (rotary.hpp): pair i's frequency as 2^64 (f_i / 2 pi mod 1), the first
+// `rotated` dims of a row turned, in pairs (2 i, 2 i + 1) if interleaved, else
+// (i, rotated / 2 + i).  turns null: nothing is turned.
+struct RotaryArgs {
+  const uint64_t* turns = nullptr;
+  float amplitude = 1.f;
+  int rotated = 0;
+  bool interleaved = false;
+};
+// Rows of fp16 values with strides in elements, the values of a row contiguous.
+struct Rows {
+  const uint16_t* at = nullptr;
+  int64_t batch = 0, head = 0, row = 0;
+};
+// y [batch][heads][rows][dim] from x: row i of request b at position positions[b] + i, or
+// positions[b * rows + i] if per_row.
+struct RotateArgs {
+  RotaryArgs rotary;
+  Rows x;
+  uint16_t* y = nullptr;
+  const int32_t* positions = nullptr;
+  bool per_row = false;
+  int batch = 0, heads = 0, rows = 0, dim = 0;
+};
+hipError_t rotate(const RotateArgs& args, hipStream_t stream);
+
+// The paged fp16 KV cache (layout in paged_cache.hip): page_size a power of two of 32
+// tokens and more.
+struct KvPaged {
+  uint16_t* pages = nullptr;
+  int page_count = 0, kv_heads = 0, page_size = 0, head_dim = 64;
+};
+// Which pages a request's tokens lie on: token t on page table[b * width + t / page_size].
+// What lies past the table or on a page outside the cache does not exist.
+struct PageTable {
+  const int32_t* table = nullptr;
+  int width = 0;
+};
+// k, v [batch][kv_heads][rows][D]: row i < lengths[b] (null: all) becomes token positions[b]
+// + i, keys turned by it if rotary.turns.  q [batch][heads][rows][D], if given, is turned
+// alike into q_out (contiguous; zeros past lengths[b]).
+struct PagedAppendArgs {
+  KvPaged cache;
+  PageTable pages;
+  RotaryArgs rotary;
+  Rows q, k, v;
+  uint16_t* q_out = nullptr;
+  const int32_t* positions = nullptr;
+  const int32_t* lengths = nullptr;
+  int batch = 0, heads = 0, rows = 0;
+};
+hipError_t paged_append(const PagedAppendArgs& args, hipStream_t stream);
+// The way back: k, v [batch][kv_heads][rows][D], zeros past lengths[b] and where no token is.
+struct PagedReadArgs {
+  KvPaged cache;
+  PageTable pages;
+  uint16_t* k = nullptr;
+  uint16_t* v = nullptr;
+  const int32_t* positions = nullptr;
+  const int32_t* lengths = nullptr;
+  int batch = 0, rows = 0;
+};
+hipError_t paged_read(const PagedReadArgs& args, hipStream_t stream);
+
+// Attention over the paged cache: as KvAttnArgs without a prefix; a token on a page
+// outside the cache is not seen.
+struct PagedAttnArgs {
+  KvPaged cache;
+  PageTable pages;
+  const uint16_t* q = nullptr;
+  uint16_t* out = nullptr;
+  const int32_t* kv_lengths = nullptr;
+  const int32_t* q_lengths = nullptr;
+  const int32_t* offsets = nullptr;
+  int batch = 0, heads = 0, q_len = 0, max_kv = 0;
+  bool causal = true;
+  float* workspace = nullptr;  // paged_attention_workspace() bytes, 16-byte aligned
+};
+int64_t paged_attention_workspace(const PagedAttnArgs& args);
+hipError_t paged_attention(const PagedAttnArgs& args, hipStream_t stream);
+
+// Log probabilities of rows of logits [batch][vocab] (logprobs.hip has the definition):
+// of tokens [batch][given], the rows' entropy, and the `top` likeliest tokens.
+struct LogprobsArgs {
+  const void* logits = nullptr;
+  bool f32 = true;
+  const int32_t* tokens = nullptr;
+  float* logprobs = nullptr;
+  float* entropy = nullptr;
+  float* top_logprobs = nullptr;
+  int32_t* top_tokens = nullptr;
+  int batch = 0, vocab = 0, given = 0, top = 0;
+};
+constexpr int kLogprobsTopMax = 64, kLogprobsGivenMax = 1 << 16;
+hipError_t logprobs(const LogprobsArgs& args, hipStream_t stream);
+
 }  // namespace tia

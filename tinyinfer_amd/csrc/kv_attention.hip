@@ -44,6 +44,7 @@
 #include <algorithm>
 
 #include "common.hpp"
+#include "divisor.hpp"
 #include "kernels.hpp"
 #include "lds_limit.hpp"
 
@@ -58,20 +59,6 @@ constexpr float kNegInf = -__builtin_huge_valf();
 // still keeps 11 bits.  The scale of a row of zeros counts as 2^kLeast, below every
 // other (2^-24 / 127 at least): probabilities are fp32 and stay below 2^(14 - kLeast).
 constexpr float kBelow = 6.f, kRaise = 14.f, kLeast = -40.f;
-
-// n / d for 0 <= n < 2^31 by a multiplication: with 2^(shift-1) < d <= 2^shift and mul =
-// floor(2^32 (2^shift - d) / d) + 1, n / d = (hi32(n mul) + n) >> shift.
-struct Divisor {
-  uint32_t d, mul, shift;
-};
-Divisor divisor(uint32_t d) {
-  uint32_t shift = 0;
-  while ((uint64_t(1) << shift) < d) ++shift;
-  return {d, uint32_t(((uint64_t(1) << 32) * ((uint64_t(1) << shift) - d)) / d + 1), shift};
-}
-__device__ __forceinline__ int div_by(int n, Divisor v) {
-  return int((uint64_t(__umulhi(uint32_t(n), v.mul)) + uint32_t(n)) >> v.shift);
-}
 
 struct AttnPlan {
   KvAttnArgs a;

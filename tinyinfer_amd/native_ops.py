@@ -11,7 +11,10 @@ extent, device, integer argument or a tensor that requires grad,
 Beyond it: an int8 KV cache (``kv_cache_int8``, ``kv_append_int8``,
 ``kv_read_int8``), attention over it for single tokens and prompts
 (``attention_int8kv``, ``attention_shared_prefix``) and ``sample``, one token per
-row of logits.
+row of logits; rotary positions (``rotary``, ``rotate``), a paged fp16 KV cache
+(``kv_cache_paged``, ``kv_append_paged`` with the rotation on the way,
+``kv_read_paged``), attention over it (``attention_paged``) and ``logprobs``, the log
+probabilities of given tokens with their row's entropy and likeliest tokens.
 
 How it is built here: every native symbol is described by a string of
 parameter codes (``_ABI``); each call goes through a ``_Call`` that validates
@@ -63,6 +66,11 @@ _ABI = {
     "ti_amd_kv_read_i8": "ppppppii",
     "ti_amd_attention_i8kv": "ppppppppqiiiiiii",
     "ti_amd_sample": "pippppp" "fiff" "ppii",
+    "ti_amd_rotate": "pqqqppipiifiiii",
+    "ti_amd_kv_append_paged": "ppqqqpqqqpqqqp" "pippp" "iifiii",
+    "ti_amd_kv_read_paged": "ppppippii",
+    "ti_amd_attention_paged": "ppppipppp" "qiiiii",
+    "ti_amd_logprobs": "pipppppiiii",
 }
 _CTYPE = {"p": ctypes.c_void_p, "i": ctypes.c_int, "f": ctypes.c_float, "q": ctypes.c_int64}
 _TRAILER = [ctypes.c_size_t, ctypes.c_int]   # hipStream_t as uintptr_t, device ordinal
@@ -100,14 +108,15 @@ class _Call:
     device is switched only when it is not current.  ``gemm_int8`` at M = 1,
     768 -> 2304, call after call: 15.6 -> 11.7 us."""
 
-    __slots__ = ("ops", "symbol", "args", "held", "made", "device", "index", "over")
+    __slots__ = ("ops", "symbol", "args", "held", "made", "device", "index", "over", "turned")
 
     def __init__(self, ops, symbol):
         self.ops, self.symbol = ops, symbol
         self.args = []
         self.held, self.made = [], []   # the caller's tensors, and this call's own
         self.device = self.index = None
-        self.over = None                # the int8 cache it works on
+        self.over = None                # the cache it works on
+        self.turned = None              # the rotary positions it turns rows by
 
     def operand(self, x, dtype, name, rank=None, shape=None):
         tensor = self.ops.tensor_type
@@ -124,15 +133,18 @@ class _Call:
         self.args.append(x.data_ptr())
         return x
 
-    def _checked(self, x, dtype, name, rank, shape):
-        """The operand checks one by one, each with its own exception."""
+    def _checked(self, x, dtype, name, rank, shape, strided=False):
+        """The operand checks one by one, each with its own exception (strided: the last axis
+        alone must be contiguous)."""
         torch = self.ops.torch
         if not isinstance(x, torch.Tensor) or x.device.type != "cuda":
             raise TypeError(f"{name}: a GPU (torch 'cuda' device) tensor is required")
         if x.dtype != dtype:
             raise TypeError(f"{name}: dtype {x.dtype} given, {dtype} required")
-        if not x.is_contiguous():
+        if not x.is_contiguous() and not strided:
             raise TypeError(f"{name}: contiguous row-major storage required")
+        if strided and x.dim() and x.shape[-1] > 1 and x.stride(-1) != 1:
+            raise TypeError(f"{name}: a last axis of contiguous values required")
         if x.requires_grad:
             raise ValueError(f"{name}: tensors that require grad are not accepted (inference only)")
         if rank is not None and x.dim() != rank:
@@ -153,6 +165,22 @@ class _Call:
             self.args.append(None)
             return None
         return self.operand(x, dtype, name, shape=shape)
+
+    def rows(self, x, name, shape):
+        """fp16 rows [B,H,Q,D] of the given shape (None: any) in any layout whose dims
+        are contiguous, a slice of a projection for one: pointer and three strides."""
+        if not (isinstance(x, self.ops.tensor_type) and x.dtype == self.ops.torch.float16 and x.dim() == 4
+                and (x.stride(3) == 1 or x.shape[3] == 1) and not x.requires_grad and 0 < x.numel() <= INT32_MAX
+                and (shape is None or x.shape == shape) and x.is_cuda
+                and (self.index is None or x.get_device() == self.index)):
+            self._checked(x, self.ops.torch.float16, name, 4, shape, strided=True)
+        if self.index is None:
+            self.device = x.device
+            self.index = x.get_device()
+        self.held.append(x)
+        self.args.append(x.data_ptr())
+        self.args.extend(x.stride()[:3])
+        return x
 
     def output(self, shape, dtype):
         y = self.ops.torch.empty(shape, dtype=dtype, device=self.device)
@@ -190,13 +218,33 @@ class _Call:
         at = held.data_ptr()
         self.args.extend(at + 4 * len(lists[0]) * i for i in range(len(lists)))
 
-    def cache(self, cache):
-        if type(cache) is not Int8KVCache:
-            raise TypeError("cache: an Int8KVCache (NativeOps.kv_cache_int8) is required")
+    def cache(self, cache, kind=None):
+        if type(cache) is not (kind or Int8KVCache):
+            raise TypeError("cache: an Int8KVCache (NativeOps.kv_cache_int8) is required" if kind is None else
+                            "cache: a PagedKVCache (NativeOps.kv_cache_paged) is required")
         self.device = cache.buffer.device
         self.index = cache.buffer.get_device()
         self.over = cache
         self.args.append(cache._at)
+
+    def page_table(self, table, batch):
+        """int32 [B,W] on the call's device, W pages to a request."""
+        self.operand(table, self.ops.torch.int32, "page_table", rank=2)
+        if table.shape[0] != batch:
+            raise ValueError(f"page_table: a row for each of {batch} requests required, got {table.shape[0]}")
+        width = table.shape[1]
+        self.args.append(width)
+        return width
+
+    def turn(self, rotary):
+        """The frequencies' pointer, the turned dims, the layout and the factor."""
+        if rotary is None:
+            self.args.extend((None, 0, 0, 1.0))
+            return
+        if self.index is not None and rotary.turns.get_device() != self.index:
+            raise ValueError(f"rotary: on {rotary.turns.device}, the call's operands are on {self.device}")
+        self.turned = rotary
+        self.args.extend((rotary._at, rotary.rotated, int(rotary.interleaved), rotary.amplitude))
 
     def per_request(self, batch, *items):
         """One int per request, each item (value, upper, name): int32 [batch] tensors on
@@ -237,6 +285,9 @@ class _Call:
         if self.over is not None and handle not in self.over._streams:
             self.over.buffer.record_stream(stream)
             self.over._streams.add(handle)
+        if self.turned is not None and handle not in self.turned._streams:
+            self.turned.turns.record_stream(stream)
+            self.turned._streams.add(handle)
         if ops.current_device() == index:
             status = getattr(ops.lib, self.symbol)(*self.args, handle, index)
         else:
@@ -287,6 +338,66 @@ class Int8KVCache:
         return self.buffer.device
 
 
+class _KvPaged(ctypes.Structure):
+    """ti_amd_kv_paged."""
+    _fields_ = [("pages", ctypes.c_void_p), ("page_count", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+class PagedKVCache:
+    """A paged fp16 KV cache, made by ``NativeOps.kv_cache_paged``.
+
+    ``buffer`` [pages, kv_heads * 2 * page_size * head_dim] is zeroed; a page's inner order
+    is the kernels' own, so rows go in through ``kv_append_paged`` and come back through
+    ``kv_read_paged``, but a page is one row of it: ``cache.buffer[a] = cache.buffer[b]``
+    copies page b to page a.  Which pages a request's tokens lie on is the caller's
+    table: token t of request b on page ``table[b, t // page_size]``; a number outside the
+    cache, -1 for one, stands for no page."""
+
+    __slots__ = ("pages", "kv_heads", "page_size", "head_dim", "buffer", "_native", "_at", "_workspace", "_streams")
+
+    def __init__(self, torch, pages, kv_heads, page_size, head_dim, device):
+        buffer = torch.zeros((pages, kv_heads * 2 * page_size * head_dim), dtype=torch.float16, device=device)
+        native = _KvPaged(buffer.data_ptr(), pages, kv_heads, page_size, head_dim)
+        for name, value in (("pages", pages), ("kv_heads", kv_heads), ("page_size", page_size), ("head_dim", head_dim),
+                            ("buffer", buffer), ("_native", native), ("_at", ctypes.addressof(native)),
+                            ("_workspace", {}), ("_streams", set())):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"{name}: a cache's buffer and extents stay as they were made")
+
+    @property
+    def device(self):
+        return self.buffer.device
+
+
+class Rotary:
+    """Rotary positions, made by ``NativeOps.rotary``: the first `rotated` dims of a row are
+    turned, pair i by ``frequencies[i]`` radians a position; turned values are multiplied by
+    `amplitude`.  ``turns`` holds the frequencies on the device, as 2^64 (f / 2 pi mod 1)."""
+
+    __slots__ = ("rotated", "interleaved", "amplitude", "frequencies", "turns", "_at", "_streams")
+
+    def __init__(self, torch, frequencies, interleaved, amplitude, device):
+        whole = [round(math.fmod(f / (2 * math.pi), 1.0) * 2.0 ** 64) % 2 ** 64 for f in frequencies]
+        turns = torch.tensor([n - 2 ** 64 if n >= 2 ** 63 else n for n in whole], dtype=torch.int64, device=device)
+        for name, value in (("rotated", 2 * len(frequencies)), ("interleaved", interleaved), ("amplitude", float(amplitude)),
+                            ("frequencies", tuple(frequencies)), ("turns", turns), ("_at", turns.data_ptr()),
+                            ("_streams", set())):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"{name}: rotary positions stay as they were made")
+
+
+def _number(value, name, low=-math.inf, above=False):
+    """A finite number >= low (> low if above), else ValueError."""
+    if type(value) not in (int, float) or not math.isfinite(value) or value < low or (above and value == low):
+        raise ValueError(f"{name} must be a finite number {'above' if above else 'of at least'} {low}")
+    return value
+
+
 class NativeOps:
     """Inference-only device ops over the v2 ABI; operands are torch GPU tensors,
     work is queued on the current torch stream of their device."""
@@ -311,6 +422,7 @@ class NativeOps:
         if self.lib.ti_v2_abi_version() != 2:
             raise RuntimeError("native v2 ABI version mismatch: version 2 required")
         self._declare("ti_amd_attention_i8kv_workspace", [ctypes.c_void_p] + [ctypes.c_int] * 5, ctypes.c_int64)
+        self._declare("ti_amd_attention_paged_workspace", [ctypes.c_void_p] + [ctypes.c_int] * 5, ctypes.c_int64)
         self.catalog = json.loads(self.lib.ti_v2_gemm_catalog_json())
         listed = tuple({**entry, "tile": tuple(entry["tile"])} for entry in self.catalog["configs"])
         if listed != GEMM_CATALOG:
@@ -625,3 +737,253 @@ class NativeOps:
         call.scalars(batch, vocab)
         call.run()
         return tokens, probs
+
+    def logprobs(self, logits, tokens, *, top=0):
+        """Log probabilities (natural) under the softmax of each row of logits [B,V] (fp16 or
+        fp32): (logprobs of `tokens` int32 [B] or [B,N], in their shape; the rows' entropy
+        [B], in nats; top_logprobs [B,top] and top_tokens int32 [B,top], the likeliest tokens
+        by logit, ties by index), all fp32 but the last.
+
+        A token outside the vocabulary, or with a logit of -inf or NaN, has the log
+        probability -inf and is no alternative: places left over hold 2^31 - 1 and -inf.
+        `top` is at most 64; 0 gives two tensors [B,0]."""
+        torch = self.torch
+        call = _Call(self, "ti_amd_logprobs")
+        wide = isinstance(logits, self.tensor_type) and logits.dtype == torch.float32
+        call.operand(logits, torch.float32 if wide else torch.float16, "logits", rank=2)
+        batch, vocab = logits.shape
+        if vocab > 1 << 18 or batch > 1 << 20:
+            raise ValueError("logits: at most 2^20 rows of 2^18")
+        _count(top, "top", 0, 64)
+        call.scalars(int(wide))
+        call.operand(tokens, torch.int32, "tokens")
+        if tokens.dim() > 2 or tokens.shape[0] != batch or tokens.numel() > batch << 16:
+            raise ValueError(f"tokens: shape [{batch}] or [{batch}, N] with N at most 2^16 required, got {list(tokens.shape)}")
+        logprobs = call.output(tokens.shape, torch.float32)
+        entropy = call.output((batch,), torch.float32)
+        if top:
+            top_logprobs, top_tokens = call.output((batch, top), torch.float32), call.output((batch, top), torch.int32)
+        else:
+            top_logprobs, top_tokens = (torch.empty((batch, 0), dtype=d, device=call.device) for d in (torch.float32, torch.int32))
+            call.scalars(None, None)
+        call.scalars(batch, vocab, tokens.numel() // batch, top)
+        call.run()
+        return logprobs, entropy, top_logprobs, top_tokens
+
+    # -- rotary positions ----------------------------------------------------------
+    def rotary(self, rotated, *, base=10000.0, interleaved=False, scaling=None, factor=1.0, original_length=None, fast=32.0,
+               slow=1.0, frequencies=None, amplitude=1.0, device=None):
+        """Rotary positions that turn the first `rotated` dims of a row (even), in pairs
+        (i, rotated / 2 + i), or (2 i, 2 i + 1) if interleaved, by base^(-2 i / rotated)
+        radians a position.
+
+        scaling stretches them for contexts `factor` times as long: "linear" divides every
+        frequency by it; "base" multiplies the base by factor^(rotated / (rotated - 2)), so
+        that the slowest pair alone is divided; "parts" keeps pairs that turn `fast` times
+        or more over original_length, divides those that turn `slow` times or fewer, and
+        goes over linearly in between.  frequencies gives all of them instead (radians a
+        position, rotated / 2 numbers).  Turned values are multiplied by amplitude."""
+        torch = self.torch
+        if type(rotated) is not int or rotated < 2 or rotated % 2 or rotated > 65536:
+            raise ValueError("rotated must be an even integer in [2, 65536]")
+        if type(interleaved) is not bool:
+            raise ValueError("interleaved must be a bool")
+        _number(base, "base", 0, True)
+        _number(factor, "factor", 0, True)
+        _number(amplitude, "amplitude")
+        if scaling not in (None, "linear", "base", "parts"):
+            raise ValueError('scaling must be None, "linear", "base" or "parts"')
+        if scaling is None and factor != 1:
+            raise ValueError("a factor needs a scaling")
+        count = rotated // 2
+        if frequencies is not None:
+            if scaling is not None or base != 10000.0:
+                raise ValueError("frequencies stand in place of a base and a scaling")
+            got = [float(_number(f, "frequencies")) for f in frequencies]
+            if len(got) != count:
+                raise ValueError(f"frequencies must hold {count} numbers, got {len(got)}")
+        else:
+            if scaling == "base" and count > 1:
+                base = base * factor ** (count / (count - 1))
+            got = [float(base) ** (-i / count) for i in range(count)]
+            if scaling == "linear":
+                got = [f / factor for f in got]
+            if scaling == "parts":
+                _count(original_length, "original_length")
+                _number(slow, "slow")
+                if _number(fast, "fast") <= slow:
+                    raise ValueError("fast must be above slow")
+                for i, f in enumerate(got):
+                    keep = min(max((original_length * f / (2 * math.pi) - slow) / (fast - slow), 0.0), 1.0)
+                    got[i] = f * keep + f / factor * (1.0 - keep)
+        where = torch.device("cuda" if device is None else device)
+        if where.type != "cuda":
+            raise TypeError("device: a GPU (torch 'cuda' device) is required")
+        return Rotary(torch, got, interleaved, amplitude, where)
+
+    def rotate(self, x, rotary, positions):
+        """x fp16 [B,H,Q,D] (its dims contiguous, any other strides) turned by ``rotary``:
+        row i of request b at position positions[b] + i.  positions is an int32 [B] tensor,
+        host ints (one for all, or B of them), or an int32 [B,Q] tensor with a position for
+        every row.  The result is contiguous."""
+        call = _Call(self, "ti_amd_rotate")
+        self._rotary(rotary)
+        call.rows(x, "x", None)
+        batch, heads, rows, dim = x.shape
+        if rotary.rotated > dim:
+            raise ValueError(f"rotary turns {rotary.rotated} dims, x has {dim}")
+        if batch > 65535 or heads > 65535 or rows * dim > 1 << 31:
+            raise ValueError("x: batch and heads must be at most 65535, rows * dims at most 2^31")
+        if positions is None:
+            raise ValueError("positions are required")
+        y = call.output(x.shape, x.dtype)
+        each = isinstance(positions, self.tensor_type) and positions.dim() == 2
+        if each:
+            call.operand(positions, self.torch.int32, "positions", shape=(batch, rows))
+        else:
+            call.per_request(batch, (positions, INT32_MAX - rows, "positions"))
+        call.scalars(int(each))
+        call.turn(rotary)
+        call.scalars(batch, heads, rows, dim)
+        call.run()
+        return y
+
+    def _rotary(self, rotary):
+        if type(rotary) is not Rotary:
+            raise TypeError("rotary: a Rotary (NativeOps.rotary) is required")
+
+    # -- paged KV cache --------------------------------------------------------------
+    def kv_cache_paged(self, pages, kv_heads, page_size, head_dim, *, device=None):
+        """A zeroed fp16 cache of `pages` pages of `page_size` tokens (a power of two from 32
+        to 1024), `kv_heads` key heads of 64 or 128 dims."""
+        torch = self.torch
+        _count(pages, "pages")
+        _count(kv_heads, "kv_heads", high=65535)
+        if type(page_size) is not int or page_size not in (32, 64, 128, 256, 512, 1024):
+            raise ValueError("page_size must be a power of two from 32 to 1024")
+        if type(head_dim) is not int or head_dim not in (64, 128):
+            raise ValueError("head_dim must be 64 or 128")
+        where = torch.device("cuda" if device is None else device)
+        if where.type != "cuda":
+            raise TypeError("device: a GPU (torch 'cuda' device) is required")
+        return PagedKVCache(torch, pages, kv_heads, page_size, head_dim, where)
+
+    def kv_append_paged(self, cache, k, v, page_table, positions, *, lengths=None, rotary=None, q=None):
+        """Put k, v fp16 [B,G,Q,D] into the cache: row i < lengths[b] (None: Q) becomes token
+        positions[b] + i of request b, on the page that page_table (int32 [B,W]) names for it.
+        With ``rotary`` (turning a multiple of 16 dims) keys are turned by their positions on
+        the way, and so is q fp16 [B,H,Q,D], whose turned rows are returned (zeros past
+        lengths[b]); None without q.
+
+        k, v and q may have any strides but the dims', as the slices of one projection do.
+        positions and lengths are int32 [B] tensors, or host ints (one for all, or B of them).
+        Host values must lie inside the table; rows that device values put outside it, or on a
+        page outside the cache, are not written.  Rows of one call must not share a place."""
+        call = _Call(self, "ti_amd_kv_append_paged")
+        call.cache(cache, PagedKVCache)
+        call.rows(k, "k", None)
+        batch, heads, rows, dim = k.shape
+        if heads != cache.kv_heads or dim != cache.head_dim:
+            raise ValueError(f"k must be [B, {cache.kv_heads}, Q, {cache.head_dim}], got {list(k.shape)}")
+        call.rows(v, "v", k.shape)
+        if rotary is not None:
+            self._rotary(rotary)
+            if rotary.rotated % 16 or rotary.rotated > dim:
+                raise ValueError(f"rotary must turn a multiple of 16 of the head's {dim} dims, not {rotary.rotated}")
+        q_heads, turned = 0, None
+        if q is None:
+            call.scalars(None, 0, 0, 0, None)
+        else:
+            if rotary is None:
+                raise ValueError("q is only turned: it needs rotary")
+            call.rows(q, "q", None)
+            q_heads = q.shape[1]
+            if q.shape[0] != batch or q.shape[2] != rows or q.shape[3] != dim or q_heads > 65535:
+                raise ValueError(f"q must be [{batch}, H, {rows}, {dim}] with H at most 65535, got {list(q.shape)}")
+            turned = call.output(q.shape, q.dtype)
+        self._paged_rows(call, cache, page_table, positions, lengths, batch, rows)
+        call.turn(rotary)
+        call.scalars(batch, q_heads, rows)
+        call.run()
+        return turned
+
+    def kv_read_paged(self, cache, page_table, positions, lengths, rows):
+        """fp16 k, v [B,G,rows,D]: row i < lengths[b] (None: rows) is token positions[b] + i of
+        request b; zeros past the length and where no token is.  page_table, positions and
+        lengths as in ``kv_append_paged``."""
+        torch = self.torch
+        call = _Call(self, "ti_amd_kv_read_paged")
+        call.cache(cache, PagedKVCache)
+        _count(rows, "rows")
+        if not isinstance(page_table, self.tensor_type):
+            raise TypeError("page_table: a GPU (torch 'cuda' device) tensor is required")
+        batch = page_table.shape[0] if page_table.dim() else 0
+        k = call.output((batch, cache.kv_heads, rows, cache.head_dim), torch.float16)
+        v = call.output_like(k)
+        self._paged_rows(call, cache, page_table, positions, lengths, batch, rows)
+        call.scalars(batch, rows)
+        call.run()
+        return k, v
+
+    def _paged_rows(self, call, cache, page_table, positions, lengths, batch, rows):
+        """The table, positions and lengths; host values must stay inside the table."""
+        if positions is None:
+            raise ValueError("positions are required")
+        if batch > 65535 or rows > 1 << 28:
+            raise ValueError("batch must be at most 65535, rows at most 2^28")
+        held = min(call.page_table(page_table, batch) * cache.page_size, INT32_MAX)
+        tensor = self.tensor_type
+        if not isinstance(positions, tensor) and not isinstance(lengths, tensor):
+            first = _per_request(positions, batch, 0, held - 1, "positions")
+            count = _per_request(lengths, batch, rows, rows, "lengths")
+            if max(map(int.__add__, first, count)) > held:
+                raise ValueError(f"positions + lengths pass the {held} tokens of the page table")
+        call.per_request(batch, (positions, held - 1, "positions"), (lengths, rows, "lengths"))
+
+    def attention_paged(self, q, cache, page_table, kv_lengths, *, q_lengths=None, query_offsets=None, causal=True,
+                        max_kv_length=None):
+        """q [B,H,Q,D] fp16 over the paged cache, H a multiple of its key heads (query head h
+        reads key head h // (H // G)): request b's keys are tokens 0 .. kv_lengths[b] - 1 on
+        the pages that page_table (int32 [B,W]) names; those on no page of the cache are not
+        seen.
+
+        Causal: query i sees keys up to query_offsets[b] + i; None means
+        kv_lengths[b] - q_lengths[b], the queries being the request's last tokens
+        (append first, then attend).  Rows that see no key and queries past
+        q_lengths[b] are 0.  kv_lengths, q_lengths and query_offsets are int32 [B]
+        tensors or host ints; tensors make a call that a graph can capture.
+        max_kv_length: what kv_lengths stay within where the table holds much more
+        (it plans the launch only)."""
+        call = _Call(self, "ti_amd_attention_paged")
+        call.cache(cache, PagedKVCache)
+        call.operand(q, self.torch.float16, "q", rank=4)
+        batch, heads, nq, dim = q.shape
+        if dim != cache.head_dim or heads % cache.kv_heads:
+            raise ValueError(f"q must be [B, H, Q, {cache.head_dim}] with H a multiple of {cache.kv_heads}, got {list(q.shape)}")
+        if batch > 65535 or heads > 65535:
+            raise ValueError("batch and heads must each be at most 65535")
+        if batch * heads * nq > 1 << 23:
+            raise ValueError("at most 2^23 query rows (batch * heads * queries)")
+        if type(causal) is not bool:
+            raise ValueError("causal must be a bool")
+        if kv_lengths is None:
+            raise ValueError("kv_lengths are required")
+        bound = 0 if max_kv_length is None else _count(max_kv_length, "max_kv_length", 0)
+        y = call.output_like(q)
+        width = call.page_table(page_table, batch)
+        held = min(width * cache.page_size, INT32_MAX)
+        call.per_request(batch, (kv_lengths, held, "kv_lengths"), (q_lengths, nq, "q_lengths"),
+                         (query_offsets, INT32_MAX - nq, "query_offsets"))
+        shape = (width, batch, heads, nq, bound)
+        needed = cache._workspace.get(shape)
+        if needed is None:
+            if len(cache._workspace) >= 1024:  # (a caller whose lengths are all different)
+                cache._workspace.clear()
+            needed = cache._workspace[shape] = max(0, self.lib.ti_amd_attention_paged_workspace(cache._at, *shape))
+        if needed:
+            call.output((needed,), self.torch.uint8)
+        else:
+            call.args.append(None)
+        call.scalars(needed, batch, heads, nq, bound, int(causal))
+        call.run()
+        return y
