@@ -3,15 +3,18 @@
 //   m = max x,  Z = sum e^(x - m),  log p(t) = x_t - m - log Z,
 //   H = -sum p log p = log Z - (sum e^(x - m) (x - m)) / Z
 //
-// One workgroup per row reads it once.  A thread keeps the largest x it has met, how many
-// times, the sum of e^(x - m) over the others and sum e^(x - m) (x - m): a likely token's
-// log probability, log1p of a small sum, and a sure row's entropy keep their digits, and a
-// larger maximum rescales three numbers.  Tokens are ordered by logit, ties by index.  The
-// alternatives come from a list of the tokens at or above a bar that `top` tokens reach for
-// certain: of the threads' largest first tokens, the least one that is among the r largest of
-// its wave, where r times the waves are `top` or more.  Where the list does not hold them
-// (many equal logits, rising ones) the range of the tokens above the bar is cut into runs
-// and read again until it does.
+// One workgroup per row reads it once.  A wave keeps the largest x it has met and how many
+// logits equal it, its lanes the sum of e^(x - m) over the others and sum e^(x - m) (x - m): a
+// likely token's log probability, log1p of a small sum, and a sure row's entropy keep their
+// digits, and a larger maximum rescales three numbers.
+//
+// Alternatives, by logit, ties by index.  A thread takes 32 tokens a round; the largest of them
+// stands for this piece.  Every wave gives the largest few of its first pieces, and the
+// `top`-th of all these is a bar that `top` tokens reach for certain; pieces that reach it are
+// listed.  The `top`-th of the list is a second bar, so only the pieces at or above that one,
+// `top` and ties, are looked at again.  Where a list does not hold them (many equal logits,
+// rising ones) the range of the tokens at or above the bar is cut into runs and read again until
+// it does.
 //
 // NaN logits count as -inf.  A row with a +inf has all its probability on the first one, a
 // row without a logit above -inf none anywhere: log probabilities of -inf, entropy 0.
@@ -24,7 +27,7 @@ namespace {
 typedef unsigned long long u64;
 constexpr int kNoToken = 0x7fffffff;
 constexpr float kNegInf = -__builtin_huge_valf(), kLog2e = 1.4426950408889634f;
-constexpr int kList = 1024, kRuns = 2048;
+constexpr int kThreads = 512, kList = 1024, kRuns = 2048, kFirsts = 128;
 
 // 64-bit key whose descending order is the row's: value, then the lower index.  Never 0.
 __device__ __forceinline__ u64 key_of(float x, int i) {
@@ -38,54 +41,66 @@ __device__ __forceinline__ float value_of(u64 key) {
 }
 __device__ __forceinline__ int index_of(u64 key) { return int(~unsigned(key)); }
 
-__device__ __forceinline__ u64 wave_max_key(u64 v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const u64 w = __shfl_xor(v, o, 64);
-    v = v > w ? v : w;
-  }
-  return v;
+// The largest x of a wave, in every lane, and the sum, by operand modifiers: no trip through LDS.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp(float old, float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, old), __builtin_bit_cast(int, x), CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ float last_lane(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+__device__ __forceinline__ float max_of_wave(float x) {
+  x = fmaxf(x, dpp<0x111, 0xF>(kNegInf, x));  // 1, 2, 4, 8 lanes back within rows of 16
+  x = fmaxf(x, dpp<0x112, 0xF>(kNegInf, x));
+  x = fmaxf(x, dpp<0x114, 0xF>(kNegInf, x));
+  x = fmaxf(x, dpp<0x118, 0xF>(kNegInf, x));
+  x = fmaxf(x, dpp<0x142, 0xA>(kNegInf, x));  // rows 0 and 2's last lane to rows 1 and 3
+  x = fmaxf(x, dpp<0x143, 0xC>(kNegInf, x));  // row 1's to rows 2 and 3
+  return last_lane(x);
+}
+__device__ __forceinline__ float sum_of_wave(float x) {
+  x += dpp<0x111, 0xF>(0.f, x);
+  x += dpp<0x112, 0xF>(0.f, x);
+  x += dpp<0x114, 0xF>(0.f, x);
+  x += dpp<0x118, 0xF>(0.f, x);
+  x += dpp<0x142, 0xA>(0.f, x);
+  x += dpp<0x143, 0xC>(0.f, x);
+  return last_lane(x);
 }
 
-// What a thread knows of the tokens it has met: their maximum m, how many there are of it,
-// and over the others rest = sum e^(x - m), spread = sum e^(x - m) (x - m).
+// What a wave knows of the logits it has met: their maximum m and how many equal it (the
+// same in all lanes), and per lane over the others rest = sum e^(x - m), spread = sum
+// e^(x - m) (x - m).
 struct Stats {
   float m, count, rest, spread;
-  // To a maximum of at least this one's.  (Differences end at -200, where e^ is 0.)
-  __device__ __forceinline__ void raise(float to) {
-    const float d = fmaxf(m - to, -200.f), f = m == to ? 1.f : __builtin_amdgcn_exp2f(d * kLog2e);
-    spread = m == to ? spread : f * fmaf(d, rest + count, spread);
-    rest = m == to ? rest : f * (rest + count);
-    count = m == to ? count : 0.f;
+  // To a maximum of at least this one; `counted` of the count are this lane's to carry over.
+  // (Differences end at -200, where e^ is 0.)
+  __device__ __forceinline__ void raise(float to, float counted) {
+    if (m == to) return;
+    const float d = fmaxf(m - to, -200.f), f = __builtin_amdgcn_exp2f(d * kLog2e);
+    spread = f * fmaf(d, rest + counted, spread);
+    rest = f * (rest + counted);
+    count = 0.f;
     m = to;
   }
-  __device__ __forceinline__ void join(Stats o) {
-    const float to = fmaxf(m, o.m);
-    raise(to);
-    o.raise(to);
-    count += o.count;
-    rest += o.rest;
-    spread += o.spread;
-  }
-  __device__ __forceinline__ Stats from(int lane) const {
-    return {__shfl_xor(m, lane, 64), __shfl_xor(count, lane, 64), __shfl_xor(rest, lane, 64), __shfl_xor(spread, lane, 64)};
-  }
+  // x, and their maximum (called by whole waves).
   template <int N>
-  __device__ __forceinline__ void add(const float (&x)[N]) {
-    float high = kNegInf;
+  __device__ __forceinline__ void add(float (&x)[N], float high) {
+    if (__ballot(high > m)) raise(max_of_wave(fmaxf(high, m)), (threadIdx.x & 63) == 0 ? count : 0.f);
+    if (__ballot(high == m)) {
+      int equal = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) high = fmaxf(high, x[i]);  // (NaN loses)
-    const bool equal = __ballot(high >= m);
-    raise(fmaxf(m, high));
+      for (int i = 0; i < N; ++i) {
+        equal += __popcll(__ballot(x[i] == m));
+        x[i] = x[i] == m ? kNegInf : x[i];
+      }
+      count += float(equal);
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float d = fmaxf(x[i] - m, -200.f);  // (NaN and -inf too: e^-200 is 0)
-      float e = __builtin_amdgcn_exp2f(d * kLog2e);
+      const float e = __builtin_amdgcn_exp2f(d * kLog2e);
       spread = fmaf(d, e, spread);
-      if (equal) {
-        count += x[i] == m ? 1.f : 0.f;
-        e = x[i] == m ? 0.f : e;
-      }
       rest += e;
     }
   }
@@ -95,43 +110,60 @@ template <typename T>
 struct Vec {
   static constexpr int W = 16 / int(sizeof(T));
   typedef T type __attribute__((ext_vector_type(W)));
+  typedef type loose __attribute__((aligned(sizeof(T))));  // (the device allows unaligned vector accesses)
 };
 
 template <typename T, int THREADS>
 struct Lds {
-  u64 list[kList];
-  u64 bar[THREADS / 64];
+  u64 keys[2][kList];  // two lists, one the other's order
+  float firsts[kFirsts];  // the waves' largest first logits
   Stats stats[THREADS / 64];
-  unsigned run[kRuns];
-  unsigned count, pick, above;
+  union {
+    unsigned run[kRuns];
+    unsigned rank[kList];
+  };
+  unsigned count, found, pick, above;
   u64 low, high;
 };
 
-// The row as threads see it: token `head` on starts a 16-byte boundary, vector v of it is
-// tokens head + W v ..; the few in front and behind are one token each of the first threads.
-template <typename T, int THREADS>
+// The row as threads see it: vector v is tokens W v .., wherever in memory the row starts
+// (so an answer does not depend on that), the few behind the last one are one token each of
+// the first threads.  A thread takes N tokens, A vectors, a round.
+template <typename T, int THREADS, int TOKENS>
 struct Row {
-  static constexpr int W = Vec<T>::W, A = 4;  // vectors of a thread at a time
+  static constexpr int W = Vec<T>::W, N = TOKENS, A = N / W;
   const T* p;
-  int n, head, vectors;
-  __device__ __forceinline__ Row(const T* row, int length) : p(row), n(length) {
-    head = min(n, int(-(reinterpret_cast<uintptr_t>(row) / sizeof(T))) & (W - 1));
-    vectors = (n - head) / W;
-  }
+  int n, vectors;
+  __device__ __forceinline__ Row(const T* row, int length) : p(row), n(length), vectors(length / W) {}
   __device__ __forceinline__ int rounds() const { return (vectors + A * THREADS - 1) / (A * THREADS); }
-  // This thread's token in front of or behind the vectors, or -1.
+  // This thread's token behind the vectors, or -1.
   __device__ __forceinline__ int edge() const {
-    const int t = int(threadIdx.x), at = t < head ? t : t + vectors * W;
-    return at < n && (t < head || t < n - vectors * W) ? at : -1;
+    const int at = vectors * W + int(threadIdx.x);
+    return at < n ? at : -1;
+  }
+  __device__ __forceinline__ int vector(int round, int c) const { return (round * A + c) * THREADS + int(threadIdx.x); }
+  __device__ __forceinline__ int token(int round, int i) const { return vector(round, i / W) * W + i % W; }
+  // Token i (0 .. N - 1) of a piece, numbered by round and thread (behind the last round: the
+  // threads' edges), or -1.
+  __device__ __forceinline__ int token_of(int piece, int i) const {
+    const int round = piece / THREADS, t = piece % THREADS, v = (round * A + i / W) * THREADS + t;
+    if (round == rounds()) return i == 0 ? vectors * W + t : -1;
+    return v < vectors ? v * W + i % W : -1;
   }
   __device__ __forceinline__ void load(typename Vec<T>::type (&x)[A], int round) const {
 #pragma unroll
-    for (int c = 0; c < A; ++c) {
-      const int v = (round * A + c) * THREADS + int(threadIdx.x);
-      x[c] = *reinterpret_cast<const typename Vec<T>::type*>(p + head + min(v, vectors - 1) * W);
+    for (int c = 0; c < A; ++c)
+      x[c] = __builtin_nontemporal_load(reinterpret_cast<const typename Vec<T>::loose*>(p + min(vector(round, c), vectors - 1) * W));
+  }
+  // A round's values; -inf past the last vector.
+  __device__ __forceinline__ void values(float (&x)[N], const typename Vec<T>::type (&v)[A], int round) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = float(v[i / W][i % W]);
+    if ((round + 1) * A * THREADS > vectors) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = vector(round, i / W) < vectors ? x[i] : kNegInf;
     }
   }
-  __device__ __forceinline__ int token(int round, int c) const { return head + ((round * A + c) * THREADS + int(threadIdx.x)) * W; }
   // f(value, index) for every token.
   template <typename F>
   __device__ void each(F f) const {
@@ -141,19 +173,17 @@ struct Row {
       typename Vec<T>::type x[A];
       load(x, r);
 #pragma unroll
-      for (int c = 0; c < A; ++c)
-#pragma unroll
-        for (int i = 0; i < W; ++i)
-          if (token(r, c) + i < head + vectors * W) f(float(x[c][i]), token(r, c) + i);
+      for (int i = 0; i < N; ++i)
+        if (vector(r, i / W) < vectors) f(float(x[i / W][i % W]), token(r, i));
     }
   }
 };
 
-// The list again, for a row whose tokens at or above `bar` (keys) are more than it holds: the
+// The list again, for a row of which it does not hold all tokens at or above `bar`: the
 // range of their keys is cut into kRuns runs, and the one in which the `top`-th lies is cut
 // again, until it and the runs above fit.  (Keys are distinct, so this ends.)
-template <typename T, int THREADS>
-__device__ __noinline__ void refill(Lds<T, THREADS>& s, const Row<T, THREADS>& row, u64 bar, unsigned top) {
+template <typename T, int THREADS, int N>
+__device__ __noinline__ void refill(Lds<T, THREADS>& s, const Row<T, THREADS, N>& row, int to_list, float bar, unsigned top) {
   u64 low = ~u64(0), high = 0;
   if (threadIdx.x == 0) {
     s.low = low;
@@ -161,9 +191,8 @@ __device__ __noinline__ void refill(Lds<T, THREADS>& s, const Row<T, THREADS>& r
   }
   __syncthreads();
   row.each([&](float x, int i) {
-    if (!(x > kNegInf)) return;
+    if (!(x >= bar)) return;
     const u64 k = key_of(x, i);
-    if (k < bar) return;
     low = min(low, k);
     high = max(high, k);
   });
@@ -178,7 +207,7 @@ __device__ __noinline__ void refill(Lds<T, THREADS>& s, const Row<T, THREADS>& r
     for (int i = int(threadIdx.x); i < kRuns; i += THREADS) s.run[i] = 0;
     __syncthreads();
     row.each([&](float x, int i) {
-      if (!(x > kNegInf)) return;
+      if (!(x >= bar)) return;
       const u64 k = key_of(x, i);
       if (k >= low && k <= high) atomicAdd(&s.run[(high - k) / width], 1u);
     });
@@ -202,148 +231,238 @@ __device__ __noinline__ void refill(Lds<T, THREADS>& s, const Row<T, THREADS>& r
     high = from;
     low = to;
   }
-  if (threadIdx.x == 0) s.count = 0;
+  if (threadIdx.x == 0) s.found = 0;
   __syncthreads();
   row.each([&](float x, int i) {
-    if (!(x > kNegInf)) return;
+    if (!(x >= bar)) return;
     const u64 k = key_of(x, i);
     if (k < low) return;
-    const unsigned at = atomicAdd(&s.count, 1u);
-    if (at < kList) s.list[at] = k;
+    const unsigned at = atomicAdd(&s.found, 1u);
+    if (at < kList) s.keys[to_list][at] = k;
   });
   __syncthreads();
 }
 
+// The top-th largest of many >= top numbers, 64 H at most, by every wave for itself.
+template <int H>
+__device__ __forceinline__ float nth_of(const float* numbers, int many, int top) {
+  const int lane = int(threadIdx.x & 63);
+  float mine[H], least = kNegInf;
+  int above[H];
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    mine[h] = lane + 64 * h < many ? numbers[lane + 64 * h] : kNegInf;
+    above[h] = 0;
+  }
+#pragma unroll
+  for (int from = 0; from < H; ++from)
+#pragma unroll 8
+    for (int i = 0; i < min(many - 64 * from, 64); ++i) {
+      const float other = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine[from]), i));
+#pragma unroll
+      for (int h = 0; h < H; ++h) above[h] += other > mine[h];
+    }
+#pragma unroll
+  for (int h = 0; h < H; ++h) least = fmaxf(least, lane + 64 * h < many && above[h] < top ? -mine[h] : kNegInf);
+  return -max_of_wave(least);
+}
+
+// List `from`'s n keys in their order, into the other one; several threads to a key, each comparing it with a part
+// of the others.
 template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void logprobs_kernel(LogprobsArgs a) {
-  constexpr int WAVES = THREADS / 64;
-  using R = Row<T, THREADS>;
+__device__ __forceinline__ void sort_list(Lds<T, THREADS>& s, int from, unsigned n) {
+  const u64* list = s.keys[from];
+  const unsigned tid = threadIdx.x;
+  unsigned wide = 64;
+  while (wide < n) wide *= 2;
+  for (unsigned i = tid; i < n; i += THREADS) s.rank[i] = 0;
+  __syncthreads();
+  const unsigned parts = max(unsigned(THREADS) / wide, 1u), part = tid / wide, chunk = (n + parts - 1) / parts;
+  for (unsigned i = tid & (wide - 1); i < n; i += THREADS) {
+    const u64 k = list[i];
+    const unsigned end = min(n, (part + 1) * chunk);
+    unsigned before = 0;
+#pragma unroll 8
+    for (unsigned o = part * chunk; o < end; ++o) before += list[o] > k;
+    if (before) atomicAdd(&s.rank[i], before);
+  }
+  __syncthreads();
+  for (unsigned i = tid; i < n; i += THREADS) s.keys[1 - from][s.rank[i]] = list[i];
+  __syncthreads();
+}
+
+template <typename T, int N>
+__global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
+  constexpr int THREADS = kThreads, WAVES = THREADS / 64;
+  using R = Row<T, THREADS, N>;
   __shared__ Lds<T, THREADS> s;
-  const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
+  const int tid = int(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const T* logits = static_cast<const T*>(a.logits) + int64_t(blockIdx.x) * a.vocab;
   const R row(logits, a.vocab);
-  const int rounds = row.rounds();
+  const int rounds = row.rounds(), edge = row.edge();
   typename Vec<T>::type next[R::A];
   if (rounds > 0) row.load(next, 0);
-  const int edge = row.edge();
   const float edge_x = edge >= 0 ? float(logits[edge]) : kNegInf;
-  if (tid == 0) s.count = 0;
-  Stats mine{kNegInf, 0.f, 0.f, 0.f};
-  u64 bar = ~u64(0);
-  const auto offer = [&](float x, int i) {
-    if (x > kNegInf && key_of(x, i) >= bar) {
-      const unsigned at = atomicAdd(&s.count, 1u);
-      if (at < kList) s.list[at] = key_of(x, i);
-    }
+  float x[R::N];
+#pragma unroll
+  for (int i = 0; i < R::N; ++i) x[i] = kNegInf;
+  if (rounds > 0) row.values(x, next, 0);
+  if (rounds > 1) row.load(next, 1);
+  const auto largest = [&] {
+    float high = x[0];
+#pragma unroll
+    for (int i = 1; i < R::N; ++i) high = fmaxf(high, x[i]);  // (NaN loses)
+    return fmaxf(high, kNegInf);
   };
-  {
-    const float x[1] = {edge_x};
-    mine.add(x);
-  }
-  float bar_x = __builtin_huge_valf();  // the bar's value: no token below it counts
-  for (int r = 0; r < rounds || r == 0; ++r) {
-    float x[R::A * R::W];
-    float high = kNegInf;
-    int high_at = 0;
-#pragma unroll
-    for (int c = 0; c < R::A; ++c)
-#pragma unroll
-      for (int i = 0; i < R::W; ++i) {
-        const bool is = row.token(r, c) < row.head + row.vectors * R::W;  // (a vector is whole or not there)
-        x[c * R::W + i] = is ? float(next[c][i]) : kNegInf;
-      }
-    if (r + 1 < rounds) row.load(next, r + 1);
-    mine.add(x);
-    if (a.top > 0) {
-      if (r == 0) {
-        // The bar, from every thread's first tokens.
-        high = edge_x;
-        high_at = edge;
-#pragma unroll
-        for (int i = 0; i < R::A * R::W; ++i) {
-          const int at = row.token(0, i / R::W) + i % R::W;
-          const bool more = x[i] > high || (x[i] == high && at < high_at);
-          high_at = more ? at : high_at;
-          high = more ? x[i] : high;
-        }
-        u64 best = high > kNegInf ? key_of(high, high_at) : 0, bound = best;
-        const int ranks = (a.top + WAVES - 1) / WAVES;
-        for (int i = 0; i < ranks; ++i) {
-          bound = wave_max_key(best);
-          best = best == bound ? 0 : best;
-        }
-        if (lane == 0) s.bar[wave] = bound;
-        __syncthreads();  // (and the count is 0)
-        bar = s.bar[0];
-#pragma unroll
-        for (int w = 1; w < WAVES; ++w) bar = min(bar, s.bar[w]);
-        bar_x = bar == 0 ? kNegInf : value_of(bar);
-        offer(edge_x, edge);
-      }
-      high = kNegInf;
-#pragma unroll
-      for (int i = 0; i < R::A * R::W; ++i) high = fmaxf(high, x[i]);
-      if (high >= bar_x) {
-#pragma unroll
-        for (int i = 0; i < R::A * R::W; ++i)
-          if (x[i] >= bar_x) offer(x[i], row.token(r, i / R::W) + i % R::W);
+  float high = largest();
+
+  // The bar: `top` tokens at least are not below it.
+  float bar = __builtin_huge_valf();
+  if (a.top > 0) {
+    if (tid == 0) s.count = s.found = 0;
+    // Waves with vectors, how many logits each gives, and all of them.
+    const int active = min(max((row.vectors + 63) / 64, 1), WAVES), each = min((a.top + active - 1) / active + 1, kFirsts / active);
+    const int many = each * active;
+    if (wave < active) {
+      float left = fmaxf(high, edge_x);
+      for (int i = 0; i < each; ++i) {
+        const float best = max_of_wave(left);
+        const u64 who = __ballot(left == best);
+        if (lane == 0) s.firsts[each * wave + i] = best;
+        if (lane == __builtin_ctzll(who)) left = kNegInf;
       }
     }
+    __syncthreads();
+    // The least of those with fewer than `top` above them.
+    if (many < a.top) {
+      bar = kNegInf;
+    } else if (many <= 64) {
+      bar = nth_of<1>(s.firsts, many, a.top);
+    } else {
+      bar = nth_of<2>(s.firsts, many, a.top);
+    }
+    bar = fmaxf(bar, -3.402823466e38f);  // (a logit of -inf is none)
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) mine.join(mine.from(o));
-  if (lane == 0) s.stats[wave] = mine;
-  __syncthreads();
-  mine = s.stats[0];
-#pragma unroll
-  for (int w = 1; w < WAVES; ++w) mine.join(s.stats[w]);
+  const auto offer = [&](float v, int piece) {
+    const unsigned at = atomicAdd(&s.count, 1u);
+    if (at < kList) s.keys[0][at] = key_of(v, piece);
+  };
 
-  const bool none = mine.m == kNegInf, sure = mine.m == __builtin_huge_valf();
-  const float log_z = logf(mine.count) + log1pf(mine.rest / mine.count);
+  Stats stats{kNegInf, 0.f, 0.f, 0.f};
+  for (int r = 0;;) {
+    if (high >= bar) offer(high, r * THREADS + tid);
+    stats.add(x, high);
+    if (++r >= rounds) break;
+    row.values(x, next, r);
+    if (r + 1 < rounds) row.load(next, r + 1);
+    high = largest();
+  }
+  if (wave == 0) {  // (the first threads have them)
+    float e[1] = {edge_x};
+    stats.add(e, fmaxf(edge_x, kNegInf));
+    if (edge_x >= bar) offer(edge_x, rounds * THREADS + tid);
+  }
+  stats.rest = sum_of_wave(stats.rest);
+  stats.spread = sum_of_wave(stats.spread);
+  if (lane == 0) s.stats[wave] = stats;
+  __syncthreads();
+  float m = kNegInf, count = 0.f, rest = 0.f, spread = 0.f;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) m = fmaxf(m, s.stats[w].m);
+  stats = s.stats[lane % WAVES];
+  stats.raise(m, stats.count);
+  count = stats.count, rest = stats.rest, spread = stats.spread;
+#pragma unroll
+  for (int o = WAVES / 2; o > 0; o >>= 1) {
+    count += __shfl_xor(count, o, 64);
+    rest += __shfl_xor(rest, o, 64);
+    spread += __shfl_xor(spread, o, 64);
+  }
+
+  const bool none = m == kNegInf, sure = m == __builtin_huge_valf();
+  const float log_z = logf(count) + log1pf(rest / count);
   int first = kNoToken;  // sure: the first +inf
   if (sure) {
     if (tid == 0) s.pick = unsigned(kNoToken);
     __syncthreads();
-    row.each([&](float x, int i) {
-      if (x == __builtin_huge_valf()) atomicMin(&s.pick, unsigned(i));
-    });
+    for (int i = tid; i < a.vocab; i += THREADS)
+      if (float(logits[i]) == __builtin_huge_valf()) {
+        atomicMin(&s.pick, unsigned(i));
+        break;
+      }
     __syncthreads();
     first = int(s.pick);
   }
-  const auto log_p = [&](float x, int i) {
+  const auto log_p = [&](float v, int i) {
     if (sure) return i == first ? 0.f : kNegInf;
-    return x > kNegInf ? (x - mine.m) - log_z : kNegInf;
+    return v > kNegInf ? (v - m) - log_z : kNegInf;
   };
-  if (tid == 0) a.entropy[blockIdx.x] = none || sure ? 0.f : log_z - mine.spread / (mine.count + mine.rest);
+  if (tid == 0) a.entropy[blockIdx.x] = none || sure ? 0.f : log_z - spread / (count + rest);
   for (int i = tid; i < a.given; i += THREADS) {
     const int64_t at = int64_t(blockIdx.x) * a.given + i;
     const int token = a.tokens[at];
     a.logprobs[at] = token >= 0 && token < a.vocab ? log_p(float(logits[token]), token) : kNegInf;
   }
   if (a.top == 0) return;
-  if (s.count > kList) refill(s, row, bar, unsigned(a.top));
-  const unsigned n = min(s.count, unsigned(kList));
-  const int64_t out = int64_t(blockIdx.x) * a.top;
-  for (unsigned i = unsigned(tid); i < n; i += THREADS) {
-    const u64 k = s.list[i];
-    unsigned before = 0;
-    for (unsigned o = 0; o < n; ++o) before += s.list[o] > k;
-    if (before < unsigned(a.top)) {
-      a.top_tokens[out + before] = index_of(k);
-      a.top_logprobs[out + before] = log_p(value_of(k), index_of(k));
+  int at_list = 0;  // where the tokens are listed
+  if (s.count > kList) {
+    refill(s, row, 0, bar, unsigned(a.top));
+  } else {
+    // (Few pieces are looked at in one go.)
+    constexpr unsigned AT_ONCE = THREADS / N, DEEP = 4;
+    const unsigned pieces = s.count;
+    at_list = 1;
+    if (pieces > DEEP * AT_ONCE) {
+      sort_list(s, 0, pieces);
+      at_list = 0;
+      if (pieces >= unsigned(a.top)) bar = value_of(s.keys[1][a.top - 1]);
     }
+    const u64* list = s.keys[1 - at_list];
+    for (unsigned e = unsigned(tid) / N; e < pieces; e += DEEP * AT_ONCE) {
+      int token[DEEP];
+      float v[DEEP];
+#pragma unroll
+      for (unsigned c = 0; c < DEEP; ++c) {
+        const u64 k = list[min(e + c * AT_ONCE, pieces - 1)];
+        token[c] = e + c * AT_ONCE < pieces && value_of(k) >= bar ? row.token_of(index_of(k), tid % N) : -1;
+      }
+      if (__ballot(token[0] >= 0) == 0) break;  // (none from here on: they are in order, or this is the only go)
+#pragma unroll
+      for (unsigned c = 0; c < DEEP; ++c) v[c] = token[c] >= 0 ? float(logits[token[c]]) : kNegInf;
+#pragma unroll
+      for (unsigned c = 0; c < DEEP; ++c)
+        if (v[c] >= bar) {
+          const unsigned at = atomicAdd(&s.found, 1u);
+          if (at < kList) s.keys[at_list][at] = key_of(v[c], token[c]);
+        }
+    }
+    __syncthreads();
+    if (s.found > kList) refill(s, row, at_list, bar, unsigned(a.top));
   }
-  for (unsigned i = n + unsigned(tid); i < unsigned(a.top); i += THREADS) {
-    a.top_tokens[out + i] = kNoToken;
-    a.top_logprobs[out + i] = kNegInf;
+  const unsigned n = s.found;
+  sort_list(s, at_list, n);
+  const int64_t out = int64_t(blockIdx.x) * a.top;
+  for (unsigned i = unsigned(tid); i < unsigned(a.top); i += THREADS) {
+    const u64 k = i < n ? s.keys[1 - at_list][i] : 0;
+    a.top_tokens[out + i] = i < n ? index_of(k) : kNoToken;
+    a.top_logprobs[out + i] = i < n ? log_p(value_of(k), index_of(k)) : kNegInf;
   }
+}
+
+// Tokens of a thread's piece: 16, or 32 from here on.
+constexpr int kWideVocab = 65536;
+
+void launch(void (*kernel)(LogprobsArgs), const LogprobsArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL(kernel, dim3(unsigned(a.batch)), dim3(kThreads), 0, stream, a);
 }
 
 }  // namespace
 
 hipError_t logprobs(const LogprobsArgs& a, hipStream_t stream) {
-  if (a.f32) hipLaunchKernelGGL((logprobs_kernel<float, 1024>), dim3(unsigned(a.batch)), dim3(1024), 0, stream, a);
-  else hipLaunchKernelGGL((logprobs_kernel<f16, 1024>), dim3(unsigned(a.batch)), dim3(1024), 0, stream, a);
+  // (By the vocabulary alone: a row's answer does not depend on the others of the call.)
+  const bool wide = a.vocab > kWideVocab;
+  if (a.f32) launch(wide ? logprobs_kernel<float, 32> : logprobs_kernel<float, 16>, a, stream);
+  else launch(wide ? logprobs_kernel<f16, 32> : logprobs_kernel<f16, 16>, a, stream);
   return hipGetLastError();
 }
 
