@@ -6,7 +6,10 @@
 // lane: eight loads of 16 bytes, an 8 x 8 turn in registers (32 byte permutations, the rest
 // of it is naming), eight stores of 16 bytes that with the neighbouring lanes' fill whole
 // records.  Tokens that are not the call's own keep what they hold: a lane whose 8 are not
-// all to be written stores single values.
+// all to be written stores single values.  One launch: a workgroup takes some heads of the
+// queries, the keys or the values of a range of tokens that starts where a record does, and
+// neighbouring ones the same tokens of other heads, which lie side by side where q, k and v are
+// slices of one projection.
 #include "paged_cache.hpp"
 #include "rotary.hpp"
 
@@ -27,17 +30,9 @@ __device__ __forceinline__ uint16_t* head_at(const KvPaged& c, const PageTable& 
   return c.pages + (int64_t(page) * c.kv_heads + head) * paged_head_size(c);
 }
 
-// Queries and keys, 16 values to a lane.  Grid: (rows x D / 16, chunks of heads, batch); a
-// chunk holds query heads or key heads.
-template <int D>
-__global__ __launch_bounds__(256) void append_turned_kernel(PagedAppendArgs a, int q_chunks, int chunk) {
-  constexpr unsigned units = D / 16;
-  const unsigned at = blockIdx.x * 256 + threadIdx.x;
-  const int b = int(blockIdx.z), row = int(at / units), u = int(at % units);
-  if (row >= a.rows) return;
-  const bool keys = int(blockIdx.y) >= q_chunks;
-  const int heads = keys ? a.cache.kv_heads : a.heads;
-  const int h0 = (int(blockIdx.y) - (keys ? q_chunks : 0)) * chunk, h1 = min(heads, h0 + chunk);
+// 16 values of heads [h0, h1) of one row of the queries (keys: false) or the keys.
+template <int D, int HC>
+__device__ __forceinline__ void append_turned(const PagedAppendArgs& a, bool keys, int b, int row, int u, int h0, int h1) {
   const Rows& from = keys ? a.k : a.q;
   const uint16_t* x = from.at + b * from.batch + row * from.row;
   const bool live = row < live_rows(a.lengths, b, a.rows);
@@ -64,22 +59,7 @@ __global__ __launch_bounds__(256) void append_turned_kernel(PagedAppendArgs a, i
       return;
     }
   }
-  if (!unit.turned) {
-#pragma unroll 4
-    for (int h = h0; h < h1; ++h) {
-      store_half8(y + h * step, load_half8(x + h * from.head + unit.first));
-      store_half8(y + h * step + second, load_half8(x + h * from.head + unit.second));
-    }
-    return;
-  }
-  const Turns turns(a.rotary, u, t);
-#pragma unroll 4
-  for (int h = h0; h < h1; ++h) {
-    half8_t p = load_half8(x + h * from.head + unit.first), q = load_half8(x + h * from.head + unit.second);
-    turn_unit(turns, a.rotary.interleaved, p, q);
-    store_half8(y + h * step, p);
-    store_half8(y + h * step + second, q);
-  }
+  turn_heads<HC>(a.rotary, unit, u, t, x, from.head, y, step, second, h0, h1);
 }
 
 // 8 rows of 8 values the other way round.
@@ -97,15 +77,13 @@ __device__ __forceinline__ void transpose8(u32x4_t (&x)[8]) {
 // Token number i (0 .. 7) of a lane's 8 of a block of 32.
 __device__ __forceinline__ int block_token(int g, int i) { return 16 * (i >> 2) + 4 * g + (i & 3); }
 
-// Values: D / 2 lanes to a head's block of 32 tokens.  Grid: (blocks, head groups, batch).
+// 8 dims (from 8 s) of 8 tokens (group g of the block of 32 from t0 on) of one head's values.
 template <int D>
-__global__ __launch_bounds__(256) void append_values_kernel(PagedAppendArgs a) {
-  constexpr int LPB = D / 2, HEADS = 256 / LPB, PIECES = D / 8, PER = D / 16;
-  const int b = int(blockIdx.z), lane = int(threadIdx.x) % LPB, s = lane % PIECES, g = lane / PIECES;
-  const int head = int(blockIdx.y) * HEADS + int(threadIdx.x) / LPB;
+__device__ __forceinline__ void append_values(const PagedAppendArgs& a, int b, int64_t t0, int head, int s, int g) {
+  constexpr int PER = D / 16;
   const int n = live_rows(a.lengths, b, a.rows);
-  const int64_t pos = a.positions[b], t0 = ((pos >> 5) + blockIdx.x) << 5;
-  if (head >= a.cache.kv_heads || n <= 0 || t0 >= pos + n) return;
+  const int64_t pos = a.positions[b];
+  if (n <= 0 || t0 >= pos + n || t0 + 32 <= pos) return;
   uint16_t* y = head_at(a.cache, a.pages, b, t0, head);
   if (!y) return;
   y += int64_t(a.cache.page_size) * D + paged_v_at(int(t0) & (a.cache.page_size - 1), 0, D) + 128 * g;
@@ -119,30 +97,68 @@ __global__ __launch_bounds__(256) void append_values_kernel(PagedAppendArgs a) {
     all = all && live[i];
     v[i] = __builtin_bit_cast(u32x4_t, load_half8(x + min(max(row, int64_t(0)), int64_t(n - 1)) * a.v.row));
   }
-  if (all) transpose8(v);
+  if (all) {
+    transpose8(v);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int dim = 8 * s + e;
-    if (all) {
-      *reinterpret_cast<u32x4_t*>(y + dim % PER * 512 + dim / PER * 8) = v[e];
-    } else {
-      // (Value e of token i.)
+    for (int e = 0; e < 8; ++e) *reinterpret_cast<u32x4_t*>(y + (8 * s + e) % PER * 512 + (8 * s + e) / PER * 8) = v[e];
+  } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (live[i]) y[dim % PER * 512 + dim / PER * 8 + i] = uint16_t(v[i][e >> 1] >> (16 * (e & 1)));
+    for (int i = 0; i < 8; ++i) {
+      if (!live[i]) continue;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[(8 * s + e) % PER * 512 + (8 * s + e) / PER * 8 + i] = uint16_t(v[i][e >> 1] >> (16 * (e & 1)));
     }
   }
 }
 
-// A few rows (single tokens): 8 dims of one row to a lane, stored one by one.
+// Many rows.  A workgroup takes the tokens [t0, t0 + RANGE), t0 a multiple of 32, of `chunk`
+// heads (of the values: v_chunk).  Grid: (chunks of q, k and v, ranges, batch).
 template <int D>
-__global__ __launch_bounds__(256) void append_value_rows_kernel(PagedAppendArgs a) {
-  constexpr unsigned PIECES = D / 8;
+struct Range {
+  static constexpr int LANES = D / 16, RANGE = 256 / LANES;                // 64 or 32 tokens
+  static constexpr int BLOCKS = RANGE / 32, HEADS = 256 / (D / 2) / BLOCKS;  // of values: heads at a time
+};
+template <int D, int HC>
+__global__ __launch_bounds__(256) void append_range_kernel(PagedAppendArgs a, int q_chunks, int k_chunks, int chunk, int v_chunk) {
+  using R = Range<D>;
+  const int b = int(blockIdx.z), tid = int(threadIdx.x);
+  const int64_t pos = a.positions[b], t0 = (pos & ~int64_t(31)) + int64_t(blockIdx.y) * R::RANGE;
+  if (t0 >= pos + a.rows) return;
+  int c = int(blockIdx.x);
+  if (c < q_chunks + k_chunks) {
+    const bool keys = c >= q_chunks;
+    if (keys) c -= q_chunks;
+    const int64_t row = t0 + tid / R::LANES - pos;
+    if (row < 0 || row >= a.rows) return;
+    append_turned<D, HC>(a, keys, b, int(row), tid % R::LANES, c * chunk, min(keys ? a.cache.kv_heads : a.heads, (c + 1) * chunk));
+    return;
+  }
+  c -= q_chunks + k_chunks;
+  const int lane = tid % (D / 2), block = tid / (D / 2) % R::BLOCKS;
+  for (int h = c * v_chunk + tid / (D / 2) / R::BLOCKS; h < min(a.cache.kv_heads, (c + 1) * v_chunk); h += R::HEADS)
+    append_values<D>(a, b, t0 + 32 * block, h, lane % (D / 8), lane / (D / 8));
+}
+
+// A few rows (single tokens): a lane has 16 values of a query or key, or 8 of a value, which it
+// stores one by one.  Grid: (lanes, batch).
+template <int D>
+__global__ __launch_bounds__(256) void append_few_kernel(PagedAppendArgs a) {
+  constexpr unsigned UNITS = D / 16, PIECES = D / 8;
   constexpr int PER = D / 16;
-  const unsigned at = blockIdx.x * 256 + threadIdx.x;
-  const int b = int(blockIdx.y), s = int(at % PIECES);
+  const unsigned rows = unsigned(a.rows), turned = unsigned(a.heads + a.cache.kv_heads) * rows * UNITS;
+  unsigned at = blockIdx.x * 256 + threadIdx.x;
+  const int b = int(blockIdx.y);
+  if (at < turned) {
+    const unsigned u = at % UNITS, hr = at / UNITS, head = hr / rows;
+    const bool keys = int(head) >= a.heads;
+    const int h = int(head) - (keys ? a.heads : 0);
+    append_turned<D, 1>(a, keys, b, int(hr % rows), int(u), h, h + 1);
+    return;
+  }
+  at -= turned;
+  const int s = int(at % PIECES);
   const unsigned hr = at / PIECES;
-  const int head = int(hr / unsigned(a.rows)), row = int(hr % unsigned(a.rows));
+  const int head = int(hr / rows), row = int(hr % rows);
   if (head >= a.cache.kv_heads || row >= live_rows(a.lengths, b, a.rows)) return;
   const int64_t t = int64_t(a.positions[b]) + row;
   uint16_t* y = head_at(a.cache, a.pages, b, t, head);
@@ -150,10 +166,7 @@ __global__ __launch_bounds__(256) void append_value_rows_kernel(PagedAppendArgs 
   const u16x8_t v = __builtin_bit_cast(u16x8_t, load_half8(a.v.at + b * a.v.batch + head * a.v.head + row * a.v.row + 8 * s));
   y += int64_t(a.cache.page_size) * D + paged_v_at(int(t) & (a.cache.page_size - 1), 0, D);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int dim = 8 * s + e;
-    y[dim % PER * 512 + dim / PER * 8] = v[e];
-  }
+  for (int e = 0; e < 8; ++e) y[(8 * s + e) % PER * 512 + (8 * s + e) / PER * 8] = v[e];
 }
 
 // Rows back: a lane takes 8 dims of a token's key and turns 8 dims of 8 tokens' values
@@ -192,27 +205,34 @@ __global__ __launch_bounds__(256) void read_kernel(PagedReadArgs a) {
 // Blocks of 32 tokens that `rows` rows from any position on can touch.
 unsigned blocks_of(int rows) { return unsigned((int64_t(rows) + 30) / 32 + 1); }
 
-constexpr int kValueRowsMax = 8;
+// Whether a row's lanes lie side by side, values stored one by one, in place of whole records:
+// few rows to a request leave most of a range idle, and few rows in all are done sooner by more
+// lanes.  One by one against ranges, us, with queries: 32 requests of 25 heads of 64, 4 / 16 / 64
+// rows 5.4 / 7.2 / 13.8 and 7.8 / 14.9 / 21.3; 64 of 32 over 8 of 128, 5.5 / 10 / 25.2 and 8.4 /
+// 15.5 / 25.7; one of 12 heads, 1000 rows 5.8 and 6.1; 8 of 12, 200 / 400 / 1000 rows 8.0 / 12.2 /
+// 20.1 and 9.0 / 11.5 / 18.7; 16 of 32 over 8, 128 / 200 / 1000 14.5 / 19.2 / 93 and 15.3 /
+// 18.4 / 83.
+bool one_by_one(const PagedAppendArgs& a) { return a.rows <= 64 || int64_t(a.batch) * a.rows <= 2048; }
 
 template <int D>
 hipError_t append(const PagedAppendArgs& a, hipStream_t stream) {
-  constexpr int HEADS = 512 / D;
-  const int64_t groups = (int64_t(a.rows) * (D / 16) + 255) / 256;
-  const int q_heads = a.q.at ? a.heads : 0, kv_heads = a.cache.kv_heads;
-  int chunk = q_heads > kv_heads ? q_heads : kv_heads;
-  while (chunk > 1 && groups * a.batch * ((q_heads + chunk - 1) / chunk + (kv_heads + chunk - 1) / chunk) < 1024) chunk = (chunk + 1) / 2;
-  const int q_chunks = (q_heads + chunk - 1) / chunk, k_chunks = (kv_heads + chunk - 1) / chunk;
-  hipLaunchKernelGGL((append_turned_kernel<D>), dim3(unsigned(groups), unsigned(q_chunks + k_chunks), unsigned(a.batch)), dim3(256), 0,
-                     stream, a, q_chunks, chunk);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  if (a.rows <= kValueRowsMax) {
-    const int64_t lanes = int64_t(kv_heads) * a.rows * (D / 8);
-    hipLaunchKernelGGL((append_value_rows_kernel<D>), dim3(unsigned((lanes + 255) / 256), unsigned(a.batch)), dim3(256), 0, stream, a);
-  } else {
-    hipLaunchKernelGGL((append_values_kernel<D>), dim3(blocks_of(a.rows), unsigned((kv_heads + HEADS - 1) / HEADS), unsigned(a.batch)),
-                       dim3(256), 0, stream, a);
+  using R = Range<D>;
+  const int q_heads = a.heads, kv_heads = a.cache.kv_heads;
+  if (one_by_one(a)) {
+    const int64_t lanes = int64_t(a.rows) * ((q_heads + kv_heads) * (D / 16) + kv_heads * (D / 8));
+    hipLaunchKernelGGL((append_few_kernel<D>), dim3(unsigned((lanes + 255) / 256), unsigned(a.batch)), dim3(256), 0, stream, a);
+    return hipGetLastError();
   }
+  // (From any position on, rows touch one range more than they fill, or two.)
+  const int64_t ranges = (int64_t(a.rows) + 30) / R::RANGE + 1;
+  const auto chunks = [](int heads, int chunk) { return (heads + chunk - 1) / chunk; };
+  const int v_chunk = R::HEADS, v_chunks = chunks(kv_heads, v_chunk);
+  int chunk = 4;
+  while (chunk > 1 && ranges * a.batch * (chunks(q_heads, chunk) + chunks(kv_heads, chunk) + v_chunks) < 1024) chunk /= 2;
+  const int q_chunks = chunks(q_heads, chunk), k_chunks = chunks(kv_heads, chunk);
+  const dim3 grid(unsigned(q_chunks + k_chunks + v_chunks), unsigned(ranges), unsigned(a.batch));
+  const auto kernel = chunk == 1 ? append_range_kernel<D, 1> : chunk == 2 ? append_range_kernel<D, 2> : append_range_kernel<D, 4>;
+  hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a, q_chunks, k_chunks, chunk, v_chunk);
   return hipGetLastError();
 }
 

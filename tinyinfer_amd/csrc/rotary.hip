@@ -14,56 +14,54 @@ __device__ __forceinline__ int64_t position_of(const RotateArgs& a, int b, int i
   return a.per_row ? int64_t(a.positions[int64_t(b) * a.rows + i]) : int64_t(a.positions[b]) + i;
 }
 
-// D and R multiples of 16: units of 16 values.
+// D and R multiples of 16: units of 16 values.  flat (HC 1): heads lie side by side, too.
+template <int HC>
 __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a, int units, int chunk) {
+  constexpr bool flat = HC == 1;
   const unsigned at = blockIdx.x * 256 + threadIdx.x, up = unsigned(units);  // (below 2^31: rows * dim is)
-  const int b = int(blockIdx.z), row = int(at / up), u = int(at % up);
-  if (row >= a.rows) return;
+  const unsigned rows = unsigned(a.rows), piece = at / up, above = flat ? piece / rows : 0;
+  const int b = int(blockIdx.z), row = int(piece - above * rows), u = int(at % up);
+  const int h0 = flat ? int(above) : int(blockIdx.y) * chunk, h1 = min(a.heads, h0 + chunk);
+  if (row >= a.rows || h0 >= a.heads) return;
   const RowUnit unit = row_unit(a.rotary, u);
-  const int h0 = int(blockIdx.y) * chunk, h1 = min(a.heads, h0 + chunk);
-  const uint16_t* x = a.x.at + b * a.x.batch + row * a.x.row;
-  uint16_t* y = a.y + (int64_t(b) * a.heads * a.rows + row) * a.dim;
-  const int64_t step = int64_t(a.rows) * a.dim;
-  if (!unit.turned) {
-#pragma unroll 4
-    for (int h = h0; h < h1; ++h) {
-      store_half8(y + h * step + unit.first, load_half8(x + h * a.x.head + unit.first));
-      store_half8(y + h * step + unit.second, load_half8(x + h * a.x.head + unit.second));
-    }
-    return;
-  }
-  const Turns t(a.rotary, u, position_of(a, b, row));
-#pragma unroll 4
-  for (int h = h0; h < h1; ++h) {
-    half8_t p = load_half8(x + h * a.x.head + unit.first), q = load_half8(x + h * a.x.head + unit.second);
-    turn_unit(t, a.rotary.interleaved, p, q);
-    store_half8(y + h * step + unit.first, p);
-    store_half8(y + h * step + unit.second, q);
-  }
+  uint16_t* y = a.y + (int64_t(b) * a.heads * a.rows + row) * a.dim + unit.first;
+  turn_heads<HC>(a.rotary, unit, u, position_of(a, b, row), a.x.at + b * a.x.batch + row * a.x.row, a.x.head, y,
+                 int64_t(a.rows) * a.dim, unit.second - unit.first, h0, h1);
 }
 
-// Any D and even R: a lane has one pair, or one value from R on.
+// Any D and even R: a lane has W pairs, or W values from R on (W divides both counts).
+template <int W>
 __global__ __launch_bounds__(256) void rotate_pairs_kernel(RotateArgs a, int chunk) {
-  const int pairs = a.rotary.rotated / 2, units = a.dim - pairs;
-  const unsigned at = blockIdx.x * 256 + threadIdx.x, up = unsigned(units);  // (below 2^31: rows * dim is)
-  const int b = int(blockIdx.z), row = int(at / up), u = int(at % up);
+  const int pairs = a.rotary.rotated / 2, units = (a.dim - pairs) / W;
+  const unsigned at = blockIdx.x * 256 + threadIdx.x;
+  const int b = int(blockIdx.z), row = int(at / unsigned(units)), u = W * int(at % unsigned(units));
   if (row >= a.rows) return;
   const int h0 = int(blockIdx.y) * chunk, h1 = min(a.heads, h0 + chunk);
   const uint16_t* x = a.x.at + b * a.x.batch + row * a.x.row;
   uint16_t* y = a.y + (int64_t(b) * a.heads * a.rows + row) * a.dim;
   const int64_t step = int64_t(a.rows) * a.dim;
   if (u >= pairs) {
-    for (int h = h0; h < h1; ++h) y[h * step + pairs + u] = x[h * a.x.head + pairs + u];
+    for (int h = h0; h < h1; ++h) __builtin_memcpy(y + h * step + pairs + u, x + h * a.x.head + pairs + u, 2 * W);
     return;
   }
-  const int first = a.rotary.interleaved ? 2 * u : u, second = a.rotary.interleaved ? 2 * u + 1 : pairs + u;
-  float c, s;
-  turn_of(a.rotary.turns[u], position_of(a, b, row), a.rotary.amplitude, c, s);
+  const bool interleaved = a.rotary.interleaved;
+  const int first = interleaved ? 2 * u : u, second = interleaved ? 2 * u + W : pairs + u;
+  float c[W], s[W];
+  const int64_t t = position_of(a, b, row);
+#pragma unroll
+  for (int i = 0; i < W; ++i) turn_of(a.rotary.turns[u + i], t, a.rotary.amplitude, c[i], s[i]);
+#pragma unroll 2
   for (int h = h0; h < h1; ++h) {
-    f16 p = __builtin_bit_cast(f16, x[h * a.x.head + first]), q = __builtin_bit_cast(f16, x[h * a.x.head + second]);
-    turn_pair(c, s, p, q);
-    y[h * step + first] = __builtin_bit_cast(uint16_t, p);
-    y[h * step + second] = __builtin_bit_cast(uint16_t, q);
+    f16 v[2 * W];
+    __builtin_memcpy(v, x + h * a.x.head + first, 2 * W);
+    __builtin_memcpy(v + W, x + h * a.x.head + second, 2 * W);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if (interleaved) turn_pair(c[i], s[i], v[2 * i], v[2 * i + 1]);
+      else turn_pair(c[i], s[i], v[i], v[W + i]);
+    }
+    __builtin_memcpy(y + h * step + first, v, 2 * W);
+    __builtin_memcpy(y + h * step + second, v + W, 2 * W);
   }
 }
 
@@ -71,14 +69,27 @@ __global__ __launch_bounds__(256) void rotate_pairs_kernel(RotateArgs a, int chu
 
 hipError_t rotate(const RotateArgs& a, hipStream_t stream) {
   const bool wide = a.dim % 16 == 0 && a.rotary.rotated % 16 == 0;
-  const int units = wide ? a.dim / 16 : a.dim - a.rotary.rotated / 2;
-  const int64_t groups = (int64_t(a.rows) * units + 255) / 256;
+  const int pairs = a.rotary.rotated / 2, plain = a.dim - a.rotary.rotated;
+  const int w = (pairs | plain) % 4 == 0 ? 4 : (pairs | plain) % 2 == 0 ? 2 : 1;  // (of the narrow kernel)
+  const int units = wide ? a.dim / 16 : (pairs + plain) / w;
+  const int64_t lanes = int64_t(a.rows) * units;
+  if (wide && lanes < 256) {  // (short rows: one head to a lane)
+    const dim3 grid(unsigned((lanes * a.heads + 255) / 256), 1, unsigned(a.batch));
+    hipLaunchKernelGGL(rotate_kernel<1>, grid, dim3(256), 0, stream, a, units, 1);
+    return hipGetLastError();
+  }
+  const int64_t groups = (lanes + 255) / 256;
   int64_t chunks = 1;
   while (chunks < a.heads && groups * a.batch * chunks < 1024) chunks *= 2;
   const int chunk = int((a.heads + chunks - 1) / chunks);
   const dim3 grid(unsigned(groups), unsigned((a.heads + chunk - 1) / chunk), unsigned(a.batch));
-  if (wide) hipLaunchKernelGGL(rotate_kernel, grid, dim3(256), 0, stream, a, units, chunk);
-  else hipLaunchKernelGGL(rotate_pairs_kernel, grid, dim3(256), 0, stream, a, chunk);
+  if (!wide) {
+    const auto kernel = w == 4 ? rotate_pairs_kernel<4> : w == 2 ? rotate_pairs_kernel<2> : rotate_pairs_kernel<1>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a, chunk);
+    return hipGetLastError();
+  }
+  if (chunk < 4) hipLaunchKernelGGL(rotate_kernel<2>, grid, dim3(256), 0, stream, a, units, chunk);
+  else hipLaunchKernelGGL(rotate_kernel<4>, grid, dim3(256), 0, stream, a, units, chunk);
   return hipGetLastError();
 }
 

@@ -56,11 +56,12 @@ __device__ __forceinline__ half8_t load_half8(const uint16_t* p) {  // (any even
 }
 __device__ __forceinline__ void store_half8(uint16_t* p, half8_t x) { __builtin_memcpy(p, &x, 16); }
 
-// One rounding to fp16 of fp32 products: a and b of a pair's two values.
+// A pair's two values, rounded to fp16 once.  (Which product is fused with the sum is written
+// down, so every kernel gives the same bits.)
 __device__ __forceinline__ void turn_pair(float c, float s, f16& a, f16& b) {
   const float x = float(a), y = float(b);
-  a = f16r(x * c - y * s);
-  b = f16r(x * s + y * c);
+  a = f16r(fmaf(x, c, -(y * s)));
+  b = f16r(fmaf(x, s, y * c));
 }
 __device__ __forceinline__ void turn_unit(const Turns& t, bool interleaved, half8_t& first, half8_t& second) {
 #pragma unroll
@@ -77,6 +78,47 @@ __device__ __forceinline__ void turn_unit(const Turns& t, bool interleaved, half
       first[e] = a;
       second[e] = b;
     }
+  }
+}
+
+// A lane's unit of heads [h0, h1) of a row from x to y (each given at head 0, y at the
+// first piece, its second one y_second behind), HC heads at a time: their loads are on the
+// way while the angles, or the heads in front of them, are worked on.
+template <int HC>
+__device__ __forceinline__ void turn_heads(const RotaryArgs& r, RowUnit unit, int u, int64_t t, const uint16_t* x, int64_t x_step,
+                                           uint16_t* y, int64_t y_step, int y_second, int h0, int h1) {
+  half8_t p[HC], q[HC];
+  const auto load = [&](int h) {
+#pragma unroll
+    for (int i = 0; i < HC; ++i) {
+      const uint16_t* at = x + int64_t(min(h + i, h1 - 1)) * x_step;
+      p[i] = load_half8(at + unit.first);
+      q[i] = load_half8(at + unit.second);
+    }
+  };
+  const auto store = [&](int h) {
+#pragma unroll
+    for (int i = 0; i < HC; ++i) {
+      if (h + i >= h1) break;
+      store_half8(y + int64_t(h + i) * y_step, p[i]);
+      store_half8(y + int64_t(h + i) * y_step + y_second, q[i]);
+    }
+  };
+  load(h0);
+  if (!unit.turned) {
+    for (int h = h0;;) {
+      store(h);
+      if ((h += HC) >= h1) return;
+      load(h);
+    }
+  }
+  const Turns turns(r, u, t);
+  for (int h = h0;;) {
+#pragma unroll
+    for (int i = 0; i < HC; ++i) turn_unit(turns, r.interleaved, p[i], q[i]);
+    store(h);
+    if ((h += HC) >= h1) return;
+    load(h);
   }
 }
 
