@@ -163,7 +163,7 @@ bool strides_fit(int64_t batch, int64_t head, int64_t row) { return batch >= 0 &
 int check_paged(const ti_amd_kv_paged* c, const int32_t* table, int width, tia::KvPaged& out, tia::PageTable& pages) {
   if (!c || (c->head_dim != 64 && c->head_dim != 128) || c->page_count <= 0 || c->kv_heads <= 0 || c->kv_heads > 65535 ||
       c->page_size < 32 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)) != 0 ||
-      !shape_fits({c->page_count, c->kv_heads, c->page_size, c->head_dim}, 4) || !aligned(c->pages, 16))
+      int64_t(c->page_count) * c->kv_heads > (int64_t(1) << 34) / c->page_size || !aligned(c->pages, 16))
     return fail(TI_V2_INVALID_ARGUMENT,
                 "paged cache: 16-byte aligned pages, page_size a power of two from 32 to 1024, head_dim 64 or 128 and positive extents");
   if (!aligned(table, 4) || width <= 0) return fail(TI_V2_INVALID_ARGUMENT, "page table: int32 [batch][width], width positive");

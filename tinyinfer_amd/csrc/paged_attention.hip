@@ -21,10 +21,23 @@
 //
 // What memory holds in masked places is anybody's, an infinity or NaN too, and 0 times that
 // is NaN: a tile in which something is masked is searched for such values, and if it has one
-// they count as 0 in the product and a second product of ones, over the keys that a row
-// sees, says which sums must be NaN all the same.
+// they count as some number, times a weight of 0, and a product of ones, over the keys that a
+// row sees, says which sums must be NaN all the same.
+//
+// What bounds it.  Single tokens: memory where caches are long (16 requests of 8 x 128, 12000
+// to 32768 keys: 248 us, 6.3 TB/s), launch and one tile's chain of latencies where they are
+// short (one request of 12 heads, 300 keys: 6.2 us; 32 of them, 128 to 1024 keys: 15 us, 5.6 of
+// them without keys).  Prompts: a tile of 64 keys x 32 rows at D 128 is 68 matrix instructions, 1088
+// cycles of a SIMD, about 105 vector instructions and 32 exponentials, 930 cycles, and a
+// quarter of the CU's LDS for 256 cycles at least; two workgroups a CU overlap these in part.  2
+// requests of 777 queries, 32 heads over 8 of 128, 4500 to 6001 keys: 170 us, 791 TFLOP/s (400
+// workgroups, so 78 % of the CUs' time); 4096 queries of 32 heads over as many keys 149 us, 920
+// TFLOP/s; 4 prompts of 1024, 25 heads of 64: 28 us, 473 TFLOP/s.  Tried for the shared tiles and no
+// faster: the next tile's scores under this one's weights (192 us for 179 then), eight waves of which
+// four multiply while four work out weights (169, but 46 for 30 at D 64: products and weights of
+// two waves of a SIMD take as long together as one after the other), operands read from LDS 4 to 16 ahead
+// by hand (181).
 #include <algorithm>
-#include <type_traits>
 
 #include "divisor.hpp"
 #include "lds_limit.hpp"
@@ -90,96 +103,313 @@ __device__ __forceinline__ half4_t output_of(float4_t o, float total, float inv)
   return half4_t{f16r(x[0]), f16r(x[1]), f16r(x[2]), f16r(x[3])};
 }
 
-// Waves' states as they meet in LDS: of lane (j, g)'s dims, number v of 4 and b of D / 16
-// lie next to each other in b.
-template <int D, int QB, int KW>
-struct Merge {
-  float4_t acc[KW][QB][4][D / 64][64];
-  float m[KW][QB][16], l[KW][QB][16];
-};
+// A wave's rows, QB blocks of 16, lane (j, g) holding its part of row j of each: what they
+// ask, see and have summed up.
+template <int D, int QB>
+struct Rows {
+  static constexpr int PER = D / 16, ROWS = 16 * QB;
+  // One block of rows (single tokens): a second product with what the weights' rounding to
+  // fp16 leaves out costs nothing that shows, so the result is as near as fp32 weights would
+  // bring it.  Two blocks (prompts) take the rounded weights alone, a third less matrix work,
+  // and sum up these too: by one more product, with ones, in place of 32 additions.
+  static constexpr bool FINE = QB == 1;
 
-// A tile's operands as the waves of a workgroup share them, in the order in which a
-// lane reads them: 16 bytes per lane, one conflict-free kilobyte per operand.
-template <int D>
-struct Tiles {
-  half8_t k[2][4][D / 32][64], v[2][2][D / 16][64];
-};
-
-// KW waves share a row block, each with its own tiles; kShared: 4 waves have a row block
-// each (`rb` counts those groups) and share every tile, each bringing a quarter of it into
-// LDS while the tile before is worked on.
-constexpr int kShared = 0;
-template <int D, int QB, int KW>
-__device__ __forceinline__ void attend(const AttnPlan& p, uint8_t* lds, int b, int head, int rb, int split) {
-  const PagedAttnArgs& a = p.a;
-  const int lane = int(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-  const int j = lane & 15, g = lane >> 4;
-  constexpr bool SHARED = KW == kShared;
-  constexpr int ROWS = 16 * QB, GROUP = SHARED ? 4 * ROWS : ROWS, STEP = SHARED ? 1 : KW, PER = D / 16;
-  const int group0 = rb * GROUP, r0 = SHARED ? group0 + wave * ROWS : group0, row_count = int(p.rows.d);
-
-  const int64_t held = int64_t(a.pages.width) * a.cache.page_size;
-  const int kv = int(min(int64_t(max(a.kv_lengths[b], 0)), held));
-
-  // This lane's rows: block u, column j.
-  const int ql = a.q_lengths ? min(max(a.q_lengths[b], 0), a.q_len) : a.q_len;
-  const int64_t off = a.offsets ? int64_t(a.offsets[b]) : int64_t(kv) - ql;
-  const auto seen = [&](int qi) { return int(max(a.causal ? min(int64_t(kv), off + qi + 1) : int64_t(kv), int64_t(0))); };
+  const AttnPlan& p;
+  int lane, j, g, b, head, kv, ql;
+  int64_t off;
   int row_id[QB];  // in q's order, -1 past the last row
   int end[QB];     // keys [0, end) are visible
-#pragma unroll
-  for (int u = 0; u < QB; ++u) {
-    const int r = r0 + 16 * u + j, rc = min(r, row_count - 1);
-    const int qi = div_by(rc, p.group), hg = rc - qi * int(p.group.d);
-    row_id[u] = r < row_count ? (b * a.heads + head * int(p.group.d) + hg) * a.q_len + qi : -1;
-    end[u] = r < row_count && qi < ql ? seen(qi) : 0;
-  }
-  // Keys that some row of the wave sees, and keys that every row of it with a query sees
-  // (a row without one may compute anything: it is cleared at the end); keys that some
-  // row of the workgroup sees.
-  const auto last_of = [&](int from, int rows) {
-    const int q_last = min(div_by(min(from + rows, row_count) - 1, p.group), ql - 1);
-    return from >= row_count || q_last < div_by(from, p.group) ? 0 : seen(q_last);
-  };
-  const int last = last_of(r0, ROWS), first = last == 0 ? 0 : seen(div_by(r0, p.group));
-  const int group_last = SHARED ? last_of(group0, GROUP) : last, group_first = seen(div_by(group0, p.group));
-  const int tiles = (group_last + kTile - 1) / kTile, per = (tiles + p.splits - 1) / p.splits;
-  const int t_end = min(tiles, (split + 1) * per);
-  int t = split * per + (SHARED ? 0 : wave);
+  int last, first; // keys that some row of the wave sees, and that every row with a query sees
+  half8_t qf[QB][D / 32];
+  float m[QB];
+  float4_t l[QB];  // FINE: [0] is this lane's part of the sum; else all are the row's sum
+  float4_t acc[QB][PER];
+  unsigned spoilt[QB];  // bit 4 d + e: the sum acc[u][d][e] is over an infinity or NaN that is not in it
+  half8_t pp[QB][2], rest[2];
 
-  // Pages of the halves of this wave's tiles from `t0` on, tile t0 + STEP i in lane i.
-  const int32_t* table = a.pages.table + int64_t(b) * a.pages.width;
-  int ids[2], ids_from = t;
-  const auto look_up = [&](int t0) {
-    ids_from = t0;
+  // Keys that query qi sees, and keys that some of `rows` rows from `from` on see.
+  __device__ __forceinline__ int seen(int qi) const {
+    return int(max(p.a.causal ? min(int64_t(kv), off + qi + 1) : int64_t(kv), int64_t(0)));
+  }
+  __device__ __forceinline__ int last_of(int from, int rows) const {
+    const int count = int(p.rows.d), q_last = min(div_by(min(from + rows, count) - 1, p.group), ql - 1);
+    return from >= count || q_last < div_by(from, p.group) ? 0 : seen(q_last);
+  }
+  __device__ __forceinline__ int first_of(int from) const { return seen(div_by(min(from, int(p.rows.d) - 1), p.group)); }
+
+  __device__ __forceinline__ Rows(const AttnPlan& plan, int request, int kv_head, int r0)
+      : p(plan), lane(int(threadIdx.x & 63)), j(lane & 15), g(lane >> 4), b(request), head(kv_head) {
+    const PagedAttnArgs& a = p.a;
+    kv = int(min(int64_t(max(a.kv_lengths[b], 0)), int64_t(a.pages.width) * a.cache.page_size));
+    ql = a.q_lengths ? min(max(a.q_lengths[b], 0), a.q_len) : a.q_len;
+    off = a.offsets ? int64_t(a.offsets[b]) : int64_t(kv) - ql;
+    const int count = int(p.rows.d), group = int(p.group.d);
+#pragma unroll
+    for (int u = 0; u < QB; ++u) {
+      const int r = r0 + 16 * u + j, rc = min(r, count - 1), qi = div_by(rc, p.group);
+      row_id[u] = r < count ? (b * a.heads + head * group + rc - qi * group) * a.q_len + qi : -1;
+      end[u] = r < count && qi < ql ? seen(qi) : 0;
+    }
+    last = last_of(r0, ROWS);
+    // (A row without a query may compute anything: it is cleared at the end.)
+    first = last == 0 ? 0 : first_of(r0);
+  }
+  __device__ __forceinline__ void load() {
+#pragma unroll
+    for (int u = 0; u < QB; ++u) {
+      u16x8_t top = {};
+      const uint16_t* qp = p.a.q + int64_t(max(row_id[u], 0)) * D + 8 * g;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        half8_t x;
+        __builtin_memcpy(&x, qp + 32 * c, 16);
+        top = top_bits(top, x);
+        qf[u][c] = end[u] > 0 ? x : half8_t{};
+      }
+      // A row's sum starts at NaN if its query has an infinity or NaN: its scores are infinite, of
+      // either sign, or NaN (and all of -inf would pass for a row without a key).
+      const float start = __ballot(any_not_finite(top)) >> j & 0x0001000100010001u ? __builtin_nanf("") : 0.f;
+      l[u] = float4_t{start, start, start, start};
+      m[u] = kNegInf;
+      spoilt[u] = 0;
+#pragma unroll
+      for (int d = 0; d < PER; ++d) acc[u][d] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+
+  // Key 16 kb + v of this lane, of tile t, is visible to row (u, j) iff it is below its half's limit.
+  __device__ __forceinline__ bool sees(int u, int t, bool held0, bool held1, int kb, int v) const {
+    return 16 * kb + v < ((kb < 2 ? held0 : held1) ? end[u] - t * kTile - 4 * g : 0);
+  }
+  __device__ __forceinline__ bool full(int t, bool held0, bool held1) const { return (t + 1) * kTile <= first && held0 && held1; }
+
+  // Scores, key(kb, c) being the operand of 16 keys x 32 dims.
+  template <typename K>
+  __device__ __forceinline__ void score(float4_t (&sc)[QB][4], K key) const {
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+#pragma unroll
+      for (int u = 0; u < QB; ++u) sc[u][kb] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        const half8_t kf = key(kb, c);
+#pragma unroll
+        for (int u = 0; u < QB; ++u) sc[u][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[u][c], sc[u][kb], 0, 0, 0);
+      }
+    }
+  }
+  // Masks the scores of block u and raises its reference where it must be.
+  __device__ __forceinline__ void refer(int u, float4_t (&sc)[QB][4], int t, bool held0, bool held1) {
+    if (!full(t, held0, held1)) {
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) sc[u][kb][v] = sees(u, t, held0, held1, kb, v) ? sc[u][kb][v] : kNegInf;
+    }
+    float high = kNegInf;
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) high = fmaxf(high, sc[u][kb][v]);
+    high *= p.scale;
+    if (__ballot(high > m[u] + kRaise)) {
+      high = fmaxf(high, __shfl_xor(high, 16, 64));
+      high = fmaxf(high, __shfl_xor(high, 32, 64));
+      const float nm = high > m[u] + kRaise ? high - kBelow : m[u];
+      const float f = m[u] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[u] - nm);
+      l[u] *= f;
+#pragma unroll
+      for (int d = 0; d < PER; ++d) acc[u][d] *= f;
+      m[u] = nm;
+    }
+  }
+  // Its weights.
+  __device__ __forceinline__ void weigh(int u, const float4_t (&sc)[QB][4]) {
+    const float ref = m[u] == kNegInf ? 0.f : -m[u];  // -inf while every key so far is masked
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float w = __builtin_amdgcn_exp2f(fmaf(sc[u][kb][v], p.scale, ref));
+        pp[u][kb >> 1][4 * (kb & 1) + v] = f16(w);
+        if constexpr (FINE) {
+          l[u][0] += w;
+          rest[kb >> 1][4 * (kb & 1) + v] = f16(w - float(f16(w)));
+        }
+      }
+  }
+  // Adds the tile's values, value(d, h) being the operand of 16 dims x 32 keys.
+  template <typename V>
+  __device__ __forceinline__ void product(V value) {
+    if constexpr (!FINE) {
+      const f16 one = f16(1.f);
+      const half8_t ones = {one, one, one, one, one, one, one, one};
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int u = 0; u < QB; ++u) l[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pp[u][h], l[u], 0, 0, 0);
+    }
+#pragma unroll
+    for (int d = 0; d < PER; ++d)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const half8_t vf = value(d, h);
+#pragma unroll
+        for (int u = 0; u < QB; ++u) acc[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pp[u][h], acc[u][d], 0, 0, 0);
+        if constexpr (FINE) acc[0][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, rest[h], acc[0][d], 0, 0, 0);
+      }
+  }
+  // Of a tile of which a row may not see everything: whether it has an infinity or NaN, and the
+  // sums that must be NaN for one that their row sees.
+  template <typename V>
+  __device__ __forceinline__ bool any_odd(V value) const {
+    u16x8_t top = {};
+#pragma unroll
+    for (int d = 0; d < PER; ++d) top = top_bits(top_bits(top, value(d, 0)), value(d, 1));
+    return __ballot(any_not_finite(top)) != 0;
+  }
+  template <typename V>
+  __device__ __forceinline__ void spoil(int t, bool held0, bool held1, V value) {
+    half8_t seen_ones[QB][2];
+#pragma unroll
+    for (int u = 0; u < QB; ++u)
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) seen_ones[u][kb >> 1][4 * (kb & 1) + v] = sees(u, t, held0, held1, kb, v) ? f16(1.f) : f16(0.f);
+    // (Rolled, and the values read once more: this is rare, and registers are not.)
+#pragma unroll 1
+    for (int d = 0; d < PER; ++d) {
+      float4_t hits[QB];
+#pragma unroll
+      for (int u = 0; u < QB; ++u) hits[u] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const half8_t x = value(d, h);
+        half8_t bad;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) bad[e] = (__builtin_bit_cast(u16x8_t, x)[e] & 0x7fff) >= 0x7c00 ? f16(1.f) : f16(0.f);
+#pragma unroll
+        for (int u = 0; u < QB; ++u) hits[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bad, seen_ones[u][h], hits[u], 0, 0, 0);
+      }
+#pragma unroll
+      for (int u = 0; u < QB; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) spoilt[u] |= hits[u][e] > 0.f ? 1u << (4 * d + e) : 0u;
+    }
+  }
+  // The rows' sums of weights in l[u][0], 0 for rows without a key, and of spoilt ones NaN.
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int u = 0; u < QB; ++u) {
+      if constexpr (FINE) {
+        l[u][0] += __shfl_xor(l[u][0], 16, 64);
+        l[u][0] += __shfl_xor(l[u][0], 32, 64);
+      }
+      if (end[u] == 0) l[u][0] = 0.f;
+      if (__ballot(spoilt[u] != 0)) {
+#pragma unroll
+        for (int d = 0; d < PER; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[u][d][e] = spoilt[u] >> (4 * d + e) & 1 ? __builtin_nanf("") : acc[u][d][e];
+      }
+    }
+  }
+  // Of this lane's dims: D / 16 (4 g + v) + 4 c .. + 3.
+  __device__ __forceinline__ float4_t piece(int u, int v, int c) const {
+    return float4_t{acc[u][4 * c][v], acc[u][4 * c + 1][v], acc[u][4 * c + 2][v], acc[u][4 * c + 3][v]};
+  }
+  // These of row (u, j), of `total` weight, to the output, or to the state of a split.
+  __device__ __forceinline__ void put(int u, int v, int c, int split, float4_t o, float total) const {
+    if (row_id[u] < 0) return;
+    const int dim = PER * (4 * g + v) + 4 * c;
+    if (p.splits > 1) {
+      const int64_t at = int64_t(split) * p.all_rows + row_id[u];
+      if (total != 0.f) *reinterpret_cast<float4_t*>(p.a.workspace + at * D + dim) = o;
+      return;
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const half4_t y = output_of(o, total, inv);
+    __builtin_memcpy(p.a.out + int64_t(row_id[u]) * D + dim, &y, 8);
+  }
+  // And their exponents' reference.
+  __device__ __forceinline__ void put_weight(int u, int split, float top, float total) const {
+    if (p.splits == 1 || g != 0 || row_id[u] < 0) return;
+    float* ml = p.a.workspace + p.splits * p.all_rows * D + 2 * (int64_t(split) * p.all_rows + row_id[u]);
+    ml[0] = top;
+    ml[1] = total;
+  }
+};
+
+__device__ __forceinline__ half8_t finite(half8_t x) {  // an infinity or NaN: some number
+  const f16 most = f16(65504.f);
+  const half8_t high = {most, most, most, most, most, most, most, most};
+  return __builtin_elementwise_max(__builtin_elementwise_min(x, high), -high);
+}
+
+// Where a (request, key head)'s tiles lie.  The pages of the halves of the wave's next 64
+// tiles, STEP apart, are read at once, one tile to a lane.
+template <int D, int STEP>
+struct Pages {
+  const AttnPlan& p;
+  const int32_t* table;
+  int head, ids[2], from;
+
+  __device__ __forceinline__ Pages(const AttnPlan& plan, int b, int kv_head)
+      : p(plan), table(plan.a.pages.table + int64_t(b) * plan.a.pages.width), head(kv_head) {}
+  __device__ __forceinline__ void look_up(int t0) {
+    from = t0;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int entry = (2 * (t0 + STEP * lane) + h) >> p.page_shift;
-      const int id = entry < a.pages.width ? table[entry] : -1;
-      ids[h] = id < a.cache.page_count ? id : -1;
+      const int entry = (2 * (t0 + STEP * int(threadIdx.x & 63)) + h) >> p.page_shift;
+      const int id = entry < p.a.pages.width ? table[entry] : -1;
+      ids[h] = id < p.a.cache.page_count ? id : -1;
     }
-  };
-  const auto page_of = [&](int tt, int h) { return __builtin_amdgcn_readlane(ids[h], (tt - ids_from) / STEP & 63); };
-  // Tokens 64 tt + 32 h .. + 31 of the head: K (V is `to_v` behind).
-  const int64_t head_size = paged_head_size(a.cache), to_v = int64_t(a.cache.page_size) * D;
-  const auto half_on = [&](int page, int half) {
-    return a.cache.pages + (int64_t(page) * a.cache.kv_heads + head) * head_size + (half & ((1 << p.page_shift) - 1)) * (32 * D);
-  };
-  const auto half_at = [&](int tt, int h) { return half_on(max(page_of(tt, h), 0), 2 * tt + h); };
+  }
+  // (Behind these calls tiles in front of t are no longer at hand.)
+  __device__ __forceinline__ void reach(int t) {
+    if (t - from >= 64 * STEP) look_up(t);
+  }
+  __device__ __forceinline__ int page(int t, int h) const {
+    return __builtin_amdgcn_readlane(h ? ids[1] : ids[0], (t - from) / STEP & 63);
+  }
+  __device__ __forceinline__ bool held(int t, int h) const { return page(t, h) >= 0; }
+  // Tokens 64 t + 32 h .. + 31 of the head on a page (none: the first): the number of their
+  // keys' block of 32 x D, and that of their values.
+  __device__ __forceinline__ int block(int page, int t, int h) const {
+    const int blocks = 1 << p.page_shift;
+    return (max(page, 0) * p.a.cache.kv_heads + head) * 2 * blocks + ((2 * t + h) & (blocks - 1));
+  }
+  __device__ __forceinline__ int values(int block) const { return block + (1 << p.page_shift); }
+  __device__ __forceinline__ const uint16_t* at(int block) const { return p.a.cache.pages + int64_t(block) * (32 * D); }
+};
 
-  // One block of rows (single tokens): memory has no use for the keys again, and a second
-  // product with what the weights' rounding to fp16 leaves out costs nothing that shows,
-  // so the result is as near as fp32 weights would bring it.  Two blocks (prompts) take
-  // the rounded weights alone: a third less matrix work.
-  constexpr bool NT = QB == 1, FINE = QB == 1;
-  // Two blocks of 128 dims leave no registers to load ahead into.
-  constexpr bool AHEAD = QB == 1 || D == 64;
-  half8_t kr[SHARED ? 1 : 4][D / 32], vr[SHARED ? 1 : PER][2];
-  auto& shared = *reinterpret_cast<Tiles<D>*>(lds);
+// Four waves share a row block, each with its own tiles.  Their states meet in LDS: of lane
+// (j, g)'s dims, number v of 4 and b of D / 16 lie next to each other in b.
+constexpr int kWaves = 4;
+template <int D, int QB>
+struct Merge {
+  float4_t acc[kWaves][QB][4][D / 64][64];
+  float m[kWaves][QB][16], l[kWaves][QB][16];
+};
+template <int D, int QB>
+__device__ __forceinline__ void attend(const AttnPlan& p, uint8_t* lds, int b, int head, int rb, int split) {
+  constexpr int PER = D / 16;
+  const int lane = int(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
+  Pages<D, kWaves> pages(p, b, head);
+  if (p.splits == 1) pages.look_up(wave);  // (the lengths are still on their way)
+  Rows<D, QB> rows(p, b, head, rb * 16 * QB);
+  const int tiles = (rows.last + kTile - 1) / kTile, per = (tiles + p.splits - 1) / p.splits, t_end = min(tiles, (split + 1) * per);
+  int t = split * per + wave;
+
+  // One block: memory has no use for the keys again.  The next tile's keys are loaded once the
+  // scores have used this one's; two blocks of 128 dims leave no registers for that.
+  constexpr bool NT = QB == 1, AHEAD = QB == 1 || D == 64;
+  half8_t kr[4][D / 32], vr[PER][2];
   const auto load_k = [&](int tt) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint16_t* at = half_at(tt, h);
+      const uint16_t* at = pages.at(pages.block(pages.page(tt, h), tt, h));
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -189,317 +419,189 @@ __device__ __forceinline__ void attend(const AttnPlan& p, uint8_t* lds, int b, i
   const auto load_v = [&](int tt) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint16_t* at = half_at(tt, h) + to_v;
+      const uint16_t* at = pages.at(pages.values(pages.block(pages.page(tt, h), tt, h)));
 #pragma unroll
       for (int d = 0; d < PER; ++d) vr[d][h] = load16<NT>(at + 512 * d + uint32_t(8 * lane));
     }
   };
-  // This wave's quarter of a tile into LDS: 16 keys, and half the dims of a half's values.
-  const auto share = [&](int tt, int buf) {
-    const uint16_t* at = half_at(tt, wave >> 1) + 8 * lane;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c)
-      __builtin_amdgcn_global_load_lds((global_ptr)(at + (wave & 1) * 16 * D + 512 * c), (lds_ptr)&shared.k[buf][wave][c][0], 16, 0, 0);
-#pragma unroll
-    for (int d = 0; d < PER / 2; ++d)
-      __builtin_amdgcn_global_load_lds((global_ptr)(at + to_v + ((wave & 1) * (PER / 2) + d) * 512),
-                                       (lds_ptr)&shared.v[buf][wave >> 1][(wave & 1) * (PER / 2) + d][0], 16, 0, 0);
-  };
   if (t < t_end) {
-    look_up(t);
-    if constexpr (SHARED) share(t, 0);
-    else if (AHEAD) load_k(t);
+    if (p.splits > 1) pages.look_up(t);
+    if (AHEAD) load_k(t);
   }
-
-  half8_t qf[QB][D / 32];
-  // A row's sum starts at NaN if its query has an infinity or NaN: its scores are infinite, of
-  // either sign, or NaN (and all of -inf would pass for a row without a key).
-  float l[QB], m[QB];
-  unsigned spoilt[QB];  // bit 4 d + e: the sum acc[u][d][e] is over an infinity or NaN that is not in it
-  float4_t acc[QB][PER];
-#pragma unroll
-  for (int u = 0; u < QB; ++u) {
-    u16x8_t top = {};
-    const uint16_t* qp = a.q + int64_t(max(row_id[u], 0)) * D + 8 * g;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-      half8_t x;
-      __builtin_memcpy(&x, qp + 32 * c, 16);
-      top = top_bits(top, x);
-      qf[u][c] = end[u] > 0 ? x : half8_t{};
-    }
-    l[u] = __ballot(any_not_finite(top)) >> j & 0x0001000100010001u ? __builtin_nanf("") : 0.f;
-    m[u] = kNegInf;
-    spoilt[u] = 0;
-#pragma unroll
-    for (int d = 0; d < PER; ++d) acc[u][d] = float4_t{0.f, 0.f, 0.f, 0.f};
-  }
-
-  const auto value = [&](int buf, int d, int h) { return SHARED ? shared.v[buf][h][d][lane] : vr[SHARED ? 0 : d][h]; };
-  // Key 16 kb + v of this lane, of the tile from key0 on, is visible to row (u, j) iff it is
-  // below its half's limit.
-  const auto sees = [&](int u, int key0, bool held0, bool held1, int kb, int v) {
-    return 16 * kb + v < ((kb < 2 ? held0 : held1) ? end[u] - key0 - 4 * g : 0);
-  };
-  // A tile of which a row may not see everything: whether it has an infinity or NaN, the sums
-  // that must be NaN for one that their row sees, and a value with a finite number in its place.
-  const auto any_odd = [&](int buf) {
-    u16x8_t top = {};
-#pragma unroll
-    for (int d = 0; d < PER; ++d) top = top_bits(top_bits(top, value(buf, d, 0)), value(buf, d, 1));
-    return __ballot(any_not_finite(top)) != 0;
-  };
-  const auto spoil = [&](int t, int buf, bool held0, bool held1) {
-    half8_t ones[QB][2];
-#pragma unroll
-    for (int u = 0; u < QB; ++u)
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) ones[u][kb >> 1][4 * (kb & 1) + v] = sees(u, t * kTile, held0, held1, kb, v) ? f16(1.f) : f16(0.f);
-    // (Rolled, and the values read once more: this is rare, and registers are not.)
-#pragma unroll 1
-    for (int d = 0; d < PER; ++d) {
-      float4_t hits[QB];
-#pragma unroll
-      for (int u = 0; u < QB; ++u) hits[u] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        half8_t x, bad;
-        if constexpr (SHARED) x = shared.v[buf][h][d][lane];
-        else x = load16<false>(half_on((h ? held1 : held0) ? table[(2 * t + h) >> p.page_shift] : 0, 2 * t + h) + to_v + 512 * d + uint32_t(8 * lane));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) bad[e] = (__builtin_bit_cast(u16x8_t, x)[e] & 0x7fff) >= 0x7c00 ? f16(1.f) : f16(0.f);
-#pragma unroll
-        for (int u = 0; u < QB; ++u) hits[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bad, ones[u][h], hits[u], 0, 0, 0);
-      }
-#pragma unroll
-      for (int u = 0; u < QB; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) spoilt[u] |= hits[u][e] > 0.f ? 1u << (4 * d + e) : 0u;
-    }
-  };
-  const auto finite = [](half8_t x) {
-    const f16 most = f16(65504.f);
-    const half8_t high = {most, most, most, most, most, most, most, most};
-    return __builtin_elementwise_max(__builtin_elementwise_min(x, high), -high);
-  };
-
-  const auto tile = [&](int t, int buf, bool held0, bool held1, auto after_scores) {
-    const int key0 = t * kTile;
-    const bool full = key0 + kTile <= first && held0 && held1;
+  rows.load();
+  for (; t < t_end; t += kWaves) {
+    const bool held0 = pages.held(t, 0), held1 = pages.held(t, 1);
+    if (!AHEAD) load_k(t);
+    else load_v(t);
+    __builtin_amdgcn_sched_barrier(0);
     float4_t sc[QB][4];
-#pragma unroll
-    for (int kb = 0; kb < 4; ++kb) {
-#pragma unroll
-      for (int u = 0; u < QB; ++u) sc[u][kb] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        const half8_t kf = SHARED ? shared.k[buf][kb][c][lane] : kr[SHARED ? 0 : kb][c];
-#pragma unroll
-        for (int u = 0; u < QB; ++u) sc[u][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[u][c], sc[u][kb], 0, 0, 0);
-      }
+    rows.score(sc, [&](int kb, int c) { return kr[kb][c]; });
+    __builtin_amdgcn_sched_barrier(0);
+    if (!AHEAD) load_v(t);
+    if (t + kWaves < t_end) {
+      pages.reach(t + kWaves);
+      if (AHEAD) load_k(t + kWaves);
     }
-    after_scores();
-    half8_t pp[QB][2], rest[2];
-    const auto visible = [&](int u, int kb, int v) { return sees(u, key0, held0, held1, kb, v); };
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < QB; ++u) {
-      if (!full) {
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) sc[u][kb][v] = visible(u, kb, v) ? sc[u][kb][v] : kNegInf;
-      }
-      float high = kNegInf;
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) high = fmaxf(high, sc[u][kb][v]);
-      high *= p.scale;
-      if (__ballot(high > m[u] + kRaise)) {
-        high = fmaxf(high, __shfl_xor(high, 16, 64));
-        high = fmaxf(high, __shfl_xor(high, 32, 64));
-        const float nm = high > m[u] + kRaise ? high - kBelow : m[u];
-        const float f = m[u] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[u] - nm);
-        l[u] *= f;
-#pragma unroll
-        for (int d = 0; d < PER; ++d) acc[u][d] *= f;
-        m[u] = nm;
-      }
-      const float ref = m[u] == kNegInf ? 0.f : -m[u];  // -inf while every key so far is masked
-#pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const float w = __builtin_amdgcn_exp2f(fmaf(sc[u][kb][v], p.scale, ref));
-          l[u] += w;
-          pp[u][kb >> 1][4 * (kb & 1) + v] = f16(w);
-          if constexpr (FINE) rest[kb >> 1][4 * (kb & 1) + v] = f16(w - float(f16(w)));
-        }
+      rows.refer(u, sc, t, held0, held1);
+      rows.weigh(u, sc);
     }
-    if constexpr (!SHARED) {
-      if (!full && any_odd(0)) {
-        spoil(t, 0, held0, held1);
-#pragma unroll
-        for (int d = 0; d < PER; ++d)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) vr[d][h] = finite(vr[d][h]);
-      }
-    }
-#pragma unroll
-    for (int d = 0; d < PER; ++d)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const half8_t vf = value(buf, d, h);
-#pragma unroll
-        for (int u = 0; u < QB; ++u) acc[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pp[u][h], acc[u][d], 0, 0, 0);
-        if constexpr (FINE) acc[0][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, rest[h], acc[0][d], 0, 0, 0);
-      }
-  };
-  // (The pages of tile t are at hand; those of t + STEP afterwards.)
-  const auto next_pages = [&](int tt) {
-    if (tt - ids_from >= 64 * STEP) look_up(tt);
-  };
-  if constexpr (SHARED) {
-    for (int buf = 0; t < t_end; ++t, buf ^= 1) {
-      const bool held0 = page_of(t, 0) >= 0, held1 = page_of(t, 1) >= 0;
-      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's quarter has landed
-      lds_barrier();                        // everyone's has, and nobody reads the other buffer any more
-      if (t + 1 < t_end) {
-        next_pages(t + 1);
-        share(t + 1, buf ^ 1);
-      }
-      // (The same for all waves: what they find lies in LDS.)
-      if (((t + 1) * kTile > group_first || !held0 || !held1) && any_odd(buf)) {
-        spoil(t, buf, held0, held1);
-        lds_barrier();
-#pragma unroll
-        for (int d = 0; d < PER / 2; ++d) {
-          half8_t& x = shared.v[buf][wave >> 1][(wave & 1) * (PER / 2) + d][lane];
-          x = finite(x);
-        }
-        lds_barrier();
-      }
-      if (t * kTile < last) tile(t, buf, held0, held1, [] {});
-    }
-  } else {
-    for (; t < t_end; t += KW) {
-      const bool held0 = page_of(t, 0) >= 0, held1 = page_of(t, 1) >= 0;
-      if (!AHEAD) load_k(t);
-      else load_v(t);
-      __builtin_amdgcn_sched_barrier(0);
-      tile(t, 0, held0, held1, [&] {
-        __builtin_amdgcn_sched_barrier(0);
-        if (!AHEAD) load_v(t);
-        if (t + KW < t_end) {
-          next_pages(t + KW);
-          if (AHEAD) load_k(t + KW);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+    const auto value = [&](int d, int h) { return vr[d][h]; };
+    if (!rows.full(t, held0, held1) && rows.any_odd(value)) {
+      rows.spoil(t, held0, held1, [&](int d, int h) {
+        const int page = (h ? held1 : held0) ? pages.table[(2 * t + h) >> p.page_shift] : 0;
+        return load16<false>(pages.at(pages.values(pages.block(page, t, h))) + 512 * d + uint32_t(8 * lane));
       });
-    }
-  }
-
-#pragma unroll
-  for (int u = 0; u < QB; ++u) {
-    l[u] += __shfl_xor(l[u], 16, 64);
-    l[u] += __shfl_xor(l[u], 32, 64);
-    if (end[u] == 0) l[u] = 0.f;
-    if (__ballot(spoilt[u] != 0)) {
 #pragma unroll
       for (int d = 0; d < PER; ++d)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[u][d][e] = spoilt[u] >> (4 * d + e) & 1 ? __builtin_nanf("") : acc[u][d][e];
+        for (int h = 0; h < 2; ++h) vr[d][h] = finite(vr[d][h]);
+    }
+    rows.product(value);
+  }
+  rows.finish();
+
+  auto& mg = *reinterpret_cast<Merge<D, QB>*>(lds);
+#pragma unroll
+  for (int u = 0; u < QB; ++u) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) mg.acc[wave][u][v][c][lane] = rows.piece(u, v, c);
+    if (rows.g == 0) {
+      mg.m[wave][u][rows.j] = rows.m[u];
+      mg.l[wave][u][rows.j] = rows.l[u][0];
     }
   }
-  // Dims PER (4 g + v) + 4 c .. + 3 of row (u, j), of `total` weight at exponent reference `top`.
-  const auto put = [&](int u, int v, int c, float4_t o, float total) {
-    if (row_id[u] < 0) return;
-    const int dim = PER * (4 * g + v) + 4 * c;
-    if (p.splits > 1) {
-      const int64_t at = int64_t(split) * p.all_rows + row_id[u];
-      if (total != 0.f) *reinterpret_cast<float4_t*>(a.workspace + at * D + dim) = o;
-      return;
+  __syncthreads();
+  // Wave w joins number v = w of the dims.
+#pragma unroll
+  for (int u = 0; u < QB; ++u) {
+    float top = kNegInf, total = 0.f, f[kWaves];
+    bool empty[kWaves];  // (what it holds is no row's; a state with keys counts however little it weighs: 0 times NaN is NaN)
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = mg.l[w][u][rows.j] == 0.f ? top : fmaxf(top, mg.m[w][u][rows.j]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float lw = mg.l[w][u][rows.j];
+      empty[w] = lw == 0.f;
+      f[w] = empty[w] ? 0.f : __builtin_amdgcn_exp2f(mg.m[w][u][rows.j] - top);
+      total += lw * f[w];
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    const half4_t y = output_of(o, total, inv);
-    __builtin_memcpy(a.out + int64_t(row_id[u]) * D + dim, &y, 8);
-  };
-  const auto put_weight = [&](int u, float top, float total) {
-    if (p.splits == 1 || g != 0 || row_id[u] < 0) return;
-    float* ml = a.workspace + p.splits * p.all_rows * D + 2 * (int64_t(split) * p.all_rows + row_id[u]);
-    ml[0] = top;
-    ml[1] = total;
-  };
-  const auto piece = [&](int u, int v, int c) {
-    return float4_t{acc[u][4 * c][v], acc[u][4 * c + 1][v], acc[u][4 * c + 2][v], acc[u][4 * c + 3][v]};
-  };
-  if constexpr (SHARED) {
 #pragma unroll
-    for (int u = 0; u < QB; ++u) {
+    for (int c = 0; c < D / 64; ++c) {
+      float4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int v = 0; v < 4; ++v)
+      for (int w = 0; w < kWaves; ++w) {
+        const float4_t x = mg.acc[w][u][wave][c][lane];
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) put(u, v, c, piece(u, v, c), l[u]);
-      put_weight(u, m[u], l[u]);
-    }
-  } else {
-    // The waves' states meet in LDS; wave w joins every KW-th v.
-    auto& mg = *reinterpret_cast<Merge<D, QB, KW>*>(lds);
-#pragma unroll
-    for (int u = 0; u < QB; ++u) {
-#pragma unroll
-      for (int v = 0; v < 4; ++v)
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) mg.acc[wave][u][v][c][lane] = piece(u, v, c);
-      if (g == 0) {
-        mg.m[wave][u][j] = m[u];
-        mg.l[wave][u][j] = l[u];
+        for (int e = 0; e < 4; ++e) o[e] = empty[w] ? o[e] : fmaf(x[e], f[w], o[e]);
       }
+      rows.put(u, wave, c, split, o, total);
     }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < QB; ++u) {
-      float top = kNegInf, total = 0.f, f[KW];
-      bool empty[KW];  // (what it holds is no row's; a state with keys counts however little it weighs: 0 times NaN is NaN)
-#pragma unroll
-      for (int w = 0; w < KW; ++w) top = mg.l[w][u][j] == 0.f ? top : fmaxf(top, mg.m[w][u][j]);
-#pragma unroll
-      for (int w = 0; w < KW; ++w) {
-        const float lw = mg.l[w][u][j];
-        empty[w] = lw == 0.f;
-        f[w] = empty[w] ? 0.f : __builtin_amdgcn_exp2f(mg.m[w][u][j] - top);
-        total += lw * f[w];
-      }
-#pragma unroll
-      for (int v0 = 0; v0 < 4; v0 += KW)
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          float4_t o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int w = 0; w < KW; ++w) {
-            const float4_t x = mg.acc[w][u][v0 + wave][c][lane];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = empty[w] ? o[e] : fmaf(x[e], f[w], o[e]);
-          }
-          put(u, v0 + wave, c, o, total);
-        }
-      if (wave == 0) put_weight(u, top, total);
-    }
+    if (wave == 0) rows.put_weight(u, split, top, total);
   }
 }
 
+// Four waves have a pair of row blocks each and share every tile, brought into LDS operand by
+// operand, one conflict-free kilobyte each, straight from memory: the next one while all work on
+// this one, two buffers and one barrier a tile.
+constexpr int kSharers = 4;
+template <int D>
+struct Tiles {
+  half8_t k[2][4 * D / 32][64], v[2][2 * D / 16][64];
+};
+template <int D>
+__device__ __forceinline__ void attend_shared(const AttnPlan& p, uint8_t* lds, int b, int head, int rb, int split) {
+  constexpr int QB = 2, PER = D / 16, GROUP = kSharers * 16 * QB, PIECE = D / 32;  // PIECE: records of keys, and of values, that a wave loads
+  const int lane = int(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)), half = wave >> 1;
+  auto& shared = *reinterpret_cast<Tiles<D>*>(lds);
+  Pages<D, 1> pages(p, b, head);
+  if (p.splits == 1) pages.look_up(0);
+  Rows<D, QB> rows(p, b, head, rb * GROUP + wave * 16 * QB);
+  const int group_last = rows.last_of(rb * GROUP, GROUP), group_first = rows.first_of(rb * GROUP);
+  const int tiles = (group_last + kTile - 1) / kTile, per = (tiles + p.splits - 1) / p.splits, t_end = min(tiles, (split + 1) * per);
+  int t = split * per;
+
+  // This wave's quarter of a tile's keys or values (records PIECE * wave .. of it, all of them of
+  // half `wave / 2`) from their half's block to a buffer.
+  const auto bring = [&](int block, half8_t (*to)[64]) {
+    const uint16_t* at = pages.at(block) + (wave & 1) * (PIECE * 512);
+#pragma unroll
+    for (int i = 0; i < PIECE; ++i)
+      __builtin_amdgcn_global_load_lds((global_ptr)(at + 512 * i + uint32_t(8 * lane)), (lds_ptr)&to[PIECE * wave + i][0], 16, 0, 0);
+  };
+  int flags = 0;  // two bits for each of tiles t and t + 1: their halves are on a page
+  const auto fetch = [&](int tt, int buf) {
+    const int block = pages.block(pages.page(tt, half), tt, half);
+    bring(block, shared.k[buf]);
+    bring(pages.values(block), shared.v[buf]);
+    flags |= int(pages.held(tt, 0)) << 2 | int(pages.held(tt, 1)) << 3;
+  };
+  if (t < t_end) {
+    if (p.splits > 1) pages.look_up(t);
+    fetch(t, 0);
+  }
+  rows.load();
+  for (int buf = 0; t < t_end; ++t, buf ^= 1) {
+    flags >>= 2;
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): what this wave has brought
+    lds_barrier();                        // everyone's has landed, and nobody reads the other buffer any more
+    if (t + 1 < t_end) {
+      pages.reach(t + 1);
+      fetch(t + 1, buf ^ 1);
+    }
+    const auto value = [&](int d, int h) { return shared.v[buf][h * PER + d][lane]; };
+    // (The same for all waves: what they find lies in LDS.)
+    if (((t + 1) * kTile > group_first || (flags & 3) != 3) && rows.any_odd(value)) {
+      rows.spoil(t, flags & 1, flags & 2, value);
+      lds_barrier();
+#pragma unroll
+      for (int i = 0; i < PIECE; ++i) {
+        half8_t& x = shared.v[buf][PIECE * wave + i][lane];
+        x = finite(x);
+      }
+      lds_barrier();
+    }
+    if (t * kTile >= rows.last) continue;
+    float4_t sc[QB][4];
+    rows.score(sc, [&](int kb, int c) { return shared.k[buf][kb * (D / 32) + c][lane]; });
+#pragma unroll
+    for (int u = 0; u < QB; ++u) rows.refer(u, sc, t, flags & 1, flags & 2);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < QB; ++u) rows.weigh(u, sc);
+    rows.product(value);
+  }
+  rows.finish();
+#pragma unroll
+  for (int u = 0; u < QB; ++u) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) rows.put(u, v, c, split, rows.piece(u, v, c), rows.l[u][0]);
+    rows.put_weight(u, split, rows.m[u], rows.l[u][0]);
+  }
+}
+
+// Waves per SIMD that the registers are budgeted for.  What the compiler takes: 64 dims, one
+// block 149 of 168, two 206, shared 117; 128 dims 240, 253 and 165, none spilled.
 constexpr int waves_for(int dim, int qb) { return dim == 64 && qb == 1 ? 3 : 2; }
 
-template <int D, int QB, int KW>
-__global__ __launch_bounds__(KW == kShared ? 256 : 64 * KW, waves_for(D, QB)) void paged_attention_kernel(AttnPlan p) {
+// QB: row blocks per wave; kShared: waves that share tiles.
+constexpr int kShared = 0;
+template <int D, int QB>
+__global__ __launch_bounds__(QB == kShared ? 64 * kSharers : 64 * kWaves, waves_for(D, QB)) void paged_attention_kernel(AttnPlan p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   // The last row blocks of all (request, key head) pairs first: under the causal mask
   // they are the longest.
   const int id = int(blockIdx.x), block = div_by(id, p.pairs), at = id - block * int(p.pairs.d), b = div_by(at, p.heads);
   const int split = div_by(block, p.row_block_div), blocks = int(p.row_block_div.d);
-  attend<D, QB, KW>(p, lds, b, at - b * int(p.heads.d), blocks - 1 - (block - split * blocks), split);
+  const int rb = blocks - 1 - (block - split * blocks), head = at - b * int(p.heads.d);
+  if constexpr (QB == kShared) attend_shared<D>(p, lds, b, head, rb, split);
+  else attend<D, QB>(p, lds, b, head, rb, split);
 }
 
 // W waves of a workgroup of 4 join a row's states: D / 4 lanes a state, 2 or 4 states at a
@@ -556,19 +658,33 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(AttnPlan p) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// How a call is walked: `blocks` row blocks of 16 per wave, `waves` waves to a row block
-// or kShared, `splits` workgroups to its keys.
+// How a call is walked: `blocks` row blocks of 16 per wave or kShared, `splits` workgroups to
+// its keys.
 struct Walk {
-  int blocks, waves, splits;
+  int blocks, splits;
 };
+// From the number of (request, key head) pairs, the rows of one and the tiles of 64 keys of
+// the longest; us, of the three ways that follow.
+// Two blocks of 16 rows use every key and value twice.  They pay where one block to a
+// workgroup makes many workgroups of many tiles (D 64: 12 pairs of 300 rows over 4096 keys 18.5
+// against 22.5, 192 of 40 over 4096 56 and 87; not 48 of 40 over 1024, 9.9 and 8.5, nor 192 of 20
+// over 256, 7.3 and 6.9), or at 128 dims, of which a CU holds two, more than one a CU (32 pairs
+// of 400 rows over 256 keys 11.7 and 14.1, 128 of 80 over 4096 87 and 164; 8 of 400 over 1024 12.9
+// and 10.8, 32 of 32 over 4096 21.5 and 19.9).
+// Tiles shared by 128 rows pay where these blocks are plenty (D 64: 192 pairs of 100 rows over
+// 4096 keys 70 against 96 in blocks of two, 48 of 1000 over 1024 24.8 and 26.5, 192 of 300 over 1024 36 and 46, 48
+// of 300 over 1024 24 and 13; D 128: 128 pairs of 400 rows over 1024 44 and 68, 32 of 4000 over
+// 4096 239 and 312, 8 of 4000 over 1024 35 and 27).
+// Splits: a second launch and the states' traffic cost 2 us and more, and 4 us of the
+// caller's time, so short caches are not split (12 pairs of 1 row over 1024 keys 8.7 us).
+// Longer ones are, into at most one workgroup a CU (12 pairs over 4096 keys 10.1, over 16384
+// 15.3; 8 pairs of 4 rows over 32768, D 128, 30) and 64 splits, but where the pairs alone take
+// more than half of the CUs into about 512.
 Walk walk_for(int64_t pairs, int rows, int keys, int dim) {
-  const int64_t tiles = ceil_div(keys, kTile), twos = pairs * ceil_div(rows, 32), plenty = dim == 64 ? 1024 : 512;
-  Walk w{1, 4, 1};
-  if (rows > 16 && (twos >= plenty || tiles >= 128 || (twos >= 128 && twos * tiles > 4096))) w.blocks = 2;
-  if (w.blocks == 2 && twos >= plenty) {
-    w.waves = kShared;
-    return w;
-  }
+  const int64_t tiles = ceil_div(keys, kTile), ones = pairs * ceil_div(rows, 16), twos = pairs * ceil_div(rows, 32);
+  Walk w{1, 1};
+  if (rows > 16 && (dim == 64 ? ones * tiles > 5000 : ones > 256 || ones * tiles > 8000)) w.blocks = 2;
+  if (w.blocks == 2 && twos >= (dim == 64 ? 768 : 1200)) return {kShared, 1};
   const int64_t wgs = pairs * ceil_div(rows, 16 * w.blocks);
   if (tiles > (dim == 64 ? 24 : 16))
     w.splits = int(wgs > 128 && tiles >= 64 ? ceil_div(512, wgs) : std::max<int64_t>(1, std::min<int64_t>({256 / wgs, tiles / 4, 64})));
@@ -588,22 +704,22 @@ AttnPlan plan_of(const PagedAttnArgs& a, Walk& w) {
   p.pairs = divisor(uint32_t(pairs));
   p.all_rows = pairs * rows;
   w = walk_for(pairs, rows, a.max_kv, a.cache.head_dim);
-  const int64_t blocks = ceil_div(rows, 16 * w.blocks * (w.waves == kShared ? 4 : 1));
+  const int64_t blocks = ceil_div(rows, w.blocks == kShared ? 32 * kSharers : 16 * w.blocks);
   p.row_block_div = divisor(uint32_t(blocks));
   p.workgroups = pairs * blocks * w.splits;
   p.splits = w.splits;
   return p;
 }
 
-template <int D, int QB, int KW>
+template <int D, int QB>
 hipError_t launch(const AttnPlan& p, hipStream_t stream) {
-  constexpr int bytes = KW == kShared ? int(sizeof(Tiles<D>)) : int(sizeof(Merge<D, QB, (KW > 0 ? KW : 1)>));
+  constexpr int bytes = QB == kShared ? int(sizeof(Tiles<D>)) : int(sizeof(Merge<D, (QB > 0 ? QB : 1)>));
   if constexpr (bytes > 64 * 1024) {  // (two blocks of 128-dim rows)
     static LdsLimit limit;
-    const hipError_t e = limit.raise(reinterpret_cast<const void*>(&paged_attention_kernel<D, QB, KW>), bytes);
+    const hipError_t e = limit.raise(reinterpret_cast<const void*>(&paged_attention_kernel<D, QB>), bytes);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((paged_attention_kernel<D, QB, KW>), dim3(unsigned(p.workgroups)), dim3(KW == kShared ? 256 : 64 * KW), bytes, stream, p);
+  hipLaunchKernelGGL((paged_attention_kernel<D, QB>), dim3(unsigned(p.workgroups)), dim3(QB == kShared ? 64 * kSharers : 64 * kWaves), bytes, stream, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
   if (p.splits > 16)
@@ -615,8 +731,8 @@ hipError_t launch(const AttnPlan& p, hipStream_t stream) {
 
 template <int D>
 hipError_t launch_walk(const AttnPlan& p, const Walk& w, hipStream_t stream) {
-  if (w.waves == kShared) return launch<D, 2, kShared>(p, stream);
-  return w.blocks == 1 ? launch<D, 1, 4>(p, stream) : launch<D, 2, 4>(p, stream);
+  if (w.blocks == kShared) return launch<D, kShared>(p, stream);
+  return w.blocks == 1 ? launch<D, 1>(p, stream) : launch<D, 2>(p, stream);
 }
 
 }  // namespace
