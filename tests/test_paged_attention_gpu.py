@@ -155,6 +155,29 @@ def test_masks_that_leave_nothing(ops, q_rows):
     y = host(ops.attention_paged(dev(q), cache, dev(table), i32([2 ** 31 - 1] * batch), causal=False))
     full = [np.concatenate([x, np.zeros((batch, 3, table.shape[1] * page - n, 64), np.float16)], 2) for x in (k, v)]
     check(y, q, *full, [table.shape[1] * page] * batch, [q_rows] * batch, None, False)
+    # Causal, with the last 20 tokens past it: queries stay where their lengths put them.
+    held = table.shape[1] * page
+    y = host(ops.attention_paged(dev(q), cache, dev(table), i32([held + 20] * batch)))
+    check(y, q, *full, [held] * batch, [q_rows] * batch, [held + 20 - q_rows] * batch, True)
+
+
+@pytest.mark.parametrize("dim,q_rows,heads", [(64, 1, 3), (128, 1, 4), (64, 40, 2), (128, 300, 40)])
+def test_keys_of_no_weight(ops, dim, q_rows, heads):
+    """Scores of -inf: such keys are as if masked, and a row with no others is 0."""
+    say("no weight", dim, q_rows, heads)
+    rng = np.random.default_rng(dim)
+    n = 130
+    cache, table, k, v = filled(ops, rng, 1, heads, dim, 32, n)
+    q = rng.standard_normal((1, heads, q_rows, dim)).astype(np.float16)
+    q[..., 3] = -1
+    k[:, :, :70, 3] = np.inf
+    ops.kv_append_paged(cache, dev(k), dev(v), dev(table), 0)
+    y = host(ops.attention_paged(dev(q), cache, dev(table), n, causal=False))
+    sees = np.tile(np.arange(n) >= 70, (q_rows, 1))
+    for h in sorted({0, heads - 1}):
+        want, tol = attend(q[0, h], k[0, h], v[0, h], sees)
+        assert (np.abs(y[0, h] - want) <= tol).all(), h
+    assert (host(ops.attention_paged(dev(q), cache, dev(table), 70, causal=False)) == 0).all()
 
 
 @pytest.mark.parametrize("dim,q_rows,heads", [(64, 1, 12), (128, 1, 4), (64, 40, 2), (128, 300, 40)])

@@ -142,7 +142,7 @@ struct Rows {
     const PagedAttnArgs& a = p.a;
     kv = int(min(int64_t(max(a.kv_lengths[b], 0)), int64_t(a.pages.width) * a.cache.page_size));
     ql = a.q_lengths ? min(max(a.q_lengths[b], 0), a.q_len) : a.q_len;
-    off = a.offsets ? int64_t(a.offsets[b]) : int64_t(kv) - ql;
+    off = int64_t(a.offsets ? a.offsets[b] : a.kv_lengths[b]) - (a.offsets ? 0 : ql);
     const int count = int(p.rows.d), group = int(p.group.d);
 #pragma unroll
     for (int u = 0; u < QB; ++u) {
