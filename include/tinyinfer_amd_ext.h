@@ -225,7 +225,7 @@ typedef struct ti_amd_kv_paged {
  * turned by that position if turns is given (rotated a multiple of 16), its value as it
  * is.  With q [batch][heads][rows][head_dim] its rows are turned alike into q_out
  * (contiguous; zeros past lengths[b]; null q: none).  Rows of one call that name one
- * place leave it with the values of either.  batch is at most 65535, rows at most 2^28. */
+ * place leave it with the values of either.  batch is at most 65535, rows at most 2^20. */
 int ti_amd_kv_append_paged(const ti_amd_kv_paged* cache, const uint16_t* k, int64_t k_batch, int64_t k_head, int64_t k_row,
                            const uint16_t* v, int64_t v_batch, int64_t v_head, int64_t v_row, const uint16_t* q,
                            int64_t q_batch, int64_t q_head, int64_t q_row, uint16_t* q_out, const int32_t* table, int width,
@@ -236,11 +236,12 @@ int ti_amd_kv_read_paged(const ti_amd_kv_paged* cache, uint16_t* k, uint16_t* v,
                          const int32_t* positions, const int32_t* lengths, int batch, int rows, uintptr_t stream, int device);
 /* ti_amd_attention_paged: q, y fp16 [batch][heads][q_len][head_dim] over the paged cache;
  * query head h reads key head h / (heads / kv_heads).  Request b's keys are tokens 0 ..
- * kv_lengths[b] - 1 (as far as its table reaches).  Query i < q_lengths[b] (null: q_len) sees
+ * kv_lengths[b] - 1, as far as its table reaches.  Query i < q_lengths[b] (null: q_len) sees
  * them all, or with causal = 1 those up to offsets[b] + i; offsets null means kv_lengths[b]
  * - q_lengths[b].  Rows that see no key, and queries past q_lengths[b], are exactly 0.  A row
  * that has an infinity or NaN in its query or sees a NaN in a key is NaN; one that sees an
- * infinity or NaN in a value is not finite in that dim.  What a row does not see does not
+ * infinity or NaN in a value is not finite in that dim.  A key with a score of -inf (it holds
+ * an infinity) has no weight; a row with no other keys is 0.  What a row does not see does not
  * count, whatever memory holds there.  Scores, softmax and sums are fp32; a probability is
  * rounded to fp16 for its product (for single tokens twice: what the first rounding leaves out
  * is added).  batch and heads are at most 65535, batch * heads * q_len at most 2^23.

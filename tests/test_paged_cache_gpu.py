@@ -194,3 +194,19 @@ def test_a_cache_beyond_32_bits(ops):
     assert t.equal(ops.attention_paged(q, cache, table, 1600), ops.attention_paged(q, small, near, 1600))
     del cache
     t.cuda.empty_cache()
+
+
+def test_the_longest_append(ops):
+    """2^20 rows in one call, all the same in memory, of which the last lie where they belong."""
+    t = torch()
+    say("2^20 rows")
+    rows, page = 1 << 20, 1024
+    cache = ops.kv_cache_paged(rows // page, 1, page, 128)
+    table = i32(np.arange(rows // page)[::-1].reshape(1, -1).copy())
+    row = t.randn((1, 1, 1, 128), device="cuda", dtype=t.float16)
+    k = row.expand(1, 1, rows, 128)
+    rotary = ops.rotary(128)
+    ops.kv_append_paged(cache, k, -row.expand(1, 1, rows, 128), table, 0, rotary=rotary)
+    for at in (0, 4096, rows - 3):
+        got_k, got_v = ops.kv_read_paged(cache, table, at, None, 3)
+        assert t.equal(got_k, ops.rotate(k[:, :, :3], rotary, at)) and t.equal(got_v, -row.expand(1, 1, 3, 128)), at

@@ -186,6 +186,7 @@ def test_refusals(ops):
             lambda: ops.kv_append_paged(cache, x, x, table, [0, 62]),                     # past the table
             lambda: ops.kv_append_paged(cache, x, x, table, -1),
             lambda: ops.kv_append_paged(cache, x, x, table, 0, lengths=4),
+            lambda: ops.kv_append_paged(cache, *[x[:, :, :1].expand(2, 2, (1 << 20) + 1, 64)] * 2, table, pos),
             lambda: ops.kv_append_paged(cache, x, x, table, pos, q=q),                    # q without rotary
             lambda: ops.kv_append_paged(cache, x, x, table, pos, rotary=odd),
             lambda: ops.kv_append_paged(cache, x, x, table, pos, rotary=ops.rotary(128)),
@@ -193,6 +194,7 @@ def test_refusals(ops):
             lambda: ops.kv_read_paged(cache, table, pos, None, 0),
             lambda: ops.kv_read_paged(cache, table, [0], None, 3),
             lambda: ops.kv_read_paged(cache, table, 0, None, 65),
+            lambda: ops.kv_read_paged(cache, table, pos, None, (1 << 20) + 1),
             lambda: ops.kv_read_paged(cache, table[:0], 0, None, 3),
             lambda: ops.attention_paged(q[:, :3].contiguous(), cache, table, 3),                       # heads
             lambda: ops.attention_paged(q[..., :32].contiguous(), cache, table, 3),
@@ -238,7 +240,7 @@ def test_refusals(ops):
         assert lib.ti_v2_last_error()
     app = lambda **o: {"c": at, "k": p(x), "v": p(x), "s": s, "q": None, "qo": None, "t": p(table), "w": 2, "pos": p(pos), "turns": None,  # noqa: E731
                        "r": 0, "b": 2, "h": 0, "n": 3, **o}
-    for o in (dict(c=None), dict(k=None), dict(v=None), dict(t=None), dict(w=0), dict(pos=None), dict(b=0), dict(n=0), dict(n=(1 << 28) + 1),
+    for o in (dict(c=None), dict(k=None), dict(v=None), dict(t=None), dict(w=0), dict(pos=None), dict(b=0), dict(n=0), dict(n=(1 << 20) + 1),
               dict(s=(384, -192, 64)), dict(q=p(q), qo=p(out), h=4), dict(turns=p(odd.turns), r=24),
               dict(turns=p(rotary.turns), r=64, q=p(q), qo=None, h=4), dict(turns=p(rotary.turns), r=64, q=p(q), qo=p(out), h=0)):
         a = app(**o)

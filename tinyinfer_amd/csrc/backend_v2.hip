@@ -180,9 +180,9 @@ int check_paged(const ti_amd_kv_paged* c, const int32_t* table, int width, tia::
 int check_paged_rows(const void* k, const void* v, const int32_t* positions, const int32_t* lengths, int batch, int rows,
                      const tia::KvPaged& c) {
   if (!aligned(k, 2) || !aligned(v, 2) || !aligned(positions, 4) || !optional_aligned(lengths, 4) || batch <= 0 || batch > 65535 ||
-      rows <= 0 || rows > (1 << 28) || !shape_fits({batch, c.kv_heads, rows, c.head_dim}, 2))
+      rows <= 0 || rows > (1 << 20) || !shape_fits({batch, c.kv_heads, rows, c.head_dim}, 2))
     return fail(TI_V2_INVALID_ARGUMENT,
-                "invalid paged cache rows: shape, pointers or alignment (batch at most 65535, rows 2^28)");
+                "invalid paged cache rows: shape, pointers or alignment (batch at most 65535, rows 2^20)");
   return TI_V2_OK;
 }
 

@@ -330,7 +330,7 @@ struct RotateArgs {
 };
 hipError_t rotate(const RotateArgs& args, hipStream_t stream);
 
-// The paged fp16 KV cache (layout in paged_cache.hip): page_size a power of two of 32
+// The paged fp16 KV cache (layout in paged_cache.hpp): page_size a power of two of 32
 // tokens and more.
 struct KvPaged {
   uint16_t* pages = nullptr;

@@ -914,7 +914,7 @@ class NativeOps:
         torch = self.torch
         call = _Call(self, "ti_amd_kv_read_paged")
         call.cache(cache, PagedKVCache)
-        _count(rows, "rows")
+        _count(rows, "rows", high=1 << 20)
         if not isinstance(page_table, self.tensor_type):
             raise TypeError("page_table: a GPU (torch 'cuda' device) tensor is required")
         batch = page_table.shape[0] if page_table.dim() else 0
@@ -929,8 +929,8 @@ class NativeOps:
         """The table, positions and lengths; host values must stay inside the table."""
         if positions is None:
             raise ValueError("positions are required")
-        if batch > 65535 or rows > 1 << 28:
-            raise ValueError("batch must be at most 65535, rows at most 2^28")
+        if batch > 65535 or rows > 1 << 20:
+            raise ValueError("batch must be at most 65535, rows at most 2^20")
         held = min(call.page_table(page_table, batch) * cache.page_size, INT32_MAX)
         tensor = self.tensor_type
         if not isinstance(positions, tensor) and not isinstance(lengths, tensor):
