@@ -28,8 +28,8 @@
 // to 32768 keys: 248 us, 6.3 TB/s), launch and one tile's chain of latencies where they are
 // short (one request of 12 heads, 300 keys: 6.2 us; 32 of them, 128 to 1024 keys: 15 us, 5.6 of
 // them without keys).  Prompts: a tile of 64 keys x 32 rows at D 128 is 68 matrix instructions, 1088
-// cycles of a SIMD, about 105 vector instructions and 32 exponentials, 930 cycles, and a
-// quarter of the CU's LDS for 256 cycles at least; two workgroups a CU overlap these in part.  2
+// cycles of a SIMD, about 105 vector instructions and 32 exponentials, 930 cycles, and 32 KB
+// from LDS, 256 of the CU's cycles and 1024 for four waves; two workgroups a CU overlap these in part.  2
 // requests of 777 queries, 32 heads over 8 of 128, 4500 to 6001 keys: 170 us, 791 TFLOP/s (400
 // workgroups, so 78 % of the CUs' time); 4096 queries of 32 heads over as many keys 149 us, 920
 // TFLOP/s; 4 prompts of 1024, 25 heads of 64: 28 us, 473 TFLOP/s.  Tried for the shared tiles and no

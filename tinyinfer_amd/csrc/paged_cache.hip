@@ -10,6 +10,10 @@
 // queries, the keys or the values of a range of tokens that starts where a record does, and
 // neighbouring ones the same tokens of other heads, which lie side by side where q, k and v are
 // slices of one projection.
+//
+// What bounds it: memory (8 prompts of up to 1000 tokens, 25 heads of 64: append 26 us, of which the
+// same bytes copied take 23; read back 16.6, 5.2 TB/s), and the launch for single tokens (32
+// requests of 12 heads of 64: 4.4 and 4.1 us).
 #include "paged_cache.hpp"
 #include "rotary.hpp"
 
@@ -227,6 +231,7 @@ hipError_t append(const PagedAppendArgs& a, hipStream_t stream) {
   const int64_t ranges = (int64_t(a.rows) + 30) / R::RANGE + 1;
   const auto chunks = [](int heads, int chunk) { return (heads + chunk - 1) / chunk; };
   const int v_chunk = R::HEADS, v_chunks = chunks(kv_heads, v_chunk);
+  // Heads that share a lane's angles: 4, or fewer where that leaves fewer than 1024 workgroups.
   int chunk = 4;
   while (chunk > 1 && ranges * a.batch * (chunks(q_heads, chunk) + chunks(kv_heads, chunk) + v_chunks) < 1024) chunk /= 2;
   const int q_chunks = chunks(q_heads, chunk), k_chunks = chunks(kv_heads, chunk);

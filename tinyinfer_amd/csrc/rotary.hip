@@ -4,6 +4,10 @@
 //
 // A lane holds the cosines and sines of its 8 pairs (rotary.hpp) and walks over heads,
 // which share them: they cost about 300 vector instructions, a head's values 70.
+//
+// What bounds it: memory (2 requests of 32 heads of 128, 6001 rows: 36 us, 5.4 TB/s of reads and
+// writes, vector units 40 % busy; 8 of 25 heads of 64, 777 rows: 10.7, launch and ramp 4 of them), and
+// the launch for single tokens (32 of 24 heads of 64: 5.0 us).
 #include "rotary.hpp"
 
 namespace tia {
@@ -73,12 +77,16 @@ hipError_t rotate(const RotateArgs& a, hipStream_t stream) {
   const int w = (pairs | plain) % 4 == 0 ? 4 : (pairs | plain) % 2 == 0 ? 2 : 1;  // (of the narrow kernel)
   const int units = wide ? a.dim / 16 : (pairs + plain) / w;
   const int64_t lanes = int64_t(a.rows) * units;
-  if (wide && lanes < 256) {  // (short rows: one head to a lane)
+  // Short rows: one head to a lane, so that a request of a few tokens fills its workgroups (64
+  // requests of 32 heads of 128, one token: 4.1 us; 7.0 with lanes that walk over heads).
+  if (wide && lanes < 256) {
     const dim3 grid(unsigned((lanes * a.heads + 255) / 256), 1, unsigned(a.batch));
     hipLaunchKernelGGL(rotate_kernel<1>, grid, dim3(256), 0, stream, a, units, 1);
     return hipGetLastError();
   }
   const int64_t groups = (lanes + 255) / 256;
+  // Heads to a lane: as many as leave 1024 workgroups, four a CU (8 requests of 25 heads of 64, 777
+  // rows: 10.7 us, 11.1 with 512 and 13.1 with 4096; 2 of 32 of 128, 6001 rows: 35.6, 36.2 and 35.3).
   int64_t chunks = 1;
   while (chunks < a.heads && groups * a.batch * chunks < 1024) chunks *= 2;
   const int chunk = int((a.heads + chunks - 1) / chunks);
