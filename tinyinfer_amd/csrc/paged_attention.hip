@@ -183,19 +183,14 @@ struct Rows {
   }
   __device__ __forceinline__ bool full(int t, bool held0, bool held1) const { return (t + 1) * kTile <= first && held0 && held1; }
 
-  // Scores, key(kb, c) being the operand of 16 keys x 32 dims.
+  // Scores of block u, key(kb, c) being the operand of 16 keys x 32 dims.
   template <typename K>
-  __device__ __forceinline__ void score(float4_t (&sc)[QB][4], K key) const {
+  __device__ __forceinline__ void score(int u, float4_t (&sc)[QB][4], K key) const {
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
+      sc[u][kb] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int u = 0; u < QB; ++u) sc[u][kb] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        const half8_t kf = key(kb, c);
-#pragma unroll
-        for (int u = 0; u < QB; ++u) sc[u][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[u][c], sc[u][kb], 0, 0, 0);
-      }
+      for (int c = 0; c < D / 32; ++c) sc[u][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key(kb, c), qf[u][c], sc[u][kb], 0, 0, 0);
     }
   }
   // Masks the scores of block u and raises its reference where it must be.
@@ -238,25 +233,22 @@ struct Rows {
         }
       }
   }
-  // Adds the tile's values, value(d, h) being the operand of 16 dims x 32 keys.
+  // Adds the tile's values to block u, value(d, h) being the operand of 16 dims x 32 keys.
   template <typename V>
-  __device__ __forceinline__ void product(V value) {
+  __device__ __forceinline__ void product(int u, V value) {
     if constexpr (!FINE) {
       const f16 one = f16(1.f);
       const half8_t ones = {one, one, one, one, one, one, one, one};
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int u = 0; u < QB; ++u) l[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pp[u][h], l[u], 0, 0, 0);
+      for (int h = 0; h < 2; ++h) l[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pp[u][h], l[u], 0, 0, 0);
     }
 #pragma unroll
     for (int d = 0; d < PER; ++d)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const half8_t vf = value(d, h);
-#pragma unroll
-        for (int u = 0; u < QB; ++u) acc[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pp[u][h], acc[u][d], 0, 0, 0);
-        if constexpr (FINE) acc[0][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, rest[h], acc[0][d], 0, 0, 0);
+        acc[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pp[u][h], acc[u][d], 0, 0, 0);
+        if constexpr (FINE) acc[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, rest[h], acc[u][d], 0, 0, 0);
       }
   }
   // Of a tile of which a row may not see everything: whether it has an infinity or NaN, and the
@@ -435,7 +427,8 @@ __device__ __forceinline__ void attend(const AttnPlan& p, uint8_t* lds, int b, i
     else load_v(t);
     __builtin_amdgcn_sched_barrier(0);
     float4_t sc[QB][4];
-    rows.score(sc, [&](int kb, int c) { return kr[kb][c]; });
+#pragma unroll
+    for (int u = 0; u < QB; ++u) rows.score(u, sc, [&](int kb, int c) { return kr[kb][c]; });
     __builtin_amdgcn_sched_barrier(0);
     if (!AHEAD) load_v(t);
     if (t + kWaves < t_end) {
@@ -459,7 +452,8 @@ __device__ __forceinline__ void attend(const AttnPlan& p, uint8_t* lds, int b, i
 #pragma unroll
         for (int h = 0; h < 2; ++h) vr[d][h] = finite(vr[d][h]);
     }
-    rows.product(value);
+#pragma unroll
+    for (int u = 0; u < QB; ++u) rows.product(u, value);
   }
   rows.finish();
 
@@ -528,10 +522,14 @@ __device__ __forceinline__ void attend_shared(const AttnPlan& p, uint8_t* lds, i
   // This wave's quarter of a tile's keys or values (records PIECE * wave .. of it, all of them of
   // half `wave / 2`) from their half's block to a buffer.
   const auto bring = [&](int block, half8_t (*to)[64]) {
-    const uint16_t* at = pages.at(block) + (wave & 1) * (PIECE * 512);
-#pragma unroll
-    for (int i = 0; i < PIECE; ++i)
-      __builtin_amdgcn_global_load_lds((global_ptr)(at + 512 * i + uint32_t(8 * lane)), (lds_ptr)&to[PIECE * wave + i][0], 16, 0, 0);
+    const global_ptr from = (global_ptr)(pages.at(block) + (wave & 1) * (PIECE * 512) + uint32_t(8 * lane));
+    const lds_ptr in = (lds_ptr)&to[PIECE * wave][0];
+    __builtin_amdgcn_global_load_lds(from, in, 16, 0, 0);  // (the offset counts on both sides)
+    __builtin_amdgcn_global_load_lds(from, in, 16, 1024, 0);
+    if constexpr (PIECE == 4) {
+      __builtin_amdgcn_global_load_lds(from, in, 16, 2048, 0);
+      __builtin_amdgcn_global_load_lds(from, in, 16, 3072, 0);
+    }
   };
   int flags = 0;  // two bits for each of tiles t and t + 1: their halves are on a page
   const auto fetch = [&](int tt, int buf) {
@@ -566,14 +564,32 @@ __device__ __forceinline__ void attend_shared(const AttnPlan& p, uint8_t* lds, i
       lds_barrier();
     }
     if (t * kTile >= rows.last) continue;
+    // One block's matrix instructions stand next to the other one's exponentials; the operands
+    // stay in registers from the first block to the second.
     float4_t sc[QB][4];
-    rows.score(sc, [&](int kb, int c) { return shared.k[buf][kb * (D / 32) + c][lane]; });
+    half8_t kf[4][D / 32], vf[PER][2];
 #pragma unroll
-    for (int u = 0; u < QB; ++u) rows.refer(u, sc, t, flags & 1, flags & 2);
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) kf[kb][c] = shared.k[buf][kb * (D / 32) + c][lane];
+    const auto key = [&](int kb, int c) { return kf[kb][c]; };
+    const auto held_value = [&](int d, int h) { return vf[d][h]; };
+    rows.score(0, sc, key);
+    rows.refer(0, sc, t, flags & 1, flags & 2);
+    __builtin_amdgcn_sched_barrier(0);
+    rows.score(1, sc, key);
+    rows.weigh(0, sc);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < QB; ++u) rows.weigh(u, sc);
-    rows.product(value);
+    for (int d = 0; d < PER; ++d)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) vf[d][h] = value(d, h);
+    rows.refer(1, sc, t, flags & 1, flags & 2);
+    __builtin_amdgcn_sched_barrier(0);
+    rows.product(0, held_value);
+    rows.weigh(1, sc);
+    __builtin_amdgcn_sched_barrier(0);
+    rows.product(1, held_value);
   }
   rows.finish();
 #pragma unroll
