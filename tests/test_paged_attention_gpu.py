@@ -203,7 +203,7 @@ def test_pages_that_are_not_there(ops, dim, q_rows, heads):
 
 
 @pytest.mark.parametrize("dim,q_rows,heads,batch", [(64, 1, 12, 3), (128, 1, 4, 3), (64, 24, 2, 3), (128, 24, 2, 3), (64, 200, 25, 12),
-                                                    (128, 200, 10, 12)])
+                                                    (128, 200, 10, 12), (128, 200, 12, 12)])
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 def test_what_a_row_does_not_see_does_not_count(ops, dim, q_rows, heads, batch, value):
     """Infinities and NaN behind a request's keys, in pages of other requests, and in keys and
@@ -251,6 +251,33 @@ def test_what_a_row_does_not_see_does_not_count(ops, dim, q_rows, heads, batch, 
         want, tol = attend(q[b, h], k[b, h, :n], v[b, h, :n], sees)
         assert np.isnan(y[b, h, -8:]).all()
         assert (np.abs(y[b, h] - want) <= tol)[:-8].all(), (b, h)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("value", [0.0, math.nan])
+def test_a_few_more_row_blocks_than_a_round(ops, dim, causal, value):
+    """260 blocks of 128 rows: the last workgroups walk their rows in another way; the tokens of a
+    page that is gone and what lies behind the keys do not count for either."""
+    say("more than a round", dim, causal, value)
+    rng = np.random.default_rng(dim + causal)
+    batch, kv_heads, group, q_rows, n, page = 4, 4, 8, 257, 600, 32
+    cache, table, k, v = filled(ops, rng, batch, kv_heads, dim, page, n)
+    if value:
+        behind = np.full((batch, kv_heads, table.shape[1] * page - n, dim), value, np.float16)
+        ops.kv_append_paged(cache, dev(behind), dev(behind), dev(table), n)
+        cache.buffer[[p for p in range(cache.pages) if p not in table]] = value
+    gone = table.copy()
+    gone[3, 7] = -1
+    q = (rng.standard_normal((batch, kv_heads * group, q_rows, dim)) * 1.5).astype(np.float16)
+    ql = [q_rows, 3, 250, q_rows]
+    y = host(ops.attention_paged(dev(q), cache, dev(gone), n, q_lengths=i32(ql), causal=causal))
+    for b in range(batch):
+        held = np.repeat(gone[b] >= 0, page)[:n]
+        sees = (np.arange(n)[None] < np.array(seen_by(q_rows, n, ql[b], None, causal))[:, None]) & held
+        for h in (0, kv_heads * group - 1):
+            want, tol = attend(q[b, h], k[b, h // group], v[b, h // group], sees)
+            assert (np.abs(y[b, h] - want) <= tol).all(), (b, h)
 
 
 @pytest.mark.parametrize("dim,q_rows,n,heads", [(64, 1, 700, 4), (128, 1, 4000, 1), (64, 30, 700, 4), (128, 200, 300, 40)])

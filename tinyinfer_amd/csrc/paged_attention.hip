@@ -30,13 +30,15 @@
 // them without keys).  Prompts: a tile of 64 keys x 32 rows at D 128 is 68 matrix instructions, 1088
 // cycles of a SIMD, about 105 vector instructions and 32 exponentials, 930 cycles, and 32 KB
 // from LDS, 256 of the CU's cycles and 1024 for four waves; two workgroups a CU overlap these in part.  2
-// requests of 777 queries, 32 heads over 8 of 128, 4500 to 6001 keys: 170 us, 791 TFLOP/s (400
-// workgroups, so 78 % of the CUs' time); 4096 queries of 32 heads over as many keys 149 us, 920
-// TFLOP/s; 4 prompts of 1024, 25 heads of 64: 28 us, 473 TFLOP/s.  Tried for the shared tiles and no
-// faster: the next tile's scores under this one's weights (192 us for 179 then), eight waves of which
-// four multiply while four work out weights (169, but 46 for 30 at D 64: products and weights of
-// two waves of a SIMD take as long together as one after the other), operands read from LDS 4 to 16 ahead
-// by hand (181).
+// requests of 777 queries, 32 heads over 8 of 128, 4500 to 6001 keys: 166 us, 813 TFLOP/s (400
+// workgroups on 256 CUs); 2 of 1024 over 5120 157 us, 983 TFLOP/s, 87 % of what a large library
+// product reaches; 4 prompts of 1024, 25 heads of 64: 28 us, 480 TFLOP/s.  Left out (wrong values), 166
+// us becomes: the exponentials 158, the maximum 164, the loads 155, the second product 122.  One row
+// block's products stand beside the other's exponentials (172 with both blocks in step).  Tried for the
+// shared tiles and no faster: the next tile's scores under this one's weights (192 us for 179 then),
+// eight waves of which four multiply while four work out weights (169, but 46 for 30 at D 64), operands
+// read from LDS 4 to 16 ahead by hand (181), the loads spread over the tile (165 to 171), wave
+// priorities (167).
 #include <algorithm>
 
 #include "divisor.hpp"
@@ -61,6 +63,7 @@ struct AttnPlan {
   Divisor heads, pairs;    // key heads; (request, key head) pairs
   Divisor row_block_div;   // row blocks of a pair
   int splits;              // of a request's keys
+  int tail;                // kMixed: row blocks of a pair, from the first on, that are walked two by two
   int64_t workgroups;
   int64_t all_rows;        // batch * heads * q_len
 };
@@ -603,21 +606,29 @@ __device__ __forceinline__ void attend_shared(const AttnPlan& p, uint8_t* lds, i
 }
 
 // Waves per SIMD that the registers are budgeted for.  What the compiler takes: 64 dims, one
-// block 149 of 168, two 206, shared 117; 128 dims 240, 253 and 165, none spilled.
+// block 149 of 168, two 206, shared 154, mixed 207; 128 dims 240, 253, 234 and 256, none spilled.
 constexpr int waves_for(int dim, int qb) { return dim == 64 && qb == 1 ? 3 : 2; }
 
-// QB: row blocks per wave; kShared: waves that share tiles.
-constexpr int kShared = 0;
+// QB: blocks of 16 rows per wave; kShared: waves that share tiles, kMixed: and for the last
+// workgroups ones of two blocks.
+constexpr int kShared = 0, kMixed = -1;
+static_assert(kSharers == kWaves, "one size of workgroup");
 template <int D, int QB>
-__global__ __launch_bounds__(QB == kShared ? 64 * kSharers : 64 * kWaves, waves_for(D, QB)) void paged_attention_kernel(AttnPlan p) {
+__global__ __launch_bounds__(64 * kWaves, waves_for(D, QB)) void paged_attention_kernel(AttnPlan p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   // The last row blocks of all (request, key head) pairs first: under the causal mask
   // they are the longest.
   const int id = int(blockIdx.x), block = div_by(id, p.pairs), at = id - block * int(p.pairs.d), b = div_by(at, p.heads);
-  const int split = div_by(block, p.row_block_div), blocks = int(p.row_block_div.d);
-  const int rb = blocks - 1 - (block - split * blocks), head = at - b * int(p.heads.d);
-  if constexpr (QB == kShared) attend_shared<D>(p, lds, b, head, rb, split);
-  else attend<D, QB>(p, lds, b, head, rb, split);
+  const int blocks = int(p.row_block_div.d), head = at - b * int(p.heads.d);
+  if constexpr (QB == kMixed) {
+    const int behind = block - (blocks - p.tail);
+    if (behind < 0) attend_shared<D>(p, lds, b, head, blocks - 1 - block, 0);
+    else attend<D, 2>(p, lds, b, head, kSharers * p.tail - 1 - behind, 0);
+  } else {
+    const int split = div_by(block, p.row_block_div), rb = blocks - 1 - (block - split * blocks);
+    if constexpr (QB == kShared) attend_shared<D>(p, lds, b, head, rb, split);
+    else attend<D, QB>(p, lds, b, head, rb, split);
+  }
 }
 
 // W waves of a workgroup of 4 join a row's states: D / 4 lanes a state, 2 or 4 states at a
@@ -674,33 +685,47 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(AttnPlan p) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// How a call is walked: `blocks` row blocks of 16 per wave or kShared, `splits` workgroups to
-// its keys.
+// How a call is walked: `blocks` row blocks of 16 per wave, kShared or kMixed, `splits` workgroups
+// to its keys; kMixed: `tail` blocks of 128 rows of every pair by waves of two.
 struct Walk {
-  int blocks, splits;
+  int blocks, splits, tail = 0;
 };
-// From the number of (request, key head) pairs, the rows of one and the tiles of 64 keys of
-// the longest; us, of the three ways that follow.
+// From the number of (request, key head) pairs, the rows of one, the tiles of 64 keys of the
+// longest, and whether rows see about as many keys (even); us, of the ways that follow.
 // Two blocks of 16 rows use every key and value twice.  They pay where one block to a
 // workgroup makes many workgroups of many tiles (D 64: 12 pairs of 300 rows over 4096 keys 18.5
 // against 22.5, 192 of 40 over 4096 56 and 87; not 48 of 40 over 1024, 9.9 and 8.5, nor 192 of 20
 // over 256, 7.3 and 6.9), or at 128 dims, of which a CU holds two, more than one a CU (32 pairs
 // of 400 rows over 256 keys 11.7 and 14.1, 128 of 80 over 4096 87 and 164; 8 of 400 over 1024 12.9
 // and 10.8, 32 of 32 over 4096 21.5 and 19.9).
-// Tiles shared by 128 rows pay where these blocks are plenty (D 64: 192 pairs of 100 rows over
-// 4096 keys 70 against 96 in blocks of two, 48 of 1000 over 1024 24.8 and 26.5, 192 of 300 over 1024 36 and 46, 48
-// of 300 over 1024 24 and 13; D 128: 128 pairs of 400 rows over 1024 44 and 68, 32 of 4000 over
-// 4096 239 and 312, 8 of 4000 over 1024 35 and 27).
+// Tiles shared by 128 rows pay where there is about one such block a CU, or, of 64 dims and
+// few pairs of many keys, more (D 128: 16 pairs of 2048 rows over 4096 keys 84 against 91, 128 of 256 91
+// and 162, 16 of 1536 81 and 71; D 64: 16 of 1536 over 512 12.5 and 14.2, over 4096 55 and 43, 256
+// of 128 over 4096 59 and 151).
+// Mixed: a CU works on two blocks in 1.35 times one's time, so a few more blocks than CUs, or than
+// a multiple of them, cost nearly a round.  Up to half a round is done by waves of two blocks
+// instead, four workgroups to 128 rows, which spread over all CUs (D 128, 4096 keys, blocks: 288
+// 89.7 against 113.6 shared, 384 112 and 123, 528 148 and 198, 800 214 and 247, but 448 133 and
+// 130; over 512 keys 320 23 and 27, 384 28.2 and 27.8; D 64: 288 58 and 79, 528 91 and 109, 2080 319 and
+// 324, 3104 479 and 466).  Blocks of uneven rows, a prompt on its own, fill the CUs by themselves (25
+// heads of 64, 4 of 1024 rows: 33 and 27).
 // Splits: a second launch and the states' traffic cost 2 us and more, and 4 us of the
 // caller's time, so short caches are not split (12 pairs of 1 row over 1024 keys 8.7 us).
 // Longer ones are, into at most one workgroup a CU (12 pairs over 4096 keys 10.1, over 16384
 // 15.3; 8 pairs of 4 rows over 32768, D 128, 30) and 64 splits, but where the pairs alone take
 // more than half of the CUs into about 512.
-Walk walk_for(int64_t pairs, int rows, int keys, int dim) {
+Walk walk_for(int64_t pairs, int rows, int keys, bool even, int dim) {
+  constexpr int kCus = 256;
   const int64_t tiles = ceil_div(keys, kTile), ones = pairs * ceil_div(rows, 16), twos = pairs * ceil_div(rows, 32);
   Walk w{1, 1};
   if (rows > 16 && (dim == 64 ? ones * tiles > 5000 : ones > 256 || ones * tiles > 8000)) w.blocks = 2;
-  if (w.blocks == 2 && twos >= (dim == 64 ? 768 : 1200)) return {kShared, 1};
+  const int64_t shared = ceil_div(twos, kSharers);
+  if (w.blocks == 2 && shared >= (dim == 128 ? 240 : tiles >= 32 && pairs < 128 ? kCus + 1 : 192)) {
+    const int64_t more = shared % kCus, tail = ceil_div(more, pairs);
+    if (even && more > 0 && shared > kCus && shared < 9 * kCus && pairs * tail <= (tiles >= 16 ? kCus / 2 : kCus / 4))
+      return {kMixed, 1, int(tail)};
+    return {kShared, 1};
+  }
   const int64_t wgs = pairs * ceil_div(rows, 16 * w.blocks);
   if (tiles > (dim == 64 ? 24 : 16))
     w.splits = int(wgs > 128 && tiles >= 64 ? ceil_div(512, wgs) : std::max<int64_t>(1, std::min<int64_t>({256 / wgs, tiles / 4, 64})));
@@ -719,23 +744,25 @@ AttnPlan plan_of(const PagedAttnArgs& a, Walk& w) {
   p.heads = divisor(a.cache.kv_heads);
   p.pairs = divisor(uint32_t(pairs));
   p.all_rows = pairs * rows;
-  w = walk_for(pairs, rows, a.max_kv, a.cache.head_dim);
-  const int64_t blocks = ceil_div(rows, w.blocks == kShared ? 32 * kSharers : 16 * w.blocks);
+  w = walk_for(pairs, rows, a.max_kv, !a.causal || a.max_kv / 2 >= a.q_len, a.cache.head_dim);
+  const int64_t blocks = ceil_div(rows, w.blocks <= kShared ? 32 * kSharers : 16 * w.blocks);
   p.row_block_div = divisor(uint32_t(blocks));
-  p.workgroups = pairs * blocks * w.splits;
+  p.workgroups = pairs * (blocks * w.splits + (kSharers - 1) * w.tail);
+  p.tail = w.tail;
   p.splits = w.splits;
   return p;
 }
 
 template <int D, int QB>
 hipError_t launch(const AttnPlan& p, hipStream_t stream) {
-  constexpr int bytes = QB == kShared ? int(sizeof(Tiles<D>)) : int(sizeof(Merge<D, (QB > 0 ? QB : 1)>));
+  constexpr int tiles = QB <= kShared ? int(sizeof(Tiles<D>)) : 0, merge = QB == kShared ? 0 : int(sizeof(Merge<D, QB == 1 ? 1 : 2>));
+  constexpr int bytes = tiles > merge ? tiles : merge;
   if constexpr (bytes > 64 * 1024) {  // (two blocks of 128-dim rows)
     static LdsLimit limit;
     const hipError_t e = limit.raise(reinterpret_cast<const void*>(&paged_attention_kernel<D, QB>), bytes);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((paged_attention_kernel<D, QB>), dim3(unsigned(p.workgroups)), dim3(QB == kShared ? 64 * kSharers : 64 * kWaves), bytes, stream, p);
+  hipLaunchKernelGGL((paged_attention_kernel<D, QB>), dim3(unsigned(p.workgroups)), dim3(64 * kWaves), bytes, stream, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
   if (p.splits > 16)
@@ -747,6 +774,7 @@ hipError_t launch(const AttnPlan& p, hipStream_t stream) {
 
 template <int D>
 hipError_t launch_walk(const AttnPlan& p, const Walk& w, hipStream_t stream) {
+  if (w.blocks == kMixed) return launch<D, kMixed>(p, stream);
   if (w.blocks == kShared) return launch<D, kShared>(p, stream);
   return w.blocks == 1 ? launch<D, 1>(p, stream) : launch<D, 2>(p, stream);
 }
