@@ -16,10 +16,11 @@
 // rising ones) the range of the tokens at or above the bar is cut into runs and read again until
 // it does.
 //
-// What bounds it: memory for hundreds of rows (768 rows of 128257 in fp32, 5 alternatives: 80 us, 4.9
-// TB/s), for a few the vector units of one CU (about 11 instructions a token) and the alternatives'
-// chain of barriers (50257 tokens: none 9.1 us, 5 alternatives 12.3, 20 14.9, 64 23.3; 32 such rows, 20
-// alternatives 16.7).  512 threads: with 256 the row of 5 alternatives takes 15.0 us and the 32 rows
+// What bounds it: memory for hundreds of rows (768 rows of 128257 in fp32, 5 alternatives: 79 us, 5.0
+// TB/s), for a few what one CU fetches, about 9 bytes a cycle (loads two to four rounds ahead, or a
+// quarter fewer vector instructions, change nothing), and the alternatives' chain of barriers (50257
+// tokens: none 9.2 us, 5 alternatives 12.1, 20 14.9, 64 23.3; 32 such rows, 20 alternatives 16.7: 1 us
+// of the first loads' latency, 2 of the bar, 5 of the pass, 2.5 of sums and waits, 5 of the list).  512 threads: with 256 the row of 5 alternatives takes 15.0 us and the 32 rows
 // 29, with 1024 13.2 and 17.0, and the 768 rows 92.
 //
 // NaN logits count as -inf.  A row with a +inf has all its probability on the first one, a
@@ -355,13 +356,14 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobsArgs a) {
   };
 
   Stats stats{kNegInf, 0.f, 0.f, 0.f};
-  for (int r = 0;;) {
-    if (high >= bar) offer(high, r * THREADS + tid);
-    stats.add(x, high);
-    if (++r >= rounds) break;
+  if (high >= bar) offer(high, tid);
+  stats.add(x, high);
+  for (int r = 1; r < rounds; ++r) {
     row.values(x, next, r);
     if (r + 1 < rounds) row.load(next, r + 1);
     high = largest();
+    if (high >= bar) offer(high, r * THREADS + tid);
+    stats.add(x, high);
   }
   if (wave == 0) {  // (the first threads have them)
     float e[1] = {edge_x};

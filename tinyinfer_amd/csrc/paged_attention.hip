@@ -28,8 +28,8 @@
 // to 32768 keys: 248 us, 6.3 TB/s), launch and one tile's chain of latencies where they are
 // short (one request of 12 heads, 300 keys: 6.2 us; 32 of them, 128 to 1024 keys: 15 us, 5.6 of
 // them without keys).  Prompts: a tile of 64 keys x 32 rows at D 128 is 68 matrix instructions, 1088
-// cycles of a SIMD, about 105 vector instructions and 32 exponentials, 930 cycles, and 32 KB
-// from LDS, 256 of the CU's cycles and 1024 for four waves; two workgroups a CU overlap these in part.  2
+// cycles of a SIMD, about 105 vector instructions and 32 exponentials, 700 cycles, and 32 KB
+// from LDS, 128 of the CU's cycles and 512 for four waves; two workgroups a CU overlap these in part.  2
 // requests of 777 queries, 32 heads over 8 of 128, 4500 to 6001 keys: 166 us, 813 TFLOP/s (400
 // workgroups on 256 CUs); 2 of 1024 over 5120 157 us, 983 TFLOP/s, 87 % of what a large library
 // product reaches; 4 prompts of 1024, 25 heads of 64: 28 us, 480 TFLOP/s.  Left out (wrong values), 166
