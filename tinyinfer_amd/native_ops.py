@@ -200,9 +200,9 @@ class _Call:
         self.args.append(y.data_ptr())
         return y
 
-    def output_like(self, x):
+    def output_like(self, x, strided=False):
         torch = self.ops.torch
-        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        y = torch.empty_like(x, memory_format=torch.contiguous_format) if strided else torch.empty_like(x)
         self.made.append(y)
         self.args.append(y.data_ptr())
         return y
@@ -848,7 +848,7 @@ class NativeOps:
             raise ValueError("x: batch and heads must be at most 65535, rows * dims at most 2^31")
         if positions is None:
             raise ValueError("positions are required")
-        y = call.output_like(x)
+        y = call.output_like(x, strided=True)
         each = isinstance(positions, self.tensor_type) and positions.dim() == 2
         if each:
             call.operand(positions, self.torch.int32, "positions", shape=(batch, rows))
@@ -910,7 +910,7 @@ class NativeOps:
             q_shape = q_batch, q_heads, q_rows, q_dim = call.rows(q, "q", None)
             if q_batch != batch or q_rows != rows or q_dim != dim or q_heads > 65535:
                 raise ValueError(f"q must be [{batch}, H, {rows}, {dim}] with H at most 65535, got {list(q_shape)}")
-            turned = call.output_like(q)
+            turned = call.output_like(q, strided=True)
         self._paged_rows(call, cache, page_table, positions, lengths, batch, rows)
         call.turn(rotary)
         call.scalars(batch, q_heads, rows)
