@@ -530,8 +530,8 @@ __device__ __forceinline__ void attend_shared(const AttnPlan& p, uint8_t* lds, i
     __builtin_amdgcn_global_load_lds(from, in, 16, 0, 0);  // (the offset counts on both sides)
     __builtin_amdgcn_global_load_lds(from, in, 16, 1024, 0);
     if constexpr (PIECE == 4) {
-      __builtin_amdgcn_global_load_lds(from, in, 16, 2048, 0);
-      __builtin_amdgcn_global_load_lds(from, in, 16, 3072, 0);
+      __builtin_amdgcn_global_load_lds(from, in, 16, 2 * 1024, 0);
+      __builtin_amdgcn_global_load_lds(from, in, 16, 3 * 1024, 0);
     }
   };
   int flags = 0;  // two bits for each of tiles t and t + 1: their halves are on a page
