@@ -90,7 +90,8 @@ def check(ops, logits, tokens, top):
 
 @pytest.mark.parametrize("batch,vocab,top", [
     (1, 1, 1), (2, 1, 0), (3, 2, 5), (2, 3, 64), (4, 7, 3), (3, 17, 20), (2, 64, 64), (5, 65, 64), (2, 1000, 1), (3, 1023, 5),
-    (2, 4097, 33), (3, 16385, 20), (2, 50257, 0), (3, 50257, 5), (1, 50257, 64), (2, 65536, 17), (2, 128257, 20), (1, 2 ** 18, 64)])
+    (2, 4097, 33), (3, 16385, 20), (2, 50257, 0), (3, 50257, 5), (1, 50257, 64), (2, 65536, 17), (2, 128257, 20), (1, 2 ** 18, 64),
+    (130, 50257, 5), (60, 50257, 20), (20, 131003, 64), (2, 32768, 33)])
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
 def test_against_the_formula(ops, batch, vocab, top, dtype):
     say("logprobs", batch, vocab, top, dtype.__name__)
@@ -172,7 +173,32 @@ def test_unaligned_rows(ops):
             check(ops, host(x), host(tokens), 20)
 
 
+def test_calls_on_streams_at_once(ops):
+    """Rows split over workgroups, several calls in flight: each as on its own."""
+    say("streams")
+    t = torch()
+    rng = np.random.default_rng(9)
+    work = []
+    for i, (batch, vocab, top) in enumerate([(1, 50257, 5), (32, 50257, 20), (9, 128257, 64), (40, 70001, 0)]):
+        logits = dev((rng.standard_normal((batch, vocab)) * 3).astype(np.float16 if i % 2 else np.float32))
+        tokens = dev(rng.integers(0, vocab, batch).astype(np.int32))
+        work.append((logits, tokens, top, ops.logprobs(logits, tokens, top=top)))
+    t.cuda.synchronize()
+    streams = [t.cuda.Stream() for _ in range(4)]
+    got = []
+    for turn in range(6):
+        for i, stream in enumerate(streams):
+            logits, tokens, top, _ = work[(i + turn) % 4]
+            with t.cuda.stream(stream):
+                got.append(((i + turn) % 4, ops.logprobs(logits, tokens, top=top)))
+    t.cuda.synchronize()
+    for i, y in got:
+        for a, b in zip(y, work[i][3]):
+            assert t.equal(a, b), i
+
+
 def test_an_answer_depends_on_its_row_alone(ops):
+    """Rows that one workgroup reads whatever their number."""
     say("rows alone")
     t = torch()
     rng = np.random.default_rng(4)
