@@ -261,7 +261,9 @@ int ti_amd_attention_paged(const ti_amd_kv_paged* cache, const uint16_t* q, uint
  * ties by index.  A token outside the vocabulary, or with a logit of -inf or NaN, has the log
  * probability -inf and is no alternative: places left over hold 2^31 - 1 and -inf.  A
  * logit of +inf has all the probability (the first such one).  A row without a logit above -inf
- * has the entropy 0. */
+ * has the entropy 0.  Sums are fp32; few rows are read by several workgroups each, which meet in
+ * static memory of the library, a slot per hardware queue as for ti_amd_gemm_ex_i8_noalloc: in the
+ * last bits they may differ from the same rows in a call of many. */
 int ti_amd_logprobs(const void* logits, int dtype, const int32_t* tokens, float* logprobs, float* entropy,
                     float* top_logprobs, int32_t* top_tokens, int batch, int vocab, int given, int top, uintptr_t stream,
                     int device);
