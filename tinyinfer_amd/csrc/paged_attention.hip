@@ -712,8 +712,10 @@ struct Walk {
 // Splits: a second launch and the states' traffic cost 2 us and more, and 4 us of the
 // caller's time, so short caches are not split (12 pairs of 1 row over 1024 keys 8.7 us).
 // Longer ones are, into at most one workgroup a CU (12 pairs over 4096 keys 10.1, over 16384
-// 15.3; 8 pairs of 4 rows over 32768, D 128, 30) and 64 splits, but where the pairs alone take
-// more than half of the CUs into about 512.
+// 15.3; 8 pairs of 4 rows over 32768, D 128, 30) and 64 splits.  Workgroups for more than half of the
+// CUs are cut in three where that fills two a CU (D 128: 160 of one token over 8192 to 16384 keys 164
+// against 184 whole and 175 in four, 144 of two blocks over 6000 33.6, 39.5 and 39.7), else left whole
+// (192 over 4096 to 8192 105 against 112 in two and 115 in three, 240 of two blocks over 6000 40 and 42).
 Walk walk_for(int64_t pairs, int rows, int keys, bool even, int dim) {
   constexpr int kCus = 256;
   const int64_t tiles = ceil_div(keys, kTile), ones = pairs * ceil_div(rows, 16), twos = pairs * ceil_div(rows, 32);
@@ -727,8 +729,8 @@ Walk walk_for(int64_t pairs, int rows, int keys, bool even, int dim) {
     return {kShared, 1};
   }
   const int64_t wgs = pairs * ceil_div(rows, 16 * w.blocks);
-  if (tiles > (dim == 64 ? 24 : 16))
-    w.splits = int(wgs > 128 && tiles >= 64 ? ceil_div(512, wgs) : std::max<int64_t>(1, std::min<int64_t>({256 / wgs, tiles / 4, 64})));
+  if (wgs > kCus / 2) w.splits = tiles >= 64 && 3 * wgs <= 2 * kCus ? 3 : 1;
+  else if (tiles > (dim == 64 ? 24 : 16)) w.splits = int(std::max<int64_t>(1, std::min<int64_t>({kCus / wgs, tiles / 4, 64})));
   return w;
 }
 
