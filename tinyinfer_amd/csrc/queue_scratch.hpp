@@ -1,5 +1,5 @@
 // Scratch for kernels that finish their own split work inside one launch
-// (split-K GEMMs, split-key decode attention) without any allocation: static
+// (split-K GEMMs, split-key decode attention, log probabilities of few rows) without any allocation: static
 // device arrays, one slot per hardware queue.
 //
 // Why per queue: HIP enqueues every kernel dispatch with the AQL barrier bit
