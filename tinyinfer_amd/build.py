@@ -5,6 +5,7 @@ Outputs, next to this file:
   libtinyinfer_llm.so         GPT-2 runtime C ABI (include/tinyinfer_llm.h)
   libtinyinfer_host_codec.so  host INT8 codec (include/tinyinfer_host_codec.h)
   ikernels<ext>               pybind11 module, next to libtinyinfer_backend.so
+  _operands<ext>              NativeOps' checks of torch tensors (no GPU code)
 Usage: python -m tinyinfer_amd.build  (or __graft_entry__.build()).
 """
 from __future__ import annotations
@@ -64,6 +65,22 @@ def _link(target: Path, objs: list[Path], extra: list[str]) -> None:
     os.replace(tmp, target)
 
 
+def _operands() -> None:
+    """The extension over torch's C++ interface, for the torch that is installed; NativeOps
+    is what needs both."""
+    try:
+        import torch
+    except ImportError:
+        return
+    from torch.utils.cpp_extension import include_paths, library_paths
+    target = PKG / ("_operands" + sysconfig.get_config_var("EXT_SUFFIX"))
+    tmp = target.with_suffix(".so.tmp")
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+          *(f"-I{path}" for path in include_paths()), "-I", sysconfig.get_paths()["include"], str(CSRC / "operands.cpp"),
+          "-o", str(tmp), *(f"-L{path}" for path in library_paths()), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"])
+    os.replace(tmp, target)
+
+
 def ikernels_name() -> str:
     return "ikernels" + sysconfig.get_config_var("EXT_SUFFIX")
 
@@ -75,8 +92,10 @@ def build(verbose: bool = True) -> None:
         hip_jobs = {s: pool.submit(_hip_obj, s) for s in hip_sources}
         cpu_job = pool.submit(_host_obj, "cpu_ops.cpp", ["-fopenmp"])
         codec_job = pool.submit(_host_obj, "host_codec.cpp")
+        operands_job = pool.submit(_operands)
         objs = {s: j.result() for s, j in hip_jobs.items()}
         cpu_obj, codec_obj = cpu_job.result(), codec_job.result()
+        operands_job.result()
 
     rpath = ["-Wl,-rpath,$ORIGIN"]
     _link(PKG / "libtinyinfer_backend.so", [objs[s] for s in BACKEND_HIP] + [cpu_obj],

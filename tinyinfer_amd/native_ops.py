@@ -102,35 +102,38 @@ class _Call:
     pointers appended in the ABI's argument order.
 
     A small call's time is this Python code (a GEMV runs 5 us on the GPU), so an
-    operand that passes every check is accepted by one condition and only a
-    refused one goes through the ordered checks that name the reason; outputs
+    operand that passes every check is accepted by one native call (csrc/operands.cpp)
+    and only a refused one goes through the ordered checks that name the reason; outputs
     come from the calling stream's own pool and need no record_stream; the
     device is switched only when it is not current.  ``gemm_int8`` at M = 1,
-    768 -> 2304, call after call: 15.6 -> 11.7 us."""
+    768 -> 2304, call after call: 15.6 us with every check in turn, 7.4 now."""
 
-    __slots__ = ("ops", "symbol", "args", "held", "made", "device", "index", "over", "turned")
+    __slots__ = ("ops", "symbol", "args", "held", "made", "like", "index", "over", "turned")
 
     def __init__(self, ops, symbol):
         self.ops, self.symbol = ops, symbol
         self.args = []
         self.held, self.made = [], []   # the caller's tensors, and this call's own
-        self.device = self.index = None
+        self.like = None                # a tensor where the call's operands are
+        self.index = -2                 # its GPU; -2: none yet
         self.over = None                # the cache it works on
         self.turned = None              # the rotary positions it turns rows by
 
+    @property
+    def device(self):
+        return None if self.like is None else self.like.device
+
     def operand(self, x, dtype, name, rank=None, shape=None):
-        tensor = self.ops.tensor_type
         # (At most INT32_MAX elements: then every extent and the byte count fit.)
-        if not ((type(x) is tensor or isinstance(x, tensor)) and x.dtype == dtype
-                and x.is_contiguous() and not x.requires_grad and 0 < x.numel() <= INT32_MAX
-                and (x.shape == shape if shape is not None else x.dim() == rank if rank is not None else x.dim())
-                and x.is_cuda and (self.index is None or x.get_device() == self.index)):
+        at = self.ops.operands.operand(x, dtype, self.index, -1 if rank is None else rank, shape)
+        if at is None:
             self._checked(x, dtype, name, rank, shape)
-        if self.index is None:
-            self.device = x.device
+            at = x.data_ptr()
+        if self.like is None:
+            self.like = x
             self.index = x.get_device()
         self.held.append(x)
-        self.args.append(x.data_ptr())
+        self.args.append(at)
         return x
 
     def _checked(self, x, dtype, name, rank, shape, strided=False):
@@ -171,38 +174,25 @@ class _Call:
         are contiguous, a slice of a projection for one: pointer and three strides.
         Returns its shape."""
         half = self.ops.torch.float16
-        if not isinstance(x, self.ops.tensor_type):
+        at = self.ops.operands.rows(x, half, self.index, shape)
+        if at is None:
             self._checked(x, half, name, 4, shape, strided=True)
-        extents, strides = x.shape, x.stride()
-        if not (x.dtype == half and len(extents) == 4 and (strides[3] == 1 or extents[3] == 1) and not x.requires_grad
-                and 0 < x.numel() <= INT32_MAX and (shape is None or extents == shape) and x.is_cuda
-                and (self.index is None or x.get_device() == self.index)):
-            self._checked(x, half, name, 4, shape, strided=True)
-        if self.index is None:
-            self.device = x.device
+            at = (x.data_ptr(), *x.stride()[:3])
+        if self.like is None:
+            self.like = x
             self.index = x.get_device()
         self.held.append(x)
-        self.args += (x.data_ptr(), *strides[:3])
-        return extents
+        self.args += at
+        return x.shape
 
     def output(self, shape, dtype):
-        # (torch.empty takes 0.8 us more.)
-        if len(shape) == 1:
-            strides = (1,)
-        elif len(shape) == 2:
-            strides = (shape[1], 1)
-        else:
-            strides = [1]
-            for extent in shape[:0:-1]:
-                strides.insert(0, extent * strides[0])
-        y = self.ops.torch.empty_strided(shape, strides, dtype=dtype, device=self.device)
+        y = self.ops.operands.empty_as(shape, dtype, self.like)
         self.made.append(y)
         self.args.append(y.data_ptr())
         return y
 
-    def output_like(self, x, strided=False):
-        torch = self.ops.torch
-        y = torch.empty_like(x, memory_format=torch.contiguous_format) if strided else torch.empty_like(x)
+    def output_like(self, x):
+        y = self.ops.operands.empty(x.shape, x)
         self.made.append(y)
         self.args.append(y.data_ptr())
         return y
@@ -235,7 +225,7 @@ class _Call:
         if type(cache) is not (kind or Int8KVCache):
             raise TypeError("cache: an Int8KVCache (NativeOps.kv_cache_int8) is required" if kind is None else
                             "cache: a PagedKVCache (NativeOps.kv_cache_paged) is required")
-        self.device = cache.buffer.device
+        self.like = cache.buffer
         self.index = cache.buffer.get_device()
         self.over = cache
         self.args.append(cache._at)
@@ -254,7 +244,7 @@ class _Call:
         if rotary is None:
             self.args.extend((None, 0, 0, 1.0))
             return
-        if self.index is not None and rotary.turns.get_device() != self.index:
+        if rotary.turns.get_device() != self.index:
             raise ValueError(f"rotary: on {rotary.turns.device}, the call's operands are on {self.device}")
         self.turned = rotary
         self.args.extend((rotary._at, rotary.rotated, int(rotary.interleaved), rotary.amplitude))
@@ -286,20 +276,19 @@ class _Call:
     def run(self):
         ops, index = self.ops, self.index
         cuda = ops.torch.cuda
-        # (The current stream's handle costs a tenth of making its Stream object, which
+        # (The current stream's handle costs a tenth of making its Stream object, whose number
         # record_stream wants and which stays the same for a handle.)
         handle = ops.stream_handle(index)
         stream = ops.streams.get((index, handle))
         if stream is None:
-            stream = ops.streams[index, handle] = cuda.current_stream(index)
-        for x in self.held:
-            x.record_stream(stream)
+            stream = ops.streams[index, handle] = cuda.current_stream(index).stream_id
+        ops.operands.record(self.held, stream, index)
         # (The allocator keeps a stream with a block until the block is freed: once does.)
         if self.over is not None and handle not in self.over._streams:
-            self.over.buffer.record_stream(stream)
+            ops.operands.record([self.over.buffer], stream, index)
             self.over._streams.add(handle)
         if self.turned is not None and handle not in self.turned._streams:
-            self.turned.turns.record_stream(stream)
+            ops.operands.record([self.turned.turns], stream, index)
             self.turned._streams.add(handle)
         if ops.current_device() == index:
             status = getattr(ops.lib, self.symbol)(*self.args, handle, index)
@@ -417,7 +406,11 @@ class NativeOps:
 
     def __init__(self, library_path=None):
         import torch
-        self.torch, self.tensor_type = torch, torch.Tensor
+        try:
+            from . import _operands  # (after torch, whose libraries it uses)
+        except ImportError as e:
+            raise ImportError(f"tinyinfer_amd._operands is not built for this torch ({e}): python -m tinyinfer_amd.build") from e
+        self.torch, self.tensor_type, self.operands = torch, torch.Tensor, _operands
         # torch's own short ways to both (operands are on a GPU: it is initialised), which
         # are not part of its interface and missing in a torch without GPU support.
         self.stream_handle = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
@@ -848,7 +841,7 @@ class NativeOps:
             raise ValueError("x: batch and heads must be at most 65535, rows * dims at most 2^31")
         if positions is None:
             raise ValueError("positions are required")
-        y = call.output_like(x, strided=True)
+        y = call.output_like(x)
         each = isinstance(positions, self.tensor_type) and positions.dim() == 2
         if each:
             call.operand(positions, self.torch.int32, "positions", shape=(batch, rows))
@@ -910,7 +903,7 @@ class NativeOps:
             q_shape = q_batch, q_heads, q_rows, q_dim = call.rows(q, "q", None)
             if q_batch != batch or q_rows != rows or q_dim != dim or q_heads > 65535:
                 raise ValueError(f"q must be [{batch}, H, {rows}, {dim}] with H at most 65535, got {list(q_shape)}")
-            turned = call.output_like(q, strided=True)
+            turned = call.output_like(q)
         self._paged_rows(call, cache, page_table, positions, lengths, batch, rows)
         call.turn(rotary)
         call.scalars(batch, q_heads, rows)
