@@ -25,7 +25,10 @@ bool has_shape(const at::Tensor& t, PyObject* shape) {
   if (shape == Py_None) return true;
   if (!PyTuple_Check(shape) || PyTuple_GET_SIZE(shape) != t.dim()) return false;
   for (int64_t i = 0; i < t.dim(); ++i)
-    if (PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i)) != t.size(i)) return false;
+    if (PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i)) != t.size(i)) {
+      PyErr_Clear();  // (an extent that is no number is another shape)
+      return false;
+    }
   return true;
 }
 
