@@ -1,0 +1,106 @@
+"""GPU tests of attention over the paged fp16 KV cache at extents that reach every way its rows
+and keys are walked, with scores that stress the running reference of the exponents.
+
+The formula and its tolerance are those of test_paged_attention_gpu.py.  Where scores are so far
+apart that a row's weights are 1 or 0, its answer is one key's values, or the mean of a few: a
+weight w cancels but for the fp32 roundings of its sum, its reciprocal and their product (2^-22 of
+the values' sizes at most), less than half a step of fp16, so one key's values come back as they
+are and the mean of two is off by half a step, 2^-11, and 2^-21 of the sizes."""
+import numpy as np
+import pytest
+
+from test_paged_attention_gpu import dev, say, torch
+
+pytestmark = pytest.mark.gpu
+
+# (batch, kv_heads, group, dim, page, q_rows, keys): blocks of 16 rows whole, cut in parts and in three;
+# two blocks whole, cut in parts and in three; tiles shared by 128 rows; and with the last row blocks of
+# a pair, one or two of them, by waves of two.
+WALKS = {
+    "one 64": (2, 3, 1, 64, 32, 1, 200), "one 128": (2, 3, 1, 128, 32, 5, 200),
+    "one cut 64": (1, 2, 4, 64, 64, 1, 4000), "one cut 128": (1, 2, 4, 128, 64, 2, 2100),
+    "one in three 128": (12, 11, 1, 128, 64, 1, 4100), "one in three 64": (12, 11, 2, 64, 64, 1, 4100),
+    "two 64": (13, 10, 1, 64, 64, 32, 1300), "two 128": (13, 10, 4, 128, 32, 8, 300),
+    "two cut 64": (1, 2, 16, 64, 128, 19, 9100), "two cut 128": (2, 1, 16, 128, 128, 19, 13500),
+    "two in three 64": (9, 4, 4, 64, 64, 25, 4200), "two in three 128": (9, 4, 4, 128, 64, 25, 4200),
+    "shared 64": (8, 16, 1, 64, 64, 512, 640), "shared 128": (8, 16, 1, 128, 64, 512, 640),
+    "mixed 64": (4, 4, 8, 64, 32, 257, 600), "mixed 128": (4, 4, 8, 128, 32, 257, 600),
+    "two mixed 64": (4, 4, 8, 64, 64, 288, 1100), "two mixed 128": (4, 4, 8, 128, 64, 288, 1100)}
+walks = pytest.mark.parametrize("walk", WALKS)
+
+
+def filled(ops, rng, batch, kv_heads, dim, page, n):
+    """A cache with n tokens of every request, its table and the contents [B, G, n, D]: of one row of
+    tokens a head, those from another place on for every request."""
+    width = -(-n // page)
+    table = rng.permutation(batch * width + 2)[:batch * width].reshape(batch, width).astype(np.int32)
+    cache = ops.kv_cache_paged(batch * width + 2, kv_heads, page, dim)
+    k, v = (np.stack([x[:, b:b + n] for b in range(batch)])
+            for x in rng.standard_normal((2, kv_heads, n + batch, dim), np.float32).astype(np.float16))
+    ops.kv_append_paged(cache, dev(k), dev(v), dev(table), 0)
+    return cache, table, k, v
+
+
+@walks
+def test_scores_of_any_size(ops, walk):
+    """Scores from thousands to 5e10: one key, two equal ones, rising ones, two that are near."""
+    t = torch()
+    batch, kv_heads, group, dim, page, q_rows, n = WALKS[walk]
+    say("scores", walk)
+    rng = np.random.default_rng(8)
+    cache, table, _, v = filled(ops, rng, batch, kv_heads, dim, page, n)
+    table, v = dev(table), dev(v)
+    signs = rng.choice([-1.0, 1.0], dim)
+    # Whole numbers of at most 7 bits times a power of two: products and sums of these are exact in fp32.
+    rows = rng.integers(64, 128, (batch, kv_heads * group, q_rows, 1)) * signs
+
+    def answers(keys, scale):
+        """keys [n]: signs * keys, times scale, as queries are."""
+        k = t.from_numpy((keys[:, None] * signs * scale).astype(np.float16)).cuda().expand(batch, kv_heads, n, dim)
+        ops.kv_append_paged(cache, k, v, table, 0)
+        return ops.attention_paged(dev((rows * scale).astype(np.float16)), cache, table, n, causal=False)
+
+    def values(at):
+        return v[:, :, at].repeat_interleave(group, 1)[:, :, None]
+
+    first, second = n // 5, n - 1 - n // 7
+    for power in range(-2, 10):  # scores x = sqrt(dim) log2(e) 2^(12 + 2 power) and up
+        scale, below = 2.0 ** power, np.full(n, -64.0)
+        keys = below.copy()
+        keys[first] = 100
+        assert t.equal(answers(keys, scale), values(first).expand(-1, -1, q_rows, -1)), (power, "one")
+        keys[second] = 100
+        y, a, b = answers(keys, scale).double(), values(first).double(), values(second).double()
+        off, tol = (y - (a + b) / 2).abs(), 2.0 ** -11 * ((a + b) / 2).abs() + 2.0 ** -21 * (a.abs() + b.abs()) + 2.0 ** -25
+        assert (off <= tol).all(), (power, "two", off.max().item())
+        rising = np.floor(np.linspace(-127, 126, n))
+        rising[-1] = 127
+        for keys, at in ((rising, n - 1), (rising[::-1], 0)):
+            assert t.equal(answers(keys, scale), values(at).expand(-1, -1, q_rows, -1)), (power, "rising")
+
+
+@walks
+def test_far_scores_that_are_near_each_other(ops, walk):
+    """Two keys in different tiles with scores of 1e7 to 1e9 that differ by a few units: weights are what
+    fp32 scores make of them, and answers lie between the two keys' values."""
+    t = torch()
+    batch, kv_heads, group, dim, page, q_rows, n = WALKS[walk]
+    say("near", walk)
+    rng = np.random.default_rng(9)
+    cache, table, _, v = filled(ops, rng, batch, kv_heads, dim, page, n)
+    table, v = dev(table), dev(v)
+    first, second = n // 5, n - 1 - n // 7
+    low, high = (f(v[:, :, first], v[:, :, second]).float().repeat_interleave(group, 1)[:, :, None]
+                 for f in (t.minimum, t.maximum))
+    slack = 2.0 ** -10 * t.maximum(low.abs(), high.abs()) + 2.0 ** -24
+    q = np.zeros((batch, kv_heads * group, q_rows, dim), np.float16)
+    q[..., 0] = 16384 + 16 * rng.integers(0, 512, q.shape[:3])
+    q[..., 1] = rng.integers(1, 9, q.shape[:3])
+    for big in (4096, 16384, 50000):
+        for step in (1, 4, 16, 64):
+            for at, other in ((first, second), (second, first)):
+                k = np.zeros((n, dim), np.float16)
+                k[:, 0], k[[at, other], 0], k[other, 1] = -big, big, step
+                ops.kv_append_paged(cache, dev(k).expand(batch, kv_heads, n, dim), v, table, 0)
+                y = ops.attention_paged(dev(q), cache, table, n, causal=False).float()
+                assert ((y >= low - slack) & (y <= high + slack)).all(), (big, step, at)

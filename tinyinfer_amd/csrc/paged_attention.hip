@@ -51,9 +51,13 @@ namespace {
 constexpr int kTile = 64;   // keys per wave and step
 constexpr float kNegInf = -__builtin_huge_valf();
 // The reference of a row's exponents: 6 below its largest x when set, raised when one is
-// 14 above it.  Weights then lie around 2^6 and below 2^14: rounded to fp16, whose smallest
-// normal number is 2^-14, a weight 2^-20 times the heaviest still keeps 11 bits.
-constexpr float kBelow = 6.f, kRaise = 14.f;
+// more than 14 above it.  Weights then lie around 2^6 and below 2^15: rounded to fp16, whose
+// smallest normal number is 2^-14, a weight 2^-20 times the heaviest still keeps 11 bits.
+// A weight's exponent is one fused multiply-add of a score and the reference, which was set from
+// a rounded product: the two are apart by up to 1.5 half steps of x, a factor that all weights
+// share and that cancels, but not out of fp16's range.  From a reference of 2^22 on, steps of
+// half a unit, it is the rounded product less the reference: a number of at most 14, exactly.
+constexpr float kBelow = 6.f, kRaise = 14.f, kFar = 4194304.f;
 
 struct AttnPlan {
   PagedAttnArgs a;
@@ -69,6 +73,7 @@ struct AttnPlan {
 };
 
 typedef unsigned short u16x8_t __attribute__((ext_vector_type(8)));
+typedef unsigned long long u64;
 
 typedef __attribute__((address_space(1))) void* global_ptr;
 typedef __attribute__((address_space(3))) void* lds_ptr;
@@ -106,6 +111,13 @@ __device__ __forceinline__ half4_t output_of(float4_t o, float total, float inv)
   return half4_t{f16r(x[0]), f16r(x[1]), f16r(x[2]), f16r(x[3])};
 }
 
+// x y, rounded: a difference behind it is not made one operation with it.
+__device__ __forceinline__ float rounded_product(float x, float y) {
+  float z = x * y;
+  asm("" : "+v"(z));
+  return z;
+}
+
 // A wave's rows, QB blocks of 16, lane (j, g) holding its part of row j of each: what they
 // ask, see and have summed up.
 template <int D, int QB>
@@ -127,6 +139,7 @@ struct Rows {
   float m[QB];
   float4_t l[QB];  // FINE: [0] is this lane's part of the sum; else all are the row's sum
   float4_t acc[QB][PER];
+  u64 far[QB];     // which lanes' references are far from 0 (the same in all of them)
   unsigned spoilt[QB];  // bit 4 d + e: the sum acc[u][d][e] is over an infinity or NaN that is not in it
   half8_t pp[QB][2], rest[2];
 
@@ -174,6 +187,7 @@ struct Rows {
       const float start = __ballot(any_not_finite(top)) >> j & 0x0001000100010001u ? __builtin_nanf("") : 0.f;
       l[u] = float4_t{start, start, start, start};
       m[u] = kNegInf;
+      far[u] = 0;
       spoilt[u] = 0;
 #pragma unroll
       for (int d = 0; d < PER; ++d) acc[u][d] = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -196,7 +210,8 @@ struct Rows {
       for (int c = 0; c < D / 32; ++c) sc[u][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key(kb, c), qf[u][c], sc[u][kb], 0, 0, 0);
     }
   }
-  // Masks the scores of block u and raises its reference where it must be.
+  // Masks the scores of block u and raises its reference where it must be.  (Scores far from 0 are
+  // scaled here.)
   __device__ __forceinline__ void refer(int u, float4_t (&sc)[QB][4], int t, bool held0, bool held1) {
     if (!full(t, held0, held1)) {
 #pragma unroll
@@ -209,26 +224,34 @@ struct Rows {
     for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
       for (int v = 0; v < 4; ++v) high = fmaxf(high, sc[u][kb][v]);
-    high *= p.scale;
-    if (__ballot(high > m[u] + kRaise)) {
+    high = rounded_product(high, p.scale);
+    if (__ballot(high - m[u] > kRaise)) {  // (not against m + 14, which would be rounded)
       high = fmaxf(high, __shfl_xor(high, 16, 64));
       high = fmaxf(high, __shfl_xor(high, 32, 64));
-      const float nm = high > m[u] + kRaise ? high - kBelow : m[u];
+      const float nm = high - m[u] > kRaise ? high - kBelow : m[u];
       const float f = m[u] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[u] - nm);
       l[u] *= f;
 #pragma unroll
       for (int d = 0; d < PER; ++d) acc[u][d] *= f;
       m[u] = nm;
+      far[u] = __ballot(fabsf(nm) >= kFar && fabsf(nm) < -kNegInf);
+    }
+    if (far[u]) {
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) sc[u][kb][v] = rounded_product(sc[u][kb][v], p.scale);
     }
   }
   // Its weights.
   __device__ __forceinline__ void weigh(int u, const float4_t (&sc)[QB][4]) {
     const float ref = m[u] == kNegInf ? 0.f : -m[u];  // -inf while every key so far is masked
+    const float scale = far[u] ? 1.f : p.scale;
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        const float w = __builtin_amdgcn_exp2f(fmaf(sc[u][kb][v], p.scale, ref));
+        const float w = __builtin_amdgcn_exp2f(fmaf(sc[u][kb][v], scale, ref));
         pp[u][kb >> 1][4 * (kb & 1) + v] = f16(w);
         if constexpr (FINE) {
           l[u][0] += w;
