@@ -211,7 +211,7 @@ struct Rows {
     }
   }
   // Masks the scores of block u and raises its reference where it must be.  (Scores far from 0 are
-  // scaled here.)
+  // scaled here; one branch for both, taken rarely.)
   __device__ __forceinline__ void refer(int u, float4_t (&sc)[QB][4], int t, bool held0, bool held1) {
     if (!full(t, held0, held1)) {
 #pragma unroll
@@ -224,8 +224,8 @@ struct Rows {
     for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
       for (int v = 0; v < 4; ++v) high = fmaxf(high, sc[u][kb][v]);
-    high = rounded_product(high, p.scale);
-    if (__ballot(high - m[u] > kRaise)) {  // (not against m + 14, which would be rounded)
+    if (__builtin_expect((__ballot(fmaf(high, p.scale, -m[u]) > kRaise) | far[u]) != 0, 0)) {
+      high = rounded_product(high, p.scale);
       high = fmaxf(high, __shfl_xor(high, 16, 64));
       high = fmaxf(high, __shfl_xor(high, 32, 64));
       const float nm = high - m[u] > kRaise ? high - kBelow : m[u];
@@ -235,12 +235,12 @@ struct Rows {
       for (int d = 0; d < PER; ++d) acc[u][d] *= f;
       m[u] = nm;
       far[u] = __ballot(fabsf(nm) >= kFar && fabsf(nm) < -kNegInf);
-    }
-    if (far[u]) {
+      if (far[u]) {
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb)
+        for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) sc[u][kb][v] = rounded_product(sc[u][kb][v], p.scale);
+          for (int v = 0; v < 4; ++v) sc[u][kb][v] = rounded_product(sc[u][kb][v], p.scale);
+      }
     }
   }
   // Its weights.
