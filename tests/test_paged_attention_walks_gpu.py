@@ -9,12 +9,12 @@ are and the mean of two is off by half a step, 2^-11, and 2^-21 of the sizes."""
 import numpy as np
 import pytest
 
-from test_paged_attention_gpu import dev, say, torch
+from test_paged_attention_gpu import attend, dev, host, i32, say, seen_by, torch
 
 pytestmark = pytest.mark.gpu
 
 # (batch, kv_heads, group, dim, page, q_rows, keys): blocks of 16 rows whole, cut in parts and in three;
-# two blocks whole, cut in parts and in three; tiles shared by 128 rows; and with the last row blocks of
+# two blocks whole, cut in parts and in three; tiles shared by 128 rows; and with the first row blocks of
 # a pair, one or two of them, by waves of two.
 WALKS = {
     "one 64": (2, 3, 1, 64, 32, 1, 200), "one 128": (2, 3, 1, 128, 32, 5, 200),
@@ -39,6 +39,70 @@ def filled(ops, rng, batch, kv_heads, dim, page, n):
             for x in rng.standard_normal((2, kv_heads, n + batch, dim), np.float32).astype(np.float16))
     ops.kv_append_paged(cache, dev(k), dev(v), dev(table), 0)
     return cache, table, k, v
+
+
+def check_some(y, q, k, v, kv, ql, causal, batches=None):
+    """Some heads of some requests against the formula."""
+    batch, heads, q_rows, _ = q.shape
+    group, n = heads // k.shape[1], k.shape[2]
+    for b in batches or sorted({0, batch - 1}):
+        for h in sorted({0, heads - 1}):
+            sees = np.arange(n)[None] < np.array(seen_by(q_rows, kv[b], ql[b], None, causal))[:, None]
+            want, tol = attend(q[b, h], k[b, h // group], v[b, h // group], sees)
+            bad = ~(np.abs(y[b, h] - want) <= tol)
+            assert not bad.any(), (b, h, np.argwhere(bad)[0].tolist(), y[b, h][bad][0], want[bad][0], tol[bad][0])
+
+
+@walks
+def test_ragged_lengths(ops, walk):
+    """Full and short requests and one without a key, causal and not; equal calls give equal bits."""
+    batch, kv_heads, group, dim, page, q_rows, n = WALKS[walk]
+    say("ragged", walk)
+    rng = np.random.default_rng(n + dim)
+    cache, table, k, v = filled(ops, rng, batch, kv_heads, dim, page, n)
+    q = (rng.standard_normal((batch, kv_heads * group, q_rows, dim)) * 1.5).astype(np.float16)
+    kv = rng.integers(1, n + 1, batch)
+    kv[-1], kv[batch // 3], ql = 65, 0, np.maximum(rng.integers(q_rows // 2, q_rows + 1, batch), 1)
+    kv[0], ql[0] = n, q_rows
+    for causal in (False, True):
+        x = dev(q), cache, dev(table), i32(kv)
+        y = ops.attention_paged(*x, q_lengths=i32(ql), causal=causal)
+        for _ in range(3):
+            assert torch().equal(ops.attention_paged(*x, q_lengths=i32(ql), causal=causal), y)
+        check_some(host(y), q, k, v, kv, ql, causal, sorted({0, batch // 3, batch - 1}))
+
+
+@walks
+def test_scores_that_rise_and_fall(ops, walk):
+    """The running reference is raised tile by tile, or never again."""
+    batch, kv_heads, group, dim, page, q_rows, n = WALKS[walk]
+    say("rising", walk)
+    rng = np.random.default_rng(7)
+    cache, table, k, v = filled(ops, rng, batch, kv_heads, dim, page, n)
+    q = np.abs(rng.standard_normal((batch, kv_heads * group, q_rows, dim))).astype(np.float16)
+    k = (np.abs(k) * np.linspace(-3, 3, n)[None, None, :, None]).astype(np.float16)
+    for kk in (k, k[:, :, ::-1].copy()):
+        ops.kv_append_paged(cache, dev(kk), dev(v), dev(table), 0)
+        y = host(ops.attention_paged(dev(q), cache, dev(table), n, causal=False))
+        check_some(y, q, kk, v, [n] * batch, [q_rows] * batch, False)
+
+
+@walks
+def test_values_of_any_size(ops, walk):
+    """The largest values have a finite result; scores far apart pick one key; the smallest survive."""
+    batch, kv_heads, group, dim, page, q_rows, n = WALKS[walk]
+    say("sizes", walk)
+    rng = np.random.default_rng(6)
+    cache, table, k, v = filled(ops, rng, batch, kv_heads, dim, page, n)
+    q = rng.standard_normal((batch, kv_heads * group, q_rows, dim)).astype(np.float16)
+    for size, far in ((65504.0, 1), (1.0, 40), (2.0 ** -14, 1)):
+        vv = v * np.float16(size) if size < 2 else (size * rng.choice([-1, 1], (batch, kv_heads, 1, dim))).astype(np.float16)
+        vv = np.broadcast_to(vv, v.shape).copy()
+        kk, qq = k * np.float16(far), q * np.float16(far)
+        ops.kv_append_paged(cache, dev(kk), dev(vv), dev(table), 0)
+        y = host(ops.attention_paged(dev(qq), cache, dev(table), n, causal=False))
+        assert np.isfinite(y).all(), size
+        check_some(y, qq, kk, vv, [n] * batch, [q_rows] * batch, False)
 
 
 @walks
