@@ -14,8 +14,8 @@ from test_paged_attention_gpu import attend, dev, host, i32, say, seen_by, torch
 pytestmark = pytest.mark.gpu
 
 # (batch, kv_heads, group, dim, page, q_rows, keys): blocks of 16 rows whole, cut in parts and in three;
-# two blocks whole, cut in parts and in three; tiles shared by 128 rows; and with the first row blocks of
-# a pair, one or two of them, by waves of two.
+# two blocks whole, cut in parts and in three; tiles shared by 128 rows;
+# and with the first row blocks of a pair, one or two of them, by waves of two.
 WALKS = {
     "one 64": (2, 3, 1, 64, 32, 1, 200), "one 128": (2, 3, 1, 128, 32, 5, 200),
     "one cut 64": (1, 2, 4, 64, 64, 1, 4000), "one cut 128": (1, 2, 4, 128, 64, 2, 2100),
@@ -25,7 +25,8 @@ WALKS = {
     "two in three 64": (9, 4, 4, 64, 64, 25, 4200), "two in three 128": (9, 4, 4, 128, 64, 25, 4200),
     "shared 64": (8, 16, 1, 64, 64, 512, 640), "shared 128": (8, 16, 1, 128, 64, 512, 640),
     "mixed 64": (4, 4, 8, 64, 32, 257, 600), "mixed 128": (4, 4, 8, 128, 32, 257, 600),
-    "two mixed 64": (4, 4, 8, 64, 64, 288, 1100), "two mixed 128": (4, 4, 8, 128, 64, 288, 1100)}
+    "two mixed 64": (4, 4, 8, 64, 64, 288, 1100), "two mixed 128": (4, 4, 8, 128, 64, 288, 1100),
+    "ragged mixed 64": (5, 8, 1, 64, 64, 900, 1100), "ragged mixed 128": (5, 8, 1, 128, 64, 900, 1100)}
 walks = pytest.mark.parametrize("walk", WALKS)
 
 

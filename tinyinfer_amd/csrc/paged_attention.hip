@@ -725,6 +725,11 @@ struct Walk {
 // few pairs of many keys, more (D 128: 16 pairs of 2048 rows over 4096 keys 84 against 91, 128 of 256 91
 // and 162, 16 of 1536 81 and 71; D 64: 16 of 1536 over 512 12.5 and 14.2, over 4096 55 and 43, 256
 // of 128 over 4096 59 and 151).
+// Blocks are those that are launched, a pair's last one as long as a full one however few rows it has
+// (D 64: 75 pairs of 269 rows, 225 blocks, over 269 keys 12.2 against 18.7; 250 of 66 over 2558 44 and 75;
+// D 128: 144 of 200 over 320 19.7 and 22.2; 40 of 900, 320 blocks, over 4096 keys 95 mixed, 112 shared), but of
+// pairs with 64 rows and fewer, half a block at most, the part of it that they fill (D 64: 192 of 32 over
+// 1024 20 and 13.8, 384 of 40 27 and 32).
 // Mixed: a CU works on two blocks in 1.35 times one's time, so a few more blocks than CUs, or than
 // a multiple of them, cost nearly a round.  Up to half a round is done by waves of two blocks
 // instead, four workgroups to 128 rows, which spread over all CUs (D 128, 4096 keys, blocks: 288
@@ -741,10 +746,10 @@ struct Walk {
 // (192 over 4096 to 8192 105 against 112 in two and 115 in three, 240 of two blocks over 6000 40 and 42).
 Walk walk_for(int64_t pairs, int rows, int keys, bool even, int dim) {
   constexpr int kCus = 256;
-  const int64_t tiles = ceil_div(keys, kTile), ones = pairs * ceil_div(rows, 16), twos = pairs * ceil_div(rows, 32);
+  const int64_t tiles = ceil_div(keys, kTile), ones = pairs * ceil_div(rows, 16);
   Walk w{1, 1};
   if (rows > 16 && (dim == 64 ? ones * tiles > 5000 : ones > 256 || ones * tiles > 8000)) w.blocks = 2;
-  const int64_t shared = ceil_div(twos, kSharers);
+  const int64_t shared = rows > 64 ? pairs * ceil_div(rows, 32 * kSharers) : ceil_div(pairs * ceil_div(rows, 32), kSharers);
   if (w.blocks == 2 && shared >= (dim == 128 ? 240 : tiles >= 32 && pairs < 128 ? kCus + 1 : 192)) {
     const int64_t more = shared % kCus, tail = ceil_div(more, pairs);
     if (even && more > 0 && shared > kCus && shared < 9 * kCus && pairs * tail <= (tiles >= 16 ? kCus / 2 : kCus / 4))
