@@ -14,7 +14,7 @@ from test_paged_attention_gpu import attend, dev, host, i32, say, seen_by, torch
 pytestmark = pytest.mark.gpu
 
 # (batch, kv_heads, group, dim, page, q_rows, keys): blocks of 16 rows whole, cut in parts and in three;
-# two blocks whole, cut in parts and in three; tiles shared by 128 rows;
+# two blocks whole, cut in parts and in three; tiles shared by 128 rows, of more blocks than CUs and of fewer;
 # and with the first row blocks of a pair, one or two of them, by waves of two.
 WALKS = {
     "one 64": (2, 3, 1, 64, 32, 1, 200), "one 128": (2, 3, 1, 128, 32, 5, 200),
@@ -26,7 +26,8 @@ WALKS = {
     "shared 64": (8, 16, 1, 64, 64, 512, 640), "shared 128": (8, 16, 1, 128, 64, 512, 640),
     "mixed 64": (4, 4, 8, 64, 32, 257, 600), "mixed 128": (4, 4, 8, 128, 32, 257, 600),
     "two mixed 64": (4, 4, 8, 64, 64, 288, 1100), "two mixed 128": (4, 4, 8, 128, 64, 288, 1100),
-    "ragged mixed 64": (5, 8, 1, 64, 64, 900, 1100), "ragged mixed 128": (5, 8, 1, 128, 64, 900, 1100)}
+    "ragged mixed 64": (5, 8, 1, 64, 64, 900, 1100), "ragged mixed 128": (5, 8, 1, 128, 64, 900, 1100),
+    "few shared 64": (3, 16, 1, 64, 64, 450, 640), "few shared 128": (3, 16, 1, 128, 64, 450, 640)}
 walks = pytest.mark.parametrize("walk", WALKS)
 
 

@@ -721,22 +721,28 @@ struct Walk {
 // over 256, 7.3 and 6.9), or at 128 dims, of which a CU holds two, more than one a CU (32 pairs
 // of 400 rows over 256 keys 11.7 and 14.1, 128 of 80 over 4096 87 and 164; 8 of 400 over 1024 12.9
 // and 10.8, 32 of 32 over 4096 21.5 and 19.9).
-// Tiles shared by 128 rows pay where there is about one such block a CU, or, of 64 dims and
-// few pairs of many keys, more (D 128: 16 pairs of 2048 rows over 4096 keys 84 against 91, 128 of 256 91
-// and 162, 16 of 1536 81 and 71; D 64: 16 of 1536 over 512 12.5 and 14.2, over 4096 55 and 43, 256
-// of 128 over 4096 59 and 151).
-// Blocks are those that are launched, a pair's last one as long as a full one however few rows it has
-// (D 64: 75 pairs of 269 rows, 225 blocks, over 269 keys 12.2 against 18.7; 250 of 66 over 2558 44 and 75;
-// D 128: 144 of 200 over 320 19.7 and 22.2; 40 of 900, 320 blocks, over 4096 keys 95 mixed, 112 shared), but of
+// Tiles shared by 128 rows pay from about one such block a CU on: the blocks that are launched, a pair's
+// last one as long as a full one however few rows it has (D 64: 75 pairs of 269 rows, 225 blocks, over 269
+// keys 12.2 against 18.7; 250 of 66 over 2558 44 and 75; D 128: 144 of 200 over 320 19.7 and 22.2), but of
 // pairs with 64 rows and fewer, half a block at most, the part of it that they fill (D 64: 192 of 32 over
 // 1024 20 and 13.8, 384 of 40 27 and 32).
+// From which number on (shared against two blocks).  Short caches or many pairs, whose keys and values
+// waves on their own read more often: 192 (D 128: 24 pairs of 1024 rows over 256 keys 14.7 and 19.6, 16 of
+// 1536 over 512 19.0 and 21.3, 192 of 128 over 1024 30.5 and 47; D 64: 100 of 256 over 256 11.8 and 15.9).
+// Long ones of few pairs: more (D 128: 16 of 1536 over 2048 45.7 and 40.6, of 1792 46.0 and 47.7; D 64: 16
+// of 1536 over 4096 55 and 43, 32 of 1024 61.6 and 53.4, 256 of 128 59 and 151).  And prompts on their own,
+// whose longest block is twice the average: a CU works on more than one at a time, and four waves
+// that share its keys are through with it sooner (D 128: 8 of 4000 over 1000 28.2 and 27.4, 36 of 1000 over 1000 30.2
+// and 35.0, 4 of 8192 over 2048 46.4 and 37.8, 20 of 2048 49.1 and 46.7, 2 of 16384 over 4096 81 and 57, but 24 of
+// 512 over 512 15.7 and 25.8 at D 64; there 24 of 1000 21.8 and 17.7, 9 of 4096 63 and 41.6, 25 of 2048 35.4 and 50).
 // Mixed: a CU works on two blocks in 1.35 times one's time, so a few more blocks than CUs, or than
 // a multiple of them, cost nearly a round.  Up to half a round is done by waves of two blocks
 // instead, four workgroups to 128 rows, which spread over all CUs (D 128, 4096 keys, blocks: 288
 // 89.7 against 113.6 shared, 384 112 and 123, 528 148 and 198, 800 214 and 247, but 448 133 and
-// 130; over 512 keys 320 23 and 27, 384 28.2 and 27.8; D 64: 288 58 and 79, 528 91 and 109, 2080 319 and
-// 324, 3104 479 and 466).  Blocks of uneven rows, a prompt on its own, fill the CUs by themselves (25
-// heads of 64, 4 of 1024 rows: 33 and 27).
+// 130; over 512 keys 320 23 and 27, 384 28.2 and 27.8; 40 pairs of 900 rows, 320 blocks, over 4096 95 and
+// 112; D 64: 288 58 and 79, 528 91 and 109, 2080 319 and 324, 3104 479 and 466; 128 pairs of 270 71 and 81).
+// At D 128 of few pairs alone (100 of 330 over 4096 keys 154 and 117, 64 of 520 95 and 117).  Blocks of
+// uneven rows, a prompt on its own, fill the CUs by themselves (25 heads of 64, 4 of 1024 rows: 33 and 27).
 // Splits: a second launch and the states' traffic cost 2 us and more, and 4 us of the
 // caller's time, so short caches are not split (12 pairs of 1 row over 1024 keys 8.7 us).
 // Longer ones are, into at most one workgroup a CU (12 pairs over 4096 keys 10.1, over 16384
@@ -750,9 +756,14 @@ Walk walk_for(int64_t pairs, int rows, int keys, bool even, int dim) {
   Walk w{1, 1};
   if (rows > 16 && (dim == 64 ? ones * tiles > 5000 : ones > 256 || ones * tiles > 8000)) w.blocks = 2;
   const int64_t shared = rows > 64 ? pairs * ceil_div(rows, 32 * kSharers) : ceil_div(pairs * ceil_div(rows, 32), kSharers);
-  if (w.blocks == 2 && shared >= (dim == 128 ? 240 : tiles >= 32 && pairs < 128 ? kCus + 1 : 192)) {
+  int64_t least = 192;
+  if (!even && tiles >= 16 && pairs <= 64) least = tiles < 32 ? kCus + 1 : 330;
+  else if (dim == 64 && tiles >= 32 && pairs < 128) least = kCus + 1;
+  else if (dim == 128 && tiles >= 16 && pairs <= 64) least = 224;
+  if (w.blocks == 2 && shared >= least) {
     const int64_t more = shared % kCus, tail = ceil_div(more, pairs);
-    if (even && more > 0 && shared > kCus && shared < 9 * kCus && pairs * tail <= (tiles >= 16 ? kCus / 2 : kCus / 4))
+    if (even && (dim == 64 || pairs <= 64) && more > 0 && shared > kCus && shared < 9 * kCus &&
+        pairs * tail <= (tiles >= 16 ? kCus / 2 : kCus / 4))
       return {kMixed, 1, int(tail)};
     return {kShared, 1};
   }
