@@ -337,22 +337,21 @@ struct Rows {
   __device__ __forceinline__ float4_t piece(int u, int v, int c) const {
     return float4_t{acc[u][4 * c][v], acc[u][4 * c + 1][v], acc[u][4 * c + 2][v], acc[u][4 * c + 3][v]};
   }
-  // These of row (u, j), of `total` weight, to the output, or to the state of a split.
-  __device__ __forceinline__ void put(int u, int v, int c, int split, float4_t o, float total) const {
+  // These of row (u, j), of `total` weight, to the output.
+  __device__ __forceinline__ void put(int u, int v, int c, float4_t o, float total) const {
     if (row_id[u] < 0) return;
-    const int dim = PER * (4 * g + v) + 4 * c;
-    if (p.splits > 1) {
-      const int64_t at = int64_t(split) * p.all_rows + row_id[u];
-      if (total != 0.f) *reinterpret_cast<float4_t*>(p.a.workspace + at * D + dim) = o;
-      return;
-    }
     const float inv = total == 0.f ? 0.f : 1.f / total;
     const half4_t y = output_of(o, total, inv);
-    __builtin_memcpy(p.a.out + int64_t(row_id[u]) * D + dim, &y, 8);
+    __builtin_memcpy(p.a.out + int64_t(row_id[u]) * D + PER * (4 * g + v) + 4 * c, &y, 8);
   }
-  // And their exponents' reference.
-  __device__ __forceinline__ void put_weight(int u, int split, float top, float total) const {
-    if (p.splits == 1 || g != 0 || row_id[u] < 0) return;
+  // To the state of a split, and their exponents' reference.
+  __device__ __forceinline__ void keep(int u, int v, int c, int split, float4_t o, float total) const {
+    if (row_id[u] < 0 || total == 0.f) return;
+    const int64_t at = int64_t(split) * p.all_rows + row_id[u];
+    *reinterpret_cast<float4_t*>(p.a.workspace + at * D + PER * (4 * g + v) + 4 * c) = o;
+  }
+  __device__ __forceinline__ void keep_weight(int u, int split, float top, float total) const {
+    if (g != 0 || row_id[u] < 0) return;
     float* ml = p.a.workspace + p.splits * p.all_rows * D + 2 * (int64_t(split) * p.all_rows + row_id[u]);
     ml[0] = top;
     ml[1] = total;
@@ -519,9 +518,10 @@ __device__ __forceinline__ void attend(const AttnPlan& p, uint8_t* lds, int b, i
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = empty[w] ? o[e] : fmaf(x[e], f[w], o[e]);
       }
-      rows.put(u, wave, c, split, o, total);
+      if (p.splits > 1) rows.keep(u, wave, c, split, o, total);
+      else rows.put(u, wave, c, o, total);
     }
-    if (wave == 0) rows.put_weight(u, split, top, total);
+    if (p.splits > 1 && wave == 0) rows.keep_weight(u, split, top, total);
   }
 }
 
@@ -534,16 +534,15 @@ struct Tiles {
   half8_t k[2][4 * D / 32][64], v[2][2 * D / 16][64];
 };
 template <int D>
-__device__ __forceinline__ void attend_shared(const AttnPlan& p, uint8_t* lds, int b, int head, int rb, int split) {
+__device__ __forceinline__ void attend_shared(const AttnPlan& p, uint8_t* lds, int b, int head, int rb) {
   constexpr int QB = 2, PER = D / 16, GROUP = kSharers * 16 * QB, PIECE = D / 32;  // PIECE: records of keys, and of values, that a wave loads
   const int lane = int(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)), half = wave >> 1;
   auto& shared = *reinterpret_cast<Tiles<D>*>(lds);
   Pages<D, 1> pages(p, b, head);
-  if (p.splits == 1) pages.look_up(0);
+  pages.look_up(0);
   Rows<D, QB> rows(p, b, head, rb * GROUP + wave * 16 * QB);
   const int group_last = rows.last_of(rb * GROUP, GROUP), group_first = rows.first_of(rb * GROUP);
-  const int tiles = (group_last + kTile - 1) / kTile, per = (tiles + p.splits - 1) / p.splits, t_end = min(tiles, (split + 1) * per);
-  int t = split * per;
+  const int tiles = (group_last + kTile - 1) / kTile;
 
   // This wave's quarter of a tile's keys or values (records PIECE * wave .. of it, all of them of
   // half `wave / 2`) from their half's block to a buffer.
@@ -564,16 +563,13 @@ __device__ __forceinline__ void attend_shared(const AttnPlan& p, uint8_t* lds, i
     bring(pages.values(block), shared.v[buf]);
     flags |= int(pages.held(tt, 0)) << 2 | int(pages.held(tt, 1)) << 3;
   };
-  if (t < t_end) {
-    if (p.splits > 1) pages.look_up(t);
-    fetch(t, 0);
-  }
+  if (tiles > 0) fetch(0, 0);
   rows.load();
-  for (int buf = 0; t < t_end; ++t, buf ^= 1) {
+  for (int t = 0, buf = 0; t < tiles; ++t, buf ^= 1) {
     flags >>= 2;
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): what this wave has brought
     lds_barrier();                        // everyone's has landed, and nobody reads the other buffer any more
-    if (t + 1 < t_end) {
+    if (t + 1 < tiles) {
       pages.reach(t + 1);
       fetch(t + 1, buf ^ 1);
     }
@@ -619,13 +615,11 @@ __device__ __forceinline__ void attend_shared(const AttnPlan& p, uint8_t* lds, i
   }
   rows.finish();
 #pragma unroll
-  for (int u = 0; u < QB; ++u) {
+  for (int u = 0; u < QB; ++u)
 #pragma unroll
     for (int v = 0; v < 4; ++v)
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) rows.put(u, v, c, split, rows.piece(u, v, c), rows.l[u][0]);
-    rows.put_weight(u, split, rows.m[u], rows.l[u][0]);
-  }
+      for (int c = 0; c < D / 64; ++c) rows.put(u, v, c, rows.piece(u, v, c), rows.l[u][0]);
 }
 
 // Waves per SIMD that the registers are budgeted for.  What the compiler takes: 64 dims, one
@@ -645,12 +639,13 @@ __global__ __launch_bounds__(64 * kWaves, waves_for(D, QB)) void paged_attention
   const int blocks = int(p.row_block_div.d), head = at - b * int(p.heads.d);
   if constexpr (QB == kMixed) {
     const int behind = block - (blocks - p.tail);
-    if (behind < 0) attend_shared<D>(p, lds, b, head, blocks - 1 - block, 0);
+    if (behind < 0) attend_shared<D>(p, lds, b, head, blocks - 1 - block);
     else attend<D, 2>(p, lds, b, head, kSharers * p.tail - 1 - behind, 0);
+  } else if constexpr (QB == kShared) {
+    attend_shared<D>(p, lds, b, head, blocks - 1 - block);
   } else {
-    const int split = div_by(block, p.row_block_div), rb = blocks - 1 - (block - split * blocks);
-    if constexpr (QB == kShared) attend_shared<D>(p, lds, b, head, rb, split);
-    else attend<D, QB>(p, lds, b, head, rb, split);
+    const int split = div_by(block, p.row_block_div);
+    attend<D, QB>(p, lds, b, head, blocks - 1 - (block - split * blocks), split);
   }
 }
 
@@ -733,8 +728,8 @@ struct Walk {
 // of 1536 over 4096 55 and 43, 32 of 1024 61.6 and 53.4, 256 of 128 59 and 151).  And prompts on their own,
 // whose longest block is twice the average: a CU works on more than one at a time, and four waves
 // that share its keys are through with it sooner (D 128: 8 of 4000 over 1000 28.2 and 27.4, 36 of 1000 over 1000 30.2
-// and 35.0, 4 of 8192 over 2048 46.4 and 37.8, 20 of 2048 49.1 and 46.7, 2 of 16384 over 4096 81 and 57, but 24 of
-// 512 over 512 15.7 and 25.8 at D 64; there 24 of 1000 21.8 and 17.7, 9 of 4096 63 and 41.6, 25 of 2048 35.4 and 50).
+// and 35.0, 4 of 8192 over 2048 46.4 and 37.8, 20 of 2048 49.1 and 46.7, 2 of 16384 over 4096 81 and 57; D 64: 24 of
+// 1000 21.8 and 17.7, 9 of 4096 63 and 41.6, but 25 of 2048, 400 blocks, 35.4 and 50).
 // Mixed: a CU works on two blocks in 1.35 times one's time, so a few more blocks than CUs, or than
 // a multiple of them, cost nearly a round.  Up to half a round is done by waves of two blocks
 // instead, four workgroups to 128 rows, which spread over all CUs (D 128, 4096 keys, blocks: 288
@@ -805,7 +800,7 @@ hipError_t launch(const AttnPlan& p, hipStream_t stream) {
   }
   hipLaunchKernelGGL((paged_attention_kernel<D, QB>), dim3(unsigned(p.workgroups)), dim3(64 * kWaves), bytes, stream, p);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.splits == 1) return e;
+  if (QB <= kShared || e != hipSuccess || p.splits == 1) return e;
   if (p.splits > 16)
     hipLaunchKernelGGL((paged_attention_join_kernel<D, 4>), dim3(unsigned(p.all_rows)), dim3(256), 0, stream, p);
   else
