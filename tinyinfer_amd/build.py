@@ -70,12 +70,14 @@ def _operands() -> None:
     is what needs both."""
     try:
         import torch
-    except ImportError:
+    except ImportError as e:
+        print(f"tinyinfer_amd.build: no _operands, whose checks NativeOps then makes in Python ({e})", flush=True)
         return
     from torch.utils.cpp_extension import include_paths, library_paths
     target = PKG / ("_operands" + sysconfig.get_config_var("EXT_SUFFIX"))
     tmp = target.with_suffix(".so.tmp")
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+          f'-DTIA_TORCH_VERSION="{torch.__version__}"',
           *(f"-I{path}" for path in include_paths()), "-I", sysconfig.get_paths()["include"], str(CSRC / "operands.cpp"),
           "-o", str(tmp), *(f"-L{path}" for path in library_paths()), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"])
     os.replace(tmp, target)

@@ -9,7 +9,9 @@
 //     the same of rank 4 with contiguous values in the last axis alone;
 //   empty(shape, like) -> an empty contiguous tensor of like's dtype and device;
 //   empty_as(shape, dtype, like) -> of like's device;
-//   record(tensors, stream id, GPU): the allocator learns that the stream uses them.
+//   record(tensors, stream id, GPU): the allocator learns that the stream uses them;
+//   torch_version: the torch whose headers this was compiled with.  Under another one no
+//     function here may be called (tensors are read through inlined accessors).
 #include <Python.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -123,4 +125,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_operands", nullptr, -1, methods, 
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__operands() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__operands() {
+  PyObject* made = PyModule_Create(&module);
+  if (made && PyModule_AddStringConstant(made, "torch_version", TIA_TORCH_VERSION) < 0) Py_CLEAR(made);
+  return made;
+}

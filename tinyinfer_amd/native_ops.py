@@ -31,6 +31,7 @@ import ctypes
 import itertools
 import json
 import math
+import warnings
 from array import array
 from contextlib import nullcontext
 from pathlib import Path
@@ -281,7 +282,8 @@ class _Call:
         handle = ops.stream_handle(index)
         stream = ops.streams.get((index, handle))
         if stream is None:
-            stream = ops.streams[index, handle] = cuda.current_stream(index).stream_id
+            stream = cuda.current_stream(index)
+            stream = ops.streams[index, handle] = stream if type(ops.operands) is _PlainOperands else stream.stream_id
         ops.operands.record(self.held, stream, index)
         # (The allocator keeps a stream with a block until the block is freed: once does.)
         if self.over is not None and handle not in self.over._streams:
@@ -400,17 +402,58 @@ def _number(value, name, low=-math.inf, above=False):
     return value
 
 
+class _PlainOperands:
+    """csrc/operands.cpp in Python, for a torch that it was not compiled for."""
+
+    def __init__(self, torch):
+        self.torch = torch
+
+    def _accepts(self, x, dtype, index, shape):
+        return (isinstance(x, self.torch.Tensor) and x.dtype == dtype and x.is_cuda and index in (-2, x.get_device())
+                and not x.requires_grad and 0 < x.numel() <= INT32_MAX and (shape is None or x.shape == shape))
+
+    def operand(self, x, dtype, index, rank, shape):
+        if self._accepts(x, dtype, index, shape) and x.is_contiguous() and x.dim() and rank in (x.dim(), -1):
+            return x.data_ptr()
+        return None
+
+    def rows(self, x, dtype, index, shape):
+        if self._accepts(x, dtype, index, shape) and x.dim() == 4 and 1 in (x.stride(3), x.shape[3]):
+            return (x.data_ptr(), *x.stride()[:3])
+        return None
+
+    def empty(self, shape, like):
+        return self.empty_as(shape, like.dtype, like)
+
+    def empty_as(self, shape, dtype, like):
+        return self.torch.empty(shape, dtype=dtype, device=like.device)
+
+    def record(self, tensors, stream, index):
+        for x in tensors:
+            x.record_stream(stream)  # (a Stream object here)
+
+
+def _operand_checks(torch):
+    """csrc/operands.cpp if it is there and of this torch, else the same in Python."""
+    try:
+        from . import _operands  # (after torch, whose libraries it uses)
+        if _operands.torch_version == torch.__version__:
+            return _operands
+        found = f"compiled for torch {_operands.torch_version}"
+    except ImportError as e:
+        found = f"not importable ({e})"
+    warnings.warn(f"tinyinfer_amd._operands is {found}: calls are checked in Python, some microseconds slower each, under torch "
+                  f"{torch.__version__}; python -m tinyinfer_amd.build compiles it", RuntimeWarning, stacklevel=3)
+    return _PlainOperands(torch)
+
+
 class NativeOps:
     """Inference-only device ops over the v2 ABI; operands are torch GPU tensors,
     work is queued on the current torch stream of their device."""
 
     def __init__(self, library_path=None):
         import torch
-        try:
-            from . import _operands  # (after torch, whose libraries it uses)
-        except ImportError as e:
-            raise ImportError(f"tinyinfer_amd._operands is not built for this torch ({e}): python -m tinyinfer_amd.build") from e
-        self.torch, self.tensor_type, self.operands = torch, torch.Tensor, _operands
+        self.torch, self.tensor_type, self.operands = torch, torch.Tensor, _operand_checks(torch)
         # torch's own short ways to both (operands are on a GPU: it is initialised), which
         # are not part of its interface and missing in a torch without GPU support.
         self.stream_handle = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
