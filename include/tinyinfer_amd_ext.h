@@ -212,10 +212,10 @@ int ti_amd_rotate(const uint16_t* x, int64_t x_batch, int64_t x_head, int64_t x_
 /* The paged fp16 KV cache: no counterpart in the reference.  `pages` (16-byte aligned) is
  * page_count pages of kv_heads * 2 * page_size * head_dim values in the kernels' own order; a
  * page is contiguous and may be copied as a whole.  page_size is a power of two from 32 to
- * 1024, head_dim 64 or 128.  Which pages hold a request's tokens is the caller's to say:
- * token t of request b lies on page table[b * width + t / page_size] (int32 on the
- * device).  What lies past the table, or on a page outside [0, page_count), does not exist:
- * it is not written, reads as zeros and is not seen. */
+ * 1024, head_dim 64 or 128, page_count * kv_heads * page_size at most 2^34.  Which pages hold a
+ * request's tokens is the caller's to say: token t of request b lies on page table[b * width +
+ * t / page_size] (int32 on the device).  What lies past the table, or on a page outside [0,
+ * page_count), does not exist: it is not written, reads as zeros and is not seen. */
 typedef struct ti_amd_kv_paged {
   uint16_t* pages;
   int32_t page_count, kv_heads, page_size, head_dim;

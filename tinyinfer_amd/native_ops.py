@@ -903,7 +903,7 @@ class NativeOps:
     # -- paged KV cache --------------------------------------------------------------
     def kv_cache_paged(self, pages, kv_heads, page_size, head_dim, *, device=None):
         """A zeroed fp16 cache of `pages` pages of `page_size` tokens (a power of two from 32
-        to 1024), `kv_heads` key heads of 64 or 128 dims."""
+        to 1024), `kv_heads` key heads of 64 or 128 dims; pages * kv_heads * page_size is at most 2^34."""
         torch = self.torch
         _count(pages, "pages")
         _count(kv_heads, "kv_heads", high=65535)
@@ -911,6 +911,8 @@ class NativeOps:
             raise ValueError("page_size must be a power of two from 32 to 1024")
         if type(head_dim) is not int or head_dim not in (64, 128):
             raise ValueError("head_dim must be 64 or 128")
+        if pages * kv_heads * page_size > 1 << 34:
+            raise ValueError("pages * kv_heads * page_size must be at most 2^34")
         where = torch.device("cuda" if device is None else device)
         if where.type != "cuda":
             raise TypeError("device: a GPU (torch 'cuda' device) is required")
