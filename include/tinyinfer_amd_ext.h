@@ -241,10 +241,13 @@ int ti_amd_kv_read_paged(const ti_amd_kv_paged* cache, uint16_t* k, uint16_t* v,
  * - q_lengths[b].  Rows that see no key, and queries past q_lengths[b], are exactly 0.  A row
  * that has an infinity or NaN in its query or sees a NaN in a key is NaN; one that sees an
  * infinity or NaN in a value is not finite in that dim.  A key with a score of -inf (it holds
- * an infinity) has no weight; a row with no other keys is 0.  What a row does not see does not
- * count, whatever memory holds there.  Scores, softmax and sums are fp32; a probability is
- * rounded to fp16 for its product (for single tokens twice: what the first rounding leaves out
- * is added).  batch and heads are at most 65535, batch * heads * q_len at most 2^23.
+ * an infinity) has no weight, though an infinity or NaN in its value may count; a row with no
+ * other keys is 0.  What a row does not see does not count, whatever memory holds there.
+ * Scores, softmax and sums are fp32; a probability is rounded to fp16 for its product.  Where
+ * a key head has at most 16 rows (heads / kv_heads * q_len: single tokens of up to 16 heads to
+ * a key head) what that rounding leaves out is added; with more rows it is or is not, as the
+ * call's extents have it walked.  batch and heads are at most 65535, batch * heads * q_len at
+ * most 2^23.
  * max_kv (0: what the table holds) plans the launch and its workspace; longer requests are
  * answered too.  workspace: ti_amd_attention_paged_workspace bytes (-1 for invalid arguments,
  * 0 if none is needed), used by this call alone until its work is done. */

@@ -170,3 +170,30 @@ def test_far_scores_that_are_near_each_other(ops, walk):
                 ops.kv_append_paged(cache, dev(k).expand(batch, kv_heads, n, dim), v, table, 0)
                 y = ops.attention_paged(dev(q), cache, table, n, causal=False).float()
                 assert ((y >= low - slack) & (y <= high + slack)).all(), (big, step, at)
+
+
+@pytest.mark.parametrize("batch,kv_heads,group,dim,q_rows,n", [
+    (2, 3, 16, 64, 1, 300), (2, 3, 4, 128, 4, 300), (1, 2, 16, 128, 1, 4000), (1, 1, 8, 64, 2, 9000), (24, 6, 16, 64, 1, 4100),
+    (140, 2, 16, 128, 1, 700), (33, 4, 2, 128, 8, 700)])
+def test_few_rows_keep_the_weights_digits(ops, batch, kv_heads, group, dim, q_rows, n):
+    """16 rows of a key head and fewer: what a weight's rounding leaves out is added, whatever the batch.
+    Two sorts of keys, of weights 1 and e^(r / sqrt(D)) and values of -8 and 8 that nearly cancel.  Scores
+    are exact; a weight is off by two roundings of an exponent of at most 14 and the hardware's 2^x (2^-20
+    and 2^-22), twice rounded (2^-22), and n of them are summed up, at least 16 sums side by side in fp32
+    (n / 16 roundings, of the weights and of the products); rounded once they are off by up to 2^-11."""
+    say("few rows", batch, kv_heads, group, dim, q_rows, n)
+    rng = np.random.default_rng(n + batch)
+    cache, table, _, _ = filled(ops, rng, batch, kv_heads, dim, 64, n)
+    sort = rng.random((batch, 1, n, 1)) < 0.25
+    k, v = np.zeros((batch, kv_heads, n, dim), np.float16), np.where(sort, 8, -8) * rng.choice([-1, 1], dim)
+    k[..., :1] = sort
+    v = np.broadcast_to(v.astype(np.float16), k.shape).copy()
+    ops.kv_append_paged(cache, dev(k), dev(v), dev(table), 0)
+    q = rng.standard_normal((batch, kv_heads * group, q_rows, dim)).astype(np.float16)
+    q[..., 0] = rng.integers(4, 21, q.shape[:3])
+    y = host(ops.attention_paged(dev(q), cache, dev(table), n, causal=False))
+    many = sort.sum(2, keepdims=True)[..., 0]
+    w = many * np.exp(q[..., 0].astype(np.float64) / np.sqrt(dim))
+    want = ((w - (n - many)) / (w + (n - many)))[..., None] * 8 * np.sign(v[:, :1, :1].astype(np.float64) * np.where(sort[:, :, :1], 1, -1))
+    tol = 8 * (2.0 ** -18 + n * 2.0 ** -27) + 2.0 ** -11 * np.abs(want) + 2.0 ** -25
+    assert (np.abs(y - want) <= tol).all(), (np.abs(y - want) - tol).max()
