@@ -54,7 +54,7 @@ namespace {
 constexpr int kTile = 64;   // keys per wave and step
 constexpr float kNegInf = -__builtin_huge_valf();
 // The reference of a row's exponents: 6 below its largest x + log2 vs when set, raised
-// when one is 14 above it.  Weights then lie around 2^6 and below 2^14: rounded to
+// when one is more than 14 above it.  Weights then lie around 2^6 and below 2^14: rounded to
 // fp16, whose smallest normal number is 2^-14, a weight 2^-20 times the heaviest
 // still keeps 11 bits.  The scale of a row of zeros counts as 2^kLeast, below every
 // other (2^-24 / 127 at least): probabilities are fp32 and stay below 2^(14 - kLeast).
@@ -381,11 +381,11 @@ __device__ void attend(const AttnPlan& p, uint8_t* lds, int b0, int head, int rb
       for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
         for (int v = 0; v < 4; ++v) high = fmaxf(high, sc[u][kb][v]);
-      if (__ballot(high > m[u] + room)) {
+      if (__ballot(high - m[u] > room)) {  // (m + room would be rounded: far from 0 by more than fp16's range has left)
         high = max_row_sum(sc[u], fmaxf(__builtin_amdgcn_logf(vs), kLeast));
         high = fmaxf(high, __shfl_xor(high, 16, 64));
         high = fmaxf(high, __shfl_xor(high, 32, 64));
-        const float nm = high > m[u] + kRaise ? high - kBelow : m[u];
+        const float nm = high - m[u] > kRaise ? high - kBelow : m[u];
         const float f = m[u] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[u] - nm);
         l[u] *= f;
 #pragma unroll
