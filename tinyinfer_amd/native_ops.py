@@ -31,6 +31,7 @@ import ctypes
 import itertools
 import json
 import math
+import sys
 import warnings
 from array import array
 from contextlib import nullcontext
@@ -40,6 +41,7 @@ from . import BACKEND_LIB, require
 
 INT32_MAX = 2**31 - 1
 INT64_MAX = 2**63 - 1
+_FLOAT_MAX = sys.float_info.max
 
 # The 12 GEMM configurations the library must report, in order (the reference
 # catalog, kernels/src/cuda/tc/catalog.cuh:8-15): three CUDA tile hints, one or
@@ -397,7 +399,8 @@ class Rotary:
 
 def _number(value, name, low=-math.inf, above=False):
     """A finite number >= low (> low if above), else ValueError."""
-    if type(value) not in (int, float) or not math.isfinite(value) or value < low or (above and value == low):
+    # (An int beyond every float is not finite either.)
+    if type(value) not in (int, float) or not abs(value) <= _FLOAT_MAX or value < low or (above and value == low):
         raise ValueError(f"{name} must be a finite number {'above' if above else 'of at least'} {low}")
     return value
 
@@ -830,7 +833,8 @@ class NativeOps:
         frequency by it; "base" multiplies the base by factor^(rotated / (rotated - 2)), so
         that the slowest pair alone is divided; "parts" keeps pairs that turn `fast` times
         or more over original_length, divides those that turn `slow` times or fewer, and
-        goes over linearly in between.  frequencies gives all of them instead (radians a
+        goes over linearly in the number of turns in between (checkpoints that go over by the
+        pairs' numbers give their own frequencies).  frequencies gives all of them instead (radians a
         position, rotated / 2 numbers).  Turned values are multiplied by amplitude."""
         torch = self.torch
         if type(rotated) is not int or rotated < 2 or rotated % 2 or rotated > 65536:
@@ -839,7 +843,8 @@ class NativeOps:
             raise ValueError("interleaved must be a bool")
         _number(base, "base", 0, True)
         _number(factor, "factor", 0, True)
-        _number(amplitude, "amplitude")
+        if abs(_number(amplitude, "amplitude")) > 2.0 ** 128 - 2.0 ** 104:
+            raise ValueError("amplitude must be a finite fp32 number")
         if scaling not in (None, "linear", "base", "parts"):
             raise ValueError('scaling must be None, "linear", "base" or "parts"')
         if scaling is None and factor != 1:
@@ -852,19 +857,25 @@ class NativeOps:
             if len(got) != count:
                 raise ValueError(f"frequencies must hold {count} numbers, got {len(got)}")
         else:
-            if scaling == "base" and count > 1:
-                base = base * factor ** (count / (count - 1))
-            got = [float(base) ** (-i / count) for i in range(count)]
-            if scaling == "linear":
-                got = [f / factor for f in got]
             if scaling == "parts":
                 _count(original_length, "original_length")
                 _number(slow, "slow")
                 if _number(fast, "fast") <= slow:
                     raise ValueError("fast must be above slow")
+            try:
+                if scaling == "base" and count > 1:
+                    base = base * factor ** (count / (count - 1))
+                got = [float(base) ** (-i / count) for i in range(count)]
+            except OverflowError:
+                got = [math.inf]
+            if scaling == "linear":
+                got = [f / factor for f in got]
+            if scaling == "parts":
                 for i, f in enumerate(got):
                     keep = min(max((original_length * f / (2 * math.pi) - slow) / (fast - slow), 0.0), 1.0)
                     got[i] = f * keep + f / factor * (1.0 - keep)
+            if not all(map(math.isfinite, got)):
+                raise ValueError("base and factor give frequencies beyond every number")
         where = torch.device("cuda" if device is None else device)
         if where.type != "cuda":
             raise TypeError("device: a GPU (torch 'cuda' device) is required")
