@@ -16,8 +16,8 @@
 // rising ones) the range of the tokens at or above the bar is cut into runs and read again until
 // it does.
 //
-// What bounds it: memory for hundreds of rows (768 rows of 128257 in fp32, 5 alternatives: 71.5 us, 5.5
-// TB/s), for a few the chain of latencies (32 rows of 50257 in fp16, 20 alternatives: 14.0 us; about 2.5
+// What bounds it: memory for hundreds of rows (768 rows of 128257 in fp32, 5 alternatives: 68.4 us, 5.8
+// TB/s; of 50257 in fp16 26.2, tokens in place of bytes: fp32 30.9), for a few the chain of latencies (32 rows of 50257 in fp16, 20 alternatives: 14.0 us; about 2.5
 // of them launch, 1 the first loads, 2 the bar, 1 a round of the row, 1 sums, 3 the list, 2 joining the
 // parts, 1 their order; one row of fp32, 5 alternatives 9.6, none 6.8).  Whole rows take 16.6, and what
 // one CU fetches, about 9 bytes a cycle, bounds them: loads two to four rounds ahead, or a quarter

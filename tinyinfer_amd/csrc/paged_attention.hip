@@ -26,13 +26,14 @@
 //
 // What bounds it.  Single tokens: memory where caches are long (16 requests of 8 x 128, 12000
 // to 32768 keys: 248 us, 6.3 TB/s), launch and one tile's chain of latencies where they are
-// short (one request of 12 heads, 300 keys: 6.2 us; 32 of them, 128 to 1024 keys: 15 us, 5.6 of
+// short (one request of 12 heads, 300 keys: 6.0 us; 32 of them, 128 to 1024 keys: 14 us, 5.6 of
 // them without keys).  Prompts: a tile of 64 keys x 32 rows at D 128 is 68 matrix instructions, 1088
 // cycles of a SIMD, about 105 vector instructions and 32 exponentials, 700 cycles, and 32 KB
 // from LDS, 128 of the CU's cycles and 512 for four waves; two workgroups a CU overlap these in part.  2
-// requests of 777 queries, 32 heads over 8 of 128, 4500 to 6001 keys: 166 us, 813 TFLOP/s (400
-// workgroups on 256 CUs); 2 of 1024 over 5120 157 us, 983 TFLOP/s, 87 % of what a large library
-// product reaches; 4 prompts of 1024, 25 heads of 64: 28 us, 480 TFLOP/s.  Left out (wrong values), 166
+// requests of 777 queries, 32 heads over 8 of 128, 4500 to 6001 keys: 165 us, 817 TFLOP/s (400
+// workgroups on 256 CUs); 2 of 1024 over 5120 159 us, 973 TFLOP/s, 86 % of what a large library
+// product reaches; 4 prompts of 1024, 25 heads of 64: 28 us, 480 TFLOP/s; prompts on their own last as long
+// as their longest block's chain of tiles (one of 1000, 32 heads over 8 of 128: 27 us, 306).  Left out (wrong values), 166
 // us becomes: the exponentials 158, the maximum 164, the loads 155, the second product 122.  One row
 // block's products stand beside the other's exponentials (172 with both blocks in step).  Tried for the
 // shared tiles and no faster: the next tile's scores under this one's weights (192 us for 179 then),
@@ -128,7 +129,9 @@ struct Rows {
   // result is as near as fp32 weights would bring it.  Two blocks (prompts, and single tokens of more
   // heads where a call is large: 32 requests of 32 heads over one, 9000 keys 36.7 us, one block 37.8;
   // 64 over 16384 100 and 113) take the rounded weights alone, a third less matrix work, and sum up
-  // these too: by one more product, with ones, in place of 32 additions.
+  // these too: by one more product, with ones, in place of 32 additions.  (Twice rounded the chunk
+  // above takes 235 us in place of 167, and its error against 64 bits is 2.1e-4 in place of 2.9e-4,
+  // most of both the result's own rounding.)
   static constexpr bool FINE = QB == 1;
 
   const AttnPlan& p;

@@ -12,8 +12,8 @@
 // slices of one projection.
 //
 // What bounds it: memory (8 prompts of up to 1000 tokens, 25 heads of 64: append 26 us, of which the
-// same bytes copied take 23; read back 16.6, 5.2 TB/s), and the launch for single tokens (32
-// requests of 12 heads of 64: 4.4 and 4.1 us).
+// same bytes copied take 23; read back 20.5, 4.1 TB/s, or 16.6 where the rows are still in the last
+// cache), and the launch for single tokens (32 requests of 12 heads of 64: 4.7 and 4.1 us).
 #include "paged_cache.hpp"
 #include "rotary.hpp"
 

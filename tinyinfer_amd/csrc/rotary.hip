@@ -5,9 +5,11 @@
 // A lane holds the cosines and sines of its 8 pairs (rotary.hpp) and walks over heads,
 // which share them: they cost about 300 vector instructions, a head's values 70.
 //
-// What bounds it: memory (2 requests of 32 heads of 128, 6001 rows: 36 us, 5.4 TB/s of reads and
-// writes, vector units 40 % busy; 8 of 25 heads of 64, 777 rows: 10.7, launch and ramp 4 of them), and
-// the launch for single tokens (32 of 24 heads of 64: 5.0 us).
+// What bounds it: memory (2 requests of 32 heads of 128, 6001 rows: 41 us, 4.8 TB/s of reads and
+// writes, 35.6 where the output's block stays partly in the last cache; vector units 40 % busy; 8 of 25
+// heads of 64, 777 rows: 9.7, launch and ramp 3 of them), and the launch for single tokens (32 of 24
+// heads of 64: 3.6 us).  Dims that are no multiple of 16: 8- or 4-byte pieces (8 of 32 heads of 80, 2000 rows, 40
+// dims turned 62 us, 2.6 TB/s, 20 dims 77).
 #include "rotary.hpp"
 
 namespace tia {

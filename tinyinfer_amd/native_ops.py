@@ -1011,8 +1011,9 @@ class NativeOps:
         (append first, then attend).  Rows that see no key and queries past
         q_lengths[b] are 0.  kv_lengths, q_lengths and query_offsets are int32 [B]
         tensors or host ints; tensors make a call that a graph can capture.
-        max_kv_length: what kv_lengths stay within where the table holds much more
-        (it plans the launch only)."""
+        max_kv_length: what kv_lengths stay within where the table holds much more.  It
+        plans the launch only, but without it the plan is for a full table: a token over 300
+        keys, 12 heads, takes 8.4 us, with a table for 32768 and no max_kv_length 11.8."""
         call = _Call(self, "ti_amd_attention_paged")
         call.cache(cache, PagedKVCache)
         call.operand(q, self.torch.float16, "q", rank=4)
